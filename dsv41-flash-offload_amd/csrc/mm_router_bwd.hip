@@ -1,0 +1,356 @@
+// Backward pass of the router (mm_router_topk): with logits = x gate^T, w = softmax of the picked logits,
+//   d[t][j] = w[t][j] (dw[t][j] - sum_i w[t][i] dw[t][i]),   D = dlogits + d scattered to the picks,
+//   dx = D gate,   dgate = D^T x.
+//
+// Both products run on v_mfma_f32_16x16x32_bf16 with fp32 accumulation. The fp32 factors are split into bf16 parts
+// (D = D1 + D2 + D3 exactly, gate = G1 + G2 up to 2^-17 of it): dgate multiplies the three parts of D with the bf16 x, so
+// every product is exact and the accumulation is the only rounding; dx takes D1 G1 + D1 G2 + D2 G1, which leaves out about
+// 2^-16 of a product where the bf16 result is rounded by 2^-9.
+//
+// Launches: the parts of D, row-major for dx (its k is the expert) and transposed for dgate (its k is the token), and of
+// the transposed gate; the two products in 128 x 128 tiles; dgate's tokens are split over enough workgroups to fill the GPU
+// and their partial sums added in order.
+#include <algorithm>
+#include <type_traits>
+
+#include "mm_common.h"
+
+namespace mm {
+
+typedef float rb_f4 __attribute__((ext_vector_type(4)));
+typedef __bf16 rb_bf8 __attribute__((ext_vector_type(8)));
+typedef short rb_s4 __attribute__((ext_vector_type(4)));
+
+constexpr int RB_T = 128, RB_K = 32;
+constexpr int RB_ROW = 32;               // LDS row of a k-contiguous operand: four 16-byte chunks, swizzled
+constexpr int RB_XROW = RB_T + 16;       // LDS row of the token-major input tile (32 bytes of padding: transposed reads of four rows hit distinct banks)
+__device__ __forceinline__ int rb_at(int r, int q) { return r * RB_ROW + 8 * (q ^ ((r >> 2) & 3)); }
+
+// v = a + b + c in bf16: a truncated (no overflow), b rounded, c the rest, exact. inf and NaN stay in a.
+__device__ __forceinline__ void split3(float v, uint16_t& a, uint16_t& b, uint16_t& c)
+{
+    const uint32_t u = __float_as_uint(v);
+    const bool fin = (u & 0x7f800000u) != 0x7f800000u;
+    a = (uint16_t)((u >> 16) | ((u & 0x7fffffffu) > 0x7f800000u ? 0x40u : 0u));
+    const float r1 = fin ? v - __uint_as_float(u & 0xffff0000u) : 0.f;
+    b = f2bf(r1);
+    c = f2bf(r1 - __uint_as_float((uint32_t)b << 16));
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// D = dlogits + scattered top-k gradient, one 64-token x 64-expert tile per workgroup, as parts in both orders.
+// ---------------------------------------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void k_rb_parts(const int64_t* __restrict__ ids, const float* __restrict__ w,
+                                                  const float* __restrict__ dw, const float* __restrict__ dlogits, int T, int E,
+                                                  int k, int Ek, int Tk, uint16_t* __restrict__ d, uint16_t* __restrict__ dt)
+{
+    __shared__ float tile[64][65];
+    const int t0 = blockIdx.y * 64, e0 = blockIdx.x * 64, tid = threadIdx.x;
+    for (int i = tid; i < 64 * 64; i += 256)
+    {
+        const int r = i >> 6, c = i & 63;
+        tile[r][c] = dlogits && t0 + r < T && e0 + c < E ? dlogits[(size_t)(t0 + r) * E + e0 + c] : 0.f;
+    }
+    __syncthreads();
+    // a thread per row adds its picks in ascending j (an expert picked twice gets both)
+    if (dw && tid < 64 && t0 + tid < T)
+    {
+        const size_t at = (size_t)(t0 + tid) * k;
+        float s = 0.f;
+        for (int j = 0; j < k; ++j) s = fmaf(w[at + j], dw[at + j], s);
+        for (int j = 0; j < k; ++j)
+        {
+            const int64_t e = ids[at + j] - e0;
+            if (e >= 0 && e < 64 && e0 + e < E) tile[tid][e] += w[at + j] * (dw[at + j] - s);
+        }
+    }
+    __syncthreads();
+    // pairs of neighbours along the contiguous index of each order
+    if (d)
+        for (int i = tid; i < 64 * 32; i += 256)
+        {
+            const int r = i >> 5, c = 2 * (i & 31);
+            if (t0 + r >= T || e0 + c >= Ek) continue;
+            uint16_t p[2][3];
+            split3(tile[r][c], p[0][0], p[0][1], p[0][2]);
+            split3(tile[r][c + 1], p[1][0], p[1][1], p[1][2]);
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+                *reinterpret_cast<uint32_t*>(d + ((size_t)q * T + t0 + r) * Ek + e0 + c) = p[0][q] | ((uint32_t)p[1][q] << 16);
+        }
+    if (dt)
+        for (int i = tid; i < 64 * 32; i += 256)
+        {
+            const int r = i >> 5, c = 2 * (i & 31);
+            if (e0 + r >= E || t0 + c >= Tk) continue;
+            uint16_t p[2][3];
+            split3(tile[c][r], p[0][0], p[0][1], p[0][2]);
+            split3(tile[c + 1][r], p[1][0], p[1][1], p[1][2]);
+#pragma unroll
+            for (int q = 0; q < 3; ++q)
+                *reinterpret_cast<uint32_t*>(dt + ((size_t)q * E + e0 + r) * Tk + t0 + c) = p[0][q] | ((uint32_t)p[1][q] << 16);
+        }
+}
+
+// Two parts of the transposed gate: gt [2][H][Ek], zeros past E.
+__global__ __launch_bounds__(256) void k_rb_gate(const float* __restrict__ gate, int E, int H, int Ek, uint16_t* __restrict__ gt)
+{
+    __shared__ float tile[64][65];
+    const int h0 = blockIdx.x * 64, e0 = blockIdx.y * 64, tid = threadIdx.x;
+    for (int i = tid; i < 64 * 64; i += 256)
+    {
+        const int r = i >> 6, c = i & 63;
+        tile[r][c] = e0 + r < E && h0 + c < H ? gate[(size_t)(e0 + r) * H + h0 + c] : 0.f;
+    }
+    __syncthreads();
+    for (int i = tid; i < 64 * 32; i += 256)
+    {
+        const int r = i >> 5, c = 2 * (i & 31);
+        if (h0 + r >= H || e0 + c >= Ek) continue;
+        uint16_t p[2][3];
+        split3(tile[c][r], p[0][0], p[0][1], p[0][2]);
+        split3(tile[c + 1][r], p[1][0], p[1][1], p[1][2]);
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+            *reinterpret_cast<uint32_t*>(gt + ((size_t)q * H + h0 + r) * Ek + e0 + c) = p[0][q] | ((uint32_t)p[1][q] << 16);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// The products, 128 (hidden index h) x 128 (column c: token or expert) tiles, four waves of 64 x 64.
+// DX: rows are gt's (k = expert), columns d's, result dx[c][h] in bf16.
+// else: rows are columns of x (k = token, read transposed from LDS), columns dt's, result part[z][c][h] in fp32.
+// ---------------------------------------------------------------------------------------------------------
+template <bool DX>
+__global__ __launch_bounds__(256) void k_rb_gemm(const uint16_t* __restrict__ rows, const uint16_t* __restrict__ cols, int H,
+                                                 int C, int T, int K, int ksteps, const float* __restrict__ gate, int E,
+                                                 void* __restrict__ out)
+{
+    constexpr int PR = DX ? 2 : 1, PC = DX ? 2 : 3;
+    __shared__ __align__(16) uint16_t rs[DX ? PR * RB_T * RB_ROW : RB_K * RB_XROW];
+    __shared__ __align__(16) uint16_t cs[PC][RB_T * RB_ROW];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int h0 = blockIdx.x * RB_T, c0 = blockIdx.y * RB_T;
+    const int wh = 64 * (wave >> 1), wc = 64 * (wave & 1);
+    const int s0 = blockIdx.z * ksteps, s1 = min(K / RB_K, s0 + ksteps);
+    uint4 rv[2 * PR], cv[2 * PC];
+    auto load = [&](int s) {
+        const int k0 = s * RB_K;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+        {
+            const int i = tid + 256 * j;
+            if constexpr (DX)
+            {
+                const size_t r = min(h0 + (i >> 2), H - 1);
+#pragma unroll
+                for (int p = 0; p < PR; ++p)
+                    rv[2 * p + j] = *reinterpret_cast<const uint4*>(rows + ((size_t)p * H + r) * K + k0 + 8 * (i & 3));
+            }
+            else
+            {
+                const int t = k0 + (i >> 4), h = h0 + 8 * (i & 15);
+                rv[j] = t < T && h < H ? *reinterpret_cast<const uint4*>(rows + (size_t)t * H + h) : make_uint4(0, 0, 0, 0);
+            }
+            const size_t c = min(c0 + (i >> 2), C - 1);
+#pragma unroll
+            for (int p = 0; p < PC; ++p)
+                cv[2 * p + j] = *reinterpret_cast<const uint4*>(cols + ((size_t)p * C + c) * K + k0 + 8 * (i & 3));
+        }
+    };
+    rb_f4 acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = rb_f4{ 0.f, 0.f, 0.f, 0.f };
+    if (s0 < s1) load(s0);
+    for (int s = s0; s < s1; ++s)
+    {
+        __syncthreads();                                  // the previous step's operand reads are done
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+        {
+            const int i = tid + 256 * j;
+            if constexpr (DX)
+            {
+#pragma unroll
+                for (int p = 0; p < PR; ++p)
+                    *reinterpret_cast<uint4*>(&rs[p * RB_T * RB_ROW + rb_at(i >> 2, i & 3)]) = rv[2 * p + j];
+            }
+            else *reinterpret_cast<uint4*>(&rs[(i >> 4) * RB_XROW + 8 * (i & 15)]) = rv[j];
+#pragma unroll
+            for (int p = 0; p < PC; ++p) *reinterpret_cast<uint4*>(&cs[p][rb_at(i >> 2, i & 3)]) = cv[2 * p + j];
+        }
+        __syncthreads();
+        if (s + 1 < s1) load(s + 1);
+        rb_bf8 R[PR][4], Cc[PC][4];
+        const int r = lane & 15, q = lane >> 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+        {
+            if constexpr (DX)
+            {
+#pragma unroll
+                for (int p = 0; p < PR; ++p)
+                    R[p][i] = *reinterpret_cast<const rb_bf8*>(&rs[p * RB_T * RB_ROW + rb_at(wh + 16 * i + r, q)]);
+            }
+            else
+            {
+                // four tokens x 16 hidden indices per transposed read: lane r of a quarter names token r >> 2 and four
+                // columns, and gets column r of the four tokens; quarter q's tokens are 8 q .. 8 q + 7
+                typedef __attribute__((address_space(3))) rb_s4* lds4;
+                uint16_t* at = &rs[(8 * q + (r >> 2)) * RB_XROW + wh + 16 * i + 4 * (r & 3)];
+                const rb_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at);
+                const rb_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 4 * RB_XROW));
+                R[0][i] = __builtin_bit_cast(rb_bf8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            }
+#pragma unroll
+            for (int p = 0; p < PC; ++p)
+                Cc[p][i] = *reinterpret_cast<const rb_bf8*>(&cs[p][rb_at(wc + 16 * i + r, q)]);
+        }
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+        {
+            constexpr int rp[3] = { 0, 0, DX ? 1 : 0 }, cp[3] = { 0, 1, DX ? 0 : 2 };
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(R[rp[p]][i], Cc[cp[p]][j], acc[i][j], 0, 0, 0);
+        }
+    }
+    // lane (column l & 15, group l >> 4) holds hidden indices 4 g .. 4 g + 3 of its column; H is a multiple of 16
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+        {
+            const int h = h0 + wh + 16 * i + 4 * (lane >> 4), c = c0 + wc + 16 * j + (lane & 15);
+            if (h >= H || c >= C) continue;
+            rb_f4 v = acc[i][j];
+            if constexpr (DX)
+            {
+                // an infinite gradient times a zero part of the gate is NaN: such results are summed again from whole factors,
+                // so that they are what the formula gives (inf, or NaN)
+#pragma unroll
+                for (int m = 0; m < 4; ++m)
+                    if (v[m] != v[m])
+                    {
+                        v[m] = 0.f;
+                        for (int e = 0; e < E; ++e)
+                        {
+                            const uint16_t* d = cols + (size_t)c * K + e;
+                            v[m] = fmaf(__uint_as_float((uint32_t)d[0] << 16) + __uint_as_float((uint32_t)d[(size_t)C * K] << 16),
+                                        gate[(size_t)e * H + h + m], v[m]);
+                        }
+                    }
+            }
+            if constexpr (DX)
+                *reinterpret_cast<uint2*>((uint16_t*)out + (size_t)c * H + h) =
+                    make_uint2(f2bf(v[0]) | ((uint32_t)f2bf(v[1]) << 16), f2bf(v[2]) | ((uint32_t)f2bf(v[3]) << 16));
+            else *reinterpret_cast<rb_f4*>((float*)out + ((size_t)blockIdx.z * C + c) * H + h) = v;
+        }
+}
+
+// out[i] = part[0][i] + part[1][i] + ... in order, four values a thread.
+__global__ __launch_bounds__(256) void k_rb_sum(const float* __restrict__ part, int S, size_t n, float* __restrict__ out)
+{
+    const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    rb_f4 s = *reinterpret_cast<const rb_f4*>(part + i);
+    for (int z = 1; z < S; ++z) s += *reinterpret_cast<const rb_f4*>(part + z * n + i);
+    *reinterpret_cast<rb_f4*>(out + i) = s;
+}
+
+// Workgroups dgate's tokens are split over: two per CU in all, at least four steps of 32 tokens each.
+static int rb_splits(int T, int H, int E)
+{
+    const int tiles = ((H + RB_T - 1) / RB_T) * ((E + RB_T - 1) / RB_T), steps = (T + RB_K - 1) / RB_K;
+    return std::max(1, std::min(512 / tiles, steps / 4));
+}
+struct RouterBwdWs
+{
+    size_t d, dt, gt, part, total;
+};
+static RouterBwdWs router_bwd_ws(int T, int H, int E)
+{
+    RouterBwdWs w{};
+    size_t at = 0;
+    auto take = [&](size_t b) { const size_t o = at; at += (b + 255) & ~(size_t)255; return o; };
+    const size_t Ek = (E + 31) & ~31, Tk = (T + 31) & ~31;
+    w.d = take(2 * (size_t)T * Ek * 2);
+    w.dt = take(3 * (size_t)E * Tk * 2);
+    w.gt = take(2 * (size_t)H * Ek * 2);
+    const int S = rb_splits(T, H, E);
+    w.part = take(S > 1 ? (size_t)S * E * H * 4 : 0);
+    w.total = at;
+    return w;
+}
+
+}  // namespace mm
+
+using namespace mm;
+
+extern "C" {
+
+size_t mm_router_backward_workspace(int T, int H, int E)
+{
+    if (T <= 0 || H <= 0 || E <= 0) return 0;
+    return router_bwd_ws(T, H, E).total;
+}
+
+int mm_router_backward(const void* x_bf16, int T, int H, const float* gate, int E, int k, const int64_t* ids, const float* w,
+                       const float* dw, const float* dlogits, void* dx_bf16, float* dgate, void* workspace,
+                       size_t workspace_bytes, mm_stream_t stream)
+{
+    MM_CHECK_ARG(T >= 0 && H > 0 && H % 16 == 0, "mm_router_backward: need T >= 0, H > 0, H %% 16 == 0 (T=%d H=%d)", T, H);
+    MM_CHECK_ARG(E > 0 && E <= 1024 && k > 0 && k <= 32, "mm_router_backward: need 0 < E <= 1024, 0 < k <= 32 (E=%d k=%d)", E, k);
+    MM_CHECK_ARG(T <= (1 << 21), "mm_router_backward: more than 2^21 tokens (%d)", T);
+    MM_CHECK_ARG(T == 0 || dw || dlogits, "mm_router_backward: neither dw nor dlogits given");
+    MM_CHECK_ARG(!dw || T == 0 || (ids && w), "mm_router_backward: dw needs ids and w");
+    MM_CHECK_ARG(!dgate || T == 0 || x_bf16, "mm_router_backward: dgate needs x");
+    MM_CHECK_ARG(!dx_bf16 || gate, "mm_router_backward: dx needs the gate");
+    MM_CHECK_ARG((((uintptr_t)x_bf16 | (uintptr_t)dx_bf16 | (uintptr_t)dgate) & 15) == 0,
+                 "mm_router_backward: x, dx and dgate must be 16-byte aligned");
+    if (!dx_bf16 && !dgate) return MM_OK;
+    const hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
+    if (T == 0)
+    {
+        // no token: a gate gradient of zeros (one empty partial sum per tile)
+        if (dgate)
+            hipLaunchKernelGGL((k_rb_gemm<false>), dim3((H + RB_T - 1) / RB_T, (E + RB_T - 1) / RB_T), dim3(256), 0, hs, nullptr,
+                               nullptr, H, E, 0, 0, 0, nullptr, E, dgate);
+        return check_launch("mm_router_backward");
+    }
+    const RouterBwdWs s = router_bwd_ws(T, H, E);
+    MM_CHECK_ARG(workspace && workspace_bytes >= s.total && ((uintptr_t)workspace & 15) == 0,
+                 "mm_router_backward: workspace too small or misaligned (%zu < %zu)", workspace_bytes, s.total);
+    unsigned char* p = static_cast<unsigned char*>(workspace);
+    const int Ek = (E + 31) & ~31, Tk = (T + 31) & ~31, S = rb_splits(T, H, E);
+    uint16_t* d = dx_bf16 ? (uint16_t*)(p + s.d) : nullptr;
+    uint16_t* dt = dgate ? (uint16_t*)(p + s.dt) : nullptr;
+    hipLaunchKernelGGL(k_rb_parts, dim3((E + 63) / 64, (T + 63) / 64), dim3(256), 0, hs, ids, w, dw, dlogits, T, E, k, Ek, Tk, d,
+                       dt);
+    if (dx_bf16)
+    {
+        uint16_t* gt = (uint16_t*)(p + s.gt);
+        hipLaunchKernelGGL(k_rb_gate, dim3((H + 63) / 64, (E + 63) / 64), dim3(256), 0, hs, gate, E, H, Ek, gt);
+        hipLaunchKernelGGL((k_rb_gemm<true>), dim3((H + RB_T - 1) / RB_T, (T + RB_T - 1) / RB_T), dim3(256), 0, hs, gt, d, H, T, T,
+                           Ek, Ek / RB_K, gate, E, dx_bf16);
+    }
+    if (dgate)
+    {
+        float* part = S > 1 ? (float*)(p + s.part) : dgate;
+        const int steps = Tk / RB_K, per = (steps + S - 1) / S;
+        hipLaunchKernelGGL((k_rb_gemm<false>), dim3((H + RB_T - 1) / RB_T, (E + RB_T - 1) / RB_T, S), dim3(256), 0, hs,
+                           (const uint16_t*)x_bf16, dt, H, E, T, Tk, per, nullptr, E, part);
+        if (S > 1)
+        {
+            const size_t n = (size_t)E * H;
+            hipLaunchKernelGGL(k_rb_sum, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, hs, part, S, n, dgate);
+        }
+    }
+    return check_launch("mm_router_backward");
+}
+
+}  // extern "C"

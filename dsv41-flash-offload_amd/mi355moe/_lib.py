@@ -3,6 +3,7 @@
 There is no fallback: if the HIP library is missing or fails to load, every entry point raises. PyTorch is
 used only for device memory and streams; tensors are passed as raw device pointers.
 """
+import contextlib
 import ctypes
 import os
 
@@ -29,6 +30,19 @@ class MMLayer(ctypes.Structure):
     EXACT = 1     # MM_LAYER_EXACT: fp16-rounded weights (the reference's EXACT expert) instead of AFFINE
 
 
+class MMW4(ctypes.Structure):
+    """Mirror of mm_w4_t."""
+
+    _fields_ = [("q", vp), ("scales", vp), ("zeros", vp)]
+
+
+class MMW4Layer(ctypes.Structure):
+    """Mirror of mm_w4_layer_t."""
+
+    _fields_ = [("w13", MMW4), ("w2", MMW4), ("E", i32), ("H", i32), ("I", i32), ("group", i32), ("scale_dtype", i32),
+                ("limit", f32)]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     "mm_version": (i32, []),
@@ -36,6 +50,11 @@ _SIGS = {
     "mm_host_alloc": (i32, [ctypes.POINTER(vp), sz]),
     "mm_host_free": (i32, [vp]),
     "mm_router_topk": (i32, [vp, i32, i32, vp, i32, i32, vp, vp, vp, vp]),
+    "mm_router_backward_workspace": (sz, [i32, i32, i32]),
+    "mm_router_backward": (i32, [vp, i32, i32, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
+    "mm_balance_workspace": (sz, [i32, i32, i32]),
+    "mm_balance_loss": (i32, [vp, i32, vp, vp, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, sz, vp]),
+    "mm_balance_loss_backward": (i32, [vp, vp, i32, vp, vp, vp, i32, i32, i32, i32, i32, vp, vp]),
     "mm_split": (i32, [vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
     "mm_combine_host": (i32, [vp, i32, vp, vp, vp, vp, i64, vp]),
     "mm_permute_workspace": (sz, [i32, i32]),
@@ -53,6 +72,10 @@ _SIGS = {
     "mm_fused_moe": (i32, [ctypes.POINTER(MMLayer), vp, i32, i32, i32, vp, vp, i32, vp, vp, sz, vp]),
     "mm_fat_batched_workspace": (sz, [i32, i32, i32, i32, i32]),
     "mm_fat_batched": (i32, [ctypes.POINTER(MMLayer), vp, i32, i32, i32, vp, vp, vp, vp, i32, vp, vp, sz, vp]),
+    "mm_w4_linear_workspace": (sz, [i32, i32, i32]),
+    "mm_w4_linear": (i32, [vp, i32, i32, i32, i32, ctypes.POINTER(MMW4), i32, i32, vp, i32, vp, sz, vp]),
+    "mm_w4_moe_workspace": (sz, [i32, i32, i32, i32, i32, i32, i32]),
+    "mm_w4_moe": (i32, [ctypes.POINTER(MMW4Layer), vp, i32, i32, i32, vp, vp, i32, vp, vp, sz, vp]),
     "mm_slot_point": (i32, [vp, vp, vp, vp, i32, vp, i32, vp]),
     "mm_stage_copy": (i32, [vp, vp, vp, i32, vp]),
     "mm_copy_stream": (i32, [i32, i32, vp, ctypes.POINTER(vp)]),
@@ -124,6 +147,37 @@ def stream_ptr(stream=None):
     import torch
     s = stream if stream is not None else torch.cuda.current_stream()
     return s.cuda_stream
+
+
+@contextlib.contextmanager
+def _entered(device, stream):
+    import torch
+    with torch.cuda.device(device), torch.cuda.stream(stream):
+        yield
+
+
+def on(device, stream=None):
+    """Context in which a call's buffers are allocated and its kernels launched: `device` current (a call's tensors may
+    live on another device than the current one), and `stream` (default: the device's current stream)."""
+    import torch
+    if stream is None and torch.cuda.current_device() == device.index:
+        return contextlib.nullcontext()
+    return _entered(device, stream)
+
+
+def check_tensors(what, device, **tensors):
+    """Every given tensor is on `device`, a GPU."""
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: {name} is on {t.device}, expected {device}")
+    if device.type != "cuda":
+        raise ValueError(f"{what}: needs GPU tensors (got {device})")
+
+
+def aligned(t):
+    """t with contiguous elements at a 16-byte boundary (a copy if it is not so)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 # copy stream roles (index of mm_copy_stream)

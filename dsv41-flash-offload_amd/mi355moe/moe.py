@@ -4,7 +4,7 @@ Every computation runs in libmi355moe.so; this module allocates buffers and laun
 """
 import torch
 
-from . import _lib
+from . import _lib, w4
 
 # Default fat-expert threshold of moe_forward (the reference image's VLLM_EXL3_FAT_THRESHOLD, docker/entrypoint.sh:69): calls
 # of at most this many tokens run on the decode path, larger ones go to mm_fused_moe.
@@ -118,7 +118,11 @@ def moe_forward(store, x, ids, w, shared_expert=None, fat_threshold=FAT_THRESHOL
     Routes with ids outside [0, E) contribute nothing. As the reference's fused-MoE call does
     (patches/vllm-exl3-host-dma.patch:241-290), a call of at most `fat_threshold` tokens runs every route on the
     decode path. A larger call goes to mm_fused_moe, which takes the decode path or the grouped GEMM by its routes and
-    experts. No call synchronises the host, so every call can be captured in a HIP graph."""
+    experts. No call synchronises the host, so every call can be captured in a HIP graph.
+
+    A layer of 4-bit experts (w4.W4Store) runs on w4.moe, whatever the threshold."""
+    if isinstance(store, w4.W4Store):
+        return w4.moe(store, x, ids, w, shared_expert=shared_expert, stream=stream)
     T = x.shape[0]
     ids, w = _with_shared(ids, w, T, shared_expert)
     k = ids.shape[1]

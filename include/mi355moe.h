@@ -62,6 +62,40 @@ int mm_host_free(void* ptr);
 int mm_router_topk(const void* x_bf16, int T, int H, const float* gate, int E, int k, float* logits, int64_t* ids,
                    float* w, mm_stream_t stream);
 
+/* Backward pass of mm_router_topk. With w = softmax of the picked logits and the gradients dw fp32 [T][k] (NULL: none) and
+ * dlogits fp32 [T][E] (NULL: none; of a loss on the logits such as mm_balance_loss) of its outputs,
+ *   D = dlogits + scatter(w[t][j] (dw[t][j] - sum_i w[t][i] dw[t][i]) at ids[t][j]),
+ *   dx bf16 [T][H] = D gate, dgate fp32 [E][H] = D^T x   (either NULL: not computed).
+ * x, gate, ids and w as mm_router_topk took and gave them (ids outside [0, E) get no gradient, a pick named twice gets
+ * both). fp32 factors are multiplied as exact sums of bf16 parts with fp32 accumulation (dx leaves out products below 2^-16 of
+ * the largest part). T <= 2^21, H a multiple of 16, E <= 1024, k <= 32; x, dx, dgate and the workspace 16-byte aligned. */
+size_t mm_router_backward_workspace(int T, int H, int E);
+int mm_router_backward(const void* x_bf16, int T, int H, const float* gate, int E, int k, const int64_t* ids, const float* w,
+                       const float* dw, const float* dlogits, void* dx_bf16, float* dgate, void* workspace,
+                       size_t workspace_bytes, mm_stream_t stream);
+
+/* Load-balance loss over B sequences of T tokens, with the per-expert counts. p[t] = the scores of token t over the E
+ * experts: softmax of its logits, or (MM_SCORE_SIGMOID) their sigmoids divided by the sum of the sigmoids. Per sequence, over
+ * the tokens with mask != 0 (mask uint8 [B][T]; NULL: all),
+ *   counts int32 [B][E] = picks of each expert (ids int64 [B][T][k]; ids outside [0, E) are not counted),
+ *   tokens int32 [B] = tokens that take part, load fp32 [B][E] = sum_t p[t],
+ *   loss fp32 [B] = E / (k tokens^2) sum_e counts[e] load[e]   (0 for a sequence without tokens).
+ * One loss over a whole batch is B = 1. logits [B][T][E] of type MM_DTYPE_*; a logit of -inf is an expert that cannot be
+ * picked, and a token whose logits are all -inf has no scores. Masked tokens' logits are never used. Sums are fp32 in a fixed order.
+ * E <= 1024, k <= 32, B <= 65535. Workspace: mm_balance_workspace(B, T, E) bytes (0: none). */
+#define MM_SCORE_SOFTMAX 0
+#define MM_SCORE_SIGMOID 1
+size_t mm_balance_workspace(int B, int T, int E);
+int mm_balance_loss(const void* logits, int dtype, const int64_t* ids, const uint8_t* mask, int B, int T, int E, int k,
+                    int score, float* loss, int32_t* counts, int32_t* tokens, float* load, void* workspace,
+                    size_t workspace_bytes, mm_stream_t stream);
+
+/* Gradient of mm_balance_loss: dlogits [B][T][E] (the logits' type) from dloss fp32 [B] and the forward's counts and tokens
+ * (constants of the gradient; summed over data-parallel ranks they give the gradient of the loss over all of them);
+ * zeros in masked rows. */
+int mm_balance_loss_backward(const float* dloss, const void* logits, int dtype, const uint8_t* mask, const int32_t* counts,
+                             const int32_t* tokens, int B, int T, int E, int k, int score, void* dlogits, mm_stream_t stream);
+
 /* Decode-tier split; replaces ft_split (ct/ft_tier_cu_v.cu:129-143), same buffers and semantics:
  * sel int64 [n], w fp32 [n], z fp16 [bsz][H] (n = bsz * topk), slotof int32 [E], score fp32 [E], pol fp32 [9];
  * ctrl int64 [16], hx fp16 [bsz*H] and hpicks int32 [n*3] are host-mapped; seqc, dflag int64 [1] and
@@ -231,6 +265,44 @@ size_t mm_fat_batched_workspace(int n, int T, int E, int H, int I);
 int mm_fat_batched(const mm_layer_t* layer, const void* x, int x_dtype, int T, int n, const int64_t* token_sorted,
                    const uint16_t* weight_sorted, const int32_t* counts, const uint8_t* skip, int cap, float* out,
                    void* workspace, size_t workspace_bytes, mm_stream_t stream);
+
+/* ------------------------------------------------------------------------------------ 4-bit weights */
+
+/* A matrix [N][K] of 4-bit weights with group scales, in the storage of the checkpoints: w[n][k] = (q - z) s with q = bits
+ * 4 (k % 8) .. + 3 of q[n][k / 8], s = scales[n][k / group] (fp16 or bf16) and z = zeros[n][k / group] (NULL: 8). group is
+ * 32, 64 or 128 and divides K. q is 16-byte aligned; rows are contiguous. */
+typedef struct mm_w4
+{
+    const int32_t* q;           /* [N][K / 8] */
+    const uint16_t* scales;     /* [N][K / group] */
+    const uint8_t* zeros;       /* [N][K / group] or NULL */
+} mm_w4_t;
+
+/* y [M][N] (y_dtype) = x [M][K] (x_dtype) W^T. Products are exact, sums fp32, the result is rounded once. x 16-byte
+ * aligned. Built for few rows (decode steps); any M works, at 64 rows per pass over the weights. Workspace:
+ * mm_w4_linear_workspace bytes (fp32 inputs only), 16-byte aligned. */
+size_t mm_w4_linear_workspace(int x_dtype, int M, int K);
+int mm_w4_linear(const void* x, int x_dtype, int M, int K, int N, const mm_w4_t* W, int group, int scale_dtype, void* y,
+                 int y_dtype, void* workspace, size_t workspace_bytes, mm_stream_t stream);
+
+/* The experts of one layer in 4 bits: w13 = [E][2][I] rows of H inputs (gate, then up), w2 = [E][H] rows of I inputs. */
+typedef struct mm_w4_layer
+{
+    mm_w4_t w13, w2;
+    int E, H, I;
+    int group, scale_dtype;     /* MM_DTYPE_F16 or MM_DTYPE_BF16 */
+    float limit;                /* SwiGLU clamp (0 = off) */
+} mm_w4_layer_t;
+
+/* One MoE layer on 4-bit experts: out fp32 [T][H] = sum_j w[t,j] * expert_{ids[t,j]}(x_t) in ascending j (fp32 fma), ids
+ * int64 [T*topk] (outside [0, E): contributes nothing), expert(x) = W2 (act(Wg x) * Wu x) with mm_moe_decode's activation and
+ * clamp, nothing rounded below fp32 between x and out. shared >= 0 names an expert that every token is routed to besides, with
+ * weight 1, added last (-1: none). The weights of an expert are read once per 16, 32 or 64 of its routes. No host
+ * synchronisation. E <= 1024, H and I multiples of the group; x and out 16-byte aligned. Workspace: mm_w4_moe_workspace
+ * bytes, 16-byte aligned (topk without the shared expert). */
+size_t mm_w4_moe_workspace(int x_dtype, int T, int topk, int shared, int E, int H, int I);
+int mm_w4_moe(const mm_w4_layer_t* layer, const void* x, int x_dtype, int T, int topk, const int64_t* ids, const float* w,
+              int shared, float* out, void* workspace, size_t workspace_bytes, mm_stream_t stream);
 
 /* ------------------------------------------------------------------------------------ expert placement */
 
