@@ -20,6 +20,7 @@ namespace mm {
 typedef float rb_f4 __attribute__((ext_vector_type(4)));
 typedef __bf16 rb_bf8 __attribute__((ext_vector_type(8)));
 typedef short rb_s4 __attribute__((ext_vector_type(4)));
+typedef uint32_t rb_u4 __attribute__((ext_vector_type(4)));
 
 constexpr int RB_T = 128, RB_K = 32;
 constexpr int RB_ROW = 32;               // LDS row of a k-contiguous operand: four 16-byte chunks, swizzled
@@ -133,7 +134,7 @@ __global__ __launch_bounds__(256) void k_rb_gemm(const uint16_t* __restrict__ ro
     const int h0 = blockIdx.x * RB_T, c0 = blockIdx.y * RB_T;
     const int wh = 64 * (wave >> 1), wc = 64 * (wave & 1);
     const int s0 = blockIdx.z * ksteps, s1 = min(K / RB_K, s0 + ksteps);
-    uint4 rv[2 * PR], cv[2 * PC];
+    rb_u4 rv[2 * PR], cv[2 * PC];                          // (a plain vector type: HIP's uint4 arrays went to scratch memory here)
     auto load = [&](int s) {
         const int k0 = s * RB_K;
 #pragma unroll
@@ -145,17 +146,17 @@ __global__ __launch_bounds__(256) void k_rb_gemm(const uint16_t* __restrict__ ro
                 const size_t r = min(h0 + (i >> 2), H - 1);
 #pragma unroll
                 for (int p = 0; p < PR; ++p)
-                    rv[2 * p + j] = *reinterpret_cast<const uint4*>(rows + ((size_t)p * H + r) * K + k0 + 8 * (i & 3));
+                    rv[2 * p + j] = *reinterpret_cast<const rb_u4*>(rows + ((size_t)p * H + r) * K + k0 + 8 * (i & 3));
             }
             else
             {
                 const int t = k0 + (i >> 4), h = h0 + 8 * (i & 15);
-                rv[j] = t < T && h < H ? *reinterpret_cast<const uint4*>(rows + (size_t)t * H + h) : make_uint4(0, 0, 0, 0);
+                rv[j] = t < T && h < H ? *reinterpret_cast<const rb_u4*>(rows + (size_t)t * H + h) : rb_u4{ 0, 0, 0, 0 };
             }
             const size_t c = min(c0 + (i >> 2), C - 1);
 #pragma unroll
             for (int p = 0; p < PC; ++p)
-                cv[2 * p + j] = *reinterpret_cast<const uint4*>(cols + ((size_t)p * C + c) * K + k0 + 8 * (i & 3));
+                cv[2 * p + j] = *reinterpret_cast<const rb_u4*>(cols + ((size_t)p * C + c) * K + k0 + 8 * (i & 3));
         }
     };
     rb_f4 acc[4][4];
@@ -175,11 +176,11 @@ __global__ __launch_bounds__(256) void k_rb_gemm(const uint16_t* __restrict__ ro
             {
 #pragma unroll
                 for (int p = 0; p < PR; ++p)
-                    *reinterpret_cast<uint4*>(&rs[p * RB_T * RB_ROW + rb_at(i >> 2, i & 3)]) = rv[2 * p + j];
+                    *reinterpret_cast<rb_u4*>(&rs[p * RB_T * RB_ROW + rb_at(i >> 2, i & 3)]) = rv[2 * p + j];
             }
-            else *reinterpret_cast<uint4*>(&rs[(i >> 4) * RB_XROW + 8 * (i & 15)]) = rv[j];
+            else *reinterpret_cast<rb_u4*>(&rs[(i >> 4) * RB_XROW + 8 * (i & 15)]) = rv[j];
 #pragma unroll
-            for (int p = 0; p < PC; ++p) *reinterpret_cast<uint4*>(&cs[p][rb_at(i >> 2, i & 3)]) = cv[2 * p + j];
+            for (int p = 0; p < PC; ++p) *reinterpret_cast<rb_u4*>(&cs[p][rb_at(i >> 2, i & 3)]) = cv[2 * p + j];
         }
         __syncthreads();
         if (s + 1 < s1) load(s + 1);
