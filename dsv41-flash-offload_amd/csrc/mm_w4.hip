@@ -20,6 +20,7 @@
 namespace mm {
 
 typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 
@@ -27,7 +28,7 @@ typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 // Operands
 // ---------------------------------------------------------------------------------------------------------
 template <int XT>
-__device__ __forceinline__ f4_t mfma(uint4 a, uint4 b, f4_t c)
+__device__ __forceinline__ f4_t mfma(u4_t a, u4_t b, f4_t c)
 {
     if constexpr (XT == MM_DTYPE_F16)
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
@@ -43,18 +44,22 @@ __device__ __forceinline__ uint32_t two_weights(uint32_t v)
     constexpr int at = XT == MM_DTYPE_F16 ? 6 : 3;
     constexpr uint32_t mask = 0x000f000fu << at, one = XT == MM_DTYPE_F16 ? 0x4c004c00u : 0x41804180u;
     constexpr int ror = (4 * P - at) & 31;
-    return (__builtin_amdgcn_alignbit(v, v, ror) & mask) | one;
+    // one instruction for the and-or: it takes one constant from a scalar register and the other from a vector register (as
+    // literals they make two)
+    uint32_t r;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(__builtin_amdgcn_alignbit(v, v, ror)), "s"(mask), "v"(one));
+    return r;
 }
 template <int XT>
-__device__ __forceinline__ uint4 eight_weights(uint32_t v)
+__device__ __forceinline__ u4_t eight_weights(uint32_t v)
 {
-    return make_uint4(two_weights<XT, 0>(v), two_weights<XT, 1>(v), two_weights<XT, 2>(v), two_weights<XT, 3>(v));
+    return u4_t{ two_weights<XT, 0>(v), two_weights<XT, 1>(v), two_weights<XT, 2>(v), two_weights<XT, 3>(v) };
 }
 // Eight inputs in the order the weights come in: 0 4 1 5 2 6 3 7.
-__device__ __forceinline__ uint4 weight_order(uint4 x)
+__device__ __forceinline__ u4_t weight_order(u4_t x)
 {
-    return make_uint4(__builtin_amdgcn_perm(x.z, x.x, 0x05040100u), __builtin_amdgcn_perm(x.z, x.x, 0x07060302u),
-                      __builtin_amdgcn_perm(x.w, x.y, 0x05040100u), __builtin_amdgcn_perm(x.w, x.y, 0x07060302u));
+    return u4_t{ __builtin_amdgcn_perm(x.z, x.x, 0x05040100u), __builtin_amdgcn_perm(x.z, x.x, 0x07060302u),
+                 __builtin_amdgcn_perm(x.w, x.y, 0x05040100u), __builtin_amdgcn_perm(x.w, x.y, 0x07060302u) };
 }
 __device__ __forceinline__ int weight_place(int i) { return (i & 3) * 2 + (i >> 2); }      // of input i among its eight
 
@@ -112,53 +117,177 @@ struct W4Ptr
     const uint8_t* z;
 };
 
-// tot[mt][nt] += the products of blocks b0 .. b1 - 1 (128 inputs each; the last may be short of whole groups). xr: this
-// lane's row of x for each row tile (P parts, xplane elements apart; XO: already in weight order), w: this lane's row of
-// each weight tile.
-template <int XT, int P, bool XO, int G, int MT, int NT>
-__device__ __forceinline__ void w4_blocks(const uint16_t* const (&xr)[MT], size_t xplane, const W4Ptr (&w)[NT], bool sbf,
-                                          int K, int b0, int b1, f4_t (&tot)[MT][NT])
+// Row n of a matrix of K inputs.
+__device__ __forceinline__ W4Ptr w4_at(const W4Ptr& w, size_t n, int K, int group)
 {
-    constexpr int GJ = G / 32;                                        // MFMA steps of a group
-    const int quarter = (threadIdx.x >> 4) & 3;
-    const uint32_t o = XT == MM_DTYPE_F16 ? 0x3c003c00u : 0x3f803f80u;
-    const uint4 ones = make_uint4(o, o, o, o);
-    auto load_w = [&](int b, uint4 (&v)[NT]) {
-        int k = 128 * b + 32 * quarter;
-        if (k >= K) k = 0;                                            // groups past K are not multiplied
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) v[nt] = *reinterpret_cast<const uint4*>(w[nt].q + (k >> 3));
-    };
-    uint4 nv[NT];
-    if (b0 < b1) load_w(b0, nv);
-    for (int b = b0; b < b1; ++b)
+    return { w.q + n * (K / 8), w.s + n * (K / group), w.z ? w.z + n * (K / group) : nullptr };
+}
+
+// The NG scales (or zero points) of a block as one word of their size, at any alignment of their own type. The word stays as it
+// was loaded until it is used: widening it at once would wait for it, and for every load before it.
+template <int BYTES>
+using few_t = std::conditional_t<BYTES == 1, uint8_t, std::conditional_t<BYTES == 2, uint16_t, std::conditional_t<BYTES == 4, uint32_t, uint64_t>>>;
+template <int BYTES>
+__device__ __forceinline__ few_t<BYTES> load_few(const void* p)
+{
+    typedef few_t<BYTES> __attribute__((aligned(1), may_alias)) any_t;
+    return *reinterpret_cast<const any_t*>(p);
+}
+
+// LDS written by some lanes of a wave is read by others: in order, without a wait, but not to be reordered.
+__device__ __forceinline__ void wave_fence()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// 16 MT rows of x times 16 NT rows of W for one wave, block by block of 128 inputs.
+//
+// Both operands go through LDS: the multiplier wants the 16 rows of a tile in neighbouring lanes, but a load of 16 bytes a lane
+// whose neighbours lie in different rows costs the address unit four times what one of neighbours in one row does. So four
+// lanes read the 64 bytes that a block has of a row of W, sixteen lanes the 256 bytes of a row of x, and the operands
+// are read back from LDS, where 16-byte chunk c of row r lies at c ^ r (x) or c ^ (r / 4) (W), so that neither side conflicts in the
+// banks. The next block's loads are in flight while a block is multiplied.
+//
+// With OWN the wave keeps its rows of x to itself (waves split K); otherwise the NW waves of the workgroup share them (waves
+// split the columns), double-buffered, with a barrier a block.
+template <int XT, bool XO, int G, bool ZP, int MT, int NT, int NW, bool OWN>
+struct W4Wave
+{
+    static constexpr int GJ = G / 32, NG = 4 / GJ;                    // MFMA steps of a group, groups of a block
+    static constexpr int XROWS = OWN ? 4 : 4 * NW;                    // rows of x that one load covers
+    static constexpr int XI = 16 * MT / XROWS;
+    static constexpr int XBYTES = 16 * MT * 256, WBYTES = NT * 1024;
+    // LDS of a workgroup; the sums of a tile come to the same place when the products are done
+    static constexpr int LDS = OWN ? NW * (XBYTES + WBYTES) : 2 * XBYTES + NW * WBYTES;
+    static_assert(XI * XROWS == 16 * MT && NW * MT * NT * 1024 <= LDS, "tile shape");
+    // x times -(16 + z) as one MFMA more per weight tile and nothing on the vector ALUs, or the row sums of x once for all
+    // weight tiles and one more fma per output and group: the first for one row tile and for small groups
+    static constexpr bool DIRECT = MT == 1 || G == 32;
+    using scales_t = few_t<2 * NG>;
+    using zeros_t = few_t<NG>;
+
+    u4_t xv[XI], wv[NT];
+    scales_t sv[NT], sc[NT];
+    zeros_t zv[NT], zc[NT];
+    // bases that are the same for all lanes, and the lanes' byte offsets
+    const unsigned char *xb, *qb, *sb, *zb;
+    uint32_t xo[XI], qo[NT], so[NT];
+    int nx;                                // loads of x that cover the rows in use
+
+    // x, w: bases; rows: number of tile rows in use; row(v): elements from x to tile row v < rows; col(nt, c): rows from w to column c
+    // of weight tile nt
+    template <typename Row, typename Col>
+    __device__ __forceinline__ void init(const uint16_t* x, Row row, int rows, const W4Ptr& w, Col col, int K)
     {
+        const int t = OWN ? threadIdx.x & 63 : threadIdx.x, lane = threadIdx.x & 63;
+        xb = reinterpret_cast<const unsigned char*>(x);
+        qb = reinterpret_cast<const unsigned char*>(w.q);
+        sb = reinterpret_cast<const unsigned char*>(w.s);
+        zb = w.z;
+        nx = (rows + XROWS - 1) / XROWS;
+#pragma unroll
+        for (int i = 0; i < XI; ++i) xo[i] = 2 * row(min(XROWS * i + (t >> 4), rows - 1)) + 16 * (t & 15);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+        {
+            qo[nt] = col(nt, lane >> 2) * (K / 2) + 16 * ((lane & 3) ^ (lane >> 4));
+            so[nt] = col(nt, lane & 15) * (K / G);
+        }
+    }
+
+    __device__ __forceinline__ void load(int b, int K)
+    {
+        if (G == 128 || 128 * b + 128 <= K)
+        {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+            {
+                wv[nt] = *reinterpret_cast<const u4_t*>(qb + 64 * (size_t)b + qo[nt]);
+                sv[nt] = load_few<2 * NG>(sb + 2 * NG * (size_t)b + 2 * so[nt]);
+                if constexpr (ZP) zv[nt] = load_few<NG>(zb + NG * (size_t)b + so[nt]);
+            }
+#pragma unroll
+            for (int i = 0; i < XI; ++i)
+                if (i < nx) xv[i] = *reinterpret_cast<const u4_t*>(xb + 256 * (size_t)b + xo[i]);
+            return;
+        }
+        // the last block of a K that is no multiple of 128: nothing past K is read (what is not loaded is not multiplied)
+        const int groups = (K - 128 * b) / G, lane = threadIdx.x & 63;
+        const int cq = (lane & 3) ^ (lane >> 4), cx = lane & 15;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+        {
+            wv[nt] = *reinterpret_cast<const u4_t*>(qb + 64 * (size_t)b + qo[nt] - (128 * b + 32 * cq < K ? 0 : 16 * cq));
+            sv[nt] = 0;
+            zv[nt] = 0;
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+                if (g < groups)
+                {
+                    sv[nt] |= (scales_t)reinterpret_cast<const uint16_t*>(sb)[so[nt] + b * NG + g] << (16 * g);
+                    if constexpr (ZP) zv[nt] |= (zeros_t)zb[so[nt] + b * NG + g] << (8 * g);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < XI; ++i)
+            if (i < nx) xv[i] = *reinterpret_cast<const u4_t*>(xb + 256 * (size_t)b + xo[i] - (128 * b + 8 * cx < K ? 0 : 16 * cx));
+    }
+
+    // the loaded block into LDS
+    __device__ __forceinline__ void store(unsigned char* x, unsigned char* w)
+    {
+        const int t = OWN ? threadIdx.x & 63 : threadIdx.x, lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < XI; ++i)
+            if (i < nx)
+            {
+                const int r = XROWS * i + (t >> 4);
+                *reinterpret_cast<u4_t*>(x + r * 256 + 16 * ((t & 15) ^ (r & 15))) = XO ? xv[i] : weight_order(xv[i]);
+            }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+        {
+            *reinterpret_cast<u4_t*>(w + nt * 1024 + lane * 16) = wv[nt];
+            sc[nt] = sv[nt];
+            if constexpr (ZP) zc[nt] = zv[nt];
+        }
+    }
+
+    // one value in every place of a B operand
+    __device__ __forceinline__ static u4_t splat(float f)
+    {
+        const uint32_t h = XT == MM_DTYPE_F16 ? (uint32_t)f2h(f) * 0x10001u : (__float_as_uint(f) >> 16) * 0x10001u;
+        return u4_t{ h, h, h, h };
+    }
+
+    __device__ __forceinline__ void multiply(const unsigned char* x, const unsigned char* w, int groups, bool sbf, f4_t (&tot)[MT][NT])
+    {
+        const int r = threadIdx.x & 15, quarter = (threadIdx.x >> 4) & 3;
         uint32_t v[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
         {
-            v[nt][0] = nv[nt].x;
-            v[nt][1] = nv[nt].y;
-            v[nt][2] = nv[nt].z;
-            v[nt][3] = nv[nt].w;
+            const u4_t u = *reinterpret_cast<const u4_t*>(w + nt * 1024 + (4 * r + (quarter ^ (r >> 2))) * 16);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[nt][j] = u[j];
+            regroup<G>(v[nt]);
         }
-        if (b + 1 < b1) load_w(b + 1, nv);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) regroup<G>(v[nt]);
-#pragma unroll
-        for (int g = 0; g < 4 / GJ; ++g)
+        for (int g = 0; g < NG; ++g)
         {
-            if (128 * b + G * g >= K) break;
-            const int gi = b * (128 / G) + g;
-            float s[NT], c[NT];
+            if (G < 128 && g >= groups) break;
+            // large tiles: one group's sums at a time in the registers
+            if constexpr (MT * NT >= 4) __builtin_amdgcn_sched_barrier(0);
+            f4_t acc[MT][NT], xs[MT];
+            float zero[NT];
+            u4_t Z[NT];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
             {
-                const uint16_t u = w[nt].s[gi];
-                s[nt] = sbf ? __uint_as_float((uint32_t)u << 16) : h2f(u);
-                c[nt] = -16.f - (w[nt].z ? (float)w[nt].z[gi] : 8.f);
+                zero[nt] = ZP ? -16.f - (float)((zc[nt] >> (8 * g)) & 255u) : -24.f;
+                if constexpr (DIRECT) Z[nt] = splat(zero[nt]);
             }
-            f4_t acc[MT][NT], xs[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
             {
@@ -169,40 +298,127 @@ __device__ __forceinline__ void w4_blocks(const uint16_t* const (&xr)[MT], size_
 #pragma unroll
             for (int jj = 0; jj < GJ; ++jj)
             {
-                const int j = g * GJ + jj, k = 128 * b + input_of<G>(quarter, j);
-                uint4 B[NT];
+                const int j = g * GJ + jj, c = input_of<G>(quarter, j) / 8;
+                u4_t B[NT];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) B[nt] = eight_weights<XT>(v[nt][j]);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
+                {
+                    const u4_t A = *reinterpret_cast<const u4_t*>(x + (16 * mt + r) * 256 + 16 * (c ^ r));
+                    if constexpr (!DIRECT) xs[mt] = mfma<XT>(A, splat(1.f), xs[mt]);
 #pragma unroll
-                    for (int p = 0; p < P; ++p)
+                    for (int nt = 0; nt < NT; ++nt)
                     {
-                        uint4 A = *reinterpret_cast<const uint4*>(xr[mt] + p * xplane + k);
-                        if constexpr (!XO) A = weight_order(A);
-                        xs[mt] = mfma<XT>(A, ones, xs[mt]);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = mfma<XT>(A, B[nt], acc[mt][nt]);
+                        acc[mt][nt] = mfma<XT>(A, B[nt], acc[mt][nt]);
+                        if constexpr (DIRECT) acc[mt][nt] = mfma<XT>(A, Z[nt], acc[mt][nt]);
                     }
+                }
             }
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int nt = 0; nt < NT; ++nt)
+            {
+                const uint16_t u = (uint16_t)(sc[nt] >> (16 * g));
+                const float s = sbf ? __uint_as_float((uint32_t)u << 16) : h2f(u);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        tot[mt][nt][i] = fmaf(s[nt], fmaf(c[nt], xs[mt][i], acc[mt][nt][i]), tot[mt][nt][i]);
+                        tot[mt][nt][i] = fmaf(s, DIRECT ? acc[mt][nt][i] : fmaf(zero[nt], xs[mt][i], acc[mt][nt][i]), tot[mt][nt][i]);
+            }
         }
     }
-}
 
-// Adds the waves' totals of a workgroup in wave order: tile t's sum ends in wave t % WK.
-template <int WK, int TILES>
-__device__ __forceinline__ f4_t add_waves(float (*part)[TILES][64][4], int wave, int lane, int t)
+    // products of blocks b0 .. b1 - 1 (with !OWN the same for all waves)
+    __device__ __forceinline__ void run(unsigned char* lds, int b0, int b1, int K, bool sbf, f4_t (&tot)[MT][NT])
+    {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        unsigned char* x = OWN ? lds + wave * (XBYTES + WBYTES) : lds;
+        unsigned char* w = OWN ? x + XBYTES : lds + 2 * XBYTES + wave * WBYTES;
+        if (b0 >= b1) return;
+        load(b0, K);
+        if constexpr (!OWN)
+        {
+            store(x, w);
+            __syncthreads();
+        }
+        for (int b = b0; b < b1; ++b)
+        {
+            if constexpr (OWN)
+            {
+                store(x, w);
+                wave_fence();
+            }
+            if (b + 1 < b1) load(b + 1, K);
+            multiply(x + (OWN ? 0 : ((b - b0) & 1) * XBYTES), w, G == 128 ? 1 : min(NG, (K - 128 * b) / G), sbf, tot);
+            wave_fence();
+            if constexpr (!OWN)
+            {
+                if (b + 1 < b1) store(x + ((b + 1 - b0) & 1) * XBYTES, w);
+                __syncthreads();
+            }
+        }
+    }
+};
+
+// A workgroup's tile: `cnt` rows of x (at most W4_ROWS<P, MT>) times 16 NT rows of W (OWN: each wave a run of the blocks of K) or
+// 16 NT rows per wave. Rows of P parts take P rows of the MFMA tiles (part p of row m is tile row p cnt + m), so a few fp32 rows
+// cost what a few bf16 rows do. row(m): elements from x to row m's first part, the next parts xpart elements on; col(nt, c): row
+// of W that is column c of weight tile nt. Byte offsets from x and w fit 32 bits.
+// On return tile_value() gives the threads of the wave (OWN: of the workgroup) any output of its tile; the caller
+// synchronises before the next tile.
+template <int P, int MT>
+constexpr int W4_ROWS = 16 * MT / P;
+
+template <int XT, int P, int G, bool ZP, int MT, int NT, int NW, bool OWN, typename Row, typename Col>
+__device__ __forceinline__ void w4_tile(unsigned char* lds, const uint16_t* x, Row row, uint32_t xpart, int cnt, const W4Ptr& w, Col col,
+                                        bool sbf, int K)
 {
-    f4_t s = f4_t{ 0.f, 0.f, 0.f, 0.f };
+    using Wave = W4Wave<XT, P == 3, G, ZP, MT, NT, NW, OWN>;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nb = (K + 127) / 128;
+    f4_t tot[MT][NT];
 #pragma unroll
-    for (int v = 0; v < WK; ++v) s += *reinterpret_cast<const f4_t*>(part[v][t][lane]);
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) tot[mt][nt] = f4_t{ 0.f, 0.f, 0.f, 0.f };
+    Wave wv;
+    wv.init(x, [&](int v) {
+        const int q = P == 1 ? 0 : (v >= cnt) + (v >= 2 * cnt);
+        return row(v - q * cnt) + q * xpart;
+    }, P * cnt, w, col, K);
+    wv.run(lds, OWN ? nb * wave / NW : 0, OWN ? nb * (wave + 1) / NW : nb, K, sbf, tot);
+    // the sums into LDS: OWN in the wave's own place, else where the inputs were (every wave is past its last barrier)
+    f4_t* part = reinterpret_cast<f4_t*>(lds + (OWN ? wave * (Wave::XBYTES + Wave::WBYTES) : wave * MT * NT * 1024));
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) part[(mt * NT + nt) * 64 + lane] = tot[mt][nt];
+    if constexpr (OWN)
+    {
+        // the waves' sums in wave order, left in the first wave's place
+        __syncthreads();
+        for (int t = wave; t < MT * NT; t += NW)
+        {
+            f4_t s = reinterpret_cast<const f4_t*>(lds)[t * 64 + lane];
+#pragma unroll
+            for (int v = 1; v < NW; ++v) s += reinterpret_cast<const f4_t*>(lds + v * (Wave::XBYTES + Wave::WBYTES))[t * 64 + lane];
+            reinterpret_cast<f4_t*>(lds)[t * 64 + lane] = s;
+        }
+        __syncthreads();
+    }
+    else wave_fence();
+}
+// Output (m, column c of weight tile nt) of a tile's sums: the sum of its parts, the smallest first.
+template <int P, int NT>
+__device__ __forceinline__ float tile_value(const unsigned char* sums, int cnt, int m, int nt, int c)
+{
+    float s = 0.f;
+#pragma unroll
+    for (int q = P - 1; q >= 0; --q)
+    {
+        const int v = q * cnt + m;
+        s += reinterpret_cast<const float*>(sums)[(((v >> 4) * NT + nt) * 64 + ((v & 15) >> 2) * 16 + c) * 4 + (v & 3)];
+    }
     return s;
 }
 
@@ -220,12 +436,13 @@ __device__ __forceinline__ void store_out(int ot, void* y, size_t i, float v)
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// fp32 rows as three bf16 parts in weight order: out [3][rows][K].
+// fp32 rows as three bf16 parts in weight order: out [rows][3][K].
 // ---------------------------------------------------------------------------------------------------------
-__global__ __launch_bounds__(256) void k_w4_parts(const float* __restrict__ x, size_t n8, uint16_t* __restrict__ out)
+__global__ __launch_bounds__(256) void k_w4_parts(const float* __restrict__ x, size_t n8, int K8, uint16_t* __restrict__ out)
 {
     const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n8) return;
+    const size_t row = i / K8;
     uint16_t p[3][8];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -239,69 +456,46 @@ __global__ __launch_bounds__(256) void k_w4_parts(const float* __restrict__ x, s
         uint32_t u[4];
 #pragma unroll
         for (int d = 0; d < 4; ++d) u[d] = p[c][2 * d] | ((uint32_t)p[c][2 * d + 1] << 16);
-        *reinterpret_cast<uint4*>(out + 8 * (c * n8 + i)) = make_uint4(u[0], u[1], u[2], u[3]);
+        *reinterpret_cast<u4_t*>(out + 8 * (i + (2 * row + c) * K8)) = u4_t{ u[0], u[1], u[2], u[3] };
     }
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// Dense: a workgroup takes 16 MT rows x 16 NT columns, its WK waves each a run of the blocks of K.
+// Dense. OWN: a workgroup takes 16 NT columns and its waves split K (few rows); else 16 NT columns a wave.
 // ---------------------------------------------------------------------------------------------------------
 struct LinearArgs
 {
     const uint16_t* x;
-    size_t xplane;
     W4Ptr w;
     void* y;
     int M, K, N, sbf, out;
 };
 
-template <int XT, int P, int G, int MT, int NT, int WK>
-__global__ __launch_bounds__(64 * WK) void k_w4_linear(LinearArgs a)
+template <int XT, int P, int G, bool ZP, int MT, int NT, int NW, bool OWN>
+__global__ __launch_bounds__(64 * NW) void k_w4_linear(LinearArgs a)
 {
-    __shared__ __align__(16) float part[WK][MT * NT][64][4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15;
-    const int m0 = blockIdx.y * 16 * MT, n0 = blockIdx.x * 16 * NT;
-    const int nb = (a.K + 127) / 128, ng = a.K / G;
-    const uint16_t* xr[MT];
-    W4Ptr w[NT];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) xr[mt] = a.x + (size_t)min(m0 + 16 * mt + r, a.M - 1) * a.K;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    constexpr int ROWS = W4_ROWS<P, MT>;
+    __shared__ __align__(16) unsigned char lds[W4Wave<XT, P == 3, G, ZP, MT, NT, NW, OWN>::LDS];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int m0 = blockIdx.y * ROWS, n0 = OWN ? blockIdx.x * 16 * NT : (blockIdx.x * NW + wave) * 16 * NT, cnt = min(ROWS, a.M - m0);
+    const int n1 = min(n0, a.N - 1);                                 // a wave past the last column works on it again
+    w4_tile<XT, P, G, ZP, MT, NT, NW, OWN>(
+        lds, a.x + (size_t)m0 * P * a.K, [&](int m) { return (uint32_t)m * P * a.K; }, a.K, cnt, w4_at(a.w, n1, a.K, G),
+        [&](int nt, int c) { return (uint32_t)min(16 * nt + c, a.N - 1 - n1); }, a.sbf, a.K);
+    const unsigned char* sums = OWN ? lds : lds + wave * MT * NT * 1024;
+    for (int o = OWN ? threadIdx.x : threadIdx.x & 63; o < cnt * 16 * NT; o += OWN ? 64 * NW : 64)
     {
-        const size_t n = min(n0 + 16 * nt + r, a.N - 1);
-        w[nt] = { a.w.q + n * (a.K / 8), a.w.s + n * ng, a.w.z ? a.w.z + n * ng : nullptr };
-    }
-    f4_t tot[MT][NT];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) tot[mt][nt] = f4_t{ 0.f, 0.f, 0.f, 0.f };
-    w4_blocks<XT, P, P == 3, G, MT, NT>(xr, a.xplane, w, a.sbf, a.K, nb * wave / WK, nb * (wave + 1) / WK, tot);
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) *reinterpret_cast<f4_t*>(part[wave][mt * NT + nt][lane]) = tot[mt][nt];
-    __syncthreads();
-    for (int t = wave; t < MT * NT; t += WK)
-    {
-        const f4_t s = add_waves<WK, MT * NT>(part, wave, lane, t);
-        const int n = n0 + 16 * (t % NT) + r;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-        {
-            const int m = m0 + 16 * (t / NT) + 4 * (lane >> 4) + i;
-            if (m < a.M && n < a.N) store_out(a.out, a.y, (size_t)m * a.N + n, s[i]);
-        }
+        const int m = o / (16 * NT), c = o % (16 * NT);
+        if (n0 + c < a.N) store_out(a.out, a.y, (size_t)(m0 + m) * a.N + n0 + c, tile_value<P, NT>(sums, cnt, m, c >> 4, c & 15));
     }
 }
 
 // ---------------------------------------------------------------------------------------------------------
 // Routed experts
 // ---------------------------------------------------------------------------------------------------------
-// Up to W4_ROWS_MAX routes each workgroup finds its record's routes itself: record r exists if route r is the first of its
-// expert, and holds every route of that expert.
-constexpr int W4_SELF = 64;
+// Up to W4_SELF routes each workgroup finds its record's routes itself: record r exists if route r is the first of its
+// expert, and holds every route of that expert. Records of larger calls come from k_w4_plan. Neither holds more than W4_REC routes.
+constexpr int W4_SELF = 64, W4_REC = 64;
 struct W4Rec
 {
     int expert, start, count, pad;
@@ -309,8 +503,7 @@ struct W4Rec
 
 struct ExpertArgs
 {
-    const uint16_t* x;         // [T][H], or [3][T][H] parts in weight order
-    size_t xplane;
+    const uint16_t* x;         // [T][H], or [T][3][H] parts in weight order
     W4Ptr w13, w2;
     const int64_t* ids;        // [T][k]
     const float* w;            // [T][k]
@@ -318,7 +511,7 @@ struct ExpertArgs
     const int32_t* order;      // NULL: routes found in the kernel
     const W4Rec* recs;
     const int32_t* nrec;
-    uint16_t* h;               // [3][n][I] parts in weight order
+    uint16_t* h;               // [n][3][I] parts in weight order
     float* y;                  // [n][H]
     int n, k, topk, E, H, I, sbf;      // n = T topk routes, topk = k, and one more with a shared expert
     int shared;
@@ -334,8 +527,8 @@ __device__ __forceinline__ int route_expert(const ExpertArgs& a, int s)
     return e >= 0 && e < a.E ? (int)e : -1;
 }
 
-// Routes of this workgroup's record into `rows` (LDS, at most `cap`); returns their number, 0 for no record.
-__device__ __forceinline__ int record_rows(const ExpertArgs& a, int rec, int* rows, int cap, int& expert)
+// Routes of this workgroup's record into `rows` (LDS); returns their number, 0 for no record.
+__device__ __forceinline__ int record_rows(const ExpertArgs& a, int rec, int* rows, int& expert)
 {
     if (!a.order)
     {
@@ -351,106 +544,113 @@ __device__ __forceinline__ int record_rows(const ExpertArgs& a, int rec, int* ro
     if (rec >= *a.nrec) return 0;
     const W4Rec q = a.recs[rec];
     expert = q.expert;
-    if ((int)threadIdx.x < q.count && (int)threadIdx.x < cap) rows[threadIdx.x] = a.order[q.start + threadIdx.x];
+    if ((int)threadIdx.x < q.count) rows[threadIdx.x] = a.order[q.start + threadIdx.x];
     return q.count;
 }
 
-// gate and up of 16 columns for the record's routes, SwiGLU, and the result as three bf16 parts for the down product
-template <int XT, int P, int G, int MT, int WK>
-__global__ __launch_bounds__(64 * WK) void k_w4_gate_up(ExpertArgs a)
+// Gate and up of 16 columns (OWN: a workgroup's, else a wave's) for some of a record's routes, SwiGLU, and the result as three
+// bf16 parts for the down product.
+template <int XT, int P, int G, bool ZP, int MT, int NW, bool OWN>
+__device__ __forceinline__ void gate_up_rows(const ExpertArgs& a, unsigned char* lds, int expert, const int* rows, int c)
 {
-    constexpr int CAP = 64;
-    __shared__ __align__(16) float part[WK][MT * 2][64][4];
-    __shared__ int rows[CAP];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15;
-    int expert;
-    const int cnt = record_rows(a, blockIdx.y, rows, CAP, expert);
-    if (cnt == 0) return;
-    __syncthreads();
-    const int n0 = blockIdx.x * 16, nb = (a.H + 127) / 128, ng = a.H / G;
-    W4Ptr w[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = OWN ? blockIdx.x * 16 : (blockIdx.x * NW + wave) * 16;
+    w4_tile<XT, P, G, ZP, MT, 2, NW, OWN>(
+        lds, a.x, [&](int m) { return (uint32_t)(rows[m] / a.topk) * (P * a.H); }, a.H, c, w4_at(a.w13, (size_t)expert * 2 * a.I, a.H, G),
+        [&](int t, int col) { return (uint32_t)(t * a.I + min(n0 + col, a.I - 1)); }, a.sbf, a.H);
+    const unsigned char* sums = OWN ? lds : lds + wave * MT * 2 * 1024;
+    for (int o = OWN ? threadIdx.x : threadIdx.x & 63; o < c * 16; o += OWN ? 64 * NW : 64)
     {
-        const size_t n = ((size_t)expert * 2 + t) * a.I + n0 + r;
-        w[t] = { a.w13.q + n * (a.H / 8), a.w13.s + n * ng, a.w13.z ? a.w13.z + n * ng : nullptr };
+        const int m = o >> 4, col = o & 15;
+        if (n0 + col >= a.I) continue;
+        uint16_t p[3];
+        three_parts(act_gu(tile_value<P, 2>(sums, c, m, 0, col), tile_value<P, 2>(sums, c, m, 1, col), a.limit), p[0], p[1], p[2]);
+        uint16_t* h = a.h + (size_t)rows[m] * 3 * a.I + n0 + (col & 8) + weight_place(col & 7);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) h[q * a.I] = p[q];
     }
-    for (int m0 = 0; m0 < cnt; m0 += 16 * MT)
+}
+// The down product of 32 columns for some of a record's routes.
+template <int G, bool ZP, int MT, int NW, bool OWN>
+__device__ __forceinline__ void down_rows(const ExpertArgs& a, unsigned char* lds, int expert, const int* rows, int c)
+{
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = OWN ? blockIdx.x * 32 : (blockIdx.x * NW + wave) * 32;
+    w4_tile<MM_DTYPE_BF16, 3, G, ZP, MT, 2, NW, OWN>(
+        lds, a.h, [&](int m) { return (uint32_t)rows[m] * (3 * a.I); }, a.I, c, w4_at(a.w2, (size_t)expert * a.H, a.I, G),
+        [&](int t, int col) { return (uint32_t)min(n0 + 16 * t + col, a.H - 1); }, a.sbf, a.I);
+    const unsigned char* sums = OWN ? lds : lds + wave * MT * 2 * 1024;
+    for (int o = OWN ? threadIdx.x : threadIdx.x & 63; o < c * 32; o += OWN ? 64 * NW : 64)
     {
-        const uint16_t* xr[MT];
-        f4_t tot[MT][2];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-        {
-            xr[mt] = a.x + (size_t)(rows[min(m0 + 16 * mt + r, cnt - 1)] / a.topk) * a.H;
-            tot[mt][0] = tot[mt][1] = f4_t{ 0.f, 0.f, 0.f, 0.f };
-        }
-        w4_blocks<XT, P, P == 3, G, MT, 2>(xr, a.xplane, w, a.sbf, a.H, nb * wave / WK, nb * (wave + 1) / WK, tot);
-        if (m0) __syncthreads();                        // the previous rows' sums are read
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int t = 0; t < 2; ++t) *reinterpret_cast<f4_t*>(part[wave][mt * 2 + t][lane]) = tot[mt][t];
-        __syncthreads();
-        for (int mt = wave; mt < MT; mt += WK)
-        {
-            const f4_t g = add_waves<WK, MT * 2>(part, wave, lane, 2 * mt), u = add_waves<WK, MT * 2>(part, wave, lane, 2 * mt + 1);
-            const int col = n0 + (r & 8) + weight_place(r & 7);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-            {
-                const int m = m0 + 16 * mt + 4 * (lane >> 4) + i;
-                if (m >= cnt) continue;
-                uint16_t p[3];
-                three_parts(act_gu(g[i], u[i], a.limit), p[0], p[1], p[2]);
-#pragma unroll
-                for (int c = 0; c < 3; ++c) a.h[((size_t)c * a.n + rows[m]) * a.I + col] = p[c];
-            }
-        }
+        const int m = o >> 5, col = o & 31;
+        if (n0 + col < a.H) a.y[(size_t)rows[m] * a.H + n0 + col] = tile_value<3, 2>(sums, c, m, col >> 4, col & 15);
     }
 }
 
-// down product of 16 columns for the record's routes
-template <int G, int MT, int WK>
-__global__ __launch_bounds__(64 * WK) void k_w4_down(ExpertArgs a)
+// Few rows: one workgroup per record and 16 (32) columns, its four waves split K; one or two row tiles by the record's routes, more routes in
+// more passes.
+template <int XT, int P, int G, bool ZP, int MT>
+__global__ __launch_bounds__(256) void k_w4_gate_up(ExpertArgs a)
 {
-    constexpr int CAP = 64;
-    __shared__ __align__(16) float part[WK][MT][64][4];
-    __shared__ int rows[CAP];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15;
+    __shared__ __align__(16) unsigned char lds[W4Wave<XT, P == 3, G, ZP, MT, 2, 4, true>::LDS];
+    __shared__ int rows[W4_REC];
     int expert;
-    const int cnt = record_rows(a, blockIdx.y, rows, CAP, expert);
+    const int cnt = record_rows(a, blockIdx.y, rows, expert);
     if (cnt == 0) return;
     __syncthreads();
-    const int n0 = blockIdx.x * 16, nb = (a.I + 127) / 128, ng = a.I / G;
-    const size_t n = (size_t)expert * a.H + n0 + r;
-    const W4Ptr w[1] = { { a.w2.q + n * (a.I / 8), a.w2.s + n * ng, a.w2.z ? a.w2.z + n * ng : nullptr } };
-    for (int m0 = 0; m0 < cnt; m0 += 16 * MT)
+    if constexpr (MT > 1)
+        if (cnt <= W4_ROWS<P, 1>) return gate_up_rows<XT, P, G, ZP, 1, 4, true>(a, lds, expert, rows, cnt);
+    for (int m = 0; m < cnt; m += W4_ROWS<P, MT>)
     {
-        const uint16_t* xr[MT];
-        f4_t tot[MT][1];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-        {
-            xr[mt] = a.h + (size_t)rows[min(m0 + 16 * mt + r, cnt - 1)] * a.I;
-            tot[mt][0] = f4_t{ 0.f, 0.f, 0.f, 0.f };
-        }
-        w4_blocks<MM_DTYPE_BF16, 3, true, G, MT, 1>(xr, (size_t)a.n * a.I, w, a.sbf, a.I, nb * wave / WK, nb * (wave + 1) / WK,
-                                                    tot);
-        if (m0) __syncthreads();
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) *reinterpret_cast<f4_t*>(part[wave][mt][lane]) = tot[mt][0];
-        __syncthreads();
-        for (int mt = wave; mt < MT; mt += WK)
-        {
-            const f4_t s = add_waves<WK, MT>(part, wave, lane, mt);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-            {
-                const int m = m0 + 16 * mt + 4 * (lane >> 4) + i;
-                if (m < cnt) a.y[(size_t)rows[m] * a.H + n0 + r] = s[i];
-            }
-        }
+        if (m) __syncthreads();                        // the previous rows' sums are read
+        gate_up_rows<XT, P, G, ZP, MT, 4, true>(a, lds, expert, rows + m, min(W4_ROWS<P, MT>, cnt - m));
+    }
+}
+template <int G, bool ZP, int MT>
+__global__ __launch_bounds__(256) void k_w4_down(ExpertArgs a)
+{
+    __shared__ __align__(16) unsigned char lds[W4Wave<MM_DTYPE_BF16, true, G, ZP, MT, 2, 4, true>::LDS];
+    __shared__ int rows[W4_REC];
+    int expert;
+    const int cnt = record_rows(a, blockIdx.y, rows, expert);
+    if (cnt == 0) return;
+    __syncthreads();
+    if constexpr (MT > 1)
+        if (cnt <= W4_ROWS<3, 1>) return down_rows<G, ZP, 1, 4, true>(a, lds, expert, rows, cnt);
+    for (int m = 0; m < cnt; m += W4_ROWS<3, MT>)
+    {
+        if (m) __syncthreads();
+        down_rows<G, ZP, MT, 4, true>(a, lds, expert, rows + m, min(W4_ROWS<3, MT>, cnt - m));
+    }
+}
+
+// Many rows: 64 (128) columns per workgroup, four waves that share the rows of x; up to 16 MT tile rows a pass.
+template <int XT, int P, int G, bool ZP, int MT>
+__global__ __launch_bounds__(256) void k_w4_gate_up_many(ExpertArgs a)
+{
+    __shared__ __align__(16) unsigned char lds[W4Wave<XT, P == 3, G, ZP, MT, 2, 4, false>::LDS];
+    __shared__ int rows[W4_REC];
+    int expert;
+    const int cnt = record_rows(a, blockIdx.y, rows, expert);
+    if (cnt == 0) return;
+    __syncthreads();
+    for (int m = 0; m < cnt; m += W4_ROWS<P, MT>)
+    {
+        if (m) __syncthreads();
+        gate_up_rows<XT, P, G, ZP, MT, 4, false>(a, lds, expert, rows + m, min(W4_ROWS<P, MT>, cnt - m));
+    }
+}
+template <int G, bool ZP, int MT>
+__global__ __launch_bounds__(256) void k_w4_down_many(ExpertArgs a)
+{
+    __shared__ __align__(16) unsigned char lds[W4Wave<MM_DTYPE_BF16, true, G, ZP, MT, 2, 4, false>::LDS];
+    __shared__ int rows[W4_REC];
+    int expert;
+    const int cnt = record_rows(a, blockIdx.y, rows, expert);
+    if (cnt == 0) return;
+    __syncthreads();
+    for (int m = 0; m < cnt; m += W4_ROWS<3, MT>)
+    {
+        if (m) __syncthreads();
+        down_rows<G, ZP, MT, 4, false>(a, lds, expert, rows + m, min(W4_ROWS<3, MT>, cnt - m));
     }
 }
 
@@ -516,12 +716,17 @@ static int check_w4(const char* what, const mm_w4_t* w, int group, int scale_dty
 template <int V>
 using ic = std::integral_constant<int, V>;
 
+// (group, zero points)
 template <typename F>
-static void by_group(int group, F f)
+static void by_group(int group, bool zeros, F f)
 {
-    if (group == 128) f(ic<128>{});
-    else if (group == 64) f(ic<64>{});
-    else f(ic<32>{});
+    auto by_zeros = [&](auto g) {
+        if (zeros) f(g, std::true_type{});
+        else f(g, std::false_type{});
+    };
+    if (group == 128) by_zeros(ic<128>{});
+    else if (group == 64) by_zeros(ic<64>{});
+    else by_zeros(ic<32>{});
 }
 // (input type, parts)
 template <typename F>
@@ -532,10 +737,10 @@ static void by_input(int x_dtype, F f)
     else f(ic<MM_DTYPE_F16>{}, ic<1>{});
 }
 
-static void parts_launch(const void* x, size_t elements, void* out, hipStream_t hs)
+static void parts_launch(const void* x, size_t rows, int K, void* out, hipStream_t hs)
 {
-    const size_t n8 = elements / 8;
-    hipLaunchKernelGGL(k_w4_parts, dim3((unsigned)((n8 + 255) / 256)), dim3(256), 0, hs, (const float*)x, n8, (uint16_t*)out);
+    const size_t n8 = rows * (K / 8);
+    hipLaunchKernelGGL(k_w4_parts, dim3((unsigned)((n8 + 255) / 256)), dim3(256), 0, hs, (const float*)x, n8, K / 8, (uint16_t*)out);
 }
 
 struct ExpertWs
@@ -603,9 +808,8 @@ int mm_w4_linear(const void* x, int x_dtype, int M, int K, int N, const mm_w4_t*
     a.x = (const uint16_t*)x;
     if (x_dtype == MM_DTYPE_F32)
     {
-        parts_launch(x, (size_t)M * K, workspace, hs);
+        parts_launch(x, M, K, workspace, hs);
         a.x = (const uint16_t*)workspace;
-        a.xplane = (size_t)M * K;
     }
     a.w = { (const uint32_t*)W->q, (const uint16_t*)W->scales, W->zeros };
     a.y = y;
@@ -615,14 +819,17 @@ int mm_w4_linear(const void* x, int x_dtype, int M, int K, int N, const mm_w4_t*
     a.sbf = scale_dtype == MM_DTYPE_BF16;
     a.out = y_dtype;
     by_input(x_dtype, [&](auto xt, auto p) {
-        by_group(group, [&](auto g) {
+        by_group(group, W->zeros != nullptr, [&](auto g, auto zp) {
             constexpr int XT = decltype(xt)::value, P = decltype(p)::value, G = decltype(g)::value;
-            if (M <= 16)
-                hipLaunchKernelGGL((k_w4_linear<XT, P, G, 1, 1, 8>), dim3((N + 15) / 16, 1), dim3(512), 0, hs, a);
-            else if (M <= 32)
-                hipLaunchKernelGGL((k_w4_linear<XT, P, G, 2, 1, 8>), dim3((N + 15) / 16, 1), dim3(512), 0, hs, a);
+            constexpr bool ZP = decltype(zp)::value;
+            const int rows = P * M;
+            auto grid = [&](int mt, int cols) { return dim3((N + cols - 1) / cols, (M + 16 * mt / P - 1) / (16 * mt / P)); };
+            if (rows <= 16)
+                hipLaunchKernelGGL((k_w4_linear<XT, P, G, ZP, 1, 1, 8, true>), grid(1, 16), dim3(512), 0, hs, a);
+            else if (rows <= 32)
+                hipLaunchKernelGGL((k_w4_linear<XT, P, G, ZP, 2, 1, 8, true>), grid(2, 16), dim3(512), 0, hs, a);
             else
-                hipLaunchKernelGGL((k_w4_linear<XT, P, G, 4, 2, 4>), dim3((N + 31) / 32, (M + 63) / 64), dim3(256), 0, hs, a);
+                hipLaunchKernelGGL((k_w4_linear<XT, P, G, ZP, 4, 2, 4, false>), grid(4, 128), dim3(256), 0, hs, a);
         });
     });
     return check_launch("mm_w4_linear");
@@ -661,9 +868,8 @@ int mm_w4_moe(const mm_w4_layer_t* L, const void* x, int x_dtype, int T, int top
     a.x = (const uint16_t*)x;
     if (x_dtype == MM_DTYPE_F32)
     {
-        parts_launch(x, (size_t)T * H, p + s.x, hs);
+        parts_launch(x, T, H, p + s.x, hs);
         a.x = (const uint16_t*)(p + s.x);
-        a.xplane = (size_t)T * H;
     }
     a.w13 = { (const uint32_t*)L->w13.q, (const uint16_t*)L->w13.scales, L->w13.zeros };
     a.w2 = { (const uint32_t*)L->w2.q, (const uint16_t*)L->w2.scales, L->w2.zeros };
@@ -701,25 +907,23 @@ int mm_w4_moe(const mm_w4_layer_t* L, const void* x, int x_dtype, int T, int top
         a.recs = (const W4Rec*)(p + s.recs);
         a.nrec = (const int32_t*)(p + s.nrec);
     }
+    const bool many = s.rows > 16;
     by_input(x_dtype, [&](auto xt, auto parts) {
-        by_group(L->group, [&](auto g) {
+        by_group(L->group, L->w13.zeros != nullptr, [&](auto g, auto zp) {
             constexpr int XT = decltype(xt)::value, P = decltype(parts)::value, G = decltype(g)::value;
-            if (s.rows == 16)
-                hipLaunchKernelGGL((k_w4_gate_up<XT, P, G, 1, 8>), dim3(I / 16, s.nrecs), dim3(512), 0, hs, a);
-            else if (s.rows == 32)
-                hipLaunchKernelGGL((k_w4_gate_up<XT, P, G, 2, 8>), dim3(I / 16, s.nrecs), dim3(512), 0, hs, a);
-            else
-                hipLaunchKernelGGL((k_w4_gate_up<XT, P, G, 4, 4>), dim3(I / 16, s.nrecs), dim3(256), 0, hs, a);
+            constexpr bool ZP = decltype(zp)::value;
+            if (many) hipLaunchKernelGGL((k_w4_gate_up_many<XT, P, G, ZP, 4>), dim3((I + 63) / 64, s.nrecs), dim3(256), 0, hs, a);
+            else if (T <= W4_ROWS<P, 1> || (P == 1 && s.rows <= 16))
+                hipLaunchKernelGGL((k_w4_gate_up<XT, P, G, ZP, 1>), dim3(I / 16, s.nrecs), dim3(256), 0, hs, a);
+            else hipLaunchKernelGGL((k_w4_gate_up<XT, P, G, ZP, 2>), dim3(I / 16, s.nrecs), dim3(256), 0, hs, a);
         });
     });
-    by_group(L->group, [&](auto g) {
+    by_group(L->group, L->w2.zeros != nullptr, [&](auto g, auto zp) {
         constexpr int G = decltype(g)::value;
-        if (s.rows == 16)
-            hipLaunchKernelGGL((k_w4_down<G, 1, 8>), dim3(H / 16, s.nrecs), dim3(512), 0, hs, a);
-        else if (s.rows == 32)
-            hipLaunchKernelGGL((k_w4_down<G, 2, 8>), dim3(H / 16, s.nrecs), dim3(512), 0, hs, a);
-        else
-            hipLaunchKernelGGL((k_w4_down<G, 4, 4>), dim3(H / 16, s.nrecs), dim3(256), 0, hs, a);
+        constexpr bool ZP = decltype(zp)::value;
+        if (many) hipLaunchKernelGGL((k_w4_down_many<G, ZP, 4>), dim3((H + 127) / 128, s.nrecs), dim3(256), 0, hs, a);
+        else if (T <= W4_ROWS<3, 1>) hipLaunchKernelGGL((k_w4_down<G, ZP, 1>), dim3(H / 32, s.nrecs), dim3(256), 0, hs, a);
+        else hipLaunchKernelGGL((k_w4_down<G, ZP, 2>), dim3(H / 32, s.nrecs), dim3(256), 0, hs, a);
     });
     hipLaunchKernelGGL(k_w4_combine, dim3((H / 4 + 255) / 256, T), dim3(256), 0, hs, a);
     return check_launch("mm_w4_moe");
