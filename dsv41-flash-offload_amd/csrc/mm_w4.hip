@@ -167,22 +167,27 @@ struct W4Wave
     using scales_t = few_t<2 * NG>;
     using zeros_t = few_t<NG>;
 
-    u4_t xv[XI], wv[NT];
-    scales_t sv[NT], sc[NT];
-    zeros_t zv[NT], zc[NT];
-    // bases that are the same for all lanes, and the lanes' byte offsets
-    const unsigned char *xb, *qb, *sb, *zb;
+    // weights of the next AHEAD blocks and inputs of the next one in registers (loads return in order: a block's inputs are asked for
+    // before the weights that come after them)
+    static constexpr int AHEAD = 1;
+    u4_t xv[XI], wv[AHEAD][NT];
+    scales_t sv[AHEAD][NT], sc[NT];
+    zeros_t zv[AHEAD][NT], zc[NT];
+    // x and W through buffer descriptors: one register of byte offset a load, the block's place in a scalar, and what the last block
+    // reads past a row is the next row, or zero past the end
+    __amdgpu_buffer_rsrc_t xb, qb;
+    const unsigned char *sb, *zb;
     uint32_t xo[XI], qo[NT], so[NT];
     int nx;                                // loads of x that cover the rows in use
 
-    // x, w: bases; rows: number of tile rows in use; row(v): elements from x to tile row v < rows; col(nt, c): rows from w to column c
-    // of weight tile nt
+    // x, w: bases of xbytes and wrows rows; rows: number of tile rows in use; row(v): elements from x to tile row v < rows;
+    // col(nt, c): rows from w to column c of weight tile nt
     template <typename Row, typename Col>
-    __device__ __forceinline__ void init(const uint16_t* x, Row row, int rows, const W4Ptr& w, Col col, int K)
+    __device__ __forceinline__ void init(const uint16_t* x, uint32_t xbytes, Row row, int rows, const W4Ptr& w, int wrows, Col col, int K)
     {
         const int t = OWN ? threadIdx.x & 63 : threadIdx.x, lane = threadIdx.x & 63;
-        xb = reinterpret_cast<const unsigned char*>(x);
-        qb = reinterpret_cast<const unsigned char*>(w.q);
+        xb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(x), (short)0, (int)xbytes, 0x00020000);
+        qb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint32_t*>(w.q), (short)0, (int)((uint32_t)wrows * (K / 2)), 0x00020000);
         sb = reinterpret_cast<const unsigned char*>(w.s);
         zb = w.z;
         nx = (rows + XROWS - 1) / XROWS;
@@ -196,46 +201,47 @@ struct W4Wave
         }
     }
 
-    __device__ __forceinline__ void load(int b, int K)
+    __device__ __forceinline__ void load_w(int b, int K, int at)
     {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) wv[at][nt] = __builtin_amdgcn_raw_buffer_load_b128(qb, qo[nt], 64 * b, 0);
         if (G == 128 || 128 * b + 128 <= K)
         {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
             {
-                wv[nt] = *reinterpret_cast<const u4_t*>(qb + 64 * (size_t)b + qo[nt]);
-                sv[nt] = load_few<2 * NG>(sb + 2 * NG * (size_t)b + 2 * so[nt]);
-                if constexpr (ZP) zv[nt] = load_few<NG>(zb + NG * (size_t)b + so[nt]);
+                sv[at][nt] = load_few<2 * NG>(sb + 2 * NG * (size_t)b + 2 * so[nt]);
+                if constexpr (ZP) zv[at][nt] = load_few<NG>(zb + NG * (size_t)b + so[nt]);
             }
-#pragma unroll
-            for (int i = 0; i < XI; ++i)
-                if (i < nx) xv[i] = *reinterpret_cast<const u4_t*>(xb + 256 * (size_t)b + xo[i]);
-            return;
         }
-        // the last block of a K that is no multiple of 128: nothing past K is read (what is not loaded is not multiplied)
-        const int groups = (K - 128 * b) / G, lane = threadIdx.x & 63;
-        const int cq = (lane & 3) ^ (lane >> 4), cx = lane & 15;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        else
         {
-            wv[nt] = *reinterpret_cast<const u4_t*>(qb + 64 * (size_t)b + qo[nt] - (128 * b + 32 * cq < K ? 0 : 16 * cq));
-            sv[nt] = 0;
-            zv[nt] = 0;
+            // the last block of a K that is no multiple of 128: the groups that exist (what is past them is not multiplied)
+            const int groups = (K - 128 * b) / G;
 #pragma unroll
-            for (int g = 0; g < NG; ++g)
-                if (g < groups)
-                {
-                    sv[nt] |= (scales_t)reinterpret_cast<const uint16_t*>(sb)[so[nt] + b * NG + g] << (16 * g);
-                    if constexpr (ZP) zv[nt] |= (zeros_t)zb[so[nt] + b * NG + g] << (8 * g);
-                }
+            for (int nt = 0; nt < NT; ++nt)
+            {
+                sv[at][nt] = 0;
+                zv[at][nt] = 0;
+#pragma unroll
+                for (int g = 0; g < NG; ++g)
+                    if (g < groups)
+                    {
+                        sv[at][nt] |= (scales_t)reinterpret_cast<const uint16_t*>(sb)[so[nt] + b * NG + g] << (16 * g);
+                        if constexpr (ZP) zv[at][nt] |= (zeros_t)zb[so[nt] + b * NG + g] << (8 * g);
+                    }
+            }
         }
+    }
+    __device__ __forceinline__ void load_x(int b)
+    {
 #pragma unroll
         for (int i = 0; i < XI; ++i)
-            if (i < nx) xv[i] = *reinterpret_cast<const u4_t*>(xb + 256 * (size_t)b + xo[i] - (128 * b + 8 * cx < K ? 0 : 16 * cx));
+            if (i < nx) xv[i] = __builtin_amdgcn_raw_buffer_load_b128(xb, xo[i], 256 * b, 0);
     }
 
     // the loaded block into LDS
-    __device__ __forceinline__ void store(unsigned char* x, unsigned char* w)
+    __device__ __forceinline__ void store(unsigned char* x, unsigned char* w, int at)
     {
         const int t = OWN ? threadIdx.x & 63 : threadIdx.x, lane = threadIdx.x & 63;
 #pragma unroll
@@ -248,9 +254,9 @@ struct W4Wave
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
         {
-            *reinterpret_cast<u4_t*>(w + nt * 1024 + lane * 16) = wv[nt];
-            sc[nt] = sv[nt];
-            if constexpr (ZP) zc[nt] = zv[nt];
+            *reinterpret_cast<u4_t*>(w + nt * 1024 + lane * 16) = wv[at][nt];
+            sc[nt] = sv[at][nt];
+            if constexpr (ZP) zc[nt] = zv[at][nt];
         }
     }
 
@@ -336,25 +342,41 @@ struct W4Wave
         unsigned char* x = OWN ? lds + wave * (XBYTES + WBYTES) : lds;
         unsigned char* w = OWN ? x + XBYTES : lds + 2 * XBYTES + wave * WBYTES;
         if (b0 >= b1) return;
-        load(b0, K);
-        if constexpr (!OWN)
+        auto groups = [&](int b) { return G == 128 ? 1 : min(NG, (K - 128 * b) / G); };
+        load_x(b0);
+        load_w(b0, K, 0);
+        if constexpr (OWN)
         {
-            store(x, w);
-            __syncthreads();
-        }
-        for (int b = b0; b < b1; ++b)
-        {
-            if constexpr (OWN)
+            if (AHEAD == 2 && b0 + 1 < b1) load_w(b0 + 1, K, AHEAD - 1);
+            for (int b = b0; b < b1; b += AHEAD)
             {
-                store(x, w);
-                wave_fence();
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i)
+                {
+                    if (b + i >= b1) break;
+                    store(x, w, i);
+                    wave_fence();
+                    if (b + i + 1 < b1) load_x(b + i + 1);
+                    if (b + i + AHEAD < b1) load_w(b + i + AHEAD, K, i);
+                    multiply(x, w, groups(b + i), sbf, tot);
+                    wave_fence();
+                }
             }
-            if (b + 1 < b1) load(b + 1, K);
-            multiply(x + (OWN ? 0 : ((b - b0) & 1) * XBYTES), w, G == 128 ? 1 : min(NG, (K - 128 * b) / G), sbf, tot);
-            wave_fence();
-            if constexpr (!OWN)
+        }
+        else
+        {
+            store(x, w, 0);
+            __syncthreads();
+            for (int b = b0; b < b1; ++b)
             {
-                if (b + 1 < b1) store(x + ((b + 1 - b0) & 1) * XBYTES, w);
+                if (b + 1 < b1)
+                {
+                    load_x(b + 1);
+                    load_w(b + 1, K, 0);
+                }
+                multiply(x + ((b - b0) & 1) * XBYTES, w, groups(b), sbf, tot);
+                wave_fence();
+                if (b + 1 < b1) store(x + ((b + 1 - b0) & 1) * XBYTES, w, 0);
                 __syncthreads();
             }
         }
@@ -371,8 +393,8 @@ template <int P, int MT>
 constexpr int W4_ROWS = 16 * MT / P;
 
 template <int XT, int P, int G, bool ZP, int MT, int NT, int NW, bool OWN, typename Row, typename Col>
-__device__ __forceinline__ void w4_tile(unsigned char* lds, const uint16_t* x, Row row, uint32_t xpart, int cnt, const W4Ptr& w, Col col,
-                                        bool sbf, int K)
+__device__ __forceinline__ void w4_tile(unsigned char* lds, const uint16_t* x, uint32_t xbytes, Row row, uint32_t xpart, int cnt,
+                                        const W4Ptr& w, int wrows, Col col, bool sbf, int K)
 {
     using Wave = W4Wave<XT, P == 3, G, ZP, MT, NT, NW, OWN>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nb = (K + 127) / 128;
@@ -382,10 +404,10 @@ __device__ __forceinline__ void w4_tile(unsigned char* lds, const uint16_t* x, R
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) tot[mt][nt] = f4_t{ 0.f, 0.f, 0.f, 0.f };
     Wave wv;
-    wv.init(x, [&](int v) {
+    wv.init(x, xbytes, [&](int v) {
         const int q = P == 1 ? 0 : (v >= cnt) + (v >= 2 * cnt);
         return row(v - q * cnt) + q * xpart;
-    }, P * cnt, w, col, K);
+    }, P * cnt, w, wrows, col, K);
     wv.run(lds, OWN ? nb * wave / NW : 0, OWN ? nb * (wave + 1) / NW : nb, K, sbf, tot);
     // the sums into LDS: OWN in the wave's own place, else where the inputs were (every wave is past its last barrier)
     f4_t* part = reinterpret_cast<f4_t*>(lds + (OWN ? wave * (Wave::XBYTES + Wave::WBYTES) : wave * MT * NT * 1024));
@@ -480,8 +502,8 @@ __global__ __launch_bounds__(64 * NW) void k_w4_linear(LinearArgs a)
     const int m0 = blockIdx.y * ROWS, n0 = OWN ? blockIdx.x * 16 * NT : (blockIdx.x * NW + wave) * 16 * NT, cnt = min(ROWS, a.M - m0);
     const int n1 = min(n0, a.N - 1);                                 // a wave past the last column works on it again
     w4_tile<XT, P, G, ZP, MT, NT, NW, OWN>(
-        lds, a.x + (size_t)m0 * P * a.K, [&](int m) { return (uint32_t)m * P * a.K; }, a.K, cnt, w4_at(a.w, n1, a.K, G),
-        [&](int nt, int c) { return (uint32_t)min(16 * nt + c, a.N - 1 - n1); }, a.sbf, a.K);
+        lds, a.x + (size_t)m0 * P * a.K, (uint32_t)cnt * P * a.K * 2, [&](int m) { return (uint32_t)m * P * a.K; }, a.K, cnt,
+        w4_at(a.w, n1, a.K, G), min(a.N - n1, 16 * NT), [&](int nt, int c) { return (uint32_t)min(16 * nt + c, a.N - 1 - n1); }, a.sbf, a.K);
     const unsigned char* sums = OWN ? lds : lds + wave * MT * NT * 1024;
     for (int o = OWN ? threadIdx.x : threadIdx.x & 63; o < cnt * 16 * NT; o += OWN ? 64 * NW : 64)
     {
@@ -513,7 +535,7 @@ struct ExpertArgs
     const int32_t* nrec;
     uint16_t* h;               // [n][3][I] parts in weight order
     float* y;                  // [n][H]
-    int n, k, topk, E, H, I, sbf;      // n = T topk routes, topk = k, and one more with a shared expert
+    int T, n, k, topk, E, H, I, sbf;   // n = T topk routes, topk = k, and one more with a shared expert
     int shared;
     float limit;
 };
@@ -543,82 +565,90 @@ __device__ __forceinline__ int record_rows(const ExpertArgs& a, int rec, int* ro
     }
     if (rec >= *a.nrec) return 0;
     const W4Rec q = a.recs[rec];
-    expert = q.expert;
+    expert = __builtin_amdgcn_readfirstlane(q.expert);
     if ((int)threadIdx.x < q.count) rows[threadIdx.x] = a.order[q.start + threadIdx.x];
-    return q.count;
+    return __builtin_amdgcn_readfirstlane(q.count);
 }
 
-// Gate and up of 16 columns (OWN: a workgroup's, else a wave's) for some of a record's routes, SwiGLU, and the result as three
-// bf16 parts for the down product.
-template <int XT, int P, int G, bool ZP, int MT, int NW, bool OWN>
+// Gate and up of 8 NT columns (OWN: a workgroup's, else a wave's; weight tile 2 i is gate, 2 i + 1 up) for some of a record's
+// routes, SwiGLU, and the result as three bf16 parts for the down product.
+template <int XT, int P, int G, bool ZP, int MT, int NT, int NW, bool OWN>
 __device__ __forceinline__ void gate_up_rows(const ExpertArgs& a, unsigned char* lds, int expert, const int* rows, int c)
 {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = OWN ? blockIdx.x * 16 : (blockIdx.x * NW + wave) * 16;
-    w4_tile<XT, P, G, ZP, MT, 2, NW, OWN>(
-        lds, a.x, [&](int m) { return (uint32_t)(rows[m] / a.topk) * (P * a.H); }, a.H, c, w4_at(a.w13, (size_t)expert * 2 * a.I, a.H, G),
-        [&](int t, int col) { return (uint32_t)(t * a.I + min(n0 + col, a.I - 1)); }, a.sbf, a.H);
-    const unsigned char* sums = OWN ? lds : lds + wave * MT * 2 * 1024;
-    for (int o = OWN ? threadIdx.x : threadIdx.x & 63; o < c * 16; o += OWN ? 64 * NW : 64)
+    constexpr int COLS = 8 * NT;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = OWN ? blockIdx.x * COLS : (blockIdx.x * NW + wave) * COLS;
+    w4_tile<XT, P, G, ZP, MT, NT, NW, OWN>(
+        lds, a.x, (uint32_t)a.T * P * a.H * 2, [&](int m) { return (uint32_t)(rows[m] / a.topk) * (P * a.H); }, a.H, c,
+        w4_at(a.w13, (size_t)expert * 2 * a.I, a.H, G), 2 * a.I,
+        [&](int t, int col) { return (uint32_t)((t & 1) * a.I + min(n0 + 16 * (t >> 1) + col, a.I - 1)); }, a.sbf, a.H);
+    const unsigned char* sums = OWN ? lds : lds + wave * MT * NT * 1024;
+    for (int o = OWN ? threadIdx.x : threadIdx.x & 63; o < c * COLS; o += OWN ? 64 * NW : 64)
     {
-        const int m = o >> 4, col = o & 15;
+        const int m = o / COLS, col = o % COLS, t = 2 * (col >> 4);
         if (n0 + col >= a.I) continue;
         uint16_t p[3];
-        three_parts(act_gu(tile_value<P, 2>(sums, c, m, 0, col), tile_value<P, 2>(sums, c, m, 1, col), a.limit), p[0], p[1], p[2]);
-        uint16_t* h = a.h + (size_t)rows[m] * 3 * a.I + n0 + (col & 8) + weight_place(col & 7);
+        three_parts(act_gu(tile_value<P, NT>(sums, c, m, t, col & 15), tile_value<P, NT>(sums, c, m, t + 1, col & 15), a.limit), p[0],
+                    p[1], p[2]);
+        uint16_t* h = a.h + (size_t)rows[m] * 3 * a.I + n0 + (col & ~7) + weight_place(col & 7);
 #pragma unroll
         for (int q = 0; q < 3; ++q) h[q * a.I] = p[q];
     }
 }
-// The down product of 32 columns for some of a record's routes.
-template <int G, bool ZP, int MT, int NW, bool OWN>
+// The down product of 16 NT columns for some of a record's routes.
+template <int G, bool ZP, int MT, int NT, int NW, bool OWN>
 __device__ __forceinline__ void down_rows(const ExpertArgs& a, unsigned char* lds, int expert, const int* rows, int c)
 {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = OWN ? blockIdx.x * 32 : (blockIdx.x * NW + wave) * 32;
-    w4_tile<MM_DTYPE_BF16, 3, G, ZP, MT, 2, NW, OWN>(
-        lds, a.h, [&](int m) { return (uint32_t)rows[m] * (3 * a.I); }, a.I, c, w4_at(a.w2, (size_t)expert * a.H, a.I, G),
-        [&](int t, int col) { return (uint32_t)min(n0 + 16 * t + col, a.H - 1); }, a.sbf, a.I);
-    const unsigned char* sums = OWN ? lds : lds + wave * MT * 2 * 1024;
-    for (int o = OWN ? threadIdx.x : threadIdx.x & 63; o < c * 32; o += OWN ? 64 * NW : 64)
+    constexpr int COLS = 16 * NT;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = OWN ? blockIdx.x * COLS : (blockIdx.x * NW + wave) * COLS;
+    w4_tile<MM_DTYPE_BF16, 3, G, ZP, MT, NT, NW, OWN>(
+        lds, a.h, (uint32_t)a.n * 3 * a.I * 2, [&](int m) { return (uint32_t)rows[m] * (3 * a.I); }, a.I, c,
+        w4_at(a.w2, (size_t)expert * a.H, a.I, G), a.H, [&](int t, int col) { return (uint32_t)min(n0 + 16 * t + col, a.H - 1); },
+        a.sbf, a.I);
+    const unsigned char* sums = OWN ? lds : lds + wave * MT * NT * 1024;
+    for (int o = OWN ? threadIdx.x : threadIdx.x & 63; o < c * COLS; o += OWN ? 64 * NW : 64)
     {
-        const int m = o >> 5, col = o & 31;
-        if (n0 + col < a.H) a.y[(size_t)rows[m] * a.H + n0 + col] = tile_value<3, 2>(sums, c, m, col >> 4, col & 15);
+        const int m = o / COLS, col = o % COLS;
+        if (n0 + col < a.H) a.y[(size_t)rows[m] * a.H + n0 + col] = tile_value<3, NT>(sums, c, m, col >> 4, col & 15);
     }
 }
+
+// Weight tiles of a workgroup in the gate/up and the down product of few rows.
+constexpr int W4_GU = 2, W4_DN = 2;
 
 // Few rows: one workgroup per record and 16 (32) columns, its four waves split K; one or two row tiles by the record's routes, more routes in
 // more passes.
 template <int XT, int P, int G, bool ZP, int MT>
-__global__ __launch_bounds__(256) void k_w4_gate_up(ExpertArgs a)
+__global__ __launch_bounds__(256, MT == 1 ? 4 : 3) void k_w4_gate_up(ExpertArgs a)
 {
-    __shared__ __align__(16) unsigned char lds[W4Wave<XT, P == 3, G, ZP, MT, 2, 4, true>::LDS];
+    __shared__ __align__(16) unsigned char lds[W4Wave<XT, P == 3, G, ZP, MT, W4_GU, 4, true>::LDS];
     __shared__ int rows[W4_REC];
     int expert;
     const int cnt = record_rows(a, blockIdx.y, rows, expert);
     if (cnt == 0) return;
     __syncthreads();
     if constexpr (MT > 1)
-        if (cnt <= W4_ROWS<P, 1>) return gate_up_rows<XT, P, G, ZP, 1, 4, true>(a, lds, expert, rows, cnt);
+        if (cnt <= W4_ROWS<P, 1>) return gate_up_rows<XT, P, G, ZP, 1, W4_GU, 4, true>(a, lds, expert, rows, cnt);
     for (int m = 0; m < cnt; m += W4_ROWS<P, MT>)
     {
         if (m) __syncthreads();                        // the previous rows' sums are read
-        gate_up_rows<XT, P, G, ZP, MT, 4, true>(a, lds, expert, rows + m, min(W4_ROWS<P, MT>, cnt - m));
+        gate_up_rows<XT, P, G, ZP, MT, W4_GU, 4, true>(a, lds, expert, rows + m, min(W4_ROWS<P, MT>, cnt - m));
     }
 }
 template <int G, bool ZP, int MT>
-__global__ __launch_bounds__(256) void k_w4_down(ExpertArgs a)
+__global__ __launch_bounds__(256, MT == 1 ? 4 : 3) void k_w4_down(ExpertArgs a)
 {
-    __shared__ __align__(16) unsigned char lds[W4Wave<MM_DTYPE_BF16, true, G, ZP, MT, 2, 4, true>::LDS];
+    __shared__ __align__(16) unsigned char lds[W4Wave<MM_DTYPE_BF16, true, G, ZP, MT, W4_DN, 4, true>::LDS];
     __shared__ int rows[W4_REC];
     int expert;
     const int cnt = record_rows(a, blockIdx.y, rows, expert);
     if (cnt == 0) return;
     __syncthreads();
     if constexpr (MT > 1)
-        if (cnt <= W4_ROWS<3, 1>) return down_rows<G, ZP, 1, 4, true>(a, lds, expert, rows, cnt);
+        if (cnt <= W4_ROWS<3, 1>) return down_rows<G, ZP, 1, W4_DN, 4, true>(a, lds, expert, rows, cnt);
     for (int m = 0; m < cnt; m += W4_ROWS<3, MT>)
     {
         if (m) __syncthreads();
-        down_rows<G, ZP, MT, 4, true>(a, lds, expert, rows + m, min(W4_ROWS<3, MT>, cnt - m));
+        down_rows<G, ZP, MT, W4_DN, 4, true>(a, lds, expert, rows + m, min(W4_ROWS<3, MT>, cnt - m));
     }
 }
 
@@ -635,7 +665,7 @@ __global__ __launch_bounds__(256) void k_w4_gate_up_many(ExpertArgs a)
     for (int m = 0; m < cnt; m += W4_ROWS<P, MT>)
     {
         if (m) __syncthreads();
-        gate_up_rows<XT, P, G, ZP, MT, 4, false>(a, lds, expert, rows + m, min(W4_ROWS<P, MT>, cnt - m));
+        gate_up_rows<XT, P, G, ZP, MT, 2, 4, false>(a, lds, expert, rows + m, min(W4_ROWS<P, MT>, cnt - m));
     }
 }
 template <int G, bool ZP, int MT>
@@ -650,7 +680,7 @@ __global__ __launch_bounds__(256) void k_w4_down_many(ExpertArgs a)
     for (int m = 0; m < cnt; m += W4_ROWS<3, MT>)
     {
         if (m) __syncthreads();
-        down_rows<G, ZP, MT, 4, false>(a, lds, expert, rows + m, min(W4_ROWS<3, MT>, cnt - m));
+        down_rows<G, ZP, MT, 2, 4, false>(a, lds, expert, rows + m, min(W4_ROWS<3, MT>, cnt - m));
     }
 }
 
@@ -743,11 +773,21 @@ static void parts_launch(const void* x, size_t rows, int K, void* out, hipStream
     hipLaunchKernelGGL(k_w4_parts, dim3((unsigned)((n8 + 255) / 256)), dim3(256), 0, hs, (const float*)x, n8, K / 8, (uint16_t*)out);
 }
 
+// A call of many tokens runs in chunks: byte offsets into the inputs and the down inputs fit 31 bits, and a chunk's workspace
+// serves the next.
+static int expert_chunk(int T, int topk, int H, int I)
+{
+    const size_t most = ((size_t)1 << 31) - 1;
+    const size_t t = std::min(most / (6 * (size_t)H), most / (6 * (size_t)I * topk));
+    return (int)std::min((size_t)T, std::min(t, (size_t)8192));
+}
+
 struct ExpertWs
 {
     size_t x, h, y, ids, counts, offsets, order, token, recs, nrec, perm, total;
     int rows, nrecs;
 };
+// of a chunk of T tokens
 static ExpertWs expert_ws(int x_dtype, int T, int k, int shared, int E, int H, int I)
 {
     const int topk = k + (shared >= 0);
@@ -763,7 +803,7 @@ static ExpertWs expert_ws(int x_dtype, int T, int k, int shared, int E, int H, i
     {
         // rows of a record: of up to 16, 32 or 64 routes by the average of the experts
         w.rows = n > (size_t)32 * E ? 64 : n > (size_t)12 * E ? 32 : 16;
-        w.nrecs = (int)std::min(n, std::min(n, (size_t)E) + n / w.rows);
+        w.nrecs = (int)(std::min(n, (size_t)E) + n / w.rows);
         w.ids = take(shared >= 0 ? n * 8 : 0);
         w.counts = take((E + 1) * 4);
         w.offsets = take((E + 2) * 4);
@@ -776,6 +816,86 @@ static ExpertWs expert_ws(int x_dtype, int T, int k, int shared, int E, int H, i
     else w.nrecs = (int)n;
     w.total = at;
     return w;
+}
+static size_t expert_ws_bytes(int x_dtype, int T, int k, int shared, int E, int H, int I)
+{
+    // a chunk, and the last one, which may find its records in another way
+    const int c = expert_chunk(T, k + 1, H, I);
+    const size_t whole = expert_ws(x_dtype, c, k, shared, E, H, I).total;
+    return T % c ? std::max(whole, expert_ws(x_dtype, T % c, k, shared, E, H, I).total) : whole;
+}
+
+// One chunk of mm_w4_moe, its arguments checked.
+static int experts_launch(const mm_w4_layer_t* L, const void* x, int x_dtype, int T, int topk, const int64_t* ids, const float* w,
+                          int shared, float* out, unsigned char* p, mm_stream_t stream)
+{
+    const int E = L->E, H = L->H, I = L->I;
+    const ExpertWs s = expert_ws(x_dtype, T, topk, shared, E, H, I);
+    const hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
+    ExpertArgs a{};
+    a.x = (const uint16_t*)x;
+    if (x_dtype == MM_DTYPE_F32)
+    {
+        parts_launch(x, T, H, p + s.x, hs);
+        a.x = (const uint16_t*)(p + s.x);
+    }
+    a.w13 = { (const uint32_t*)L->w13.q, (const uint16_t*)L->w13.scales, L->w13.zeros };
+    a.w2 = { (const uint32_t*)L->w2.q, (const uint16_t*)L->w2.scales, L->w2.zeros };
+    a.ids = ids;
+    a.w = w;
+    a.out = out;
+    a.k = topk;
+    a.shared = shared;
+    a.h = (uint16_t*)(p + s.h);
+    a.y = (float*)(p + s.y);
+    a.T = T;
+    a.topk = topk + (shared >= 0);
+    a.n = T * a.topk;
+    a.E = E;
+    a.H = H;
+    a.I = I;
+    a.sbf = L->scale_dtype == MM_DTYPE_BF16;
+    a.limit = L->limit;
+    if (a.n > W4_SELF)
+    {
+        int32_t* order = (int32_t*)(p + s.order);
+        int32_t* counts = (int32_t*)(p + s.counts);
+        int32_t* offsets = (int32_t*)(p + s.offsets);
+        const int64_t* all = ids;
+        if (shared >= 0)
+        {
+            hipLaunchKernelGGL(k_w4_routes, dim3((a.n + 255) / 256), dim3(256), 0, hs, a, (int64_t*)(p + s.ids));
+            all = (const int64_t*)(p + s.ids);
+        }
+        const int rc = permute_launch(all, nullptr, a.n, a.topk, E, counts, offsets, order, (int32_t*)(p + s.token), nullptr, nullptr,
+                                      nullptr, nullptr, p + s.perm, mm_permute_workspace(a.n, E), stream);
+        if (rc) return rc;
+        hipLaunchKernelGGL(k_w4_plan, dim3(1), dim3(1024), 0, hs, counts, offsets, E, s.rows, (W4Rec*)(p + s.recs),
+                           (int32_t*)(p + s.nrec));
+        a.order = order;
+        a.recs = (const W4Rec*)(p + s.recs);
+        a.nrec = (const int32_t*)(p + s.nrec);
+    }
+    const bool many = s.rows > 16;
+    by_input(x_dtype, [&](auto xt, auto parts) {
+        by_group(L->group, L->w13.zeros != nullptr, [&](auto g, auto zp) {
+            constexpr int XT = decltype(xt)::value, P = decltype(parts)::value, G = decltype(g)::value;
+            constexpr bool ZP = decltype(zp)::value;
+            if (many) hipLaunchKernelGGL((k_w4_gate_up_many<XT, P, G, ZP, 4>), dim3((I + 63) / 64, s.nrecs), dim3(256), 0, hs, a);
+            else if (T <= W4_ROWS<P, 1> || (P == 1 && s.rows <= 16))
+                hipLaunchKernelGGL((k_w4_gate_up<XT, P, G, ZP, 1>), dim3((I + 8 * W4_GU - 1) / (8 * W4_GU), s.nrecs), dim3(256), 0, hs, a);
+            else hipLaunchKernelGGL((k_w4_gate_up<XT, P, G, ZP, 2>), dim3((I + 8 * W4_GU - 1) / (8 * W4_GU), s.nrecs), dim3(256), 0, hs, a);
+        });
+    });
+    by_group(L->group, L->w2.zeros != nullptr, [&](auto g, auto zp) {
+        constexpr int G = decltype(g)::value;
+        constexpr bool ZP = decltype(zp)::value;
+        if (many) hipLaunchKernelGGL((k_w4_down_many<G, ZP, 4>), dim3((H + 127) / 128, s.nrecs), dim3(256), 0, hs, a);
+        else if (T <= W4_ROWS<3, 1>) hipLaunchKernelGGL((k_w4_down<G, ZP, 1>), dim3((H + 16 * W4_DN - 1) / (16 * W4_DN), s.nrecs), dim3(256), 0, hs, a);
+        else hipLaunchKernelGGL((k_w4_down<G, ZP, 2>), dim3((H + 16 * W4_DN - 1) / (16 * W4_DN), s.nrecs), dim3(256), 0, hs, a);
+    });
+    hipLaunchKernelGGL(k_w4_combine, dim3((H / 4 + 255) / 256, T), dim3(256), 0, hs, a);
+    return check_launch("mm_w4_moe");
 }
 
 }  // namespace mm
@@ -798,6 +918,8 @@ int mm_w4_linear(const void* x, int x_dtype, int M, int K, int N, const mm_w4_t*
                  M, K, N);
     MM_CHECK_ARG(x_dtype >= MM_DTYPE_F16 && x_dtype <= MM_DTYPE_F32 && y_dtype >= MM_DTYPE_F16 && y_dtype <= MM_DTYPE_F32,
                  "mm_w4_linear: bad element type");
+    MM_CHECK_ARG(K < (1 << 22), "mm_w4_linear: K must be below 2^22 (%d)", K);
+    MM_CHECK_ARG(M <= (1 << 20), "mm_w4_linear: more than 2^20 rows (%d)", M);
     if (M == 0) return MM_OK;
     MM_CHECK_ARG(x && y && ((uintptr_t)x & 15) == 0, "mm_w4_linear: null or misaligned input (16 bytes)");
     const size_t need = mm_w4_linear_workspace(x_dtype, M, K);
@@ -838,7 +960,7 @@ int mm_w4_linear(const void* x, int x_dtype, int M, int K, int N, const mm_w4_t*
 size_t mm_w4_moe_workspace(int x_dtype, int T, int topk, int shared, int E, int H, int I)
 {
     if (T <= 0 || topk <= 0 || E <= 0 || H <= 0 || I <= 0 || (size_t)T * (topk + 1) >= ((size_t)1 << 30)) return 0;
-    return expert_ws(x_dtype, T, topk, shared, E, H, I).total;
+    return expert_chunk(T, topk + 1, H, I) > 0 ? expert_ws_bytes(x_dtype, T, topk, shared, E, H, I) : 0;
 }
 
 int mm_w4_moe(const mm_w4_layer_t* L, const void* x, int x_dtype, int T, int topk, const int64_t* ids, const float* w, int shared,
@@ -851,82 +973,25 @@ int mm_w4_moe(const mm_w4_layer_t* L, const void* x, int x_dtype, int T, int top
     const int E = L->E, H = L->H, I = L->I;
     MM_CHECK_ARG(E > 0 && E <= 1024 && H > 0 && I > 0 && H % L->group == 0 && I % L->group == 0,
                  "mm_w4_moe: need 0 < E <= 1024 and H, I multiples of the group (E=%d H=%d I=%d)", E, H, I);
+    MM_CHECK_ARG((size_t)H * I < ((size_t)1 << 31), "mm_w4_moe: an expert of more than 2^31 weights a matrix (H=%d I=%d)", H, I);
     MM_CHECK_ARG(shared < E, "mm_w4_moe: shared expert %d of %d", shared, E);
-    MM_CHECK_ARG(T >= 0 && topk > 0 && (size_t)T * (topk + 1) < ((size_t)1 << 30), "mm_w4_moe: bad number of routes (T=%d topk=%d)", T,
-                 topk);
+    MM_CHECK_ARG(T >= 0 && topk > 0 && topk <= 1024 && (size_t)T * (topk + 1) < ((size_t)1 << 30),
+                 "mm_w4_moe: bad number of routes (T=%d topk=%d)", T, topk);
     MM_CHECK_ARG(x_dtype >= MM_DTYPE_F16 && x_dtype <= MM_DTYPE_F32, "mm_w4_moe: bad input type");
     if (T == 0) return MM_OK;
     MM_CHECK_ARG(x && ids && w && out && ((uintptr_t)x & 15) == 0 && ((uintptr_t)out & 15) == 0,
                  "mm_w4_moe: null or misaligned pointer (x and out: 16 bytes)");
-    const ExpertWs s = expert_ws(x_dtype, T, topk, shared, E, H, I);
-    MM_CHECK_ARG(workspace && workspace_bytes >= s.total && ((uintptr_t)workspace & 15) == 0,
-                 "mm_w4_moe: workspace too small or misaligned (%zu < %zu)", workspace_bytes, s.total);
-    MM_CHECK_ARG(s.nrecs <= 65535 && T <= 65535, "mm_w4_moe: too many routes for one call (T=%d topk=%d)", T, topk);
-    const hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
-    unsigned char* p = static_cast<unsigned char*>(workspace);
-    ExpertArgs a{};
-    a.x = (const uint16_t*)x;
-    if (x_dtype == MM_DTYPE_F32)
-    {
-        parts_launch(x, T, H, p + s.x, hs);
-        a.x = (const uint16_t*)(p + s.x);
-    }
-    a.w13 = { (const uint32_t*)L->w13.q, (const uint16_t*)L->w13.scales, L->w13.zeros };
-    a.w2 = { (const uint32_t*)L->w2.q, (const uint16_t*)L->w2.scales, L->w2.zeros };
-    a.ids = ids;
-    a.w = w;
-    a.out = out;
-    a.k = topk;
-    a.shared = shared;
-    a.h = (uint16_t*)(p + s.h);
-    a.y = (float*)(p + s.y);
-    a.topk = topk + (shared >= 0);
-    a.n = T * a.topk;
-    a.E = E;
-    a.H = H;
-    a.I = I;
-    a.sbf = L->scale_dtype == MM_DTYPE_BF16;
-    a.limit = L->limit;
-    if (a.n > W4_SELF)
-    {
-        int32_t* order = (int32_t*)(p + s.order);
-        int32_t* counts = (int32_t*)(p + s.counts);
-        int32_t* offsets = (int32_t*)(p + s.offsets);
-        const int64_t* all = ids;
-        if (shared >= 0)
-        {
-            hipLaunchKernelGGL(k_w4_routes, dim3((a.n + 255) / 256), dim3(256), 0, hs, a, (int64_t*)(p + s.ids));
-            all = (const int64_t*)(p + s.ids);
-        }
-        rc = permute_launch(all, nullptr, a.n, a.topk, E, counts, offsets, order, (int32_t*)(p + s.token), nullptr, nullptr, nullptr,
-                            nullptr, p + s.perm, mm_permute_workspace(a.n, E), stream);
-        if (rc) return rc;
-        hipLaunchKernelGGL(k_w4_plan, dim3(1), dim3(1024), 0, hs, counts, offsets, E, s.rows, (W4Rec*)(p + s.recs),
-                           (int32_t*)(p + s.nrec));
-        a.order = order;
-        a.recs = (const W4Rec*)(p + s.recs);
-        a.nrec = (const int32_t*)(p + s.nrec);
-    }
-    const bool many = s.rows > 16;
-    by_input(x_dtype, [&](auto xt, auto parts) {
-        by_group(L->group, L->w13.zeros != nullptr, [&](auto g, auto zp) {
-            constexpr int XT = decltype(xt)::value, P = decltype(parts)::value, G = decltype(g)::value;
-            constexpr bool ZP = decltype(zp)::value;
-            if (many) hipLaunchKernelGGL((k_w4_gate_up_many<XT, P, G, ZP, 4>), dim3((I + 63) / 64, s.nrecs), dim3(256), 0, hs, a);
-            else if (T <= W4_ROWS<P, 1> || (P == 1 && s.rows <= 16))
-                hipLaunchKernelGGL((k_w4_gate_up<XT, P, G, ZP, 1>), dim3(I / 16, s.nrecs), dim3(256), 0, hs, a);
-            else hipLaunchKernelGGL((k_w4_gate_up<XT, P, G, ZP, 2>), dim3(I / 16, s.nrecs), dim3(256), 0, hs, a);
-        });
-    });
-    by_group(L->group, L->w2.zeros != nullptr, [&](auto g, auto zp) {
-        constexpr int G = decltype(g)::value;
-        constexpr bool ZP = decltype(zp)::value;
-        if (many) hipLaunchKernelGGL((k_w4_down_many<G, ZP, 4>), dim3((H + 127) / 128, s.nrecs), dim3(256), 0, hs, a);
-        else if (T <= W4_ROWS<3, 1>) hipLaunchKernelGGL((k_w4_down<G, ZP, 1>), dim3(H / 32, s.nrecs), dim3(256), 0, hs, a);
-        else hipLaunchKernelGGL((k_w4_down<G, ZP, 2>), dim3(H / 32, s.nrecs), dim3(256), 0, hs, a);
-    });
-    hipLaunchKernelGGL(k_w4_combine, dim3((H / 4 + 255) / 256, T), dim3(256), 0, hs, a);
-    return check_launch("mm_w4_moe");
+    const int chunk = expert_chunk(T, topk + 1, H, I);
+    MM_CHECK_ARG(chunk > 0, "mm_w4_moe: a token's routes pass 2^31 bytes (topk=%d I=%d)", topk, I);
+    const size_t need = expert_ws_bytes(x_dtype, T, topk, shared, E, H, I);
+    MM_CHECK_ARG(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0,
+                 "mm_w4_moe: workspace too small or misaligned (%zu < %zu)", workspace_bytes, need);
+    const size_t xsize = x_dtype == MM_DTYPE_F32 ? 4 : 2;
+    for (int t = 0; t < T && !rc; t += chunk)
+        rc = experts_launch(L, static_cast<const unsigned char*>(x) + (size_t)t * H * xsize, x_dtype, std::min(chunk, T - t), topk,
+                            ids + (size_t)t * topk, w + (size_t)t * topk, shared, out + (size_t)t * H,
+                            static_cast<unsigned char*>(workspace), stream);
+    return rc;
 }
 
 }  // extern "C"
