@@ -494,7 +494,7 @@ struct LinearArgs
 };
 
 template <int XT, int P, int G, bool ZP, int MT, int NT, int NW, bool OWN>
-__global__ __launch_bounds__(64 * NW) void k_w4_linear(LinearArgs a)
+__global__ __launch_bounds__(64 * NW, 2) void k_w4_linear(LinearArgs a)
 {
     constexpr int ROWS = W4_ROWS<P, MT>;
     __shared__ __align__(16) unsigned char lds[W4Wave<XT, P == 3, G, ZP, MT, NT, NW, OWN>::LDS];
@@ -614,11 +614,14 @@ __device__ __forceinline__ void down_rows(const ExpertArgs& a, unsigned char* ld
 
 // Weight tiles of a workgroup in the gate/up and the down product of few rows.
 constexpr int W4_GU = 2, W4_DN = 2;
+// Waves per SIMD that they are compiled for: as many as need no scratch memory.
+template <int G, bool ZP, int MT>
+constexpr int W4_OCC = MT == 1 ? (G == 128 && !ZP ? 4 : 3) : 2;
 
 // Few rows: one workgroup per record and 16 (32) columns, its four waves split K; one or two row tiles by the record's routes, more routes in
 // more passes.
 template <int XT, int P, int G, bool ZP, int MT>
-__global__ __launch_bounds__(256, MT == 1 ? 4 : 3) void k_w4_gate_up(ExpertArgs a)
+__global__ __launch_bounds__(256, (W4_OCC<G, ZP, MT>)) void k_w4_gate_up(ExpertArgs a)
 {
     __shared__ __align__(16) unsigned char lds[W4Wave<XT, P == 3, G, ZP, MT, W4_GU, 4, true>::LDS];
     __shared__ int rows[W4_REC];
@@ -635,7 +638,7 @@ __global__ __launch_bounds__(256, MT == 1 ? 4 : 3) void k_w4_gate_up(ExpertArgs 
     }
 }
 template <int G, bool ZP, int MT>
-__global__ __launch_bounds__(256, MT == 1 ? 4 : 3) void k_w4_down(ExpertArgs a)
+__global__ __launch_bounds__(256, (W4_OCC<G, ZP, MT>)) void k_w4_down(ExpertArgs a)
 {
     __shared__ __align__(16) unsigned char lds[W4Wave<MM_DTYPE_BF16, true, G, ZP, MT, W4_DN, 4, true>::LDS];
     __shared__ int rows[W4_REC];
@@ -654,7 +657,7 @@ __global__ __launch_bounds__(256, MT == 1 ? 4 : 3) void k_w4_down(ExpertArgs a)
 
 // Many rows: 64 (128) columns per workgroup, four waves that share the rows of x; up to 16 MT tile rows a pass.
 template <int XT, int P, int G, bool ZP, int MT>
-__global__ __launch_bounds__(256) void k_w4_gate_up_many(ExpertArgs a)
+__global__ __launch_bounds__(256, 2) void k_w4_gate_up_many(ExpertArgs a)
 {
     __shared__ __align__(16) unsigned char lds[W4Wave<XT, P == 3, G, ZP, MT, 2, 4, false>::LDS];
     __shared__ int rows[W4_REC];
@@ -669,7 +672,7 @@ __global__ __launch_bounds__(256) void k_w4_gate_up_many(ExpertArgs a)
     }
 }
 template <int G, bool ZP, int MT>
-__global__ __launch_bounds__(256) void k_w4_down_many(ExpertArgs a)
+__global__ __launch_bounds__(256, 2) void k_w4_down_many(ExpertArgs a)
 {
     __shared__ __align__(16) unsigned char lds[W4Wave<MM_DTYPE_BF16, true, G, ZP, MT, 2, 4, false>::LDS];
     __shared__ int rows[W4_REC];
