@@ -46,51 +46,63 @@ __global__ __launch_bounds__(256) void k_rb_parts(const int64_t* __restrict__ id
                                                   int k, int Ek, int Tk, uint16_t* __restrict__ d, uint16_t* __restrict__ dt)
 {
     __shared__ float tile[64][65];
+    __shared__ float sw[64 * 32], sd[64 * 32];
+    __shared__ int se[64 * 32];
     const int t0 = blockIdx.y * 64, e0 = blockIdx.x * 64, tid = threadIdx.x;
-    for (int i = tid; i < 64 * 64; i += 256)
+    // all loads at once: the tile's logit gradients, and the rows' picks (their expert within the tile, or -1)
+    float v[16];
+#pragma unroll
+    for (int u = 0; u < 16; ++u)
     {
-        const int r = i >> 6, c = i & 63;
-        tile[r][c] = dlogits && t0 + r < T && e0 + c < E ? dlogits[(size_t)(t0 + r) * E + e0 + c] : 0.f;
+        const int r = (tid + 256 * u) >> 6, c = tid & 63;
+        v[u] = dlogits && t0 + r < T && e0 + c < E ? dlogits[(size_t)(t0 + r) * E + e0 + c] : 0.f;
     }
+    const int picks = dw ? min(64, T - t0) * k : 0;
+#pragma unroll 2
+    for (int i = tid; i < picks; i += 256)
+    {
+        const size_t at = (size_t)t0 * k + i;
+        const int64_t e = ids[at];
+        sw[i] = w[at];
+        sd[i] = dw[at];
+        se[i] = e >= e0 && e < min(E, e0 + 64) ? (int)(e - e0) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < 16; ++u) tile[(tid + 256 * u) >> 6][tid & 63] = v[u];
     __syncthreads();
     // a thread per row adds its picks in ascending j (an expert picked twice gets both)
-    if (dw && tid < 64 && t0 + tid < T)
+    if (tid * k < picks)
     {
-        const size_t at = (size_t)(t0 + tid) * k;
+        const int at = tid * k;
         float s = 0.f;
-        for (int j = 0; j < k; ++j) s = fmaf(w[at + j], dw[at + j], s);
+        for (int j = 0; j < k; ++j) s = fmaf(sw[at + j], sd[at + j], s);
         for (int j = 0; j < k; ++j)
-        {
-            const int64_t e = ids[at + j] - e0;
-            if (e >= 0 && e < 64 && e0 + e < E) tile[tid][e] += w[at + j] * (dw[at + j] - s);
-        }
+            if (se[at + j] >= 0) tile[tid][se[at + j]] += sw[at + j] * (sd[at + j] - s);
     }
     __syncthreads();
     // pairs of neighbours along the contiguous index of each order
-    if (d)
-        for (int i = tid; i < 64 * 32; i += 256)
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+    {
+        const int r = (tid + 256 * u) >> 5, c = 2 * (tid & 31);
+        uint16_t p[2][3];
+        if (d && t0 + r < T && e0 + c < Ek)
         {
-            const int r = i >> 5, c = 2 * (i & 31);
-            if (t0 + r >= T || e0 + c >= Ek) continue;
-            uint16_t p[2][3];
             split3(tile[r][c], p[0][0], p[0][1], p[0][2]);
             split3(tile[r][c + 1], p[1][0], p[1][1], p[1][2]);
 #pragma unroll
             for (int q = 0; q < 2; ++q)
                 *reinterpret_cast<uint32_t*>(d + ((size_t)q * T + t0 + r) * Ek + e0 + c) = p[0][q] | ((uint32_t)p[1][q] << 16);
         }
-    if (dt)
-        for (int i = tid; i < 64 * 32; i += 256)
+        if (dt && e0 + r < E && t0 + c < Tk)
         {
-            const int r = i >> 5, c = 2 * (i & 31);
-            if (e0 + r >= E || t0 + c >= Tk) continue;
-            uint16_t p[2][3];
             split3(tile[c][r], p[0][0], p[0][1], p[0][2]);
             split3(tile[c + 1][r], p[1][0], p[1][1], p[1][2]);
 #pragma unroll
             for (int q = 0; q < 3; ++q)
                 *reinterpret_cast<uint32_t*>(dt + ((size_t)q * E + e0 + r) * Tk + t0 + c) = p[0][q] | ((uint32_t)p[1][q] << 16);
         }
+    }
 }
 
 // Two parts of the transposed gate: gt [2][H][Ek], zeros past E.
@@ -98,15 +110,20 @@ __global__ __launch_bounds__(256) void k_rb_gate(const float* __restrict__ gate,
 {
     __shared__ float tile[64][65];
     const int h0 = blockIdx.x * 64, e0 = blockIdx.y * 64, tid = threadIdx.x;
-    for (int i = tid; i < 64 * 64; i += 256)
+    float v[16];
+#pragma unroll
+    for (int u = 0; u < 16; ++u)
     {
-        const int r = i >> 6, c = i & 63;
-        tile[r][c] = e0 + r < E && h0 + c < H ? gate[(size_t)(e0 + r) * H + h0 + c] : 0.f;
+        const int r = (tid + 256 * u) >> 6, c = tid & 63;
+        v[u] = e0 + r < E && h0 + c < H ? gate[(size_t)(e0 + r) * H + h0 + c] : 0.f;
     }
+#pragma unroll
+    for (int u = 0; u < 16; ++u) tile[(tid + 256 * u) >> 6][tid & 63] = v[u];
     __syncthreads();
-    for (int i = tid; i < 64 * 32; i += 256)
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
     {
-        const int r = i >> 5, c = 2 * (i & 31);
+        const int r = (tid + 256 * u) >> 5, c = 2 * (tid & 31);
         if (h0 + r >= H || e0 + c >= Ek) continue;
         uint16_t p[2][3];
         split3(tile[c][r], p[0][0], p[0][1], p[0][2]);

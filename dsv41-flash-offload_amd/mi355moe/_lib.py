@@ -156,13 +156,22 @@ def _entered(device, stream):
         yield
 
 
+_HERE_NOW = contextlib.nullcontext()
+
+
 def on(device, stream=None):
     """Context in which a call's buffers are allocated and its kernels launched: `device` current (a call's tensors may
     live on another device than the current one), and `stream` (default: the device's current stream)."""
     import torch
-    if stream is None and torch.cuda.current_device() == device.index:
-        return contextlib.nullcontext()
+    if stream is None and torch._C._cuda_getDevice() == device.index:
+        return _HERE_NOW
     return _entered(device, stream)
+
+
+def raw_stream(device):
+    """Address of the device's current stream (torch.cuda.current_stream() without making a Stream object)."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def check_tensors(what, device, **tensors):

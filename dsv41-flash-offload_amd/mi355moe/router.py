@@ -36,7 +36,7 @@ def topk_forward(x, gate, k, stream=None):
         w = torch.empty((T, k), dtype=torch.float32, device=x.device)
         logits = torch.empty((T, E), dtype=torch.float32, device=x.device)
         if T:
-            _lib.call("mm_router_topk", _p(x), T, H, _p(gate), E, int(k), _p(logits), _p(ids), _p(w), _lib.stream_ptr())
+            _lib.call("mm_router_topk", _p(x), T, H, _p(gate), E, int(k), _p(logits), _p(ids), _p(w), _lib.raw_stream(x.device))
     return ids, w, logits
 
 
@@ -67,7 +67,7 @@ def topk_backward(x, gate, ids, w, dw=None, dlogits=None, need_x=True, need_gate
         wsb = _lib.load().mm_router_backward_workspace(T, H, E)
         ws = torch.empty(max(wsb, 1), dtype=torch.uint8, device=x.device)
         _lib.call("mm_router_backward", _p(x), T, H, _p(gate), E, k, _p(ids), _p(w), _p(dw), _p(dlogits), _p(dx), _p(dgate),
-                  _p(ws), wsb, _lib.stream_ptr())
+                  _p(ws), wsb, _lib.raw_stream(x.device))
     return dx, dgate
 
 
@@ -138,7 +138,7 @@ def balance_loss_forward(logits, ids, mask=None, score="softmax", stream=None):
         wsb = _lib.load().mm_balance_workspace(B, T, E)
         ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
         _lib.call("mm_balance_loss", _p(logits), _DTYPES[logits.dtype], _p(ids), _p(mask), B, T, E, k, _SCORES[score],
-                  _p(loss), _p(counts), _p(tokens), _p(load), _p(ws), wsb, _lib.stream_ptr())
+                  _p(loss), _p(counts), _p(tokens), _p(load), _p(ws), wsb, _lib.raw_stream(dev))
     return loss, counts, tokens, load
 
 
@@ -158,7 +158,7 @@ def balance_loss_backward(dloss, logits, counts, tokens, k, mask=None, score="so
         mask = None if mask is None else mask.contiguous()
         dlogits = torch.empty_like(logits)
         _lib.call("mm_balance_loss_backward", _p(dloss), _p(logits), _DTYPES[logits.dtype], _p(mask), _p(counts), _p(tokens), B, T,
-                  E, int(k), _SCORES[score], _p(dlogits), _lib.stream_ptr())
+                  E, int(k), _SCORES[score], _p(dlogits), _lib.raw_stream(dev))
     return dlogits
 
 

@@ -72,7 +72,7 @@ def linear(x, W, out_dtype=None, stream=None):
         wsb = _lib.load().mm_w4_linear_workspace(code, M, W.K)
         ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
         _lib.call("mm_w4_linear", _p(x), code, M, W.K, W.N, ctypes.byref(W._c), W.group, _DTYPES[W.scales.dtype], _p(y),
-                  _DTYPES[out_dtype], _p(ws), wsb, _lib.stream_ptr())
+                  _DTYPES[out_dtype], _p(ws), wsb, _lib.raw_stream(dev))
     return y
 
 
@@ -127,5 +127,5 @@ def moe(store, x, ids, w, shared_expert=None, stream=None):
         wsb = _lib.load().mm_w4_moe_workspace(code, T, k, shared, store.E, store.H, store.I)
         ws = torch.empty(max(wsb, 1), dtype=torch.uint8, device=dev)
         _lib.call("mm_w4_moe", ctypes.byref(store._c), _p(x), code, T, k, _p(ids), _p(w), shared, _p(out), _p(ws), wsb,
-                  _lib.stream_ptr())
+                  _lib.raw_stream(dev))
     return out
