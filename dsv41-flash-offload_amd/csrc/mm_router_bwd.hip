@@ -7,9 +7,9 @@
 // every product is exact and the accumulation is the only rounding; dx takes D1 G1 + D1 G2 + D2 G1, which leaves out about
 // 2^-16 of a product where the bf16 result is rounded by 2^-9.
 //
-// Launches: the parts of D, row-major for dx (its k is the expert) and transposed for dgate (its k is the token), and of
-// the transposed gate; the two products in 128 x 128 tiles; dgate's tokens are split over enough workgroups to fill the GPU
-// and their partial sums added in order.
+// Three launches: the parts of D, row-major for dx (its k is the expert) and transposed for dgate (its k is the token), and
+// of the transposed gate; both products; the sum of dgate's partial results in order, whose tokens are split over enough
+// workgroups to fill the GPU.
 #include <algorithm>
 #include <type_traits>
 
@@ -22,9 +22,9 @@ typedef __bf16 rb_bf8 __attribute__((ext_vector_type(8)));
 typedef short rb_s4 __attribute__((ext_vector_type(4)));
 typedef uint32_t rb_u4 __attribute__((ext_vector_type(4)));
 
-constexpr int RB_T = 128, RB_K = 32;
+constexpr int RB_H = 128, RB_C = 128, RB_K = 32;
 constexpr int RB_ROW = 32;               // LDS row of a k-contiguous operand: four 16-byte chunks, swizzled
-constexpr int RB_XROW = RB_T + 16;       // LDS row of the token-major input tile (32 bytes of padding: transposed reads of four rows hit distinct banks)
+constexpr int RB_XROW = RB_H + 16;       // LDS row of the token-major input tile (32 bytes of padding: transposed reads of four rows hit distinct banks)
 __device__ __forceinline__ int rb_at(int r, int q) { return r * RB_ROW + 8 * (q ^ ((r >> 2) & 3)); }
 
 // v = a + b + c in bf16: a truncated (no overflow), b rounded, c the rest, exact. inf and NaN stay in a.
@@ -39,16 +39,47 @@ __device__ __forceinline__ void split3(float v, uint16_t& a, uint16_t& b, uint16
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// D = dlogits + scattered top-k gradient, one 64-token x 64-expert tile per workgroup, as parts in both orders.
+// The parts, 64 x 64 tiles: of D = dlogits + scattered top-k gradient in both orders (the first `tiles` workgroups), and of the
+// transposed gate (gt [2][H][Ek], zeros past E).
 // ---------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void gate_parts(const float* __restrict__ gate, int E, int H, int Ek, uint16_t* __restrict__ gt, float (*tile)[65],
+                                           int b)
+{
+    const int nh = (H + 63) / 64, h0 = b % nh * 64, e0 = b / nh * 64, tid = threadIdx.x;
+    float v[16];
+#pragma unroll
+    for (int u = 0; u < 16; ++u)
+    {
+        const int r = (tid + 256 * u) >> 6, c = tid & 63;
+        v[u] = e0 + r < E && h0 + c < H ? gate[(size_t)(e0 + r) * H + h0 + c] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < 16; ++u) tile[(tid + 256 * u) >> 6][tid & 63] = v[u];
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+    {
+        const int r = (tid + 256 * u) >> 5, c = 2 * (tid & 31);
+        if (h0 + r >= H || e0 + c >= Ek) continue;
+        uint16_t p[2][3];
+        split3(tile[c][r], p[0][0], p[0][1], p[0][2]);
+        split3(tile[c + 1][r], p[1][0], p[1][1], p[1][2]);
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+            *reinterpret_cast<uint32_t*>(gt + ((size_t)q * H + h0 + r) * Ek + e0 + c) = p[0][q] | ((uint32_t)p[1][q] << 16);
+    }
+}
+
 __global__ __launch_bounds__(256) void k_rb_parts(const int64_t* __restrict__ ids, const float* __restrict__ w,
-                                                  const float* __restrict__ dw, const float* __restrict__ dlogits, int T, int E,
-                                                  int k, int Ek, int Tk, uint16_t* __restrict__ d, uint16_t* __restrict__ dt)
+                                                  const float* __restrict__ dw, const float* __restrict__ dlogits,
+                                                  const float* __restrict__ gate, int T, int E, int H, int k, int Ek, int Tk,
+                                                  uint16_t* __restrict__ d, uint16_t* __restrict__ dt, uint16_t* __restrict__ gt, int tiles)
 {
     __shared__ float tile[64][65];
     __shared__ float sw[64 * 32], sd[64 * 32];
     __shared__ int se[64 * 32];
-    const int t0 = blockIdx.y * 64, e0 = blockIdx.x * 64, tid = threadIdx.x;
+    if ((int)blockIdx.x >= tiles) return gate_parts(gate, E, H, Ek, gt, tile, blockIdx.x - tiles);
+    const int ne = (E + 63) / 64, t0 = (int)blockIdx.x / ne * 64, e0 = (int)blockIdx.x % ne * 64, tid = threadIdx.x;
     // all loads at once: the tile's logit gradients, and the rows' picks (their expert within the tile, or -1)
     float v[16];
 #pragma unroll
@@ -105,143 +136,133 @@ __global__ __launch_bounds__(256) void k_rb_parts(const int64_t* __restrict__ id
     }
 }
 
-// Two parts of the transposed gate: gt [2][H][Ek], zeros past E.
-__global__ __launch_bounds__(256) void k_rb_gate(const float* __restrict__ gate, int E, int H, int Ek, uint16_t* __restrict__ gt)
-{
-    __shared__ float tile[64][65];
-    const int h0 = blockIdx.x * 64, e0 = blockIdx.y * 64, tid = threadIdx.x;
-    float v[16];
-#pragma unroll
-    for (int u = 0; u < 16; ++u)
-    {
-        const int r = (tid + 256 * u) >> 6, c = tid & 63;
-        v[u] = e0 + r < E && h0 + c < H ? gate[(size_t)(e0 + r) * H + h0 + c] : 0.f;
-    }
-#pragma unroll
-    for (int u = 0; u < 16; ++u) tile[(tid + 256 * u) >> 6][tid & 63] = v[u];
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-    {
-        const int r = (tid + 256 * u) >> 5, c = 2 * (tid & 31);
-        if (h0 + r >= H || e0 + c >= Ek) continue;
-        uint16_t p[2][3];
-        split3(tile[c][r], p[0][0], p[0][1], p[0][2]);
-        split3(tile[c + 1][r], p[1][0], p[1][1], p[1][2]);
-#pragma unroll
-        for (int q = 0; q < 2; ++q)
-            *reinterpret_cast<uint32_t*>(gt + ((size_t)q * H + h0 + r) * Ek + e0 + c) = p[0][q] | ((uint32_t)p[1][q] << 16);
-    }
-}
-
 // ---------------------------------------------------------------------------------------------------------
-// The products, 128 (hidden index h) x 128 (column c: token or expert) tiles, four waves of 64 x 64.
+// The products in RB_H (hidden indices h) x RB_C (columns c: tokens or experts) tiles, four waves of RB_H / 2 x RB_C / 2.
 // DX: rows are gt's (k = expert), columns d's, result dx[c][h] in bf16.
 // else: rows are columns of x (k = token, read transposed from LDS), columns dt's, result part[z][c][h] in fp32.
 // ---------------------------------------------------------------------------------------------------------
+struct GemmArgs
+{
+    const uint16_t *rows, *cols;
+    const float* gate;
+    void* out;
+    int H, C, T, K, E, ksteps;
+};
+constexpr int RB_LDS = std::max(2 * RB_H * RB_ROW + 2 * RB_C * RB_ROW, RB_K * RB_XROW + 3 * RB_C * RB_ROW);
+
 template <bool DX>
-__global__ __launch_bounds__(256) void k_rb_gemm(const uint16_t* __restrict__ rows, const uint16_t* __restrict__ cols, int H,
-                                                 int C, int T, int K, int ksteps, const float* __restrict__ gate, int E,
-                                                 void* __restrict__ out)
+__device__ __forceinline__ void rb_tile(const GemmArgs& a, uint16_t* lds, int bh, int bc, int bz)
 {
     constexpr int PR = DX ? 2 : 1, PC = DX ? 2 : 3;
-    __shared__ __align__(16) uint16_t rs[DX ? PR * RB_T * RB_ROW : RB_K * RB_XROW];
-    __shared__ __align__(16) uint16_t cs[PC][RB_T * RB_ROW];
+    constexpr int RT = RB_H / 32, CT = RB_C / 32;          // 16 x 16 tiles per wave
+    constexpr int RI = PR * RB_H / 64, CI = RB_C / 64;     // 16-byte loads per thread and step: rows (all parts; x: 32 x RB_H), columns (a part)
+    uint16_t* rs = lds;
+    uint16_t* cs = lds + (DX ? PR * RB_H * RB_ROW : RB_K * RB_XROW);
+    const int H = a.H, C = a.C, K = a.K;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int h0 = blockIdx.x * RB_T, c0 = blockIdx.y * RB_T;
-    const int wh = 64 * (wave >> 1), wc = 64 * (wave & 1);
-    const int s0 = blockIdx.z * ksteps, s1 = min(K / RB_K, s0 + ksteps);
-    rb_u4 rv[2 * PR], cv[2 * PC];                          // (a plain vector type: HIP's uint4 arrays went to scratch memory here)
+    const int h0 = bh * RB_H, c0 = bc * RB_C;
+    const int wh = RB_H / 2 * (wave >> 1), wc = RB_C / 2 * (wave & 1);
+    const int s0 = bz * a.ksteps, s1 = min(K / RB_K, s0 + a.ksteps);
+    rb_u4 rv[RI], cv[PC * CI];                             // (a plain vector type: HIP's uint4 arrays went to scratch memory here)
     auto load = [&](int s) {
         const int k0 = s * RB_K;
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-        {
-            const int i = tid + 256 * j;
+        for (int j = 0; j < RI; ++j)
             if constexpr (DX)
             {
+                const int i = tid + 256 * (j / PR), p = j % PR;
                 const size_t r = min(h0 + (i >> 2), H - 1);
-#pragma unroll
-                for (int p = 0; p < PR; ++p)
-                    rv[2 * p + j] = *reinterpret_cast<const rb_u4*>(rows + ((size_t)p * H + r) * K + k0 + 8 * (i & 3));
+                rv[j] = *reinterpret_cast<const rb_u4*>(a.rows + ((size_t)p * H + r) * K + k0 + 8 * (i & 3));
             }
             else
             {
-                const int t = k0 + (i >> 4), h = h0 + 8 * (i & 15);
-                rv[j] = t < T && h < H ? *reinterpret_cast<const rb_u4*>(rows + (size_t)t * H + h) : rb_u4{ 0, 0, 0, 0 };
+                const int i = tid + 256 * j, t = k0 + i / (RB_H / 8), h = h0 + 8 * (i % (RB_H / 8));
+                rv[j] = t < a.T && h < H ? *reinterpret_cast<const rb_u4*>(a.rows + (size_t)t * H + h) : rb_u4{ 0, 0, 0, 0 };
             }
+#pragma unroll
+        for (int j = 0; j < CI; ++j)
+        {
+            const int i = tid + 256 * j;
             const size_t c = min(c0 + (i >> 2), C - 1);
 #pragma unroll
             for (int p = 0; p < PC; ++p)
-                cv[2 * p + j] = *reinterpret_cast<const rb_u4*>(cols + ((size_t)p * C + c) * K + k0 + 8 * (i & 3));
+                cv[PC * j + p] = *reinterpret_cast<const rb_u4*>(a.cols + ((size_t)p * C + c) * K + k0 + 8 * (i & 3));
         }
     };
-    rb_f4 acc[4][4];
+    rb_f4 acc[RT][CT];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = rb_f4{ 0.f, 0.f, 0.f, 0.f };
+        for (int j = 0; j < CT; ++j) acc[i][j] = rb_f4{ 0.f, 0.f, 0.f, 0.f };
     if (s0 < s1) load(s0);
     for (int s = s0; s < s1; ++s)
     {
         __syncthreads();                                  // the previous step's operand reads are done
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-        {
-            const int i = tid + 256 * j;
+        for (int j = 0; j < RI; ++j)
             if constexpr (DX)
             {
-#pragma unroll
-                for (int p = 0; p < PR; ++p)
-                    *reinterpret_cast<rb_u4*>(&rs[p * RB_T * RB_ROW + rb_at(i >> 2, i & 3)]) = rv[2 * p + j];
-            }
-            else *reinterpret_cast<rb_u4*>(&rs[(i >> 4) * RB_XROW + 8 * (i & 15)]) = rv[j];
-#pragma unroll
-            for (int p = 0; p < PC; ++p) *reinterpret_cast<rb_u4*>(&cs[p][rb_at(i >> 2, i & 3)]) = cv[2 * p + j];
-        }
-        __syncthreads();
-        if (s + 1 < s1) load(s + 1);
-        rb_bf8 R[PR][4], Cc[PC][4];
-        const int r = lane & 15, q = lane >> 4;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-        {
-            if constexpr (DX)
-            {
-#pragma unroll
-                for (int p = 0; p < PR; ++p)
-                    R[p][i] = *reinterpret_cast<const rb_bf8*>(&rs[p * RB_T * RB_ROW + rb_at(wh + 16 * i + r, q)]);
+                const int i = tid + 256 * (j / PR), p = j % PR;
+                *reinterpret_cast<rb_u4*>(&rs[p * RB_H * RB_ROW + rb_at(i >> 2, i & 3)]) = rv[j];
             }
             else
             {
-                // four tokens x 16 hidden indices per transposed read: lane r of a quarter names token r >> 2 and four
-                // columns, and gets column r of the four tokens; quarter q's tokens are 8 q .. 8 q + 7
-                typedef __attribute__((address_space(3))) rb_s4* lds4;
-                uint16_t* at = &rs[(8 * q + (r >> 2)) * RB_XROW + wh + 16 * i + 4 * (r & 3)];
-                const rb_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at);
-                const rb_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 4 * RB_XROW));
-                R[0][i] = __builtin_bit_cast(rb_bf8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                const int i = tid + 256 * j;
+                *reinterpret_cast<rb_u4*>(&rs[i / (RB_H / 8) * RB_XROW + 8 * (i % (RB_H / 8))]) = rv[j];
             }
 #pragma unroll
-            for (int p = 0; p < PC; ++p)
-                Cc[p][i] = *reinterpret_cast<const rb_bf8*>(&cs[p][rb_at(wc + 16 * i + r, q)]);
+        for (int j = 0; j < CI; ++j)
+        {
+            const int i = tid + 256 * j;
+#pragma unroll
+            for (int p = 0; p < PC; ++p) *reinterpret_cast<rb_u4*>(&cs[p * RB_C * RB_ROW + rb_at(i >> 2, i & 3)]) = cv[PC * j + p];
         }
+        __syncthreads();
+        if (s + 1 < s1) load(s + 1);
+        const int r = lane & 15, q = lane >> 4;
+        rb_bf8 R[RT], Cc[CT];
+        auto read_rows = [&](int p) {
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+                if constexpr (DX) R[i] = *reinterpret_cast<const rb_bf8*>(&rs[p * RB_H * RB_ROW + rb_at(wh + 16 * i + r, q)]);
+                else
+                {
+                    // four tokens x 16 hidden indices per transposed read: lane r of a quarter names token r >> 2 and four
+                    // columns, and gets column r of the four tokens; quarter q's tokens are 8 q .. 8 q + 7
+                    typedef __attribute__((address_space(3))) rb_s4* lds4;
+                    uint16_t* at = &rs[(8 * q + (r >> 2)) * RB_XROW + wh + 16 * i + 4 * (r & 3)];
+                    const rb_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at);
+                    const rb_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 4 * RB_XROW));
+                    R[i] = __builtin_bit_cast(rb_bf8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+        };
+        auto read_cols = [&](int p) {
+#pragma unroll
+            for (int j = 0; j < CT; ++j)
+                Cc[j] = *reinterpret_cast<const rb_bf8*>(&cs[p * RB_C * RB_ROW + rb_at(wc + 16 * j + r, q)]);
+        };
+        // dx: G1 D2, G1 D1, G2 D1; dgate: x D3, x D2, x D1
+        read_rows(0);
 #pragma unroll
         for (int p = 0; p < 3; ++p)
         {
-            constexpr int rp[3] = { 0, 0, DX ? 1 : 0 }, cp[3] = { 0, 1, DX ? 0 : 2 };
+            if constexpr (DX)
+            {
+                if (p < 2) read_cols(1 - p);
+                else read_rows(1);
+            }
+            else read_cols(2 - p);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < RT; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(R[rp[p]][i], Cc[cp[p]][j], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < CT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(R[i], Cc[j], acc[i][j], 0, 0, 0);
         }
     }
     // lane (column l & 15, group l >> 4) holds hidden indices 4 g .. 4 g + 3 of its column; H is a multiple of 16
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < CT; ++j)
         {
             const int h = h0 + wh + 16 * i + 4 * (lane >> 4), c = c0 + wc + 16 * j + (lane & 15);
             if (h >= H || c >= C) continue;
@@ -255,19 +276,36 @@ __global__ __launch_bounds__(256) void k_rb_gemm(const uint16_t* __restrict__ ro
                     if (v[m] != v[m])
                     {
                         v[m] = 0.f;
-                        for (int e = 0; e < E; ++e)
+                        for (int e = 0; e < a.E; ++e)
                         {
-                            const uint16_t* d = cols + (size_t)c * K + e;
+                            const uint16_t* d = a.cols + (size_t)c * K + e;
                             v[m] = fmaf(__uint_as_float((uint32_t)d[0] << 16) + __uint_as_float((uint32_t)d[(size_t)C * K] << 16),
-                                        gate[(size_t)e * H + h + m], v[m]);
+                                        a.gate[(size_t)e * H + h + m], v[m]);
                         }
                     }
-            }
-            if constexpr (DX)
-                *reinterpret_cast<uint2*>((uint16_t*)out + (size_t)c * H + h) =
+                *reinterpret_cast<uint2*>((uint16_t*)a.out + (size_t)c * H + h) =
                     make_uint2(f2bf(v[0]) | ((uint32_t)f2bf(v[1]) << 16), f2bf(v[2]) | ((uint32_t)f2bf(v[3]) << 16));
-            else *reinterpret_cast<rb_f4*>((float*)out + ((size_t)blockIdx.z * C + c) * H + h) = v;
+            }
+            else *reinterpret_cast<rb_f4*>((float*)a.out + ((size_t)bz * C + c) * H + h) = v;
         }
+}
+
+// Both products in one launch: the first dx_blocks workgroups are dx's tiles, the others dgate's (x: hidden tile, then column tile, then
+// split).
+__global__ __launch_bounds__(256, 2) void k_rb_gemm(GemmArgs dx, GemmArgs dg, int dx_blocks)
+{
+    __shared__ __align__(16) uint16_t lds[RB_LDS];
+    const int b = blockIdx.x;
+    if (b < dx_blocks)
+    {
+        const int nh = (dx.H + RB_H - 1) / RB_H;
+        rb_tile<true>(dx, lds, b % nh, b / nh, 0);
+    }
+    else
+    {
+        const int i = b - dx_blocks, nh = (dg.H + RB_H - 1) / RB_H, nc = (dg.C + RB_C - 1) / RB_C;
+        rb_tile<false>(dg, lds, i % nh, i / nh % nc, i / nh / nc);
+    }
 }
 
 // out[i] = part[0][i] + part[1][i] + ... in order, four values a thread.
@@ -280,11 +318,12 @@ __global__ __launch_bounds__(256) void k_rb_sum(const float* __restrict__ part, 
     *reinterpret_cast<rb_f4*>(out + i) = s;
 }
 
-// Workgroups dgate's tokens are split over: two per CU in all, at least four steps of 32 tokens each.
+// Workgroups dgate's tokens are split over: two per CU in all, at least RB_MIN_STEPS steps of 32 tokens each.
+constexpr int RB_MIN_STEPS = 8;
 static int rb_splits(int T, int H, int E)
 {
-    const int tiles = ((H + RB_T - 1) / RB_T) * ((E + RB_T - 1) / RB_T), steps = (T + RB_K - 1) / RB_K;
-    return std::max(1, std::min(512 / tiles, steps / 4));
+    const int tiles = ((H + RB_H - 1) / RB_H) * ((E + RB_C - 1) / RB_C), steps = (T + RB_K - 1) / RB_K;
+    return std::max(1, std::min(512 / tiles, steps / RB_MIN_STEPS));
 }
 struct RouterBwdWs
 {
@@ -332,41 +371,39 @@ int mm_router_backward(const void* x_bf16, int T, int H, const float* gate, int 
                  "mm_router_backward: x, dx and dgate must be 16-byte aligned");
     if (!dx_bf16 && !dgate) return MM_OK;
     const hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
-    if (T == 0)
-    {
-        // no token: a gate gradient of zeros (one empty partial sum per tile)
-        if (dgate)
-            hipLaunchKernelGGL((k_rb_gemm<false>), dim3((H + RB_T - 1) / RB_T, (E + RB_T - 1) / RB_T), dim3(256), 0, hs, nullptr,
-                               nullptr, H, E, 0, 0, 0, nullptr, E, dgate);
-        return check_launch("mm_router_backward");
-    }
-    const RouterBwdWs s = router_bwd_ws(T, H, E);
-    MM_CHECK_ARG(workspace && workspace_bytes >= s.total && ((uintptr_t)workspace & 15) == 0,
+    const int Ek = (E + 31) & ~31, Tk = (T + 31) & ~31, S = T ? rb_splits(T, H, E) : 1;
+    const int nh = (H + RB_H - 1) / RB_H;
+    GemmArgs gx{}, gg{};
+    int dx_blocks = 0, dg_blocks = 0;
+    // without tokens: a gate gradient of zeros (one empty partial sum per tile)
+    const RouterBwdWs s = T ? router_bwd_ws(T, H, E) : RouterBwdWs{};
+    MM_CHECK_ARG(T == 0 || (workspace && workspace_bytes >= s.total && ((uintptr_t)workspace & 15) == 0),
                  "mm_router_backward: workspace too small or misaligned (%zu < %zu)", workspace_bytes, s.total);
     unsigned char* p = static_cast<unsigned char*>(workspace);
-    const int Ek = (E + 31) & ~31, Tk = (T + 31) & ~31, S = rb_splits(T, H, E);
-    uint16_t* d = dx_bf16 ? (uint16_t*)(p + s.d) : nullptr;
-    uint16_t* dt = dgate ? (uint16_t*)(p + s.dt) : nullptr;
-    hipLaunchKernelGGL(k_rb_parts, dim3((E + 63) / 64, (T + 63) / 64), dim3(256), 0, hs, ids, w, dw, dlogits, T, E, k, Ek, Tk, d,
-                       dt);
-    if (dx_bf16)
+    uint16_t *d = (uint16_t*)(p + s.d), *dt = (uint16_t*)(p + s.dt), *gt = (uint16_t*)(p + s.gt);
+    if (dx_bf16 && T)
     {
-        uint16_t* gt = (uint16_t*)(p + s.gt);
-        hipLaunchKernelGGL(k_rb_gate, dim3((H + 63) / 64, (E + 63) / 64), dim3(256), 0, hs, gate, E, H, Ek, gt);
-        hipLaunchKernelGGL((k_rb_gemm<true>), dim3((H + RB_T - 1) / RB_T, (T + RB_T - 1) / RB_T), dim3(256), 0, hs, gt, d, H, T, T,
-                           Ek, Ek / RB_K, gate, E, dx_bf16);
+        gx = { gt, d, gate, dx_bf16, H, T, T, Ek, E, Ek / RB_K };
+        dx_blocks = nh * ((T + RB_C - 1) / RB_C);
     }
     if (dgate)
     {
-        float* part = S > 1 ? (float*)(p + s.part) : dgate;
-        const int steps = Tk / RB_K, per = (steps + S - 1) / S;
-        hipLaunchKernelGGL((k_rb_gemm<false>), dim3((H + RB_T - 1) / RB_T, (E + RB_T - 1) / RB_T, S), dim3(256), 0, hs,
-                           (const uint16_t*)x_bf16, dt, H, E, T, Tk, per, nullptr, E, part);
-        if (S > 1)
-        {
-            const size_t n = (size_t)E * H;
-            hipLaunchKernelGGL(k_rb_sum, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, hs, part, S, n, dgate);
-        }
+        const int steps = Tk / RB_K;
+        gg = { (const uint16_t*)x_bf16, dt, nullptr, S > 1 ? (void*)(p + s.part) : dgate, H, E, T, Tk, E, (steps + S - 1) / S };
+        dg_blocks = nh * ((E + RB_C - 1) / RB_C) * S;
+    }
+    if (T)
+    {
+        const int tiles = (E + 63) / 64 * ((T + 63) / 64), gate_tiles = dx_bf16 ? (H + 63) / 64 * ((E + 63) / 64) : 0;
+        hipLaunchKernelGGL(k_rb_parts, dim3(tiles + gate_tiles), dim3(256), 0, hs, ids, w, dw, dlogits, gate, T, E, H, k, Ek, Tk,
+                           dx_bf16 ? d : nullptr, dgate ? dt : nullptr, gt, tiles);
+    }
+    if (dx_blocks + dg_blocks == 0) return MM_OK;
+    hipLaunchKernelGGL(k_rb_gemm, dim3(dx_blocks + dg_blocks), dim3(256), 0, hs, gx, gg, dx_blocks);
+    if (dgate && S > 1)
+    {
+        const size_t n = (size_t)E * H;
+        hipLaunchKernelGGL(k_rb_sum, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, hs, (const float*)(p + s.part), S, n, dgate);
     }
     return check_launch("mm_router_backward");
 }
