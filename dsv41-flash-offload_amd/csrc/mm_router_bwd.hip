@@ -22,10 +22,13 @@ typedef __bf16 rb_bf8 __attribute__((ext_vector_type(8)));
 typedef short rb_s4 __attribute__((ext_vector_type(4)));
 typedef uint32_t rb_u4 __attribute__((ext_vector_type(4)));
 
-constexpr int RB_H = 128, RB_C = 128, RB_K = 32;
-constexpr int RB_ROW = 32;               // LDS row of a k-contiguous operand: four 16-byte chunks, swizzled
+constexpr int RB_H = 128, RB_C = 128, RB_K = 64;
+// LDS row of a k-contiguous operand: eight 16-byte chunks, chunk q of row r at q ^ (r / 2): the 16 rows of an operand read lie in 16
+// distinct bank groups. Steps of 64 rather than 32 inputs, so that eight lanes read one row's 128 bytes: loads of 64 bytes a row
+// kept the address unit busy for twice as long (16,384 tokens: 384 us a call, 362 now).
+constexpr int RB_ROW = RB_K;
 constexpr int RB_XROW = RB_H + 16;       // LDS row of the token-major input tile (32 bytes of padding: transposed reads of four rows hit distinct banks)
-__device__ __forceinline__ int rb_at(int r, int q) { return r * RB_ROW + 8 * (q ^ ((r >> 2) & 3)); }
+__device__ __forceinline__ int rb_at(int r, int q) { return r * RB_ROW + 8 * (q ^ ((r >> 1) & 7)); }
 
 // v = a + b + c in bf16: a truncated (no overflow), b rounded, c the rest, exact. inf and NaN stay in a.
 __device__ __forceinline__ void split3(float v, uint16_t& a, uint16_t& b, uint16_t& c)
@@ -155,7 +158,7 @@ __device__ __forceinline__ void rb_tile(const GemmArgs& a, uint16_t* lds, int bh
 {
     constexpr int PR = DX ? 2 : 1, PC = DX ? 2 : 3;
     constexpr int RT = RB_H / 32, CT = RB_C / 32;          // 16 x 16 tiles per wave
-    constexpr int RI = PR * RB_H / 64, CI = RB_C / 64;     // 16-byte loads per thread and step: rows (all parts; x: 32 x RB_H), columns (a part)
+    constexpr int RI = PR * RB_H * RB_K / 2048, CI = RB_C * RB_K / 2048;   // 16-byte loads per thread and step: rows (all parts; x: RB_K x RB_H), columns (a part)
     uint16_t* rs = lds;
     uint16_t* cs = lds + (DX ? PR * RB_H * RB_ROW : RB_K * RB_XROW);
     const int H = a.H, C = a.C, K = a.K;
@@ -171,8 +174,8 @@ __device__ __forceinline__ void rb_tile(const GemmArgs& a, uint16_t* lds, int bh
             if constexpr (DX)
             {
                 const int i = tid + 256 * (j / PR), p = j % PR;
-                const size_t r = min(h0 + (i >> 2), H - 1);
-                rv[j] = *reinterpret_cast<const rb_u4*>(a.rows + ((size_t)p * H + r) * K + k0 + 8 * (i & 3));
+                const size_t r = min(h0 + i / (RB_K / 8), H - 1);
+                rv[j] = *reinterpret_cast<const rb_u4*>(a.rows + ((size_t)p * H + r) * K + k0 + 8 * (i % (RB_K / 8)));
             }
             else
             {
@@ -183,10 +186,10 @@ __device__ __forceinline__ void rb_tile(const GemmArgs& a, uint16_t* lds, int bh
         for (int j = 0; j < CI; ++j)
         {
             const int i = tid + 256 * j;
-            const size_t c = min(c0 + (i >> 2), C - 1);
+            const size_t c = min(c0 + i / (RB_K / 8), C - 1);
 #pragma unroll
             for (int p = 0; p < PC; ++p)
-                cv[PC * j + p] = *reinterpret_cast<const rb_u4*>(a.cols + ((size_t)p * C + c) * K + k0 + 8 * (i & 3));
+                cv[PC * j + p] = *reinterpret_cast<const rb_u4*>(a.cols + ((size_t)p * C + c) * K + k0 + 8 * (i % (RB_K / 8)));
         }
     };
     rb_f4 acc[RT][CT];
@@ -203,7 +206,7 @@ __device__ __forceinline__ void rb_tile(const GemmArgs& a, uint16_t* lds, int bh
             if constexpr (DX)
             {
                 const int i = tid + 256 * (j / PR), p = j % PR;
-                *reinterpret_cast<rb_u4*>(&rs[p * RB_H * RB_ROW + rb_at(i >> 2, i & 3)]) = rv[j];
+                *reinterpret_cast<rb_u4*>(&rs[p * RB_H * RB_ROW + rb_at(i / (RB_K / 8), i % (RB_K / 8))]) = rv[j];
             }
             else
             {
@@ -215,47 +218,51 @@ __device__ __forceinline__ void rb_tile(const GemmArgs& a, uint16_t* lds, int bh
         {
             const int i = tid + 256 * j;
 #pragma unroll
-            for (int p = 0; p < PC; ++p) *reinterpret_cast<rb_u4*>(&cs[p * RB_C * RB_ROW + rb_at(i >> 2, i & 3)]) = cv[PC * j + p];
+            for (int p = 0; p < PC; ++p) *reinterpret_cast<rb_u4*>(&cs[p * RB_C * RB_ROW + rb_at(i / (RB_K / 8), i % (RB_K / 8))]) = cv[PC * j + p];
         }
         __syncthreads();
         if (s + 1 < s1) load(s + 1);
         const int r = lane & 15, q = lane >> 4;
-        rb_bf8 R[RT], Cc[CT];
-        auto read_rows = [&](int p) {
 #pragma unroll
-            for (int i = 0; i < RT; ++i)
-                if constexpr (DX) R[i] = *reinterpret_cast<const rb_bf8*>(&rs[p * RB_H * RB_ROW + rb_at(wh + 16 * i + r, q)]);
-                else
-                {
-                    // four tokens x 16 hidden indices per transposed read: lane r of a quarter names token r >> 2 and four
-                    // columns, and gets column r of the four tokens; quarter q's tokens are 8 q .. 8 q + 7
-                    typedef __attribute__((address_space(3))) rb_s4* lds4;
-                    uint16_t* at = &rs[(8 * q + (r >> 2)) * RB_XROW + wh + 16 * i + 4 * (r & 3)];
-                    const rb_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at);
-                    const rb_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 4 * RB_XROW));
-                    R[i] = __builtin_bit_cast(rb_bf8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-                }
-        };
-        auto read_cols = [&](int p) {
-#pragma unroll
-            for (int j = 0; j < CT; ++j)
-                Cc[j] = *reinterpret_cast<const rb_bf8*>(&cs[p * RB_C * RB_ROW + rb_at(wc + 16 * j + r, q)]);
-        };
-        // dx: G1 D2, G1 D1, G2 D1; dgate: x D3, x D2, x D1
-        read_rows(0);
-#pragma unroll
-        for (int p = 0; p < 3; ++p)
+        for (int u = 0; u < RB_K / 32; ++u)
         {
-            if constexpr (DX)
+            rb_bf8 R[RT], Cc[CT];
+            auto read_rows = [&](int p) {
+#pragma unroll
+                for (int i = 0; i < RT; ++i)
+                    if constexpr (DX) R[i] = *reinterpret_cast<const rb_bf8*>(&rs[p * RB_H * RB_ROW + rb_at(wh + 16 * i + r, 4 * u + q)]);
+                    else
+                    {
+                        // four tokens x 16 hidden indices per transposed read: lane r of a quarter names token r >> 2 and four
+                        // columns, and gets column r of the four tokens; quarter q's tokens are 8 q .. 8 q + 7
+                        typedef __attribute__((address_space(3))) rb_s4* lds4;
+                        uint16_t* at = &rs[(32 * u + 8 * q + (r >> 2)) * RB_XROW + wh + 16 * i + 4 * (r & 3)];
+                        const rb_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at);
+                        const rb_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 4 * RB_XROW));
+                        R[i] = __builtin_bit_cast(rb_bf8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                    }
+            };
+            auto read_cols = [&](int p) {
+#pragma unroll
+                for (int j = 0; j < CT; ++j)
+                    Cc[j] = *reinterpret_cast<const rb_bf8*>(&cs[p * RB_C * RB_ROW + rb_at(wc + 16 * j + r, 4 * u + q)]);
+            };
+            // dx: G1 D2, G1 D1, G2 D1; dgate: x D3, x D2, x D1
+            read_rows(0);
+#pragma unroll
+            for (int p = 0; p < 3; ++p)
             {
-                if (p < 2) read_cols(1 - p);
-                else read_rows(1);
+                if constexpr (DX)
+                {
+                    if (p < 2) read_cols(1 - p);
+                    else read_rows(1);
+                }
+                else read_cols(2 - p);
+#pragma unroll
+                for (int i = 0; i < RT; ++i)
+#pragma unroll
+                    for (int j = 0; j < CT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(R[i], Cc[j], acc[i][j], 0, 0, 0);
             }
-            else read_cols(2 - p);
-#pragma unroll
-            for (int i = 0; i < RT; ++i)
-#pragma unroll
-                for (int j = 0; j < CT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(R[i], Cc[j], acc[i][j], 0, 0, 0);
         }
     }
     // lane (column l & 15, group l >> 4) holds hidden indices 4 g .. 4 g + 3 of its column; H is a multiple of 16
@@ -318,8 +325,8 @@ __global__ __launch_bounds__(256) void k_rb_sum(const float* __restrict__ part, 
     *reinterpret_cast<rb_f4*>(out + i) = s;
 }
 
-// Workgroups dgate's tokens are split over: two per CU in all, at least RB_MIN_STEPS steps of 32 tokens each.
-constexpr int RB_MIN_STEPS = 8;
+// Workgroups dgate's tokens are split over: two per CU in all, at least RB_MIN_STEPS steps of RB_K tokens each.
+constexpr int RB_MIN_STEPS = 4;
 static int rb_splits(int T, int H, int E)
 {
     const int tiles = ((H + RB_H - 1) / RB_H) * ((E + RB_C - 1) / RB_C), steps = (T + RB_K - 1) / RB_K;
@@ -334,7 +341,7 @@ static RouterBwdWs router_bwd_ws(int T, int H, int E)
     RouterBwdWs w{};
     size_t at = 0;
     auto take = [&](size_t b) { const size_t o = at; at += (b + 255) & ~(size_t)255; return o; };
-    const size_t Ek = (E + 31) & ~31, Tk = (T + 31) & ~31;
+    const size_t Ek = (E + RB_K - 1) / RB_K * RB_K, Tk = (T + RB_K - 1) / RB_K * RB_K;
     w.d = take(2 * (size_t)T * Ek * 2);
     w.dt = take(3 * (size_t)E * Tk * 2);
     w.gt = take(2 * (size_t)H * Ek * 2);
@@ -371,7 +378,7 @@ int mm_router_backward(const void* x_bf16, int T, int H, const float* gate, int 
                  "mm_router_backward: x, dx and dgate must be 16-byte aligned");
     if (!dx_bf16 && !dgate) return MM_OK;
     const hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
-    const int Ek = (E + 31) & ~31, Tk = (T + 31) & ~31, S = T ? rb_splits(T, H, E) : 1;
+    const int Ek = (E + RB_K - 1) / RB_K * RB_K, Tk = (T + RB_K - 1) / RB_K * RB_K, S = T ? rb_splits(T, H, E) : 1;
     const int nh = (H + RB_H - 1) / RB_H;
     GemmArgs gx{}, gg{};
     int dx_blocks = 0, dg_blocks = 0;
