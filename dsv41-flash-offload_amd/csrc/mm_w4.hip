@@ -516,7 +516,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_w4_linear(LinearArgs a)
 // Routed experts
 // ---------------------------------------------------------------------------------------------------------
 // Up to W4_SELF routes each workgroup finds its record's routes itself: record r exists if route r is the first of its
-// expert, and holds every route of that expert. Records of larger calls come from k_w4_plan. Neither holds more than W4_REC routes.
+// expert, and holds every route of that expert. Records of larger calls come from k_w4_plan or k_w4_records. Neither holds more than W4_REC routes.
 constexpr int W4_SELF = 64, W4_REC = 64;
 struct W4Rec
 {
@@ -614,9 +614,10 @@ __device__ __forceinline__ void down_rows(const ExpertArgs& a, unsigned char* ld
 
 // Weight tiles of a workgroup in the gate/up and the down product of few rows.
 constexpr int W4_GU = 2, W4_DN = 2;
-// Waves per SIMD that they are compiled for: as many as need no scratch memory.
+// Waves per SIMD that they are compiled for: as many as need no scratch memory in the loops of the usual shapes (a few words at two
+// row tiles, which 24 tokens of 64 experts run on 3 % faster than with two waves).
 template <int G, bool ZP, int MT>
-constexpr int W4_OCC = MT == 1 ? (G == 128 && !ZP ? 4 : 3) : 2;
+constexpr int W4_OCC = MT == 1 && G == 128 && !ZP ? 4 : 3;
 
 // Few rows: one workgroup per record and 16 (32) columns, its four waves split K; one or two row tiles by the record's routes, more routes in
 // more passes.
@@ -712,24 +713,64 @@ __global__ __launch_bounds__(256) void k_w4_routes(ExpertArgs a, int64_t* __rest
     if (s < a.n) out[s] = route_expert(a, s);
 }
 
-// Records of at most `rows` routes of one expert, in ascending expert: (expert, first sorted position, routes).
-__global__ __launch_bounds__(1024) void k_w4_plan(const int32_t* __restrict__ counts, const int32_t* __restrict__ offsets, int E,
-                                                  int rows, W4Rec* __restrict__ recs, int32_t* __restrict__ nrec)
+// Where expert e = threadIdx.x (1024 threads) with cnt routes has its first route and its first record of at most `rows` routes;
+// writes its records and, from thread 0, their number. `sums`: LDS of 32 words.
+__device__ __forceinline__ int plan_records(int cnt, int rows, int* sums, W4Rec* __restrict__ recs, int32_t* __restrict__ nrec)
 {
-    __shared__ int sums[16];
     const int e = threadIdx.x, lane = e & 63, wave = e >> 6;
-    const int cnt = e < E ? counts[e] : 0, m = (cnt + rows - 1) / rows;
-    const int incl = wave_incl_scan(m);
-    if (lane == 63) sums[wave] = incl;
+    const int m = (cnt + rows - 1) / rows, ic = wave_incl_scan(cnt), im = wave_incl_scan(m);
+    if (lane == 63)
+    {
+        sums[wave] = ic;
+        sums[16 + wave] = im;
+    }
     __syncthreads();
-    int at = incl - m, all = 0;
+    int first = ic - cnt, at = im - m, all = 0;
     for (int w = 0; w < 16; ++w)
     {
-        if (w < wave) at += sums[w];
-        all += sums[w];
+        if (w < wave)
+        {
+            first += sums[w];
+            at += sums[16 + w];
+        }
+        all += sums[16 + w];
     }
-    for (int i = 0; i < m; ++i) recs[at + i] = { e, offsets[e] + i * rows, min(rows, cnt - i * rows), 0 };
+    for (int i = 0; i < m; ++i) recs[at + i] = { e, first + i * rows, min(rows, cnt - i * rows), 0 };
     if (e == 0) *nrec = all;
+    return first;
+}
+
+// Records and the routes in their order, by one workgroup: count, scan, place. The order of an expert's routes is that of the
+// atomics; no result depends on it (a route's sums do not depend on the row it takes in a tile).
+constexpr int W4_PLAN_ROUTES = 16384;
+__global__ __launch_bounds__(1024) void k_w4_plan(ExpertArgs a, int rows, int32_t* __restrict__ order, W4Rec* __restrict__ recs,
+                                                  int32_t* __restrict__ nrec)
+{
+    __shared__ int sums[32], fill[1024];
+    fill[threadIdx.x] = 0;
+    __syncthreads();
+    for (int s = threadIdx.x; s < a.n; s += 1024)
+    {
+        const int e = route_expert(a, s);
+        if (e >= 0) atomicAdd(&fill[e], 1);
+    }
+    __syncthreads();
+    const int cnt = fill[threadIdx.x];
+    const int first = plan_records(cnt, rows, sums, recs, nrec);
+    fill[threadIdx.x] = first;
+    __syncthreads();
+    for (int s = threadIdx.x; s < a.n; s += 1024)
+    {
+        const int e = route_expert(a, s);
+        if (e >= 0) order[atomicAdd(&fill[e], 1)] = s;
+    }
+}
+// The records alone, for the order that mm_permute gives.
+__global__ __launch_bounds__(1024) void k_w4_records(const int32_t* __restrict__ counts, int E, int rows, W4Rec* __restrict__ recs,
+                                                     int32_t* __restrict__ nrec)
+{
+    __shared__ int sums[32];
+    plan_records((int)threadIdx.x < E ? counts[threadIdx.x] : 0, rows, sums, recs, nrec);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -807,14 +848,17 @@ static ExpertWs expert_ws(int x_dtype, int T, int k, int shared, int E, int H, i
         // rows of a record: of up to 16, 32 or 64 routes by the average of the experts
         w.rows = n > (size_t)32 * E ? 64 : n > (size_t)12 * E ? 32 : 16;
         w.nrecs = (int)(std::min(n, (size_t)E) + n / w.rows);
-        w.ids = take(shared >= 0 ? n * 8 : 0);
-        w.counts = take((E + 1) * 4);
-        w.offsets = take((E + 2) * 4);
         w.order = take(n * 4);
-        w.token = take(n * 4);
         w.recs = take((size_t)w.nrecs * sizeof(W4Rec));
         w.nrec = take(4);
-        w.perm = take(mm_permute_workspace((int)n, E));
+        if (n > W4_PLAN_ROUTES)
+        {
+            w.ids = take(shared >= 0 ? n * 8 : 0);
+            w.counts = take((E + 1) * 4);
+            w.offsets = take((E + 2) * 4);
+            w.token = take(n * 4);
+            w.perm = take(mm_permute_workspace((int)n, E));
+        }
     }
     else w.nrecs = (int)n;
     w.total = at;
@@ -862,29 +906,38 @@ static int experts_launch(const mm_w4_layer_t* L, const void* x, int x_dtype, in
     if (a.n > W4_SELF)
     {
         int32_t* order = (int32_t*)(p + s.order);
-        int32_t* counts = (int32_t*)(p + s.counts);
-        int32_t* offsets = (int32_t*)(p + s.offsets);
-        const int64_t* all = ids;
-        if (shared >= 0)
+        W4Rec* recs = (W4Rec*)(p + s.recs);
+        int32_t* nrec = (int32_t*)(p + s.nrec);
+        if (a.n <= W4_PLAN_ROUTES)
+            hipLaunchKernelGGL(k_w4_plan, dim3(1), dim3(1024), 0, hs, a, s.rows, order, recs, nrec);
+        else
         {
-            hipLaunchKernelGGL(k_w4_routes, dim3((a.n + 255) / 256), dim3(256), 0, hs, a, (int64_t*)(p + s.ids));
-            all = (const int64_t*)(p + s.ids);
+            const int64_t* all = ids;
+            if (shared >= 0)
+            {
+                hipLaunchKernelGGL(k_w4_routes, dim3((a.n + 255) / 256), dim3(256), 0, hs, a, (int64_t*)(p + s.ids));
+                all = (const int64_t*)(p + s.ids);
+            }
+            int32_t* counts = (int32_t*)(p + s.counts);
+            const int rc = permute_launch(all, nullptr, a.n, a.topk, E, counts, (int32_t*)(p + s.offsets), order,
+                                          (int32_t*)(p + s.token), nullptr, nullptr, nullptr, nullptr, p + s.perm,
+                                          mm_permute_workspace(a.n, E), stream);
+            if (rc) return rc;
+            hipLaunchKernelGGL(k_w4_records, dim3(1), dim3(1024), 0, hs, counts, E, s.rows, recs, nrec);
         }
-        const int rc = permute_launch(all, nullptr, a.n, a.topk, E, counts, offsets, order, (int32_t*)(p + s.token), nullptr, nullptr,
-                                      nullptr, nullptr, p + s.perm, mm_permute_workspace(a.n, E), stream);
-        if (rc) return rc;
-        hipLaunchKernelGGL(k_w4_plan, dim3(1), dim3(1024), 0, hs, counts, offsets, E, s.rows, (W4Rec*)(p + s.recs),
-                           (int32_t*)(p + s.nrec));
         a.order = order;
-        a.recs = (const W4Rec*)(p + s.recs);
-        a.nrec = (const int32_t*)(p + s.nrec);
+        a.recs = recs;
+        a.nrec = nrec;
     }
     const bool many = s.rows > 16;
     by_input(x_dtype, [&](auto xt, auto parts) {
         by_group(L->group, L->w13.zeros != nullptr, [&](auto g, auto zp) {
             constexpr int XT = decltype(xt)::value, P = decltype(parts)::value, G = decltype(g)::value;
             constexpr bool ZP = decltype(zp)::value;
-            if (many) hipLaunchKernelGGL((k_w4_gate_up_many<XT, P, G, ZP, 4>), dim3((I + 63) / 64, s.nrecs), dim3(256), 0, hs, a);
+            const dim3 grid((I + 63) / 64, s.nrecs);
+            if (many && P == 3) hipLaunchKernelGGL((k_w4_gate_up_many<XT, P, G, ZP, P == 3 ? 6 : 4>), grid, dim3(256), 0, hs, a);
+            else if (s.rows == 64) hipLaunchKernelGGL((k_w4_gate_up_many<XT, P, G, ZP, P == 3 ? 6 : 4>), grid, dim3(256), 0, hs, a);
+            else if (many) hipLaunchKernelGGL((k_w4_gate_up_many<XT, P, G, ZP, P == 3 ? 6 : 2>), grid, dim3(256), 0, hs, a);
             else if (T <= W4_ROWS<P, 1> || (P == 1 && s.rows <= 16))
                 hipLaunchKernelGGL((k_w4_gate_up<XT, P, G, ZP, 1>), dim3((I + 8 * W4_GU - 1) / (8 * W4_GU), s.nrecs), dim3(256), 0, hs, a);
             else hipLaunchKernelGGL((k_w4_gate_up<XT, P, G, ZP, 2>), dim3((I + 8 * W4_GU - 1) / (8 * W4_GU), s.nrecs), dim3(256), 0, hs, a);
@@ -893,7 +946,7 @@ static int experts_launch(const mm_w4_layer_t* L, const void* x, int x_dtype, in
     by_group(L->group, L->w2.zeros != nullptr, [&](auto g, auto zp) {
         constexpr int G = decltype(g)::value;
         constexpr bool ZP = decltype(zp)::value;
-        if (many) hipLaunchKernelGGL((k_w4_down_many<G, ZP, 4>), dim3((H + 127) / 128, s.nrecs), dim3(256), 0, hs, a);
+        if (many) hipLaunchKernelGGL((k_w4_down_many<G, ZP, 6>), dim3((H + 127) / 128, s.nrecs), dim3(256), 0, hs, a);
         else if (T <= W4_ROWS<3, 1>) hipLaunchKernelGGL((k_w4_down<G, ZP, 1>), dim3((H + 16 * W4_DN - 1) / (16 * W4_DN), s.nrecs), dim3(256), 0, hs, a);
         else hipLaunchKernelGGL((k_w4_down<G, ZP, 2>), dim3((H + 16 * W4_DN - 1) / (16 * W4_DN), s.nrecs), dim3(256), 0, hs, a);
     });

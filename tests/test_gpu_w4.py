@@ -205,7 +205,9 @@ def check_experts(out, a, b, x, ids, w, shared, limit):
     (130, 4, 20, 192, 128, 64, torch.bfloat16, True, 19),
     (200, 3, 5, 256, 128, 128, torch.float16, False, None),
     (300, 8, 9, 128, 256, 128, torch.float32, True, 2),
-    (900, 6, 300, 64, 64, 32, torch.bfloat16, False, None)])
+    (900, 6, 300, 64, 64, 32, torch.bfloat16, False, None),
+    (2400, 7, 30, 64, 64, 64, torch.float32, True, 4),
+    (8300, 2, 12, 64, 32, 32, torch.bfloat16, False, 0)])
 def test_experts(dev, T, k, E, H, I, group, dtype, zeros, shared):
     from mi355moe import moe
     g = torch.Generator().manual_seed(T + E + H)
