@@ -34,43 +34,12 @@ static int balance_chunks(int T)
 }
 
 template <int DT>
-using raw_t = std::conditional_t<DT == MM_DTYPE_F32, float, uint16_t>;
-template <int DT>
-__device__ __forceinline__ float logit_value(raw_t<DT> h)
+__device__ __forceinline__ float load_logit(const void* p, size_t i)
 {
-    if constexpr (DT == MM_DTYPE_F32) return h;
-    else if constexpr (DT == MM_DTYPE_F16) return h2f(h);
-    else return __uint_as_float((uint32_t)h << 16);
-}
-// Rows that a wave has in flight at once. (One row after the other, each a round trip to memory: 12,000 tokens x 160 experts
-// @ONE@ us forward and backward, four at a time @FOUR@.)
-template <int NV>
-constexpr int BL_AT = NV <= 8 ? 4 : 2;
-// Rows r, r + step, ... (those below r1 with their mask set are live) as they are stored; lane's experts lane + 64 v.
-template <int DT, int NV, int AT>
-__device__ __forceinline__ void load_rows(const void* logits, const uint8_t* mask, size_t row0, int r, int step, int r1, int E,
-                                          raw_t<DT> (&raw)[AT][NV], bool (&live)[AT])
-{
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int i = 0; i < AT; ++i) live[i] = false;
-    if (r >= r1) return;                       // no row at all: nothing may be read
-#pragma unroll
-    for (int i = 0; i < AT; ++i)
-    {
-        const int q = min(r + i * step, r1 - 1);
-        live[i] = r + i * step < r1 && (!mask || mask[row0 + q]);
-        const raw_t<DT>* p = reinterpret_cast<const raw_t<DT>*>(logits) + (row0 + q) * E;
-#pragma unroll
-        for (int v = 0; v < NV; ++v) raw[i][v] = p[min(lane + 64 * v, E - 1)];
-    }
-}
-template <int DT, int NV>
-__device__ __forceinline__ void logits_of(const raw_t<DT> (&raw)[NV], int E, float (&l)[NV])
-{
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) l[v] = lane + 64 * v < E ? logit_value<DT>(raw[v]) : -INFINITY;
+    if constexpr (DT == MM_DTYPE_F32) return reinterpret_cast<const float*>(p)[i];
+    const uint16_t h = reinterpret_cast<const uint16_t*>(p)[i];
+    if constexpr (DT == MM_DTYPE_F16) return h2f(h);
+    return __uint_as_float((uint32_t)h << 16);
 }
 template <int DT>
 __device__ __forceinline__ void store_grad(void* p, size_t i, float v)
@@ -163,15 +132,10 @@ __global__ __launch_bounds__(64 * BL_WAVES) void k_balance(BalanceArgs a)
     __shared__ int sc[64 * NV];
     __shared__ int sn[BL_WAVES];
     __shared__ float sl[BL_WAVES];
-    constexpr int AT = BL_AT<NV>;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int b = blockIdx.y, c = blockIdx.x;
     const int r0 = c * a.rows, r1 = min(a.T, r0 + a.rows);
     const size_t row0 = (size_t)b * a.T;
-    // the wave's first rows and the first picks are asked for before anything else
-    raw_t<DT> raw[AT][NV];
-    bool live[AT];
-    load_rows<DT, NV, AT>(a.logits, a.mask, row0, r0 + wave, BL_WAVES, r1, a.E, raw, live);
     if (tid == 0 && c == 0 && a.chunks > 1) a.done[b] = 0;
     for (int e = tid; e < 64 * NV; e += 64 * BL_WAVES) sc[e] = 0;
     __syncthreads();
@@ -186,20 +150,23 @@ __global__ __launch_bounds__(64 * BL_WAVES) void k_balance(BalanceArgs a)
 #pragma unroll
     for (int v = 0; v < NV; ++v) acc[v] = 0.f;
     int n = 0;
-    float l[NV], one[NV];
-    for (int r = r0 + wave; r < r1; r += AT * BL_WAVES)
+    auto load = [&](int r, float (&l)[NV]) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+            l[v] = lane + 64 * v < a.E ? load_logit<DT>(a.logits, (row0 + r) * a.E + lane + 64 * v) : -INFINITY;
+    };
+    float l[NV], nx[NV], one[NV];
+    if (r0 + wave < r1) load(r0 + wave, nx);
+    for (int r = r0 + wave; r < r1; r += BL_WAVES)
     {
-        if (r != r0 + wave) load_rows<DT, NV, AT>(a.logits, a.mask, row0, r, BL_WAVES, r1, a.E, raw, live);
 #pragma unroll
-        for (int i = 0; i < AT; ++i)
-        {
-            if (!live[i]) continue;
-            ++n;
-            logits_of<DT, NV>(raw[i], a.E, l);
-            row_scores<NV, SIG>(l, one);
+        for (int v = 0; v < NV; ++v) l[v] = nx[v];
+        if (r + BL_WAVES < r1) load(r + BL_WAVES, nx);
+        if (a.mask && !a.mask[row0 + r]) continue;
+        ++n;
+        row_scores<NV, SIG>(l, one);
 #pragma unroll
-            for (int v = 0; v < NV; ++v) acc[v] += l[v];
-        }
+        for (int v = 0; v < NV; ++v) acc[v] += l[v];
     }
 #pragma unroll
     for (int v = 0; v < NV; ++v) sp[wave][lane + 64 * v] = acc[v];
@@ -318,37 +285,32 @@ __global__ __launch_bounds__(64 * BL_WAVES) void k_balance_sum(BalanceArgs a)
 
 template <int DT, int NV, bool SIG>
 __global__ __launch_bounds__(64 * BL_BWD_WAVES) void k_balance_bwd(const void* __restrict__ logits, const uint8_t* __restrict__ mask,
-                                                                   int T, int E, int k,
+                                                                   int T, int E, int k, int rows,
                                                                    const int32_t* __restrict__ counts,
                                                                    const int32_t* __restrict__ tokens,
                                                                    const float* __restrict__ dloss, void* __restrict__ dlogits)
 {
-    constexpr int AT = BL_AT<NV>;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int b = blockIdx.y, r = (blockIdx.x * BL_BWD_WAVES + wave) * AT;
+    const int b = blockIdx.y;
+    const int r0 = blockIdx.x * rows, r1 = min(T, r0 + rows);
     const size_t row0 = (size_t)b * T;
-    if (r >= T) return;
-    raw_t<DT> raw[AT][NV];
-    bool live[AT];
-    load_rows<DT, NV, AT>(logits, mask, row0, r, 1, T, E, raw, live);
     float cnt[NV];
 #pragma unroll
     for (int v = 0; v < NV; ++v) cnt[v] = lane + 64 * v < E ? (float)counts[(size_t)b * E + lane + 64 * v] : 0.f;
     const float g = dloss[b] * balance_factor(E, k, tokens[b]);
-#pragma unroll
-    for (int i = 0; i < AT; ++i)
+    for (int r = r0 + wave; r < r1; r += BL_BWD_WAVES)
     {
-        if (r + i >= T) break;
-        const size_t at = (row0 + r + i) * E;
+        const size_t at = (row0 + r) * E;
         float l[NV], one[NV];
-        if (!live[i])
+        if (mask && !mask[row0 + r])
         {
 #pragma unroll
             for (int v = 0; v < NV; ++v)
                 if (lane + 64 * v < E) store_grad<DT>(dlogits, at + lane + 64 * v, 0.f);
             continue;
         }
-        logits_of<DT, NV>(raw[i], E, l);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) l[v] = lane + 64 * v < E ? load_logit<DT>(logits, at + lane + 64 * v) : -INFINITY;
         row_scores<NV, SIG>(l, one);
         float dot = 0.f;
 #pragma unroll
@@ -468,11 +430,11 @@ int mm_balance_loss_backward(const float* dloss, const void* logits, int dtype, 
     if (rc) return rc;
     if (B == 0 || T == 0) return MM_OK;
     MM_CHECK_ARG(dloss && logits && counts && tokens && dlogits, "mm_balance_loss_backward: null pointer");
+    const int rows = 4 * BL_BWD_WAVES;
     const hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
     balance_dispatch(dtype, E, score, [&](auto dt, auto nv, auto sig) {
         hipLaunchKernelGGL((k_balance_bwd<decltype(dt)::value, decltype(nv)::value, decltype(sig)::value>),
-                           dim3((unsigned)((T + BL_BWD_WAVES * BL_AT<decltype(nv)::value> - 1) / (BL_BWD_WAVES * BL_AT<decltype(nv)::value>)), B),
-                           dim3(64 * BL_BWD_WAVES), 0, hs, logits, mask, T, E, k, counts,
+                           dim3((T + rows - 1) / rows, B), dim3(64 * BL_BWD_WAVES), 0, hs, logits, mask, T, E, k, rows, counts,
                            tokens, dloss, dlogits);
     });
     return check_launch("mm_balance_loss_backward");
