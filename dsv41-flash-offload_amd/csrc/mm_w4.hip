@@ -444,6 +444,37 @@ __device__ __forceinline__ float tile_value(const unsigned char* sums, int cnt, 
     return s;
 }
 
+// One output from whole weights, input by input: x (16 + q) and x (16 + z) of an infinite input, or of one near fp32's largest, do not
+// cancel, so outputs that the tiles leave infinite or NaN are summed again as the formula has them. x: a row's first part; w: the
+// row of W.
+template <int XT, int P>
+__device__ __forceinline__ float whole_value(const uint16_t* x, const W4Ptr& w, int K, int G, bool sbf)
+{
+    float y = 0.f;
+#pragma unroll 1
+    for (int j = 0; j < K / 8; ++j)
+    {
+        const int g = 8 * j / G;
+        const uint32_t q = w.q[j];
+        const float s = sbf ? __uint_as_float((uint32_t)w.s[g] << 16) : h2f(w.s[g]);
+        const int z = w.z ? w.z[g] : 8;
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i)
+        {
+            float v;
+            if constexpr (P == 3)
+            {
+                const uint16_t* at = x + 8 * j + weight_place(i);
+                v = __uint_as_float((uint32_t)at[2 * K] << 16) + __uint_as_float((uint32_t)at[K] << 16) + __uint_as_float((uint32_t)at[0] << 16);
+            }
+            else v = XT == MM_DTYPE_F16 ? h2f(x[8 * j + i]) : __uint_as_float((uint32_t)x[8 * j + i] << 16);
+            y = fmaf(v, (float)((int)((q >> (4 * i)) & 15u) - z) * s, y);
+        }
+    }
+    return y;
+}
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
+
 template <int OT>
 __device__ __forceinline__ void store_out(void* y, size_t i, float v)
 {
@@ -508,7 +539,10 @@ __global__ __launch_bounds__(64 * NW, 2) void k_w4_linear(LinearArgs a)
     for (int o = OWN ? threadIdx.x : threadIdx.x & 63; o < cnt * 16 * NT; o += OWN ? 64 * NW : 64)
     {
         const int m = o / (16 * NT), c = o % (16 * NT);
-        if (n0 + c < a.N) store_out(a.out, a.y, (size_t)(m0 + m) * a.N + n0 + c, tile_value<P, NT>(sums, cnt, m, c >> 4, c & 15));
+        if (n0 + c >= a.N) continue;
+        float v = tile_value<P, NT>(sums, cnt, m, c >> 4, c & 15);
+        if (!finite(v)) v = whole_value<XT, P>(a.x + (size_t)(m0 + m) * P * a.K, w4_at(a.w, n0 + c, a.K, G), a.K, G, a.sbf);
+        store_out(a.out, a.y, (size_t)(m0 + m) * a.N + n0 + c, v);
     }
 }
 
@@ -520,7 +554,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_w4_linear(LinearArgs a)
 constexpr int W4_SELF = 64, W4_REC = 64;
 struct W4Rec
 {
-    int expert, start, count, pad;
+    int expert, start, count, all;      // all: routes of the expert, in all its records
 };
 
 struct ExpertArgs
@@ -535,7 +569,7 @@ struct ExpertArgs
     const int32_t* nrec;
     uint16_t* h;               // [n][3][I] parts in weight order
     float* y;                  // [n][H]
-    int T, n, k, topk, E, H, I, sbf;   // n = T topk routes, topk = k, and one more with a shared expert
+    int T, n, k, topk, E, H, I, group, sbf;   // n = T topk routes, topk = k, and one more with a shared expert
     int shared;
     float limit;
 };
@@ -549,8 +583,9 @@ __device__ __forceinline__ int route_expert(const ExpertArgs& a, int s)
     return e >= 0 && e < a.E ? (int)e : -1;
 }
 
-// Routes of this workgroup's record into `rows` (LDS); returns their number, 0 for no record.
-__device__ __forceinline__ int record_rows(const ExpertArgs& a, int rec, int* rows, int& expert)
+// Routes of this workgroup's record into `rows` (LDS); returns their number, 0 for no record. `all`: those of the expert, by which
+// kernels choose how to sum (the routes of a record come in no fixed order, so their number may not).
+__device__ __forceinline__ int record_rows(const ExpertArgs& a, int rec, int* rows, int& expert, int& all)
 {
     if (!a.order)
     {
@@ -561,13 +596,26 @@ __device__ __forceinline__ int record_rows(const ExpertArgs& a, int rec, int* ro
         const uint64_t m = __ballot(ei == expert);
         if ((int)__ffsll((unsigned long long)m) - 1 != rec) return 0;
         if (threadIdx.x < 64 && ei == expert) rows[__popcll(m & ((1ull << lane) - 1))] = lane;
-        return __popcll(m);
+        return all = __popcll(m);
     }
     if (rec >= *a.nrec) return 0;
     const W4Rec q = a.recs[rec];
     expert = __builtin_amdgcn_readfirstlane(q.expert);
+    all = __builtin_amdgcn_readfirstlane(q.all);
     if ((int)threadIdx.x < q.count) rows[threadIdx.x] = a.order[q.start + threadIdx.x];
     return __builtin_amdgcn_readfirstlane(q.count);
+}
+
+// mm_moe_decode's activation and clamp; a clamp that keeps NaN.
+__device__ __forceinline__ float swiglu(float g, float u, float limit)
+{
+    float x = g / (1.0f + expf(-g));
+    if (limit != 0.0f)
+    {
+        u = u < -limit ? -limit : u > limit ? limit : u;
+        x = x > limit ? limit : x;
+    }
+    return x * u;
 }
 
 // Gate and up of 8 NT columns (OWN: a workgroup's, else a wave's; weight tile 2 i is gate, 2 i + 1 up) for some of a record's
@@ -586,9 +634,18 @@ __device__ __forceinline__ void gate_up_rows(const ExpertArgs& a, unsigned char*
     {
         const int m = o / COLS, col = o % COLS, t = 2 * (col >> 4);
         if (n0 + col >= a.I) continue;
+        float gate = tile_value<P, NT>(sums, c, m, t, col & 15), up = tile_value<P, NT>(sums, c, m, t + 1, col & 15);
+        if (!(finite(gate) && finite(up)))
+#pragma unroll 1
+            for (int i = 0; i < 2; ++i)                         // (a loop: one copy of it leaves the registers to the products)
+            {
+                float& v = i ? up : gate;
+                if (!finite(v))
+                    v = whole_value<XT, P>(a.x + (size_t)(rows[m] / a.topk) * P * a.H,
+                                           w4_at(a.w13, ((size_t)expert * 2 + i) * a.I + n0 + col, a.H, G), a.H, G, a.sbf);
+            }
         uint16_t p[3];
-        three_parts(act_gu(tile_value<P, NT>(sums, c, m, t, col & 15), tile_value<P, NT>(sums, c, m, t + 1, col & 15), a.limit), p[0],
-                    p[1], p[2]);
+        three_parts(swiglu(gate, up, a.limit), p[0], p[1], p[2]);
         uint16_t* h = a.h + (size_t)rows[m] * 3 * a.I + n0 + (col & ~7) + weight_place(col & 7);
 #pragma unroll
         for (int q = 0; q < 3; ++q) h[q * a.I] = p[q];
@@ -626,12 +683,12 @@ __global__ __launch_bounds__(256, (W4_OCC<G, ZP, MT>)) void k_w4_gate_up(ExpertA
 {
     __shared__ __align__(16) unsigned char lds[W4Wave<XT, P == 3, G, ZP, MT, W4_GU, 4, true>::LDS];
     __shared__ int rows[W4_REC];
-    int expert;
-    const int cnt = record_rows(a, blockIdx.y, rows, expert);
+    int expert, all;
+    const int cnt = record_rows(a, blockIdx.y, rows, expert, all);
     if (cnt == 0) return;
     __syncthreads();
     if constexpr (MT > 1)
-        if (cnt <= W4_ROWS<P, 1>) return gate_up_rows<XT, P, G, ZP, 1, W4_GU, 4, true>(a, lds, expert, rows, cnt);
+        if (all <= W4_ROWS<P, 1>) return gate_up_rows<XT, P, G, ZP, 1, W4_GU, 4, true>(a, lds, expert, rows, cnt);
     for (int m = 0; m < cnt; m += W4_ROWS<P, MT>)
     {
         if (m) __syncthreads();                        // the previous rows' sums are read
@@ -643,12 +700,12 @@ __global__ __launch_bounds__(256, (W4_OCC<G, ZP, MT>)) void k_w4_down(ExpertArgs
 {
     __shared__ __align__(16) unsigned char lds[W4Wave<MM_DTYPE_BF16, true, G, ZP, MT, W4_DN, 4, true>::LDS];
     __shared__ int rows[W4_REC];
-    int expert;
-    const int cnt = record_rows(a, blockIdx.y, rows, expert);
+    int expert, all;
+    const int cnt = record_rows(a, blockIdx.y, rows, expert, all);
     if (cnt == 0) return;
     __syncthreads();
     if constexpr (MT > 1)
-        if (cnt <= W4_ROWS<3, 1>) return down_rows<G, ZP, 1, W4_DN, 4, true>(a, lds, expert, rows, cnt);
+        if (all <= W4_ROWS<3, 1>) return down_rows<G, ZP, 1, W4_DN, 4, true>(a, lds, expert, rows, cnt);
     for (int m = 0; m < cnt; m += W4_ROWS<3, MT>)
     {
         if (m) __syncthreads();
@@ -662,8 +719,8 @@ __global__ __launch_bounds__(256, 2) void k_w4_gate_up_many(ExpertArgs a)
 {
     __shared__ __align__(16) unsigned char lds[W4Wave<XT, P == 3, G, ZP, MT, 2, 4, false>::LDS];
     __shared__ int rows[W4_REC];
-    int expert;
-    const int cnt = record_rows(a, blockIdx.y, rows, expert);
+    int expert, all;
+    const int cnt = record_rows(a, blockIdx.y, rows, expert, all);
     if (cnt == 0) return;
     __syncthreads();
     for (int m = 0; m < cnt; m += W4_ROWS<P, MT>)
@@ -677,8 +734,8 @@ __global__ __launch_bounds__(256, 2) void k_w4_down_many(ExpertArgs a)
 {
     __shared__ __align__(16) unsigned char lds[W4Wave<MM_DTYPE_BF16, true, G, ZP, MT, 2, 4, false>::LDS];
     __shared__ int rows[W4_REC];
-    int expert;
-    const int cnt = record_rows(a, blockIdx.y, rows, expert);
+    int expert, all;
+    const int cnt = record_rows(a, blockIdx.y, rows, expert, all);
     if (cnt == 0) return;
     __syncthreads();
     for (int m = 0; m < cnt; m += W4_ROWS<3, MT>)
@@ -688,7 +745,8 @@ __global__ __launch_bounds__(256, 2) void k_w4_down_many(ExpertArgs a)
     }
 }
 
-// Weighted sum of a token's routes in ascending j, fp32 fma; four columns a thread.
+// Weighted sum of a token's routes in ascending j, fp32 fma; four columns a thread. (The down product's infinite and NaN outputs are
+// summed again here rather than in its own kernels, whose registers are full.)
 __global__ __launch_bounds__(256) void k_w4_combine(ExpertArgs a)
 {
     const int t = blockIdx.y, h = (blockIdx.x * 256 + threadIdx.x) * 4;
@@ -697,9 +755,16 @@ __global__ __launch_bounds__(256) void k_w4_combine(ExpertArgs a)
     for (int j = 0; j < a.topk; ++j)
     {
         const int r = t * a.topk + j;
-        if (route_expert(a, r) < 0) continue;
+        const int e = route_expert(a, r);
+        if (e < 0) continue;
         const float w = j == a.k ? 1.f : a.w[(size_t)t * a.k + j];
-        const f4_t y = *reinterpret_cast<const f4_t*>(a.y + (size_t)r * a.H + h);
+        f4_t y = *reinterpret_cast<const f4_t*>(a.y + (size_t)r * a.H + h);
+        if (!(finite(y.x) && finite(y.y) && finite(y.z) && finite(y.w)))
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (!finite(y[i]))
+                    y[i] = whole_value<MM_DTYPE_BF16, 3>(a.h + (size_t)r * 3 * a.I, w4_at(a.w2, (size_t)e * a.H + h + i, a.I, a.group), a.I,
+                                                         a.group, a.sbf);
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[i] = fmaf(w, y[i], s[i]);
     }
@@ -735,13 +800,13 @@ __device__ __forceinline__ int plan_records(int cnt, int rows, int* sums, W4Rec*
         }
         all += sums[16 + w];
     }
-    for (int i = 0; i < m; ++i) recs[at + i] = { e, first + i * rows, min(rows, cnt - i * rows), 0 };
+    for (int i = 0; i < m; ++i) recs[at + i] = { e, first + i * rows, min(rows, cnt - i * rows), cnt };
     if (e == 0) *nrec = all;
     return first;
 }
 
 // Records and the routes in their order, by one workgroup: count, scan, place. The order of an expert's routes is that of the
-// atomics; no result depends on it (a route's sums do not depend on the row it takes in a tile).
+// atomics; no result depends on it (a route's sums depend neither on the row it takes in a tile nor on its record).
 constexpr int W4_PLAN_ROUTES = 16384;
 __global__ __launch_bounds__(1024) void k_w4_plan(ExpertArgs a, int rows, int32_t* __restrict__ order, W4Rec* __restrict__ recs,
                                                   int32_t* __restrict__ nrec)
@@ -817,12 +882,12 @@ static void parts_launch(const void* x, size_t rows, int K, void* out, hipStream
     hipLaunchKernelGGL(k_w4_parts, dim3((unsigned)((n8 + 255) / 256)), dim3(256), 0, hs, (const float*)x, n8, K / 8, (uint16_t*)out);
 }
 
-// A call of many tokens runs in chunks: byte offsets into the inputs and the down inputs fit 31 bits, and a chunk's workspace
-// serves the next.
+// A call of many tokens runs in chunks: byte offsets into the inputs and the down inputs fit 31 bits, the records one dimension of a
+// grid, and a chunk's workspace serves the next.
 static int expert_chunk(int T, int topk, int H, int I)
 {
     const size_t most = ((size_t)1 << 31) - 1;
-    const size_t t = std::min(most / (6 * (size_t)H), most / (6 * (size_t)I * topk));
+    const size_t t = std::min({ most / (6 * (size_t)H), most / (6 * (size_t)I * topk), ((size_t)1 << 21) / topk });
     return (int)std::min((size_t)T, std::min(t, (size_t)8192));
 }
 
@@ -901,6 +966,7 @@ static int experts_launch(const mm_w4_layer_t* L, const void* x, int x_dtype, in
     a.E = E;
     a.H = H;
     a.I = I;
+    a.group = L->group;
     a.sbf = L->scale_dtype == MM_DTYPE_BF16;
     a.limit = L->limit;
     if (a.n > W4_SELF)
@@ -974,7 +1040,7 @@ int mm_w4_linear(const void* x, int x_dtype, int M, int K, int N, const mm_w4_t*
                  M, K, N);
     MM_CHECK_ARG(x_dtype >= MM_DTYPE_F16 && x_dtype <= MM_DTYPE_F32 && y_dtype >= MM_DTYPE_F16 && y_dtype <= MM_DTYPE_F32,
                  "mm_w4_linear: bad element type");
-    MM_CHECK_ARG(K < (1 << 22), "mm_w4_linear: K must be below 2^22 (%d)", K);
+    MM_CHECK_ARG(K < (1 << 22) && N <= (1 << 30), "mm_w4_linear: K must be below 2^22 and N at most 2^30 (K=%d N=%d)", K, N);
     MM_CHECK_ARG(M <= (1 << 20), "mm_w4_linear: more than 2^20 rows (%d)", M);
     if (M == 0) return MM_OK;
     MM_CHECK_ARG(x && y && ((uintptr_t)x & 15) == 0, "mm_w4_linear: null or misaligned input (16 bytes)");

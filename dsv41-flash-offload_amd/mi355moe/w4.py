@@ -3,8 +3,9 @@
 Tensors are taken as 4-bit checkpoints store them, and read in place:
   q       int32 [N, K / 8]        weight k = 8 j + i of a row in bits 4 i .. 4 i + 3 of its word j
   scales  fp16 or bf16 [N, K / G] G = 32, 64 or 128 inputs per group
-  zeros   uint8 [N, K / G] or None (8): weight = (q - zero) * scale
-Products are exact, sums fp32. moe.moe_forward takes a W4Store as it takes an ExpertStore.
+  zeros   uint8 [N, K / G], 0 to 16, or None (8): weight = (q - zero) * scale
+Products are exact, sums fp32. For serving: nothing here records itself in autograd. moe.moe_forward takes a W4Store as it takes
+an ExpertStore.
 """
 import ctypes
 

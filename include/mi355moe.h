@@ -269,8 +269,8 @@ int mm_fat_batched(const mm_layer_t* layer, const void* x, int x_dtype, int T, i
 /* ------------------------------------------------------------------------------------ 4-bit weights */
 
 /* A matrix [N][K] of 4-bit weights with group scales, in the storage of the checkpoints: w[n][k] = (q - z) s with q = bits
- * 4 (k % 8) .. + 3 of q[n][k / 8], s = scales[n][k / group] (fp16 or bf16) and z = zeros[n][k / group] (NULL: 8). group is
- * 32, 64 or 128 and divides K. q is 16-byte aligned; rows are contiguous. */
+ * 4 (k % 8) .. + 3 of q[n][k / 8], s = scales[n][k / group] (fp16 or bf16) and z = zeros[n][k / group] (4-bit zero points, 0
+ * .. 16; NULL: 8). group is 32, 64 or 128 and divides K. q is 16-byte aligned; rows are contiguous. */
 typedef struct mm_w4
 {
     const int32_t* q;           /* [N][K / 8] */
@@ -278,9 +278,9 @@ typedef struct mm_w4
     const uint8_t* zeros;       /* [N][K / group] or NULL */
 } mm_w4_t;
 
-/* y [M][N] (y_dtype) = x [M][K] (x_dtype) W^T. Products are exact, sums fp32, the result is rounded once. x 16-byte
- * aligned. Built for few rows (decode steps); any M works, at 64 rows per pass over the weights. Workspace:
- * mm_w4_linear_workspace bytes (fp32 inputs only), 16-byte aligned. */
+/* y [M][N] (y_dtype) = x [M][K] (x_dtype) W^T. Products are exact, sums fp32, the result is rounded once. x 16-byte aligned.
+ * Built for few rows (decode steps); any M up to 2^20 works, at 64 rows (21 of fp32) per pass over the weights. K < 2^22, N <=
+ * 2^30. Workspace: mm_w4_linear_workspace bytes (fp32 inputs only), 16-byte aligned. */
 size_t mm_w4_linear_workspace(int x_dtype, int M, int K);
 int mm_w4_linear(const void* x, int x_dtype, int M, int K, int N, const mm_w4_t* W, int group, int scale_dtype, void* y,
                  int y_dtype, void* workspace, size_t workspace_bytes, mm_stream_t stream);
@@ -296,10 +296,10 @@ typedef struct mm_w4_layer
 
 /* One MoE layer on 4-bit experts: out fp32 [T][H] = sum_j w[t,j] * expert_{ids[t,j]}(x_t) in ascending j (fp32 fma), ids
  * int64 [T*topk] (outside [0, E): contributes nothing), expert(x) = W2 (act(Wg x) * Wu x) with mm_moe_decode's activation and
- * clamp, nothing rounded below fp32 between x and out. shared >= 0 names an expert that every token is routed to besides, with
- * weight 1, added last (-1: none). The weights of an expert are read once per 16, 32 or 64 of its routes. No host
- * synchronisation. E <= 1024, H and I multiples of the group; x and out 16-byte aligned. Workspace: mm_w4_moe_workspace
- * bytes, 16-byte aligned (topk without the shared expert). */
+ * clamp, nothing rounded below fp32 between x and out. shared >= 0 names an expert that every token is routed to besides, with weight 1,
+ * added last (-1: none). The result of a token does not depend on the other tokens' order. An expert's weights are read once per 16 to 64 of its routes; a call of many tokens runs in
+ * chunks of at most 8,192. No host synchronisation. E <= 1024, topk <= 1024, H and I multiples of the group, H I < 2^31; x and
+ * out 16-byte aligned. Workspace: mm_w4_moe_workspace bytes (topk without the shared expert), 16-byte aligned. */
 size_t mm_w4_moe_workspace(int x_dtype, int T, int topk, int shared, int E, int H, int I);
 int mm_w4_moe(const mm_w4_layer_t* layer, const void* x, int x_dtype, int T, int topk, const int64_t* ids, const float* w,
               int shared, float* out, void* workspace, size_t workspace_bytes, mm_stream_t stream);

@@ -306,3 +306,67 @@ def test_router_and_experts_in_a_graph(dev):
         y = moe.moe_forward(store, new, want[0], want[1], shared_expert=1, stream=side)
         side.synchronize()
         assert torch.equal(y, want[2])
+
+
+# ------------------------------------------------------------------------------------------ odd values, equal rows
+
+def alike(got, ref, tol):
+    """Same infinities and NaN, the rest within tol."""
+    got = got.cpu().double()
+    assert torch.equal(got.isnan(), ref.isnan()) and torch.equal(got == torch.inf, ref == torch.inf)
+    assert torch.equal(got == -torch.inf, ref == -torch.inf)
+    ok = ref.isfinite()
+    within(got[ok], ref[ok], tol[ok])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("M", [1, 20, 70])
+def test_linear_an_infinite_or_largest_input_gives_what_the_formula_gives(dev, M, dtype):
+    """One infinite input: +-inf by the weight's sign, NaN where the weight is zero; one input of fp32's largest: finite. Outputs summed
+    again have K roundings of 2^-24 of sum |x w|, less than the tolerance of the others (|q - z| <= 15, against 32 + q + z)."""
+    from mi355moe import w4
+    g = torch.Generator().manual_seed(M)
+    q, s, z = weights(g, 150, 256, 64, True)
+    x = torch.randn((M, 256), generator=g).to(dtype)
+    x[0, 77] = -torch.inf
+    if M > 1:
+        x[M - 1, 200] = torch.finfo(dtype).max
+    y = w4.linear(x.to(dev), w4.W4Matrix(*to(dev, (q, s, z))), out_dtype=torch.float32)
+    w, m = dense64(q, s, z)
+    ref = torch.stack([(x[i].double() * w).sum(1) for i in range(M)])
+    alike(y, ref, 84 * 2.0 ** -23 * (x.double().abs() @ m.t()) + HALF[torch.float32] * ref.abs())
+
+
+@pytest.mark.parametrize("T,k,E", [(3, 2, 6), (40, 2, 6), (90, 3, 6)])
+def test_experts_odd_tokens_stay_alone(dev, T, k, E):
+    """A token with NaN gives NaN (no clamp hides it); the others are as without it."""
+    from mi355moe import moe
+    g = torch.Generator().manual_seed(T)
+    store, a, b = make_store(g, E, 128, 64, 64, True, dev, limit=2.0)
+    x = torch.randn((T, 128), generator=g).bfloat16()
+    ids = torch.stack([torch.randperm(E, generator=g)[:k] for _ in range(T)])
+    w = torch.rand((T, k), generator=g) + 0.1
+    plain = moe.moe_forward(store, x.to(dev), ids.to(dev), w.to(dev))
+    y = x.clone()
+    y[0, 5] = float("nan")
+    out = moe.moe_forward(store, y.to(dev), ids.to(dev), w.to(dev))
+    assert out[0].isnan().all() and torch.equal(out[1:], plain[1:])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("T,E,most", [(80, 16, 17), (80, 16, 33), (200, 20, 40), (190, 20, 65), (700, 20, 130)])
+def test_experts_equal_tokens_get_equal_results(dev, T, E, most, group, dtype):
+    """Tokens that are equal and go to one expert get the same bits, in whichever row and record they come: the order of an expert's
+    routes is not fixed, the results are."""
+    from mi355moe import moe
+    g = torch.Generator().manual_seed(T + most)
+    store, a, b = make_store(g, E, 256, 128, group, True, dev)
+    x = torch.randn((T, 256), generator=g).to(dtype)
+    x[:most] = x[0]
+    ids = torch.randint(1, E, (T, 1), generator=g)
+    ids[:most] = 0
+    w = torch.ones((T, 1))
+    out = moe.moe_forward(store, x.to(dev), ids.to(dev), w.to(dev))
+    assert torch.equal(out[:most], out[:1].expand(most, -1))
+    check_experts(out, a, b, x, ids, w, None, 10.0)
