@@ -165,6 +165,8 @@ def on(device, stream=None):
     import torch
     if stream is None and torch._C._cuda_getDevice() == device.index:
         return _HERE_NOW
+    if stream is not None and stream.device != device:
+        raise ValueError(f"mi355moe: stream of {stream.device} for tensors on {device}")
     return _entered(device, stream)
 
 

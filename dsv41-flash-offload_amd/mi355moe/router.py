@@ -15,6 +15,29 @@ _SCORES = {"softmax": 0, "sigmoid": 1}        # MM_SCORE_*
 _p = _lib.ptr
 
 
+def _captured_apply(what, fn, leaves, *args):
+    """fn.apply(*args). Under stream capture, a leaf among its inputs may not have its gradient node in an autograd graph from before
+    the capture: the captured backward would go to that node's stream, which invalidates the capture and ends the process."""
+    leaves = [t for t in leaves if t.requires_grad and t.is_leaf]
+    if not (leaves and torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing()):
+        return fn.apply(*args)
+
+    def notes(t):
+        return torch.autograd.graph.get_gradient_edge(t).node.metadata
+
+    for t in leaves:
+        if notes(t).get("mi355moe") == "captured":            # used in this capture by an earlier call
+            continue
+        notes(t)["mi355moe"] = "seen"                         # gone with the node if no graph holds it
+        if notes(t).pop("mi355moe", None):
+            raise RuntimeError(f"{what}: an input has an autograd graph from before the stream capture; drop it first, or capture "
+                               f"{what}_forward and {what}_backward")
+    out = fn.apply(*args)
+    for t in leaves:
+        notes(t)["mi355moe"] = "captured"
+    return out
+
+
 # ------------------------------------------------------------------------------------------ router top-k
 
 def _check_router(what, x, gate):
@@ -91,8 +114,9 @@ class _TopK(torch.autograd.Function):
 
 
 def topk(x, gate, k):
-    """topk_forward on the current stream, with gradients of w and logits into x and gate."""
-    return _TopK.apply(x, gate, k)
+    """topk_forward on the current stream, with gradients of w and logits into x and gate. Under stream capture an input must not
+    have an autograd graph from before the capture (refused)."""
+    return _captured_apply("topk", _TopK, (x, gate), x, gate, k)
 
 
 # ------------------------------------------------------------------------------------------ load balance
@@ -183,5 +207,5 @@ class _BalanceLoss(torch.autograd.Function):
 
 def balance_loss(logits, ids, mask=None, score="softmax"):
     """(loss, counts) of balance_loss_forward on the current stream, with the gradient of the loss into the logits (the counts
-    are constants of it)."""
-    return _BalanceLoss.apply(logits, ids, mask, score)
+    are constants of it); under stream capture as topk."""
+    return _captured_apply("balance_loss", _BalanceLoss, (logits,), logits, ids, mask, score)

@@ -399,3 +399,37 @@ def test_router_step_in_a_graph_and_on_another_stream(dev):
     want = step(*new)
     for a, b in zip((ids, loss, counts, d, dx, dg), want):
         assert torch.equal(a, b)
+
+
+def test_router_step_captured_through_autograd(dev):
+    """topk and balance_loss with their backward passes captured (no eager graph of the leaves alive), replayed with new inputs."""
+    from mi355moe import router
+    T, H, E, k = 120, 256, 32, 4
+    x, gate, _, _, dw, _ = router_inputs(T, H, E, k, 7, dev)
+    x, gate = x.clone().requires_grad_(), gate.clone().requires_grad_()
+
+    def step():
+        ids, w, logits = router.topk(x, gate, k)
+        loss, _ = router.balance_loss(logits, ids)
+        return torch.autograd.grad([w, loss], [x, gate], [dw, torch.ones_like(loss)])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for seed in (8, 9, 10):
+        nx, ng, _, _, nd, _ = router_inputs(T, H, E, k, seed, dev)
+        with torch.no_grad():
+            x.copy_(nx)
+            gate.copy_(ng)
+            dw.copy_(nd)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b)

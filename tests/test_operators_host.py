@@ -117,3 +117,41 @@ def test_c_argument_errors():
         err(L.mm_w4_moe(*a), text)
     for bad in (_lib.MMW4Layer(W, W, 8, 256, 100, 64, 0, 10.0), _lib.MMW4Layer(W, W, 1025, 256, 128, 64, 0, 10.0)):
         err(L.mm_w4_moe(ctypes.byref(bad), *mo[1:]), b"multiples of the group")
+
+
+def test_a_capture_beside_an_eager_autograd_graph_is_refused(monkeypatch):
+    """As seen under stream capture: a leaf that an earlier autograd graph holds is refused, one that only calls of this capture hold is
+    not."""
+    from mi355moe import router
+
+    class Double(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, t):
+            return 2 * t
+
+        @staticmethod
+        def backward(ctx, d):
+            return 2 * d
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    t = torch.ones(3, requires_grad=True)
+    eager = t.sum()
+    with pytest.raises(RuntimeError, match="capture topk_forward and topk_backward"):
+        router._captured_apply("topk", Double, (t,), t)
+    del eager
+    a = router._captured_apply("topk", Double, (t,), t)
+    b = router._captured_apply("topk", Double, (t,), t)
+    (a + b).sum().backward()
+    assert torch.equal(t.grad, torch.full((3,), 4.0))
+    with torch.no_grad():
+        assert not router._captured_apply("topk", Double, (t,), t).requires_grad
+
+
+def test_a_stream_of_another_device_is_refused():
+    from mi355moe import _lib
+
+    class Stream:
+        device = torch.device("cuda", 1)
+
+    with pytest.raises(ValueError, match="stream of cuda:1"):
+        _lib.on(torch.device("cuda", 0), Stream())
