@@ -167,12 +167,10 @@ struct W4Wave
     using scales_t = few_t<2 * NG>;
     using zeros_t = few_t<NG>;
 
-    // weights of the next AHEAD blocks and inputs of the next one in registers (loads return in order: a block's inputs are asked for
-    // before the weights that come after them)
-    static constexpr int AHEAD = 1;
-    u4_t xv[XI], wv[AHEAD][NT];
-    scales_t sv[AHEAD][NT], sc[NT];
-    zeros_t zv[AHEAD][NT], zc[NT];
+    // the next block, on its way
+    u4_t xv[XI], wv[NT];
+    scales_t sv[NT], sc[NT];
+    zeros_t zv[NT], zc[NT];
     // x and W through buffer descriptors: one register of byte offset a load, the block's place in a scalar, and what the last block
     // reads past a row is the next row, or zero past the end
     __amdgpu_buffer_rsrc_t xb, qb;
@@ -185,7 +183,7 @@ struct W4Wave
     template <typename Row, typename Col>
     __device__ __forceinline__ void init(const uint16_t* x, uint32_t xbytes, Row row, int rows, const W4Ptr& w, int wrows, Col col, int K)
     {
-        const int t = OWN ? threadIdx.x & 63 : threadIdx.x, lane = threadIdx.x & 63;
+        const int t = threadIdx.x % (OWN ? 64 : 64 * NW), lane = threadIdx.x & 63;
         xb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(x), (short)0, (int)xbytes, 0x00020000);
         qb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint32_t*>(w.q), (short)0, (int)((uint32_t)wrows * (K / 2)), 0x00020000);
         sb = reinterpret_cast<const unsigned char*>(w.s);
@@ -201,17 +199,17 @@ struct W4Wave
         }
     }
 
-    __device__ __forceinline__ void load_w(int b, int K, int at)
+    __device__ __forceinline__ void load_w(int b, int K)
     {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) wv[at][nt] = __builtin_amdgcn_raw_buffer_load_b128(qb, qo[nt], 64 * b, 0);
+        for (int nt = 0; nt < NT; ++nt) wv[nt] = __builtin_amdgcn_raw_buffer_load_b128(qb, qo[nt], 64 * b, 0);
         if (G == 128 || 128 * b + 128 <= K)
         {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
             {
-                sv[at][nt] = load_few<2 * NG>(sb + 2 * NG * (size_t)b + 2 * so[nt]);
-                if constexpr (ZP) zv[at][nt] = load_few<NG>(zb + NG * (size_t)b + so[nt]);
+                sv[nt] = load_few<2 * NG>(sb + 2 * NG * (size_t)b + 2 * so[nt]);
+                if constexpr (ZP) zv[nt] = load_few<NG>(zb + NG * (size_t)b + so[nt]);
             }
         }
         else
@@ -221,14 +219,14 @@ struct W4Wave
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
             {
-                sv[at][nt] = 0;
-                zv[at][nt] = 0;
+                sv[nt] = 0;
+                zv[nt] = 0;
 #pragma unroll
                 for (int g = 0; g < NG; ++g)
                     if (g < groups)
                     {
-                        sv[at][nt] |= (scales_t)reinterpret_cast<const uint16_t*>(sb)[so[nt] + b * NG + g] << (16 * g);
-                        if constexpr (ZP) zv[at][nt] |= (zeros_t)zb[so[nt] + b * NG + g] << (8 * g);
+                        sv[nt] |= (scales_t)reinterpret_cast<const uint16_t*>(sb)[so[nt] + b * NG + g] << (16 * g);
+                        if constexpr (ZP) zv[nt] |= (zeros_t)zb[so[nt] + b * NG + g] << (8 * g);
                     }
             }
         }
@@ -241,9 +239,9 @@ struct W4Wave
     }
 
     // the loaded block into LDS
-    __device__ __forceinline__ void store(unsigned char* x, unsigned char* w, int at)
+    __device__ __forceinline__ void store(unsigned char* x, unsigned char* w)
     {
-        const int t = OWN ? threadIdx.x & 63 : threadIdx.x, lane = threadIdx.x & 63;
+        const int t = threadIdx.x % (OWN ? 64 : 64 * NW), lane = threadIdx.x & 63;
 #pragma unroll
         for (int i = 0; i < XI; ++i)
             if (i < nx)
@@ -254,9 +252,9 @@ struct W4Wave
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
         {
-            *reinterpret_cast<u4_t*>(w + nt * 1024 + lane * 16) = wv[at][nt];
-            sc[nt] = sv[at][nt];
-            if constexpr (ZP) zc[nt] = zv[at][nt];
+            *reinterpret_cast<u4_t*>(w + nt * 1024 + lane * 16) = wv[nt];
+            sc[nt] = sv[nt];
+            if constexpr (ZP) zc[nt] = zv[nt];
         }
     }
 
@@ -335,48 +333,50 @@ struct W4Wave
         }
     }
 
-    // products of blocks b0 .. b1 - 1 (with !OWN the same for all waves)
-    __device__ __forceinline__ void run(unsigned char* lds, int b0, int b1, int K, bool sbf, f4_t (&tot)[MT][NT])
+    // products of blocks b0 .. b1 - 1 (with !OWN the same for the waves that share x, and SPLIT: other groups of waves have other blocks,
+    // so every wave takes `steps` >= b1 - b0 barriers)
+    template <bool SPLIT>
+    __device__ __forceinline__ void run(unsigned char* lds, int b0, int b1, int steps, int K, bool sbf, f4_t (&tot)[MT][NT])
     {
-        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % NW;
         unsigned char* x = OWN ? lds + wave * (XBYTES + WBYTES) : lds;
         unsigned char* w = OWN ? x + XBYTES : lds + 2 * XBYTES + wave * WBYTES;
-        if (b0 >= b1) return;
         auto groups = [&](int b) { return G == 128 ? 1 : min(NG, (K - 128 * b) / G); };
-        load_x(b0);
-        load_w(b0, K, 0);
+        if (b0 < b1)
+        {
+            load_x(b0);
+            load_w(b0, K);
+        }
         if constexpr (OWN)
         {
-            if (AHEAD == 2 && b0 + 1 < b1) load_w(b0 + 1, K, AHEAD - 1);
-            for (int b = b0; b < b1; b += AHEAD)
+            for (int b = b0; b < b1; ++b)
             {
-#pragma unroll
-                for (int i = 0; i < AHEAD; ++i)
+                store(x, w);
+                wave_fence();
+                if (b + 1 < b1)
                 {
-                    if (b + i >= b1) break;
-                    store(x, w, i);
-                    wave_fence();
-                    if (b + i + 1 < b1) load_x(b + i + 1);
-                    if (b + i + AHEAD < b1) load_w(b + i + AHEAD, K, i);
-                    multiply(x, w, groups(b + i), sbf, tot);
-                    wave_fence();
+                    load_x(b + 1);
+                    load_w(b + 1, K);
                 }
+                multiply(x, w, groups(b), sbf, tot);
+                wave_fence();
             }
         }
         else
         {
-            store(x, w, 0);
+            if (b0 < b1) store(x, w);
             __syncthreads();
-            for (int b = b0; b < b1; ++b)
+            for (int i = 0; i < (SPLIT ? steps : b1 - b0); ++i)
             {
+                const int b = b0 + i;
                 if (b + 1 < b1)
                 {
                     load_x(b + 1);
-                    load_w(b + 1, K, 0);
+                    load_w(b + 1, K);
                 }
-                multiply(x + ((b - b0) & 1) * XBYTES, w, groups(b), sbf, tot);
+                if (!SPLIT || b < b1) multiply(x + (i & 1) * XBYTES, w, groups(b), sbf, tot);
                 wave_fence();
-                if (b + 1 < b1) store(x + ((b + 1 - b0) & 1) * XBYTES, w, 0);
+                if (b + 1 < b1) store(x + ((i + 1) & 1) * XBYTES, w);
                 __syncthreads();
             }
         }
@@ -392,12 +392,14 @@ struct W4Wave
 template <int P, int MT>
 constexpr int W4_ROWS = 16 * MT / P;
 
-template <int XT, int P, int G, bool ZP, int MT, int NT, int NW, bool OWN, typename Row, typename Col>
+template <int XT, int P, int G, bool ZP, int MT, int NT, int NW, bool OWN, int KG = 1, typename Row, typename Col>
 __device__ __forceinline__ void w4_tile(unsigned char* lds, const uint16_t* x, uint32_t xbytes, Row row, uint32_t xpart, int cnt,
                                         const W4Ptr& w, int wrows, Col col, bool sbf, int K)
 {
+    static_assert(KG == 1 || !OWN, "K is split one way");
     using Wave = W4Wave<XT, P == 3, G, ZP, MT, NT, NW, OWN>;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nb = (K + 127) / 128;
+    const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all % NW, kg = all / NW;
+    const int nb = (K + 127) / 128, steps = (nb + KG - 1) / KG;
     f4_t tot[MT][NT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -408,9 +410,10 @@ __device__ __forceinline__ void w4_tile(unsigned char* lds, const uint16_t* x, u
         const int q = P == 1 ? 0 : (v >= cnt) + (v >= 2 * cnt);
         return row(v - q * cnt) + q * xpart;
     }, P * cnt, w, wrows, col, K);
-    wv.run(lds, OWN ? nb * wave / NW : 0, OWN ? nb * (wave + 1) / NW : nb, K, sbf, tot);
+    if constexpr (OWN) wv.template run<false>(lds, nb * wave / NW, nb * (wave + 1) / NW, 0, K, sbf, tot);
+    else wv.template run<(KG > 1)>(lds + kg * Wave::LDS, kg * steps, min(nb, (kg + 1) * steps), steps, K, sbf, tot);
     // the sums into LDS: OWN in the wave's own place, else where the inputs were (every wave is past its last barrier)
-    f4_t* part = reinterpret_cast<f4_t*>(lds + (OWN ? wave * (Wave::XBYTES + Wave::WBYTES) : wave * MT * NT * 1024));
+    f4_t* part = reinterpret_cast<f4_t*>(lds + kg * Wave::LDS + (OWN ? wave * (Wave::XBYTES + Wave::WBYTES) : wave * MT * NT * 1024));
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -424,6 +427,19 @@ __device__ __forceinline__ void w4_tile(unsigned char* lds, const uint16_t* x, u
             f4_t s = reinterpret_cast<const f4_t*>(lds)[t * 64 + lane];
 #pragma unroll
             for (int v = 1; v < NW; ++v) s += reinterpret_cast<const f4_t*>(lds + v * (Wave::XBYTES + Wave::WBYTES))[t * 64 + lane];
+            reinterpret_cast<f4_t*>(lds)[t * 64 + lane] = s;
+        }
+        __syncthreads();
+    }
+    else if constexpr (KG > 1)
+    {
+        // those of the groups in order, in the first group's place
+        __syncthreads();
+        for (int t = all; t < NW * MT * NT; t += KG * NW)
+        {
+            f4_t s = reinterpret_cast<const f4_t*>(lds)[t * 64 + lane];
+#pragma unroll
+            for (int v = 1; v < KG; ++v) s += reinterpret_cast<const f4_t*>(lds + v * Wave::LDS)[t * 64 + lane];
             reinterpret_cast<f4_t*>(lds)[t * 64 + lane] = s;
         }
         __syncthreads();
@@ -514,7 +530,12 @@ __global__ __launch_bounds__(256) void k_w4_parts(const float* __restrict__ x, s
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// Dense. OWN: a workgroup takes 16 NT columns and its waves split K (few rows); else 16 NT columns a wave.
+// Dense. OWN: a workgroup takes 16 NT columns and its waves split K (up to 32 tile rows); else 16 NT columns a wave, and KG groups of
+// waves split K. A wave's block of 128 inputs is a chain of LDS reads, products and a barrier of some 1.2 us, of which more waves hide
+// more: 4 of them on a CU take 42 us for 64 rows of 8192 x 4096, 16 (KG = 4) take 20; 300 rows take 54 us in tiles of 64 rows,
+// 41 (490 TFLOP/s) in tiles of 80 with KG = 2, one workgroup a CU. Full grids have waves enough: 4,096 rows 424 us (648
+// TFLOP/s) with KG = 1, 514 with KG = 2. (Two to four blocks of loads in flight instead of one: 56-60 us at 300 rows, LDS operands a
+// block ahead: 59.) One row of 4096 x 4096 takes 3.9 us (2.2 TB/s; as many bytes copied take 3.5).
 // ---------------------------------------------------------------------------------------------------------
 struct LinearArgs
 {
@@ -524,19 +545,19 @@ struct LinearArgs
     int M, K, N, sbf, out;
 };
 
-template <int XT, int P, int G, bool ZP, int MT, int NT, int NW, bool OWN>
-__global__ __launch_bounds__(64 * NW, 2) void k_w4_linear(LinearArgs a)
+template <int XT, int P, int G, bool ZP, int MT, int NT, int NW, bool OWN, int KG>
+__global__ __launch_bounds__(64 * NW * KG, 2) void k_w4_linear(LinearArgs a)
 {
     constexpr int ROWS = W4_ROWS<P, MT>;
-    __shared__ __align__(16) unsigned char lds[W4Wave<XT, P == 3, G, ZP, MT, NT, NW, OWN>::LDS];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __shared__ __align__(16) unsigned char lds[KG * W4Wave<XT, P == 3, G, ZP, MT, NT, NW, OWN>::LDS];
+    const int all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all % NW, kg = all / NW;
     const int m0 = blockIdx.y * ROWS, n0 = OWN ? blockIdx.x * 16 * NT : (blockIdx.x * NW + wave) * 16 * NT, cnt = min(ROWS, a.M - m0);
     const int n1 = min(n0, a.N - 1);                                 // a wave past the last column works on it again
-    w4_tile<XT, P, G, ZP, MT, NT, NW, OWN>(
+    w4_tile<XT, P, G, ZP, MT, NT, NW, OWN, KG>(
         lds, a.x + (size_t)m0 * P * a.K, (uint32_t)cnt * P * a.K * 2, [&](int m) { return (uint32_t)m * P * a.K; }, a.K, cnt,
         w4_at(a.w, n1, a.K, G), min(a.N - n1, 16 * NT), [&](int nt, int c) { return (uint32_t)min(16 * nt + c, a.N - 1 - n1); }, a.sbf, a.K);
     const unsigned char* sums = OWN ? lds : lds + wave * MT * NT * 1024;
-    for (int o = OWN ? threadIdx.x : threadIdx.x & 63; o < cnt * 16 * NT; o += OWN ? 64 * NW : 64)
+    for (int o = OWN ? threadIdx.x : (threadIdx.x & 63) + 64 * kg; o < cnt * 16 * NT; o += OWN ? 64 * NW : 64 * KG)
     {
         const int m = o / (16 * NT), c = o % (16 * NT);
         if (n0 + c >= a.N) continue;
@@ -1067,13 +1088,24 @@ int mm_w4_linear(const void* x, int x_dtype, int M, int K, int N, const mm_w4_t*
             constexpr int XT = decltype(xt)::value, P = decltype(p)::value, G = decltype(g)::value;
             constexpr bool ZP = decltype(zp)::value;
             const int rows = P * M;
-            auto grid = [&](int mt, int cols) { return dim3((N + cols - 1) / cols, (M + 16 * mt / P - 1) / (16 * mt / P)); };
-            if (rows <= 16)
-                hipLaunchKernelGGL((k_w4_linear<XT, P, G, ZP, 1, 1, 8, true>), grid(1, 16), dim3(512), 0, hs, a);
-            else if (rows <= 32)
-                hipLaunchKernelGGL((k_w4_linear<XT, P, G, ZP, 2, 1, 8, true>), grid(2, 16), dim3(512), 0, hs, a);
+            auto launch = [&](auto mt, auto nt, auto nw, auto own, auto kg) {
+                constexpr int MT = decltype(mt)::value, NT = decltype(nt)::value, NW = decltype(nw)::value, KG = decltype(kg)::value;
+                constexpr bool OWN = decltype(own)::value;
+                constexpr int COLS = 16 * NT * (OWN ? 1 : NW), ROWS = W4_ROWS<P, MT>;
+                hipLaunchKernelGGL((k_w4_linear<XT, P, G, ZP, MT, NT, NW, OWN, KG>), dim3((N + COLS - 1) / COLS, (M + ROWS - 1) / ROWS),
+                                   dim3(64 * NW * KG), 0, hs, a);
+            };
+            if (rows <= 16) launch(ic<1>{}, ic<1>{}, ic<8>{}, std::true_type{}, ic<1>{});
+            else if (rows <= 32) launch(ic<2>{}, ic<1>{}, ic<8>{}, std::true_type{}, ic<1>{});
             else
-                hipLaunchKernelGGL((k_w4_linear<XT, P, G, ZP, 4, 2, 4, false>), grid(4, 128), dim3(256), 0, hs, a);
+            {
+                // workgroups of 128 columns and 16 MT tile rows: the least of the estimated times (us at 4,096 inputs)
+                auto groups = [&](int mt) { return (size_t)((N + 127) / 128) * ((M + 16 * mt / P - 1) / (16 * mt / P)); };
+                const size_t t2 = 20 * ((groups(2) + 255) / 256), t5 = 41 * ((groups(5) + 255) / 256), t4 = 18 + 26 * groups(4) / 256;
+                if (t2 <= std::min(t4, t5)) launch(ic<2>{}, ic<2>{}, ic<4>{}, std::false_type{}, ic<4>{});
+                else if (t5 <= t4) launch(ic<5>{}, ic<2>{}, ic<4>{}, std::false_type{}, ic<2>{});
+                else launch(ic<4>{}, ic<2>{}, ic<4>{}, std::false_type{}, ic<1>{});
+            }
         });
     });
     return check_launch("mm_w4_linear");

@@ -83,6 +83,21 @@ def test_linear(dev, M, K, N, group, dtype, zeros, sdtype):
     check_linear(w4.linear(x.to(dev), W, out_dtype=torch.float32), x, q, s, z)
 
 
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("M,K,N,group,dtype", [
+    (100, 128, 300, 128, torch.bfloat16), (60, 160, 140, 32, torch.float16), (40, 384, 200, 64, torch.float32),
+    (33, 640, 129, 128, torch.bfloat16), (64, 1216, 64, 64, torch.float16),
+    (20000, 128, 100, 128, torch.bfloat16), (20000, 96, 70, 32, torch.float16), (6500, 448, 100, 64, torch.float32),
+    (40000, 96, 64, 32, torch.bfloat16), (13000, 256, 50, 64, torch.float32)])
+def test_linear_of_many_rows(dev, M, K, N, group, dtype, zeros):
+    """Every split of the waves (by rows and columns), with fewer blocks of inputs than groups of waves, and K's last block cut."""
+    from mi355moe import w4
+    g = torch.Generator().manual_seed(M + K + N)
+    q, s, z = weights(g, N, K, group, zeros, torch.bfloat16)
+    x = torch.randn((M, K), generator=g).to(dtype)
+    check_linear(w4.linear(x.to(dev), w4.W4Matrix(*to(dev, (q, s, z)))), x, q, s, z)
+
+
 @pytest.mark.parametrize("group", [32, 64, 128])
 def test_linear_every_weight_value_in_every_place(dev, group):
     """x = unit vectors picks single weights: 256 columns of every nibble value at every k, exact in fp32."""
