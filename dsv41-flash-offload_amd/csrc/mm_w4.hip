@@ -697,8 +697,11 @@ constexpr int W4_GU = 2, W4_DN = 2;
 template <int G, bool ZP, int MT>
 constexpr int W4_OCC = MT == 1 && G == 128 && !ZP ? 4 : 3;
 
-// Few rows: one workgroup per record and 16 (32) columns, its four waves split K; one or two row tiles by the record's routes, more routes in
-// more passes.
+// Few rows: one workgroup per record and 16 (32) columns, its four waves split K; one or two row tiles by the expert's routes, more
+// routes in more passes. Bound by no unit that a counter shows: 9 experts of 4096 / 2048 take 20.5 + 13.0 us, 32 experts of them (4
+// fp32 tokens) 58 + 32 us, 3.5 TB/s of weights, where a read alone in this pattern reaches 5.7 to 6.4; VALU 39 % busy, MFMA 18 %, address
+// unit 57 %, LDS 22 %. Waves that split the columns instead, as for many rows, would have each expert's few columns wait for the
+// whole of K: 9 experts would be 9 x 32 workgroups of 32 blocks in a row.
 template <int XT, int P, int G, bool ZP, int MT>
 __global__ __launch_bounds__(256, (W4_OCC<G, ZP, MT>)) void k_w4_gate_up(ExpertArgs a)
 {
@@ -734,7 +737,9 @@ __global__ __launch_bounds__(256, (W4_OCC<G, ZP, MT>)) void k_w4_down(ExpertArgs
     }
 }
 
-// Many rows: 64 (128) columns per workgroup, four waves that share the rows of x; up to 16 MT tile rows a pass.
+// Many rows: 64 (128) columns per workgroup, four waves that share the rows of x; up to 16 MT tile rows a pass. 200 tokens of 32
+// experts of 1024 / 512 take 19 + 18 us (four to eight blocks in a row), 4,000 of 4096 / 1024 1.2 ms in all (330 TFLOP/s, the down
+// product's three parts counted once).
 template <int XT, int P, int G, bool ZP, int MT>
 __global__ __launch_bounds__(256, 2) void k_w4_gate_up_many(ExpertArgs a)
 {
@@ -931,8 +936,10 @@ static ExpertWs expert_ws(int x_dtype, int T, int k, int shared, int E, int H, i
     w.rows = 16;
     if (n > W4_SELF)
     {
-        // rows of a record: of up to 16, 32 or 64 routes by the average of the experts
-        w.rows = n > (size_t)32 * E ? 64 : n > (size_t)12 * E ? 32 : 16;
+        // Routes of a record, up to 16, 32 or 64 by the experts' average (us at 64 experts of 2048 / 1024, groups of 64): 6 routes an
+        // expert 92 in records of 16 and 97 of 32, 8 routes 102 and 97, 12 routes 131 and 102; 32 routes 157 in records of 32
+        // and 172 of 64, 40 routes 197 and 184, 128 routes 440 both, 256 routes 787 and 760.
+        w.rows = n > (size_t)36 * E ? 64 : n > (size_t)7 * E ? 32 : 16;
         w.nrecs = (int)(std::min(n, (size_t)E) + n / w.rows);
         w.order = take(n * 4);
         w.recs = take((size_t)w.nrecs * sizeof(W4Rec));
