@@ -641,17 +641,18 @@ __device__ __forceinline__ float swiglu(float g, float u, float limit)
 
 // Gate and up of 8 NT columns (OWN: a workgroup's, else a wave's; weight tile 2 i is gate, 2 i + 1 up) for some of a record's
 // routes, SwiGLU, and the result as three bf16 parts for the down product.
-template <int XT, int P, int G, bool ZP, int MT, int NT, int NW, bool OWN>
+template <int XT, int P, int G, bool ZP, int MT, int NT, int NW, bool OWN, int KG = 1>
 __device__ __forceinline__ void gate_up_rows(const ExpertArgs& a, unsigned char* lds, int expert, const int* rows, int c)
 {
     constexpr int COLS = 8 * NT;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = OWN ? blockIdx.x * COLS : (blockIdx.x * NW + wave) * COLS;
-    w4_tile<XT, P, G, ZP, MT, NT, NW, OWN>(
+    const int all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all % NW, kg = all / NW;
+    const int n0 = OWN ? blockIdx.x * COLS : (blockIdx.x * NW + wave) * COLS;
+    w4_tile<XT, P, G, ZP, MT, NT, NW, OWN, KG>(
         lds, a.x, (uint32_t)a.T * P * a.H * 2, [&](int m) { return (uint32_t)(rows[m] / a.topk) * (P * a.H); }, a.H, c,
         w4_at(a.w13, (size_t)expert * 2 * a.I, a.H, G), 2 * a.I,
         [&](int t, int col) { return (uint32_t)((t & 1) * a.I + min(n0 + 16 * (t >> 1) + col, a.I - 1)); }, a.sbf, a.H);
     const unsigned char* sums = OWN ? lds : lds + wave * MT * NT * 1024;
-    for (int o = OWN ? threadIdx.x : threadIdx.x & 63; o < c * COLS; o += OWN ? 64 * NW : 64)
+    for (int o = OWN ? threadIdx.x : (threadIdx.x & 63) + 64 * kg; o < c * COLS; o += OWN ? 64 * NW : 64 * KG)
     {
         const int m = o / COLS, col = o % COLS, t = 2 * (col >> 4);
         if (n0 + col >= a.I) continue;
@@ -737,13 +738,14 @@ __global__ __launch_bounds__(256, (W4_OCC<G, ZP, MT>)) void k_w4_down(ExpertArgs
     }
 }
 
-// Many rows: 64 (128) columns per workgroup, four waves that share the rows of x; up to 16 MT tile rows a pass. 200 tokens of 32
+// Many rows: 64 columns (gate and up; down 64 NT) per workgroup, four waves that share the rows of x, KG groups of them that split K; up
+// to 16 MT tile rows a pass. 200 tokens of 32
 // experts of 1024 / 512 take 19 + 18 us (four to eight blocks in a row), 4,000 of 4096 / 1024 1.2 ms in all (330 TFLOP/s, the down
 // product's three parts counted once).
-template <int XT, int P, int G, bool ZP, int MT>
-__global__ __launch_bounds__(256, 2) void k_w4_gate_up_many(ExpertArgs a)
+template <int XT, int P, int G, bool ZP, int MT, int KG>
+__global__ __launch_bounds__(256 * KG, 2) void k_w4_gate_up_many(ExpertArgs a)
 {
-    __shared__ __align__(16) unsigned char lds[W4Wave<XT, P == 3, G, ZP, MT, 2, 4, false>::LDS];
+    __shared__ __align__(16) unsigned char lds[KG * W4Wave<XT, P == 3, G, ZP, MT, 2, 4, false>::LDS];
     __shared__ int rows[W4_REC];
     int expert, all;
     const int cnt = record_rows(a, blockIdx.y, rows, expert, all);
@@ -752,13 +754,13 @@ __global__ __launch_bounds__(256, 2) void k_w4_gate_up_many(ExpertArgs a)
     for (int m = 0; m < cnt; m += W4_ROWS<P, MT>)
     {
         if (m) __syncthreads();
-        gate_up_rows<XT, P, G, ZP, MT, 2, 4, false>(a, lds, expert, rows + m, min(W4_ROWS<P, MT>, cnt - m));
+        gate_up_rows<XT, P, G, ZP, MT, 2, 4, false, KG>(a, lds, expert, rows + m, min(W4_ROWS<P, MT>, cnt - m));
     }
 }
-template <int G, bool ZP, int MT>
+template <int G, bool ZP, int MT, int NT>
 __global__ __launch_bounds__(256, 2) void k_w4_down_many(ExpertArgs a)
 {
-    __shared__ __align__(16) unsigned char lds[W4Wave<MM_DTYPE_BF16, true, G, ZP, MT, 2, 4, false>::LDS];
+    __shared__ __align__(16) unsigned char lds[W4Wave<MM_DTYPE_BF16, true, G, ZP, MT, NT, 4, false>::LDS];
     __shared__ int rows[W4_REC];
     int expert, all;
     const int cnt = record_rows(a, blockIdx.y, rows, expert, all);
@@ -767,7 +769,7 @@ __global__ __launch_bounds__(256, 2) void k_w4_down_many(ExpertArgs a)
     for (int m = 0; m < cnt; m += W4_ROWS<3, MT>)
     {
         if (m) __syncthreads();
-        down_rows<G, ZP, MT, 2, 4, false>(a, lds, expert, rows + m, min(W4_ROWS<3, MT>, cnt - m));
+        down_rows<G, ZP, MT, NT, 4, false>(a, lds, expert, rows + m, min(W4_ROWS<3, MT>, cnt - m));
     }
 }
 
@@ -1024,25 +1026,40 @@ static int experts_launch(const mm_w4_layer_t* L, const void* x, int x_dtype, in
         a.nrec = nrec;
     }
     const bool many = s.rows > 16;
+    // At most one workgroup a CU: twice the waves in gate and up, half the columns in down (200 tokens of 32 experts of 1024 / 512 44.5 ->
+    // 40 us, 60 of 8 37 -> 32; with four workgroups a CU, 300 tokens of 64 experts of 2048 / 1024, 142 -> 160 and 163 us).
+    auto few = [&](int columns) { return (size_t)columns * std::min(E, a.n) <= 256 && a.n <= 64 * E; };
     by_input(x_dtype, [&](auto xt, auto parts) {
         by_group(L->group, L->w13.zeros != nullptr, [&](auto g, auto zp) {
             constexpr int XT = decltype(xt)::value, P = decltype(parts)::value, G = decltype(g)::value;
             constexpr bool ZP = decltype(zp)::value;
-            const dim3 grid((I + 63) / 64, s.nrecs);
-            if (many && P == 3) hipLaunchKernelGGL((k_w4_gate_up_many<XT, P, G, ZP, P == 3 ? 6 : 4>), grid, dim3(256), 0, hs, a);
-            else if (s.rows == 64) hipLaunchKernelGGL((k_w4_gate_up_many<XT, P, G, ZP, P == 3 ? 6 : 4>), grid, dim3(256), 0, hs, a);
-            else if (many) hipLaunchKernelGGL((k_w4_gate_up_many<XT, P, G, ZP, P == 3 ? 6 : 2>), grid, dim3(256), 0, hs, a);
-            else if (T <= W4_ROWS<P, 1> || (P == 1 && s.rows <= 16))
-                hipLaunchKernelGGL((k_w4_gate_up<XT, P, G, ZP, 1>), dim3((I + 8 * W4_GU - 1) / (8 * W4_GU), s.nrecs), dim3(256), 0, hs, a);
-            else hipLaunchKernelGGL((k_w4_gate_up<XT, P, G, ZP, 2>), dim3((I + 8 * W4_GU - 1) / (8 * W4_GU), s.nrecs), dim3(256), 0, hs, a);
+            auto launch_many = [&](auto mt, auto kg) {
+                constexpr int MT = decltype(mt)::value, KG = decltype(kg)::value;
+                hipLaunchKernelGGL((k_w4_gate_up_many<XT, P, G, ZP, MT, KG>), dim3((I + 63) / 64, s.nrecs), dim3(256 * KG), 0, hs, a);
+            };
+            auto by_groups = [&](auto mt) {
+                if (few((I + 63) / 64)) launch_many(mt, ic<2>{});
+                else launch_many(mt, ic<1>{});
+            };
+            const dim3 grid((I + 8 * W4_GU - 1) / (8 * W4_GU), s.nrecs);
+            if (many)
+            {
+                if constexpr (P == 3) by_groups(ic<6>{});
+                else if (s.rows == 64) by_groups(ic<4>{});
+                else by_groups(ic<2>{});
+            }
+            else if (P == 1 || T <= W4_ROWS<P, 1>) hipLaunchKernelGGL((k_w4_gate_up<XT, P, G, ZP, 1>), grid, dim3(256), 0, hs, a);
+            else if constexpr (P == 3) hipLaunchKernelGGL((k_w4_gate_up<XT, P, G, ZP, 2>), grid, dim3(256), 0, hs, a);
         });
     });
     by_group(L->group, L->w2.zeros != nullptr, [&](auto g, auto zp) {
         constexpr int G = decltype(g)::value;
         constexpr bool ZP = decltype(zp)::value;
-        if (many) hipLaunchKernelGGL((k_w4_down_many<G, ZP, 6>), dim3((H + 127) / 128, s.nrecs), dim3(256), 0, hs, a);
-        else if (T <= W4_ROWS<3, 1>) hipLaunchKernelGGL((k_w4_down<G, ZP, 1>), dim3((H + 16 * W4_DN - 1) / (16 * W4_DN), s.nrecs), dim3(256), 0, hs, a);
-        else hipLaunchKernelGGL((k_w4_down<G, ZP, 2>), dim3((H + 16 * W4_DN - 1) / (16 * W4_DN), s.nrecs), dim3(256), 0, hs, a);
+        const dim3 grid((H + 16 * W4_DN - 1) / (16 * W4_DN), s.nrecs);
+        if (many && few((H + 127) / 128)) hipLaunchKernelGGL((k_w4_down_many<G, ZP, 6, 1>), dim3((H + 63) / 64, s.nrecs), dim3(256), 0, hs, a);
+        else if (many) hipLaunchKernelGGL((k_w4_down_many<G, ZP, 6, 2>), dim3((H + 127) / 128, s.nrecs), dim3(256), 0, hs, a);
+        else if (T <= W4_ROWS<3, 1>) hipLaunchKernelGGL((k_w4_down<G, ZP, 1>), grid, dim3(256), 0, hs, a);
+        else hipLaunchKernelGGL((k_w4_down<G, ZP, 2>), grid, dim3(256), 0, hs, a);
     });
     hipLaunchKernelGGL(k_w4_combine, dim3((H / 4 + 255) / 256, T), dim3(256), 0, hs, a);
     return check_launch("mm_w4_moe");

@@ -125,7 +125,8 @@ def check(rc, what=""):
 
 
 def call(name, *args):
-    return check(getattr(load(), name)(*args), name)
+    rc = getattr(_LIB or load(), name)(*args)
+    return check(rc, name) if rc else rc
 
 
 def call_count(name, *args):

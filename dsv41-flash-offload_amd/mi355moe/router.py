@@ -156,9 +156,8 @@ def balance_loss_forward(logits, ids, mask=None, score="softmax", stream=None):
         logits, ids = logits.contiguous(), ids.contiguous()
         mask = None if mask is None else mask.contiguous()
         loss = torch.empty(lead, dtype=torch.float32, device=dev)
-        counts = torch.empty(lead + (E,), dtype=torch.int32, device=dev)
-        tokens = torch.empty(lead, dtype=torch.int32, device=dev)
         load = torch.empty(lead + (E,), dtype=torch.float32, device=dev)
+        tokens, counts = torch.empty_like(loss, dtype=torch.int32), torch.empty_like(load, dtype=torch.int32)
         wsb = _lib.load().mm_balance_workspace(B, T, E)
         ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
         _lib.call("mm_balance_loss", _p(logits), _DTYPES[logits.dtype], _p(ids), _p(mask), B, T, E, k, _SCORES[score],

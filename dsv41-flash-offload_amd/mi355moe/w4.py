@@ -49,31 +49,35 @@ class W4Matrix:
         self.q, self.scales, self.zeros = q, scales, zeros
         self.N, self.K = q.shape[0], q.shape[1] * 8
         self._c = _lib.MMW4(_p(q), _p(scales), _p(zeros))
+        self._ref, self._device, self._scale_code = ctypes.byref(self._c), q.device, _DTYPES[scales.dtype]
 
 
 def linear(x, W, out_dtype=None, stream=None):
     """x [..., K] times W [N, K] transposed: [..., N] in x's type or `out_dtype` (fp16, bf16 or fp32). Built for few rows."""
-    if x.dtype not in _DTYPES:
+    # (a decode step's call takes as long as its launch: little is done twice here)
+    code = _DTYPES.get(x.dtype)
+    if code is None:
         raise TypeError(f"w4.linear: x must be fp16, bf16 or fp32 (got {x.dtype})")
     out_dtype = x.dtype if out_dtype is None else out_dtype
-    if out_dtype not in _DTYPES:
+    out_code = _DTYPES.get(out_dtype)
+    if out_code is None:
         raise TypeError(f"w4.linear: out_dtype must be fp16, bf16 or fp32 (got {out_dtype})")
-    if x.dim() < 1 or x.shape[-1] != W.K:
-        raise ValueError(f"w4.linear: x [..., {W.K}] expected (got {tuple(x.shape)})")
-    dev = W.q.device
+    shape, dev = x.shape, W._device
+    if not shape or shape[-1] != W.K:
+        raise ValueError(f"w4.linear: x [..., {W.K}] expected (got {tuple(shape)})")
     _lib.check_tensors("w4.linear", dev, x=x)
-    lead = x.shape[:-1]
     M = x.numel() // W.K
     with _lib.on(dev, stream):
-        y = torch.empty(lead + (W.N,), dtype=out_dtype, device=dev)
+        y = torch.empty(shape[:-1] + (W.N,), dtype=out_dtype, device=dev)
         if M == 0:
             return y
         x = _lib.aligned(x)
-        code = _DTYPES[x.dtype]
-        wsb = _lib.load().mm_w4_linear_workspace(code, M, W.K)
-        ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
-        _lib.call("mm_w4_linear", _p(x), code, M, W.K, W.N, ctypes.byref(W._c), W.group, _DTYPES[W.scales.dtype], _p(y),
-                  _DTYPES[out_dtype], _p(ws), wsb, _lib.raw_stream(dev))
+        ws, wsb = None, 0
+        if code == _lib.DTYPE_F32:
+            wsb = _lib.load().mm_w4_linear_workspace(code, M, W.K)
+            ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+        _lib.call("mm_w4_linear", x.data_ptr(), code, M, W.K, W.N, W._ref, W.group, W._scale_code, y.data_ptr(), out_code, _p(ws), wsb,
+                  _lib.raw_stream(dev))
     return y
 
 
@@ -111,7 +115,7 @@ def moe(store, x, ids, w, shared_expert=None, stream=None):
     if x.dim() != 2 or x.shape[1] != store.H:
         raise ValueError(f"w4.moe: x [T, {store.H}] expected (got {tuple(x.shape)})")
     T = x.shape[0]
-    if ids.numel() != w.numel() or ids.numel() == 0 and T or T and ids.numel() % T:
+    if ids.shape != w.shape or ids.numel() == 0 and T or T and ids.numel() % T:
         raise ValueError(f"w4.moe: ids and w must be [{T}, k] (got {tuple(ids.shape)} and {tuple(w.shape)})")
     shared = -1 if shared_expert is None else int(shared_expert)
     if shared_expert is not None and not 0 <= shared < store.E:

@@ -385,3 +385,13 @@ def test_experts_equal_tokens_get_equal_results(dev, T, E, most, group, dtype):
     out = moe.moe_forward(store, x.to(dev), ids.to(dev), w.to(dev))
     assert torch.equal(out[:most], out[:1].expand(most, -1))
     check_experts(out, a, b, x, ids, w, None, 10.0)
+
+
+def test_experts_picks_and_weights_must_match(dev):
+    from mi355moe import w4
+    g = torch.Generator().manual_seed(3)
+    store, _, _ = make_store(g, 4, 128, 64, 64, False, dev)
+    x, ids, w = torch.randn((2, 128)).to(dev), torch.zeros((2, 3), dtype=torch.int64, device=dev), torch.zeros((2, 3), device=dev)
+    for bad in ((ids, w.t()), (ids, w[:, :2]), (ids[:, :0], w[:, :0]), (ids[:1, :1], w[:1, :1])):
+        with pytest.raises(ValueError, match="ids and w"):
+            w4.moe(store, x, *bad)
