@@ -69,6 +69,21 @@ __device__ __forceinline__ float wave_max(float v)
     return v;
 }
 
+// e^x for x <= 0 (or NaN): 2^t of t = x / ln 2 rounded, times 1 + ln 2 times what the rounding left. Two steps of v_exp_f32 and a few
+// of t's: within 3 2^-24 of the value; results below fp32's normal numbers are zero.
+__device__ __forceinline__ float exp_neg(float x)
+{
+    x = x < -126.f ? -126.f : x;
+    const float t = x * 1.44269504f, e = __builtin_amdgcn_exp2f(t);
+    return fmaf(e, 0.693147181f * fmaf(x, 1.92596299e-8f, fmaf(x, 1.44269504f, -t)), e);
+}
+// 1 / d for d in [1, 2] (or NaN): one Newton step on v_rcp_f32.
+__device__ __forceinline__ float recip(float d)
+{
+    const float r = __builtin_amdgcn_rcpf(d);
+    return fmaf(fmaf(-d, r, 1.f), r, r);
+}
+
 // A row's scores from its logits l (lane's experts lane + 64 v; those past E hold -inf), in place. Softmax shifts by the
 // row's largest logit. Sigmoids go through sigma(l) = e^min(l, 0) / (1 + e^-|l|), whose numerator is shifted the same way
 // (the sum divides the shift out again), so logits far below zero keep their ratios; one[v] = 1 - sigma(l) without
@@ -86,10 +101,10 @@ __device__ __forceinline__ void row_scores(float (&l)[NV], float (&one)[NV])
     for (int v = 0; v < NV; ++v)
     {
         const float x = l[v];
-        float p = expf((SIG ? (x > 0.f ? 0.f : x) : x) - m);
+        float p = exp_neg((SIG ? (x > 0.f ? 0.f : x) : x) - m);
         if constexpr (SIG)
         {
-            const float u = expf(-fabsf(x)), r = 1.f / (1.f + u);
+            const float u = exp_neg(-fabsf(x)), r = recip(1.f + u);
             p *= r;
             one[v] = x >= 0.f ? u * r : r;
         }
@@ -360,7 +375,9 @@ static void balance_dispatch(int dtype, int E, int score, F f)
         else f(dt, nv, std::false_type{});
     };
     auto by_e = [&](auto dt) {
-        if (E <= 128) by_score(dt, std::integral_constant<int, 2>{});
+        if (E <= 64) by_score(dt, std::integral_constant<int, 1>{});
+        else if (E <= 128) by_score(dt, std::integral_constant<int, 2>{});
+        else if (E <= 192) by_score(dt, std::integral_constant<int, 3>{});
         else if (E <= 256) by_score(dt, std::integral_constant<int, 4>{});
         else if (E <= 384) by_score(dt, std::integral_constant<int, 6>{});
         else if (E <= 512) by_score(dt, std::integral_constant<int, 8>{});
