@@ -740,7 +740,7 @@ __global__ __launch_bounds__(256, (W4_OCC<G, ZP, MT>)) void k_w4_down(ExpertArgs
 
 // Many rows: 64 columns (gate and up; down 64 NT) per workgroup, four waves that share the rows of x, KG groups of them that split K; up
 // to 16 MT tile rows a pass. 200 tokens of 32
-// experts of 1024 / 512 take 19 + 18 us (four to eight blocks in a row), 4,000 of 4096 / 1024 1.2 ms in all (330 TFLOP/s, the down
+// experts of 1024 / 512 take 17 + 15 us (four blocks in a row), 4,000 of 4096 / 1024 1.2 ms in all (330 TFLOP/s, the down
 // product's three parts counted once).
 template <int XT, int P, int G, bool ZP, int MT, int KG>
 __global__ __launch_bounds__(256 * KG, 2) void k_w4_gate_up_many(ExpertArgs a)
