@@ -46,31 +46,42 @@ __device__ __forceinline__ void split3(float v, uint16_t& a, uint16_t& b, uint16
 // The parts, 64 x 64 tiles: of D = dlogits + scattered top-k gradient in both orders (the first `tiles` workgroups), and of the
 // transposed gate (gt [2][H][Ek], zeros past E).
 // ---------------------------------------------------------------------------------------------------------
+// Parts q < N of four neighbours v at out + q * stride (8 bytes a lane).
+template <int N>
+__device__ __forceinline__ void store_parts(const float (&v)[4], uint16_t* out, size_t stride)
+{
+    uint16_t p[4][3];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) split3(v[i], p[i][0], p[i][1], p[i][2]);
+#pragma unroll
+    for (int q = 0; q < N; ++q)
+        *reinterpret_cast<uint2*>(out + q * stride) = make_uint2(p[0][q] | ((uint32_t)p[1][q] << 16), p[2][q] | ((uint32_t)p[3][q] << 16));
+}
+
 __device__ __forceinline__ void gate_parts(const float* __restrict__ gate, int E, int H, int Ek, uint16_t* __restrict__ gt, float (*tile)[65],
                                            int b)
 {
-    const int nh = (H + 63) / 64, h0 = b % nh * 64, e0 = b / nh * 64, tid = threadIdx.x;
-    float v[16];
+    typedef rb_f4 __attribute__((aligned(4))) f4_any;
+    const int nh = (H + 63) / 64, h0 = b % nh * 64, e0 = b / nh * 64, tid = threadIdx.x, c = 4 * (tid & 15);
+    rb_f4 v[4];
 #pragma unroll
-    for (int u = 0; u < 16; ++u)
+    for (int u = 0; u < 4; ++u)
     {
-        const int r = (tid + 256 * u) >> 6, c = tid & 63;
-        v[u] = e0 + r < E && h0 + c < H ? gate[(size_t)(e0 + r) * H + h0 + c] : 0.f;
+        const int r = (tid >> 4) + 16 * u;
+        v[u] = e0 + r < E && h0 + c < H ? *reinterpret_cast<const f4_any*>(gate + (size_t)(e0 + r) * H + h0 + c) : rb_f4{ 0.f, 0.f, 0.f, 0.f };
     }
 #pragma unroll
-    for (int u = 0; u < 16; ++u) tile[(tid + 256 * u) >> 6][tid & 63] = v[u];
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tile[(tid >> 4) + 16 * u][c + i] = v[u][i];
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
+    for (int u = 0; u < 4; ++u)
     {
-        const int r = (tid + 256 * u) >> 5, c = 2 * (tid & 31);
-        if (h0 + r >= H || e0 + c >= Ek) continue;
-        uint16_t p[2][3];
-        split3(tile[c][r], p[0][0], p[0][1], p[0][2]);
-        split3(tile[c + 1][r], p[1][0], p[1][1], p[1][2]);
-#pragma unroll
-        for (int q = 0; q < 2; ++q)
-            *reinterpret_cast<uint32_t*>(gt + ((size_t)q * H + h0 + r) * Ek + e0 + c) = p[0][q] | ((uint32_t)p[1][q] << 16);
+        const int r = (tid >> 4) + 16 * u;
+        if (h0 + r >= H) continue;
+        const float w[4] = { tile[c][r], tile[c + 1][r], tile[c + 2][r], tile[c + 3][r] };
+        store_parts<2>(w, gt + (size_t)(h0 + r) * Ek + e0 + c, (size_t)H * Ek);
     }
 }
 
@@ -115,27 +126,21 @@ __global__ __launch_bounds__(256) void k_rb_parts(const int64_t* __restrict__ id
             if (se[at + j] >= 0) tile[tid][se[at + j]] += sw[at + j] * (sd[at + j] - s);
     }
     __syncthreads();
-    // pairs of neighbours along the contiguous index of each order
+    // four neighbours along the contiguous index of each order (Ek and Tk are multiples of 64)
+    const int c = 4 * (tid & 15);
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
+    for (int u = 0; u < 4; ++u)
     {
-        const int r = (tid + 256 * u) >> 5, c = 2 * (tid & 31);
-        uint16_t p[2][3];
-        if (d && t0 + r < T && e0 + c < Ek)
+        const int r = (tid >> 4) + 16 * u;
+        if (d && t0 + r < T)
         {
-            split3(tile[r][c], p[0][0], p[0][1], p[0][2]);
-            split3(tile[r][c + 1], p[1][0], p[1][1], p[1][2]);
-#pragma unroll
-            for (int q = 0; q < 2; ++q)
-                *reinterpret_cast<uint32_t*>(d + ((size_t)q * T + t0 + r) * Ek + e0 + c) = p[0][q] | ((uint32_t)p[1][q] << 16);
+            const float x[4] = { tile[r][c], tile[r][c + 1], tile[r][c + 2], tile[r][c + 3] };
+            store_parts<2>(x, d + (size_t)(t0 + r) * Ek + e0 + c, (size_t)T * Ek);
         }
-        if (dt && e0 + r < E && t0 + c < Tk)
+        if (dt && e0 + r < E)
         {
-            split3(tile[c][r], p[0][0], p[0][1], p[0][2]);
-            split3(tile[c + 1][r], p[1][0], p[1][1], p[1][2]);
-#pragma unroll
-            for (int q = 0; q < 3; ++q)
-                *reinterpret_cast<uint32_t*>(dt + ((size_t)q * E + e0 + r) * Tk + t0 + c) = p[0][q] | ((uint32_t)p[1][q] << 16);
+            const float x[4] = { tile[c][r], tile[c + 1][r], tile[c + 2][r], tile[c + 3][r] };
+            store_parts<3>(x, dt + (size_t)(e0 + r) * Tk + t0 + c, (size_t)E * Tk);
         }
     }
 }
