@@ -85,32 +85,40 @@ __device__ __forceinline__ float recip(float d)
 }
 
 // A row's scores from its logits l (lane's experts lane + 64 v; those past E hold -inf), in place. Softmax shifts by the
-// row's largest logit. Sigmoids go through sigma(l) = e^min(l, 0) / (1 + e^-|l|), whose numerator is shifted the same way
-// (the sum divides the shift out again), so logits far below zero keep their ratios; one[v] = 1 - sigma(l) without
+// row's largest logit m. Sigmoids are (l < 0 ? u : 1) / (1 + u) with u = e^-|l|; where every logit lies below -1 the numerator is
+// e^(l - m) (the sum divides the shift out again), so logits far below zero keep their ratios; one[v] = 1 - sigma(l) without
 // cancellation. A row of -inf only (every expert masked) has no scores: all zero.
 template <int NV, bool SIG>
 __device__ __forceinline__ void row_scores(float (&l)[NV], float (&one)[NV])
 {
     float m = -INFINITY;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) m = fmaxf(m, SIG ? fminf(l[v], 0.f) : l[v]);
+    for (int v = 0; v < NV; ++v) m = fmaxf(m, l[v]);
     m = wave_max(m);
     if (m == -INFINITY) m = 0.f;              // every expert masked (or NaN, which fmaxf drops and the sum passes on)
-    float sum = 0.f;
+    float sum = 0.f, p[NV];
+    if (!SIG || m < -1.f)
+    {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) p[v] = exp_neg(l[v] - m);
+    }
+    else
+    {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) p[v] = -1.f;                // from u below
+    }
 #pragma unroll
     for (int v = 0; v < NV; ++v)
     {
-        const float x = l[v];
-        float p = exp_neg((SIG ? (x > 0.f ? 0.f : x) : x) - m);
+        one[v] = 1.f;
         if constexpr (SIG)
         {
-            const float u = exp_neg(-fabsf(x)), r = recip(1.f + u);
-            p *= r;
-            one[v] = x >= 0.f ? u * r : r;
+            const float u = exp_neg(-fabsf(l[v])), r = recip(1.f + u);
+            p[v] = (p[v] >= 0.f ? p[v] : l[v] < 0.f ? u : 1.f) * r;
+            one[v] = l[v] >= 0.f ? u * r : r;
         }
-        else one[v] = 1.f;
-        l[v] = p;
-        sum += p;
+        l[v] = p[v];
+        sum += p[v];
     }
     sum = wave_sum(sum);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
