@@ -171,13 +171,15 @@ def balance_loss_backward(dloss, logits, counts, tokens, k, mask=None, score="so
     gradient of the loss over all ranks' tokens."""
     B, T, E = _check_balance("balance_loss_backward", logits, k, mask, score)
     lead, dev = logits.shape[:-2], logits.device
-    for name, t, shape, dt in (("dloss", dloss, lead, torch.float32), ("counts", counts, lead + (E,), torch.int32),
-                               ("tokens", tokens, lead, torch.int32)):
-        if t.shape != shape or t.dtype != dt:
-            raise ValueError(f"balance_loss_backward: {name} must be {dt} {list(shape)} (got {t.dtype} {tuple(t.shape)})")
+    if dloss.shape != lead or dloss.dtype != torch.float32:
+        raise ValueError(f"balance_loss_backward: dloss must be fp32 {list(lead)} (got {dloss.dtype} {tuple(dloss.shape)})")
+    if counts.shape != lead + (E,) or counts.dtype != torch.int32:
+        raise ValueError(f"balance_loss_backward: counts must be int32 {list(lead + (E,))} (got {counts.dtype} {tuple(counts.shape)})")
+    if tokens.shape != lead or tokens.dtype != torch.int32:
+        raise ValueError(f"balance_loss_backward: tokens must be int32 {list(lead)} (got {tokens.dtype} {tuple(tokens.shape)})")
     _lib.check_tensors("balance_loss_backward", dev, dloss=dloss, counts=counts, tokens=tokens, mask=mask)
     with _lib.on(dev, stream):
-        logits, dloss, counts, tokens = (t.contiguous() for t in (logits, dloss, counts, tokens))
+        logits, dloss, counts, tokens = logits.contiguous(), dloss.contiguous(), counts.contiguous(), tokens.contiguous()
         mask = None if mask is None else mask.contiguous()
         dlogits = torch.empty_like(logits)
         _lib.call("mm_balance_loss_backward", _p(dloss), _p(logits), _DTYPES[logits.dtype], _p(mask), _p(counts), _p(tokens), B, T,
