@@ -4,8 +4,8 @@
 // sigmoids), c[e] the picks of expert e and n the tokens that take part,
 //   loss = E / (k n^2) sum_e c[e] sum_t p[t][e],
 //   d loss / d logit[t][e] = E / (k n^2) p[t][e] (c[e] - sum_e' c[e'] p[t][e'])        (x (1 - sigmoid) for sigmoids);
-// the counts are constants of the gradient. Both directions read each logit once: 16,384 x 384 fp32 logits take 8.5 + 7.1 us forward
-// (2.9 TB/s in the first launch) and 13.2 backward (3.8 TB/s); small calls are bound by the launches.
+// the counts are constants of the gradient. Both directions read each logit once: 16,384 x 384 fp32 logits take 8.8 + 7.0 us forward
+// (2.9 TB/s in the first launch) and 13.6 backward (3.7 TB/s); small calls are bound by the launches.
 //
 // Forward: a wave takes a row at a time (lane l holds experts l, l + 64, ...) and keeps the sum of its rows' scores in
 // registers; a workgroup of sixteen waves adds its waves' sums through LDS in wave order and writes one partial per chunk

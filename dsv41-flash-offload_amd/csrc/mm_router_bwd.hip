@@ -9,8 +9,8 @@
 //
 // Three launches: the parts of D, row-major for dx (its k is the expert) and transposed for dgate (its k is the token), and
 // of the transposed gate; both products; the sum of dgate's partial results in order, whose tokens are split over enough
-// workgroups to fill the GPU. 16,384 tokens x 4,096 x 384 experts: 355 us a call, the products bound by MFMA at 0.88 to 0.97 PFLOP/s
-// of bf16 work (a large library product reaches 1.13); 700 tokens 38 us, bound by their few steps and the launches.
+// workgroups to fill the GPU. 16,384 tokens x 4,096 x 384 experts: 350 us a call, the products bound by MFMA at 0.88 to 0.97 PFLOP/s
+// of bf16 work (a large library product reaches 1.13); 700 tokens 36 us, bound by their few steps and the launches.
 #include <algorithm>
 #include <type_traits>
 
