@@ -236,8 +236,9 @@ __global__ __launch_bounds__(64 * BL_WAVES) void k_balance(BalanceArgs a)
 
 // Adds the chunks of one sequence for 16 experts: 64 groups of 16 lanes each take a contiguous run of chunks, their sums are
 // added in a fixed order (16 experts a workgroup rather than 64: 256 chunks of 384 experts in 24 workgroups take 7.5 us, in 6
-// they took 11.4). The last of a sequence's slices to finish adds the slices' shares of the loss, in slice order.
+// they took 11.4). The last of a sequence's slices to finish adds the slices' shares of the loss.
 constexpr int BL_SLICE = 16;
+static_assert(1024 / BL_SLICE <= 64, "a lane per slice");
 __global__ __launch_bounds__(64 * BL_WAVES) void k_balance_sum(BalanceArgs a)
 {
     constexpr int GROUPS = 64 * BL_WAVES / BL_SLICE;
@@ -290,19 +291,20 @@ __global__ __launch_bounds__(64 * BL_WAVES) void k_balance_sum(BalanceArgs a)
         a.counts[(size_t)b * a.E + e] = cnt;
     }
     const float dot = wave_sum(lane < BL_SLICE && e < a.E ? (float)cnt * s : 0.f);
+    // (at most 64 slices, a lane each: one after the other they took 0.15 us each)
+    float* pl = a.part_loss + (size_t)b * gridDim.x;
+    int before = 0;
     if (lane == 0)
     {
-        float* pl = a.part_loss + (size_t)b * gridDim.x;
         __hip_atomic_store(pl + blockIdx.x, dot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const int before = __hip_atomic_fetch_add(a.done + b, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-        if (before == (int)gridDim.x - 1)
-        {
-            float t = 0.f;
-            for (int i = 0; i < (int)gridDim.x; ++i)
-                t += __hip_atomic_load(pl + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            a.loss[b] = balance_factor(a.E, a.k, n) * t;
-            a.tokens[b] = n;
-        }
+        before = __hip_atomic_fetch_add(a.done + b, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (__builtin_amdgcn_readfirstlane(before) != (int)gridDim.x - 1) return;
+    const float t = wave_sum(lane < (int)gridDim.x ? __hip_atomic_load(pl + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.f);
+    if (lane == 0)
+    {
+        a.loss[b] = balance_factor(a.E, a.k, n) * t;
+        a.tokens[b] = n;
     }
 }
 
