@@ -4,8 +4,8 @@
 // sigmoids), c[e] the picks of expert e and n the tokens that take part,
 //   loss = E / (k n^2) sum_e c[e] sum_t p[t][e],
 //   d loss / d logit[t][e] = E / (k n^2) p[t][e] (c[e] - sum_e' c[e'] p[t][e'])        (x (1 - sigmoid) for sigmoids);
-// the counts are constants of the gradient. Both directions read each logit once: 16,384 x 384 fp32 logits take 8.8 + 7.0 us forward
-// (2.9 TB/s in the first launch) and 13.6 backward (3.7 TB/s); small calls are bound by the launches.
+// the counts are constants of the gradient. Both directions read each logit once: 16,384 x 384 fp32 logits take 8.8 + 5.1 us forward
+// (2.9 TB/s in the first launch) and 13.0 backward (3.9 TB/s); small calls are bound by the launches.
 //
 // Forward: a wave takes a row at a time (lane l holds experts l, l + 64, ...) and keeps the sum of its rows' scores in
 // registers; a workgroup of sixteen waves adds its waves' sums through LDS in wave order and writes one partial per chunk
@@ -235,8 +235,8 @@ __global__ __launch_bounds__(64 * BL_WAVES) void k_balance(BalanceArgs a)
 }
 
 // Adds the chunks of one sequence for 16 experts: 64 groups of 16 lanes each take a contiguous run of chunks, their sums are
-// added in a fixed order (16 experts a workgroup rather than 64: 256 chunks of 384 experts in 24 workgroups take 7.5 us, in 6
-// they took 11.4). The last of a sequence's slices to finish adds the slices' shares of the loss.
+// added in a fixed order (16 experts a workgroup rather than 64: 256 chunks of 384 experts in 24 workgroups took 7.5 us, in 6 11.4, both
+// before the shares of the loss were added by a wave at once: 5.1). The last of a sequence's slices to finish adds the slices' shares of the loss.
 constexpr int BL_SLICE = 16;
 static_assert(1024 / BL_SLICE <= 64, "a lane per slice");
 __global__ __launch_bounds__(64 * BL_WAVES) void k_balance_sum(BalanceArgs a)
