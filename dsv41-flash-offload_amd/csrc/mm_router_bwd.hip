@@ -2,15 +2,17 @@
 //   d[t][j] = w[t][j] (dw[t][j] - sum_i w[t][i] dw[t][i]),   D = dlogits + d scattered to the picks,
 //   dx = D gate,   dgate = D^T x.
 //
-// Both products run on v_mfma_f32_16x16x32_bf16 with fp32 accumulation. The fp32 factors are split into bf16 parts
-// (D = D1 + D2 + D3 exactly, gate = G1 + G2 up to 2^-17 of it): dgate multiplies the three parts of D with the bf16 x, so
-// every product is exact and the accumulation is the only rounding; dx takes D1 G1 + D1 G2 + D2 G1, which leaves out about
-// 2^-16 of a product where the bf16 result is rounded by 2^-9.
+// Both products run on v_mfma_f32_16x16x32 with fp32 accumulation. dgate multiplies three bf16 parts of D (D = D1 + D2 + D3
+// exactly) with the bf16 x, so every product is exact and the accumulation is the only rounding. dx takes D1 G1 + D1 G2 + D2 G1
+// of two fp16 parts each, under a power of two per token of D and per hidden index of the gate: two parts leave 2^-22 of a value
+// and what is left out of a product is 3 x 2^-22 of it (2^-33 of the row's largest where values lie far below that), so that rows of D
+// that sum to zero cancel what the gate's rows share as fp32 products do. (Two bf16 parts left up to 2^-13.7 of a product.)
 //
-// Three launches: the parts of D, row-major for dx (its k is the expert) and transposed for dgate (its k is the token), and
+// Four launches: the largest values that the powers of two come from; the parts of D, row-major for dx (its k is the expert) and transposed for dgate (its k is the token), and
 // of the transposed gate; both products; the sum of dgate's partial results in order, whose tokens are split over enough
-// workgroups to fill the GPU. 16,384 tokens x 4,096 x 384 experts: 350 us a call, the products bound by MFMA at 0.88 to 0.97 PFLOP/s
-// of bf16 work (a large library product reaches 1.13); 700 tokens 36 us, bound by their few steps and the launches.
+// workgroups to fill the GPU. 16,384 tokens x 4,096 x 384 experts: 389 us a call (357 with
+// two bf16 parts and no powers of two), the products bound by MFMA at 0.82 PFLOP/s of 16-bit work (a large library product reaches
+// 1.13); 700 tokens 39.7 us (35.9), bound by their few steps and the launches.
 #include <algorithm>
 #include <type_traits>
 
@@ -20,6 +22,7 @@ namespace mm {
 
 typedef float rb_f4 __attribute__((ext_vector_type(4)));
 typedef __bf16 rb_bf8 __attribute__((ext_vector_type(8)));
+typedef _Float16 rb_h8 __attribute__((ext_vector_type(8)));
 typedef short rb_s4 __attribute__((ext_vector_type(4)));
 typedef uint32_t rb_u4 __attribute__((ext_vector_type(4)));
 
@@ -42,24 +45,88 @@ __device__ __forceinline__ void split3(float v, uint16_t& a, uint16_t& b, uint16
     c = f2bf(r1 - __uint_as_float((uint32_t)b << 16));
 }
 
+// v 2^s = a + b in fp16 but for 2^-22 of it (and 2^-25); inf and NaN stay in a.
+__device__ __forceinline__ void split2(float v, int s, uint16_t& a, uint16_t& b)
+{
+    const float x = ldexpf(v, s);
+    a = f2h(x);
+    b = f2h(fabsf(x) < INFINITY ? x - h2f(a) : 0.f);
+}
+// Bits of |v|, 0 for inf and NaN: the largest of them over a row gives its power of two.
+__device__ __forceinline__ uint32_t finite_bits(float v)
+{
+    const uint32_t u = __float_as_uint(v) & 0x7fffffffu;
+    return u < 0x7f800000u ? u : 0u;
+}
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v)
+{
+    v = max(v, (uint32_t)xor_lane_i<1>((int)v));
+    v = max(v, (uint32_t)xor_lane_i<2>((int)v));
+    v = max(v, (uint32_t)xor_lane_i<4>((int)v));
+    v = max(v, (uint32_t)xor_lane_i<8>((int)v));
+    v = max(v, (uint32_t)xor_lane_i<16>((int)v));
+    return max(v, (uint32_t)xor_lane_i<32>((int)v));
+}
+// The power of two for values whose largest magnitude has bits u: that one comes to at least 2^8, and a sum of a logit's gradient
+// and 32 picks' of this size stays below 2^15.
+__device__ __forceinline__ int row_scale(uint32_t u) { return u == 0 ? 0 : 8 + 127 - (int)(u >> 23); }
+
 // ---------------------------------------------------------------------------------------------------------
-// The parts, 64 x 64 tiles: of D = dlogits + scattered top-k gradient in both orders (the first `tiles` workgroups), and of the
-// transposed gate (gt [2][H][Ek], zeros past E).
+// The largest finite values that the powers of two come from, as bits: of each row of dlogits (dmax [T], a wave a row), and of each
+// of the gate's columns over runs of RB_RUN experts (gmax [runs][H], four columns a lane, rows read whole; workgroups past `rows`). A
+// launch of its own: with every 64 x 64 tile below reading its rows and columns to their ends, 700 tokens took 22 us more.
 // ---------------------------------------------------------------------------------------------------------
-// Parts q < N of four neighbours v at out + q * stride (8 bytes a lane).
+constexpr int RB_RUN = 8;
+__host__ __device__ constexpr int gate_runs(int E) { return (E + RB_RUN - 1) / RB_RUN; }
+__global__ __launch_bounds__(256) void k_rb_largest(const float* __restrict__ dlogits, const float* __restrict__ gate, int T, int E, int H,
+                                                    uint32_t* __restrict__ dmax, uint32_t* __restrict__ gmax, int rows)
+{
+    if ((int)blockIdx.x < rows)
+    {
+        const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
+        if (t >= T) return;
+        uint32_t m = 0;
+#pragma unroll 8
+        for (int e = threadIdx.x & 63; e < E; e += 64) m = max(m, finite_bits(dlogits[(size_t)t * E + e]));
+        m = wave_umax(m);
+        if ((threadIdx.x & 63) == 0) dmax[t] = m;
+        return;
+    }
+    typedef rb_f4 __attribute__((aligned(4))) f4_any;
+    const int nh = (H + 1023) / 1024, b = blockIdx.x - rows, h = b % nh * 1024 + 4 * threadIdx.x, e0 = b / nh * RB_RUN;
+    if (h >= H) return;
+    uint32_t m[4] = { 0, 0, 0, 0 };
+#pragma unroll
+    for (int j = 0; j < RB_RUN; ++j)
+    {
+        const rb_f4 g = *reinterpret_cast<const f4_any*>(gate + (size_t)min(e0 + j, E - 1) * H + h);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m[i] = max(m[i], finite_bits(g[i]));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) gmax[(size_t)(b / nh) * H + h + i] = m[i];
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// The parts, 64 x 64 tiles: of D = dlogits + scattered top-k gradient in both orders (the first `tiles` workgroups; d [2][T][Ek] in
+// fp16 under 2^ds[t], dt [3][E][Tk] in bf16), and of the transposed gate (gt [2][H][Ek] in fp16 under 2^gs[h], zeros past E).
+// ---------------------------------------------------------------------------------------------------------
+// Parts q < N of four neighbours v at out + q * stride (8 bytes a lane): three of bf16, or two of fp16 under 2^s.
 template <int N>
-__device__ __forceinline__ void store_parts(const float (&v)[4], uint16_t* out, size_t stride)
+__device__ __forceinline__ void store_parts(const float (&v)[4], int s, uint16_t* out, size_t stride)
 {
     uint16_t p[4][3];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) split3(v[i], p[i][0], p[i][1], p[i][2]);
+    for (int i = 0; i < 4; ++i)
+        if constexpr (N == 3) split3(v[i], p[i][0], p[i][1], p[i][2]);
+        else split2(v[i], s, p[i][0], p[i][1]);
 #pragma unroll
     for (int q = 0; q < N; ++q)
         *reinterpret_cast<uint2*>(out + q * stride) = make_uint2(p[0][q] | ((uint32_t)p[1][q] << 16), p[2][q] | ((uint32_t)p[3][q] << 16));
 }
 
-__device__ __forceinline__ void gate_parts(const float* __restrict__ gate, int E, int H, int Ek, uint16_t* __restrict__ gt, float (*tile)[65],
-                                           int b)
+__device__ __forceinline__ void gate_parts(const float* __restrict__ gate, int E, int H, int Ek, uint16_t* __restrict__ gt, const uint32_t* __restrict__ gmax,
+                                           int32_t* __restrict__ gs, float (*tile)[65], int* scale, int b)
 {
     typedef rb_f4 __attribute__((aligned(4))) f4_any;
     const int nh = (H + 63) / 64, h0 = b % nh * 64, e0 = b / nh * 64, tid = threadIdx.x, c = 4 * (tid & 15);
@@ -74,6 +141,14 @@ __device__ __forceinline__ void gate_parts(const float* __restrict__ gate, int E
     for (int u = 0; u < 4; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) tile[(tid >> 4) + 16 * u][c + i] = v[u][i];
+    if (tid < 64 && h0 + tid < H)
+    {
+        uint32_t m = 0;
+#pragma unroll 8
+        for (int r = 0; r < gate_runs(E); ++r) m = max(m, gmax[(size_t)r * H + h0 + tid]);
+        scale[tid] = row_scale(m);
+        if (e0 == 0) gs[h0 + tid] = scale[tid];
+    }
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < 4; ++u)
@@ -81,19 +156,22 @@ __device__ __forceinline__ void gate_parts(const float* __restrict__ gate, int E
         const int r = (tid >> 4) + 16 * u;
         if (h0 + r >= H) continue;
         const float w[4] = { tile[c][r], tile[c + 1][r], tile[c + 2][r], tile[c + 3][r] };
-        store_parts<2>(w, gt + (size_t)(h0 + r) * Ek + e0 + c, (size_t)H * Ek);
+        store_parts<2>(w, scale[r], gt + (size_t)(h0 + r) * Ek + e0 + c, (size_t)H * Ek);
     }
 }
 
 __global__ __launch_bounds__(256) void k_rb_parts(const int64_t* __restrict__ ids, const float* __restrict__ w,
                                                   const float* __restrict__ dw, const float* __restrict__ dlogits,
                                                   const float* __restrict__ gate, int T, int E, int H, int k, int Ek, int Tk,
-                                                  uint16_t* __restrict__ d, uint16_t* __restrict__ dt, uint16_t* __restrict__ gt, int tiles)
+                                                  uint16_t* __restrict__ d, uint16_t* __restrict__ dt, uint16_t* __restrict__ gt,
+                                                  const uint32_t* __restrict__ dmax, const uint32_t* __restrict__ gmax,
+                                                  int32_t* __restrict__ ds, int32_t* __restrict__ gs, int tiles)
 {
     __shared__ float tile[64][65];
     __shared__ float sw[64 * 32], sd[64 * 32];
     __shared__ int se[64 * 32];
-    if ((int)blockIdx.x >= tiles) return gate_parts(gate, E, H, Ek, gt, tile, blockIdx.x - tiles);
+    __shared__ int scale[64];
+    if ((int)blockIdx.x >= tiles) return gate_parts(gate, E, H, Ek, gt, gmax, gs, tile, scale, blockIdx.x - tiles);
     const int ne = (E + 63) / 64, t0 = (int)blockIdx.x / ne * 64, e0 = (int)blockIdx.x % ne * 64, tid = threadIdx.x;
     // all loads at once: the tile's logit gradients, and the rows' picks (their expert within the tile, or -1)
     float v[16];
@@ -115,15 +193,28 @@ __global__ __launch_bounds__(256) void k_rb_parts(const int64_t* __restrict__ id
     }
 #pragma unroll
     for (int u = 0; u < 16; ++u) tile[(tid + 256 * u) >> 6][tid & 63] = v[u];
+    uint32_t m = d && dlogits && tid < min(64, T - t0) ? dmax[t0 + tid] : 0u;
     __syncthreads();
     // a thread per row adds its picks in ascending j (an expert picked twice gets both)
-    if (tid * k < picks)
+    if (tid < 64)
     {
         const int at = tid * k;
-        float s = 0.f;
-        for (int j = 0; j < k; ++j) s = fmaf(sw[at + j], sd[at + j], s);
-        for (int j = 0; j < k; ++j)
-            if (se[at + j] >= 0) tile[tid][se[at + j]] += sw[at + j] * (sd[at + j] - s);
+        if (at < picks)
+        {
+            float s = 0.f;
+            for (int j = 0; j < k; ++j) s = fmaf(sw[at + j], sd[at + j], s);
+            for (int j = 0; j < k; ++j)
+            {
+                const float p = sw[at + j] * (sd[at + j] - s);
+                m = max(m, finite_bits(p));
+                if (se[at + j] >= 0) tile[tid][se[at + j]] += p;
+            }
+        }
+        if (d)
+        {
+            scale[tid] = row_scale(m);
+            if (e0 == 0 && t0 + tid < T) ds[t0 + tid] = scale[tid];
+        }
     }
     __syncthreads();
     // four neighbours along the contiguous index of each order (Ek and Tk are multiples of 64)
@@ -135,32 +226,41 @@ __global__ __launch_bounds__(256) void k_rb_parts(const int64_t* __restrict__ id
         if (d && t0 + r < T)
         {
             const float x[4] = { tile[r][c], tile[r][c + 1], tile[r][c + 2], tile[r][c + 3] };
-            store_parts<2>(x, d + (size_t)(t0 + r) * Ek + e0 + c, (size_t)T * Ek);
+            store_parts<2>(x, scale[r], d + (size_t)(t0 + r) * Ek + e0 + c, (size_t)T * Ek);
         }
         if (dt && e0 + r < E)
         {
             const float x[4] = { tile[c][r], tile[c + 1][r], tile[c + 2][r], tile[c + 3][r] };
-            store_parts<3>(x, dt + (size_t)(e0 + r) * Tk + t0 + c, (size_t)E * Tk);
+            store_parts<3>(x, 0, dt + (size_t)(e0 + r) * Tk + t0 + c, (size_t)E * Tk);
         }
     }
 }
 
 // ---------------------------------------------------------------------------------------------------------
 // The products in RB_H (hidden indices h) x RB_C (columns c: tokens or experts) tiles, four waves of RB_H / 2 x RB_C / 2.
-// DX: rows are gt's (k = expert), columns d's, result dx[c][h] in bf16.
+// DX: rows are gt's (k = expert), columns d's, result dx[c][h] in bf16, without the powers of two of its row and column.
 // else: rows are columns of x (k = token, read transposed from LDS), columns dt's, result part[z][c][h] in fp32.
 // ---------------------------------------------------------------------------------------------------------
 struct GemmArgs
 {
     const uint16_t *rows, *cols;
+    const int32_t *rscale, *cscale;
     const float* gate;
     void* out;
     int H, C, T, K, E, ksteps;
 };
 constexpr int RB_LDS = std::max(2 * RB_H * RB_ROW + 2 * RB_C * RB_ROW, RB_K * RB_XROW + 3 * RB_C * RB_ROW);
 
+template <bool HALF>
+__device__ __forceinline__ rb_f4 rb_mfma(rb_u4 a, rb_u4 b, rb_f4 c)
+{
+    if constexpr (HALF)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(rb_h8, a), __builtin_bit_cast(rb_h8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(rb_bf8, a), __builtin_bit_cast(rb_bf8, b), c, 0, 0, 0);
+}
+
 template <bool DX>
-__device__ __forceinline__ void rb_tile(const GemmArgs& a, uint16_t* lds, int bh, int bc, int bz)
+__device__ __forceinline__ void rb_tile(const GemmArgs& a, uint16_t* lds, int* scale, int bh, int bc, int bz)
 {
     constexpr int PR = DX ? 2 : 1, PC = DX ? 2 : 3;
     constexpr int RT = RB_H / 32, CT = RB_C / 32;          // 16 x 16 tiles per wave
@@ -204,6 +304,7 @@ __device__ __forceinline__ void rb_tile(const GemmArgs& a, uint16_t* lds, int bh
 #pragma unroll
         for (int j = 0; j < CT; ++j) acc[i][j] = rb_f4{ 0.f, 0.f, 0.f, 0.f };
     if (s0 < s1) load(s0);
+    if constexpr (DX) scale[tid] = tid < RB_H ? a.rscale[min(h0 + tid, H - 1)] : a.cscale[min(c0 + tid - RB_H, C - 1)];
     for (int s = s0; s < s1; ++s)
     {
         __syncthreads();                                  // the previous step's operand reads are done
@@ -232,11 +333,11 @@ __device__ __forceinline__ void rb_tile(const GemmArgs& a, uint16_t* lds, int bh
 #pragma unroll
         for (int u = 0; u < RB_K / 32; ++u)
         {
-            rb_bf8 R[RT], Cc[CT];
+            rb_u4 R[RT], Cc[CT];
             auto read_rows = [&](int p) {
 #pragma unroll
                 for (int i = 0; i < RT; ++i)
-                    if constexpr (DX) R[i] = *reinterpret_cast<const rb_bf8*>(&rs[p * RB_H * RB_ROW + rb_at(wh + 16 * i + r, 4 * u + q)]);
+                    if constexpr (DX) R[i] = *reinterpret_cast<const rb_u4*>(&rs[p * RB_H * RB_ROW + rb_at(wh + 16 * i + r, 4 * u + q)]);
                     else
                     {
                         // four tokens x 16 hidden indices per transposed read: lane r of a quarter names token r >> 2 and four
@@ -245,13 +346,13 @@ __device__ __forceinline__ void rb_tile(const GemmArgs& a, uint16_t* lds, int bh
                         uint16_t* at = &rs[(32 * u + 8 * q + (r >> 2)) * RB_XROW + wh + 16 * i + 4 * (r & 3)];
                         const rb_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at);
                         const rb_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 4 * RB_XROW));
-                        R[i] = __builtin_bit_cast(rb_bf8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                        R[i] = __builtin_bit_cast(rb_u4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
                     }
             };
             auto read_cols = [&](int p) {
 #pragma unroll
                 for (int j = 0; j < CT; ++j)
-                    Cc[j] = *reinterpret_cast<const rb_bf8*>(&cs[p * RB_C * RB_ROW + rb_at(wc + 16 * j + r, 4 * u + q)]);
+                    Cc[j] = *reinterpret_cast<const rb_u4*>(&cs[p * RB_C * RB_ROW + rb_at(wc + 16 * j + r, 4 * u + q)]);
             };
             // dx: G1 D2, G1 D1, G2 D1; dgate: x D3, x D2, x D1
             read_rows(0);
@@ -267,7 +368,7 @@ __device__ __forceinline__ void rb_tile(const GemmArgs& a, uint16_t* lds, int bh
 #pragma unroll
                 for (int i = 0; i < RT; ++i)
 #pragma unroll
-                    for (int j = 0; j < CT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(R[i], Cc[j], acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < CT; ++j) acc[i][j] = rb_mfma<DX>(R[i], Cc[j], acc[i][j]);
             }
         }
     }
@@ -284,6 +385,7 @@ __device__ __forceinline__ void rb_tile(const GemmArgs& a, uint16_t* lds, int bh
             {
                 // an infinite gradient times a zero part of the gate is NaN: such results are summed again from whole factors,
                 // so that they are what the formula gives (inf, or NaN)
+                const int cs = scale[RB_H + c - c0];
 #pragma unroll
                 for (int m = 0; m < 4; ++m)
                     if (v[m] != v[m])
@@ -292,10 +394,10 @@ __device__ __forceinline__ void rb_tile(const GemmArgs& a, uint16_t* lds, int bh
                         for (int e = 0; e < a.E; ++e)
                         {
                             const uint16_t* d = a.cols + (size_t)c * K + e;
-                            v[m] = fmaf(__uint_as_float((uint32_t)d[0] << 16) + __uint_as_float((uint32_t)d[(size_t)C * K] << 16),
-                                        a.gate[(size_t)e * H + h + m], v[m]);
+                            v[m] = fmaf(ldexpf(h2f(d[0]) + h2f(d[(size_t)C * K]), -cs), a.gate[(size_t)e * H + h + m], v[m]);
                         }
                     }
+                    else v[m] = ldexpf(v[m], -(cs + scale[h - h0 + m]));
                 *reinterpret_cast<uint2*>((uint16_t*)a.out + (size_t)c * H + h) =
                     make_uint2(f2bf(v[0]) | ((uint32_t)f2bf(v[1]) << 16), f2bf(v[2]) | ((uint32_t)f2bf(v[3]) << 16));
             }
@@ -308,16 +410,18 @@ __device__ __forceinline__ void rb_tile(const GemmArgs& a, uint16_t* lds, int bh
 __global__ __launch_bounds__(256, 2) void k_rb_gemm(GemmArgs dx, GemmArgs dg, int dx_blocks)
 {
     __shared__ __align__(16) uint16_t lds[RB_LDS];
+    __shared__ int scale[RB_H + RB_C];                      // of dx's rows and columns
+    static_assert(RB_H + RB_C == 256, "one a thread");
     const int b = blockIdx.x;
     if (b < dx_blocks)
     {
         const int nh = (dx.H + RB_H - 1) / RB_H;
-        rb_tile<true>(dx, lds, b % nh, b / nh, 0);
+        rb_tile<true>(dx, lds, scale, b % nh, b / nh, 0);
     }
     else
     {
         const int i = b - dx_blocks, nh = (dg.H + RB_H - 1) / RB_H, nc = (dg.C + RB_C - 1) / RB_C;
-        rb_tile<false>(dg, lds, i % nh, i / nh % nc, i / nh / nc);
+        rb_tile<false>(dg, lds, scale, i % nh, i / nh % nc, i / nh / nc);
     }
 }
 
@@ -340,7 +444,7 @@ static int rb_splits(int T, int H, int E)
 }
 struct RouterBwdWs
 {
-    size_t d, dt, gt, part, total;
+    size_t d, dt, gt, dmax, gmax, ds, gs, part, total;
 };
 static RouterBwdWs router_bwd_ws(int T, int H, int E)
 {
@@ -351,6 +455,10 @@ static RouterBwdWs router_bwd_ws(int T, int H, int E)
     w.d = take(2 * (size_t)T * Ek * 2);
     w.dt = take(3 * (size_t)E * Tk * 2);
     w.gt = take(2 * (size_t)H * Ek * 2);
+    w.dmax = take((size_t)T * 4);
+    w.gmax = take((size_t)gate_runs(E) * H * 4);
+    w.ds = take((size_t)T * 4);
+    w.gs = take((size_t)H * 4);
     const int S = rb_splits(T, H, E);
     w.part = take(S > 1 ? (size_t)S * E * H * 4 : 0);
     w.total = at;
@@ -394,22 +502,30 @@ int mm_router_backward(const void* x_bf16, int T, int H, const float* gate, int 
                  "mm_router_backward: workspace too small or misaligned (%zu < %zu)", workspace_bytes, s.total);
     unsigned char* p = static_cast<unsigned char*>(workspace);
     uint16_t *d = (uint16_t*)(p + s.d), *dt = (uint16_t*)(p + s.dt), *gt = (uint16_t*)(p + s.gt);
+    uint32_t *dmax = (uint32_t*)(p + s.dmax), *gmax = (uint32_t*)(p + s.gmax);
+    int32_t *ds = (int32_t*)(p + s.ds), *gs = (int32_t*)(p + s.gs);
     if (dx_bf16 && T)
     {
-        gx = { gt, d, gate, dx_bf16, H, T, T, Ek, E, Ek / RB_K };
+        gx = { gt, d, gs, ds, gate, dx_bf16, H, T, T, Ek, E, Ek / RB_K };
         dx_blocks = nh * ((T + RB_C - 1) / RB_C);
     }
     if (dgate)
     {
         const int steps = Tk / RB_K;
-        gg = { (const uint16_t*)x_bf16, dt, nullptr, S > 1 ? (void*)(p + s.part) : dgate, H, E, T, Tk, E, (steps + S - 1) / S };
+        gg = { (const uint16_t*)x_bf16, dt, nullptr, nullptr, nullptr, S > 1 ? (void*)(p + s.part) : dgate, H, E, T, Tk, E, (steps + S - 1) / S };
         dg_blocks = nh * ((E + RB_C - 1) / RB_C) * S;
     }
     if (T)
     {
         const int tiles = (E + 63) / 64 * ((T + 63) / 64), gate_tiles = dx_bf16 ? (H + 63) / 64 * ((E + 63) / 64) : 0;
+        if (dx_bf16)
+        {
+            const int rows = dlogits ? (T + 3) / 4 : 0;
+            hipLaunchKernelGGL(k_rb_largest, dim3(rows + (H + 1023) / 1024 * gate_runs(E)), dim3(256), 0, hs, dlogits, gate, T, E, H, dmax,
+                               gmax, rows);
+        }
         hipLaunchKernelGGL(k_rb_parts, dim3(tiles + gate_tiles), dim3(256), 0, hs, ids, w, dw, dlogits, gate, T, E, H, k, Ek, Tk,
-                           dx_bf16 ? d : nullptr, dgate ? dt : nullptr, gt, tiles);
+                           dx_bf16 ? d : nullptr, dgate ? dt : nullptr, gt, dmax, gmax, ds, gs, tiles);
     }
     if (dx_blocks + dg_blocks == 0) return MM_OK;
     hipLaunchKernelGGL(k_rb_gemm, dim3(dx_blocks + dg_blocks), dim3(256), 0, hs, gx, gg, dx_blocks);

@@ -67,8 +67,8 @@ int mm_router_topk(const void* x_bf16, int T, int H, const float* gate, int E, i
  *   D = dlogits + scatter(w[t][j] (dw[t][j] - sum_i w[t][i] dw[t][i]) at ids[t][j]),
  *   dx bf16 [T][H] = D gate, dgate fp32 [E][H] = D^T x   (either NULL: not computed).
  * x, gate, ids and w as mm_router_topk took and gave them (ids outside [0, E) get no gradient, a pick named twice gets
- * both). fp32 factors are multiplied as exact sums of bf16 parts with fp32 accumulation (dx leaves out products below 2^-16 of
- * the largest part). T <= 2^21, H a multiple of 16, E <= 1024, k <= 32; x, dx, dgate and the workspace 16-byte aligned. */
+ * both). fp32 factors are multiplied in parts with fp32 accumulation: exactly in dgate, in dx to 3 x 2^-22 of each product (and
+ * 2^-33 of the largest of its row of D times the largest of its column of the gate). T <= 2^21, H a multiple of 16, E <= 1024, k <= 32; x, dx, dgate and the workspace 16-byte aligned. */
 size_t mm_router_backward_workspace(int T, int H, int E);
 int mm_router_backward(const void* x_bf16, int T, int H, const float* gate, int E, int k, const int64_t* ids, const float* w,
                        const float* dw, const float* dlogits, void* dx_bf16, float* dgate, void* workspace,
