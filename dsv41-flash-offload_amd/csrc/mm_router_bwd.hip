@@ -34,15 +34,31 @@ constexpr int RB_ROW = RB_K;
 constexpr int RB_XROW = RB_H + 16;       // LDS row of the token-major input tile (32 bytes of padding: transposed reads of four rows hit distinct banks)
 __device__ __forceinline__ int rb_at(int r, int q) { return r * RB_ROW + 8 * (q ^ ((r >> 1) & 7)); }
 
-// v = a + b + c in bf16: a truncated (no overflow), b rounded, c the rest, exact. inf and NaN stay in a.
+// v = a + b + c in bf16, exactly, all of v's sign and none of them zero (but for v below 2^-100, or zero), so that their products with
+// an infinite input are all the infinity that v's is: a and b truncated, c the rest; what is left of a value of few bits is zero, and
+// the last part that is not is taken apart into halves. Of an infinite v or NaN every part is v.
 __device__ __forceinline__ void split3(float v, uint16_t& a, uint16_t& b, uint16_t& c)
 {
-    const uint32_t u = __float_as_uint(v);
-    const bool fin = (u & 0x7f800000u) != 0x7f800000u;
-    a = (uint16_t)((u >> 16) | ((u & 0x7fffffffu) > 0x7f800000u ? 0x40u : 0u));
-    const float r1 = fin ? v - __uint_as_float(u & 0xffff0000u) : 0.f;
-    b = f2bf(r1);
-    c = f2bf(r1 - __uint_as_float((uint32_t)b << 16));
+    const uint32_t u = __float_as_uint(v), m = u & 0x7fffffffu;
+    float p = __uint_as_float(u & 0xffff0000u), r = v - p;
+    float q = __uint_as_float(__float_as_uint(r) & 0xffff0000u), s = r - q;
+    if (m >= 0x0d800000u)                     // 2^-100: the halves are exact
+    {
+        if (r == 0.f)
+        {
+            p = 0.5f * v;
+            r = p;
+        }
+        if (s == 0.f)
+        {
+            q = 0.5f * r;
+            s = q;
+        }
+    }
+    a = (uint16_t)(__float_as_uint(p) >> 16);
+    b = (uint16_t)(__float_as_uint(q) >> 16);
+    c = (uint16_t)(__float_as_uint(s) >> 16);
+    if (m >= 0x7f800000u) a = b = c = (uint16_t)((u >> 16) | (m > 0x7f800000u ? 0x40u : 0u));
 }
 
 // v 2^s = a + b in fp16 but for 2^-22 of it (and 2^-25); inf and NaN stay in a.

@@ -66,7 +66,7 @@ int mm_router_topk(const void* x_bf16, int T, int H, const float* gate, int E, i
  * dlogits fp32 [T][E] (NULL: none; of a loss on the logits such as mm_balance_loss) of its outputs,
  *   D = dlogits + scatter(w[t][j] (dw[t][j] - sum_i w[t][i] dw[t][i]) at ids[t][j]),
  *   dx bf16 [T][H] = D gate, dgate fp32 [E][H] = D^T x   (either NULL: not computed).
- * x, gate, ids and w as mm_router_topk took and gave them (ids outside [0, E) get no gradient, a pick named twice gets
+ * x, gate, ids and w as mm_router_topk took and gave them; infinite values give what IEEE products and sums of the formula give (ids outside [0, E) get no gradient, a pick named twice gets
  * both). fp32 factors are multiplied in parts with fp32 accumulation: exactly in dgate, in dx to 3 x 2^-22 of each product (and
  * 2^-33 of the largest of its row of D times the largest of its column of the gate). T <= 2^21, H a multiple of 16, E <= 1024, k <= 32; x, dx, dgate and the workspace 16-byte aligned. */
 size_t mm_router_backward_workspace(int T, int H, int E);

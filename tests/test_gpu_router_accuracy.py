@@ -83,3 +83,37 @@ def test_dx_of_picks_that_cancel_the_logits_gradient(dev):
     one = router64(x, gate, ids, w, dw, torch.zeros_like(dl))
     # ex counts D's roundings from its own magnitudes; the gradient of the picks alone has the larger ones
     close(dx, rx, 2.0 ** -8 * rx.abs() + (PRODUCT + 3 * 40 * 2.0 ** -23) * mx + ex + one[4] + 2.0 ** -33 * 40 * one[2] + 1e-37)
+
+
+@pytest.mark.parametrize("T,E", [(40, 20), (600, 33)])
+@pytest.mark.parametrize("with_picks", [False, True])
+def test_dgate_of_infinite_inputs_and_gradients(dev, T, E, with_picks):
+    """dgate = D^T x with infinities as IEEE products and sums have them: +-inf by the signs, NaN for 0 x inf and inf - inf, whatever parts
+    D is made of (values of few bits among them); the rest within the sums' roundings."""
+    from mi355moe import router
+    H = 48
+    x, gate, ids, w, dw, dl = router_inputs(T, H, E, 3, T + E, dev)
+    dl[3] = torch.tensor([1.0, -2.0, 0.375, 1 + 2.0 ** -7, -1 - 2.0 ** -8, 0.0])[torch.arange(E) % 6].to(dev)
+    dl[7, ::2] = 0.0
+    x[3, 5], x[7, 11], x[9, 13] = torch.inf, -torch.inf, torch.inf
+    x[T - 1, 13] = torch.inf
+    dl[12, 4], x[12, 20] = -torch.inf, 0.0
+    x[15, 30] = torch.finfo(torch.bfloat16).max
+    dl[15] = 2.0 ** -8
+    dw = dw if with_picks else None
+    _, dgate = router.topk_backward(x, gate, ids, w, dw, dl, need_x=False)
+    _, ref, _, _, _, err = router64(x, gate, ids, w, dw, dl)
+    if with_picks:                                             # (a pick may move D off zero, or leave it there)
+        assert (torch.isinf(ref[:, 5]) | ref[:, 5].isnan()).all()
+    got = dgate.cpu().double()
+    assert torch.equal(got.isnan(), ref.isnan())
+    assert torch.equal(got == torch.inf, ref == torch.inf) and torch.equal(got == -torch.inf, ref == -torch.inf)
+    assert (ref == torch.inf).any() and (ref == -torch.inf).any() and ref.isnan().any()
+    ok = ref.isfinite()
+    D, x64 = dl.cpu().double(), x.cpu().double()
+    if with_picks:
+        d = w * (dw - (w * dw).sum(1, keepdim=True))
+        D = D.scatter_add(1, ids.cpu(), d.cpu().double())
+    mag = torch.nan_to_num(D.abs(), posinf=0.0).t() @ torch.nan_to_num(x64.abs(), posinf=0.0)
+    tol = (3 * T + 64) * 2.0 ** -23 * mag + torch.nan_to_num(err, nan=0.0, posinf=0.0) + 1e-37
+    assert ((got - ref).abs()[ok] <= tol[ok]).all()
