@@ -15,9 +15,15 @@ _SCORES = {"softmax": 0, "sigmoid": 1}        # MM_SCORE_*
 _p = _lib.ptr
 
 
+def _capture_stream(device):
+    """Address of the device's current stream, on which a capture runs."""
+    return _lib.raw_stream(device) if device.type == "cuda" else None
+
+
 def _captured_apply(what, fn, leaves, *args):
     """fn.apply(*args). Under stream capture, a leaf among its inputs may not have its gradient node in an autograd graph from before
-    the capture: the captured backward would go to that node's stream, which invalidates the capture and ends the process."""
+    the capture: the captured backward would go to that node's stream, which invalidates the capture and ends the process. (A node that
+    a captured call made belongs to that capture's stream, and passes in captures of that stream only.)"""
     leaves = [t for t in leaves if t.requires_grad and t.is_leaf]
     if not (leaves and torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing()):
         return fn.apply(*args)
@@ -26,15 +32,15 @@ def _captured_apply(what, fn, leaves, *args):
         return torch.autograd.graph.get_gradient_edge(t).node.metadata
 
     for t in leaves:
-        if notes(t).get("mi355moe") == "captured":            # used in this capture by an earlier call
+        if notes(t).get("mi355moe captured") == (t.device, _capture_stream(t.device)):
             continue
-        notes(t)["mi355moe"] = "seen"                         # gone with the node if no graph holds it
-        if notes(t).pop("mi355moe", None):
+        notes(t)["mi355moe seen"] = True                      # gone with the node if no graph holds it
+        if notes(t).pop("mi355moe seen", None):
             raise RuntimeError(f"{what}: an input has an autograd graph from before the stream capture; drop it first, or capture "
                                f"{what}_forward and {what}_backward")
     out = fn.apply(*args)
     for t in leaves:
-        notes(t)["mi355moe"] = "captured"
+        notes(t)["mi355moe captured"] = (t.device, _capture_stream(t.device))
     return out
 
 
@@ -114,8 +120,8 @@ class _TopK(torch.autograd.Function):
 
 
 def topk(x, gate, k):
-    """topk_forward on the current stream, with gradients of w and logits into x and gate. Under stream capture an input must not
-    have an autograd graph from before the capture (refused)."""
+    """topk_forward on the current stream, with gradients of w and logits into x and gate. Under stream capture a leaf must not
+    have an autograd graph from before the capture (refused), nor may an input that is not a leaf come from one (not seen here)."""
     return _captured_apply("topk", _TopK, (x, gate), x, gate, k)
 
 

@@ -155,3 +155,42 @@ def test_a_stream_of_another_device_is_refused():
 
     with pytest.raises(ValueError, match="stream of cuda:1"):
         _lib.on(torch.device("cuda", 0), Stream())
+
+
+def test_a_later_capture_is_held_to_its_own_stream(monkeypatch):
+    """A gradient node that a call of an earlier capture made, kept alive by an eager graph, passes in a capture of that stream only."""
+    from mi355moe import router
+
+    class Double(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, t):
+            return 2 * t
+
+        @staticmethod
+        def backward(ctx, d):
+            return 2 * d
+
+    capturing, stream = True, 1
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    monkeypatch.setattr(router, "_capture_stream", lambda device: stream, raising=False)
+
+    def call():
+        return router._captured_apply("topk", Double, (t,), t)
+
+    t = torch.ones(3, requires_grad=True)
+    first = call()
+    capturing = False
+    eager = t.sum()
+    del first
+    capturing, stream = True, 2
+    with pytest.raises(RuntimeError, match="from before the stream capture"):
+        call()
+    stream = 1                                                # the node's own: refusing the other one left its mark in place
+    assert call().requires_grad
+    stream = 2
+    del eager
+    a, b = call(), call()                                     # nothing holds the old node: a new one of this capture
+    assert a.requires_grad and b.requires_grad
+    stream = 1
+    with pytest.raises(RuntimeError, match="from before the stream capture"):
+        call()
