@@ -1085,7 +1085,8 @@ int mm_w4_linear(const void* x, int x_dtype, int M, int K, int N, const mm_w4_t*
                  M, K, N);
     MM_CHECK_ARG(x_dtype >= MM_DTYPE_F16 && x_dtype <= MM_DTYPE_F32 && y_dtype >= MM_DTYPE_F16 && y_dtype <= MM_DTYPE_F32,
                  "mm_w4_linear: bad element type");
-    MM_CHECK_ARG(K < (1 << 22) && N <= (1 << 30), "mm_w4_linear: K must be below 2^22 and N at most 2^30 (K=%d N=%d)", K, N);
+    // (a launch has at most 2^32 threads a dimension, and up to 16 tile rows take 512 for 16 columns)
+    MM_CHECK_ARG(K < (1 << 22) && N <= (1 << 26), "mm_w4_linear: K must be below 2^22 and N at most 2^26 (K=%d N=%d)", K, N);
     MM_CHECK_ARG(M <= (1 << 20), "mm_w4_linear: more than 2^20 rows (%d)", M);
     if (M == 0) return MM_OK;
     MM_CHECK_ARG(x && y && ((uintptr_t)x & 15) == 0, "mm_w4_linear: null or misaligned input (16 bytes)");

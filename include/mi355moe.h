@@ -280,7 +280,7 @@ typedef struct mm_w4
 
 /* y [M][N] (y_dtype) = x [M][K] (x_dtype) W^T. Products are exact, sums fp32, the result is rounded once. x 16-byte aligned.
  * Built for few rows (decode steps); any M up to 2^20 works, at 32 to 80 rows (a third of fp32) per pass over the weights. K < 2^22, N <=
- * 2^30. Workspace: mm_w4_linear_workspace bytes (fp32 inputs only), 16-byte aligned. */
+ * 2^26. Workspace: mm_w4_linear_workspace bytes (fp32 inputs only), 16-byte aligned. */
 size_t mm_w4_linear_workspace(int x_dtype, int M, int K);
 int mm_w4_linear(const void* x, int x_dtype, int M, int K, int N, const mm_w4_t* W, int group, int scale_dtype, void* y,
                  int y_dtype, void* workspace, size_t workspace_bytes, mm_stream_t stream);

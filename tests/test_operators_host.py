@@ -194,3 +194,12 @@ def test_a_later_capture_is_held_to_its_own_stream(monkeypatch):
     stream = 1
     with pytest.raises(RuntimeError, match="from before the stream capture"):
         call()
+
+
+def test_linear_refuses_more_columns_than_a_launch_has():
+    from mi355moe import _lib
+    L = _lib.load()
+    W = _lib.MMW4(256, 256, None)
+    for N in ((1 << 26) + 1, 1 << 27, 1 << 30):
+        assert L.mm_w4_linear(256, 1, 4, 256, N, ctypes.byref(W), 64, 0, 256, 1, None, 0, None) == -1
+        assert b"N at most 2^26" in L.mm_last_error()
