@@ -369,6 +369,7 @@ static BalanceWs balance_ws(int B, int T, int E)
 static int check_balance(const char* what, int dtype, int B, int T, int E, int k, int score)
 {
     MM_CHECK_ARG(B >= 0 && T >= 0 && B <= 65535, "%s: need 0 <= B <= 65535, T >= 0 (B=%d T=%d)", what, B, T);
+    MM_CHECK_ARG(T <= (1 << 30), "%s: more than 2^30 tokens a sequence (%d)", what, T);
     MM_CHECK_ARG(E > 0 && E <= 1024 && k > 0 && k <= 32, "%s: need 0 < E <= 1024, 0 < k <= 32 (E=%d k=%d)", what, E, k);
     MM_CHECK_ARG((size_t)T * k < ((size_t)1 << 31), "%s: too many picks per sequence (T=%d k=%d)", what, T, k);
     MM_CHECK_ARG(dtype == MM_DTYPE_F16 || dtype == MM_DTYPE_BF16 || dtype == MM_DTYPE_F32, "%s: bad logits type %d", what, dtype);
@@ -457,7 +458,7 @@ int mm_balance_loss_backward(const float* dloss, const void* logits, int dtype, 
     if (rc) return rc;
     if (B == 0 || T == 0) return MM_OK;
     MM_CHECK_ARG(dloss && logits && counts && tokens && dlogits, "mm_balance_loss_backward: null pointer");
-    const int rows = 4 * BL_BWD_WAVES;
+    const int rows = 4 * BL_BWD_WAVES * (1 + T / (1 << 27));    // (a launch has at most 2^32 threads)
     const hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
     balance_dispatch(dtype, E, score, [&](auto dt, auto nv, auto sig) {
         hipLaunchKernelGGL((k_balance_bwd<decltype(dt)::value, decltype(nv)::value, decltype(sig)::value>),

@@ -117,3 +117,17 @@ def test_dgate_of_infinite_inputs_and_gradients(dev, T, E, with_picks):
     mag = torch.nan_to_num(D.abs(), posinf=0.0).t() @ torch.nan_to_num(x64.abs(), posinf=0.0)
     tol = (3 * T + 64) * 2.0 ** -23 * mag + torch.nan_to_num(err, nan=0.0, posinf=0.0) + 1e-37
     assert ((got - ref).abs()[ok] <= tol[ok]).all()
+
+
+def test_balance_gradient_of_very_many_tokens(dev):
+    """2^28 tokens: more than a launch has threads for at 16 tokens a workgroup of 256. Equal rows have equal gradients, known from the
+    formula (scores of 1 / 2)."""
+    from mi355moe import router
+    T, E = (1 << 28) + 5, 2
+    logits = torch.zeros((T, E), dtype=torch.float16, device=dev)
+    counts = torch.tensor([3, 1], dtype=torch.int32, device=dev)
+    dloss = torch.tensor(float(T) * T, device=dev)
+    d = router.balance_loss_backward(dloss, logits, counts, torch.tensor(T, dtype=torch.int32, device=dev), 1)
+    assert d.shape == logits.shape
+    assert bool((d[:, 0] == d[0, 0]).all()) and bool((d[:, 1] == -d[0, 0]).all())
+    assert abs(float(d[0, 0]) - E * 0.5 * (3 - 2)) <= 2.0 ** -10

@@ -203,3 +203,13 @@ def test_linear_refuses_more_columns_than_a_launch_has():
     for N in ((1 << 26) + 1, 1 << 27, 1 << 30):
         assert L.mm_w4_linear(256, 1, 4, 256, N, ctypes.byref(W), 64, 0, 256, 1, None, 0, None) == -1
         assert b"N at most 2^26" in L.mm_last_error()
+
+
+def test_balance_refuses_more_than_2_30_tokens():
+    from mi355moe import _lib
+    L = _lib.load()
+    T = (1 << 30) + 1
+    assert L.mm_balance_loss(256, 2, 256, None, 1, T, 8, 1, 0, 256, 256, 256, 256, 256, 1 << 40, None) == -1
+    assert b"2^30" in L.mm_last_error()
+    assert L.mm_balance_loss_backward(256, 256, 2, None, 256, 256, 1, T, 8, 1, 0, 256, None) == -1
+    assert b"2^30" in L.mm_last_error()
