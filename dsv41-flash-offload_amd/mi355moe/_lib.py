@@ -186,6 +186,22 @@ def check_tensors(what, device, **tensors):
         raise ValueError(f"{what}: needs GPU tensors (got {device})")
 
 
+def wants_gradient(**tensors):
+    """Name of the first tensor that autograd would follow into the call, or None."""
+    for name, t in tensors.items():
+        if t.requires_grad:
+            import torch
+            return name if torch.is_grad_enabled() else None
+    return None
+
+
+def no_gradient(what, **tensors):
+    """Refuses tensors that autograd would follow: the result would be cut off from them without a word."""
+    name = wants_gradient(**tensors)
+    if name:
+        raise RuntimeError(f"{what}: {name} requires a gradient, which {what} does not give (detach it, or call under torch.no_grad())")
+
+
 def aligned(t):
     """t with contiguous elements at a 16-byte boundary (a copy if it is not so)."""
     t = t.contiguous()

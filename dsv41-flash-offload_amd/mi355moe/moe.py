@@ -2,6 +2,8 @@
 
 Every computation runs in libmi355moe.so; this module allocates buffers and launches on the current stream.
 """
+import warnings
+
 import torch
 
 from . import _lib, w4
@@ -120,9 +122,16 @@ def moe_forward(store, x, ids, w, shared_expert=None, fat_threshold=FAT_THRESHOL
     decode path. A larger call goes to mm_fused_moe, which takes the decode path or the grouped GEMM by its routes and
     experts. No call synchronises the host, so every call can be captured in a HIP graph.
 
-    A layer of 4-bit experts (w4.W4Store) runs on w4.moe, whatever the threshold."""
+    A layer of 4-bit experts (w4.W4Store) runs on w4.moe, whatever the threshold.
+
+    The output records no gradient, neither into x nor into w (router.topk's weights among them): inputs that require one get a
+    warning here and are refused by w4.moe."""
     if isinstance(store, w4.W4Store):
         return w4.moe(store, x, ids, w, shared_expert=shared_expert, stream=stream)
+    name = _lib.wants_gradient(x=x, w=w)
+    if name:
+        warnings.warn(f"moe_forward: {name} requires a gradient, but the output carries no gradient (detach it, or call under "
+                      "torch.no_grad())", stacklevel=2)
     T = x.shape[0]
     ids, w = _with_shared(ids, w, T, shared_expert)
     k = ids.shape[1]

@@ -4,7 +4,8 @@ Tensors are taken as 4-bit checkpoints store them, and read in place:
   q       int32 [N, K / 8]        weight k = 8 j + i of a row in bits 4 i .. 4 i + 3 of its word j
   scales  fp16 or bf16 [N, K / G] G = 32, 64 or 128 inputs per group
   zeros   uint8 [N, K / G], 0 to 16, or None (8): weight = (q - zero) * scale
-Products are exact, sums fp32. For serving: nothing here records itself in autograd. moe.moe_forward takes a W4Store as it takes
+Products are exact, sums fp32. For serving: nothing here records itself in autograd, and inputs that
+require a gradient are refused. moe.moe_forward takes a W4Store as it takes
 an ExpertStore.
 """
 import ctypes
@@ -65,6 +66,7 @@ def linear(x, W, out_dtype=None, stream=None):
     shape, dev = x.shape, W._device
     if not shape or shape[-1] != W.K:
         raise ValueError(f"w4.linear: x [..., {W.K}] expected (got {tuple(shape)})")
+    _lib.no_gradient("w4.linear", x=x)
     _lib.check_tensors("w4.linear", dev, x=x)
     M = x.numel() // W.K
     with _lib.on(dev, stream):
@@ -121,6 +123,7 @@ def moe(store, x, ids, w, shared_expert=None, stream=None):
     if shared_expert is not None and not 0 <= shared < store.E:
         raise ValueError(f"w4.moe: shared expert {shared} of {store.E}")
     dev = store.q13.device
+    _lib.no_gradient("w4.moe", x=x, w=w)
     _lib.check_tensors("w4.moe", dev, x=x, ids=ids, w=w)
     with _lib.on(dev, stream):
         out = torch.empty((T, store.H), dtype=torch.float32, device=dev)

@@ -213,3 +213,36 @@ def test_balance_refuses_more_than_2_30_tokens():
     assert b"2^30" in L.mm_last_error()
     assert L.mm_balance_loss_backward(256, 256, 2, None, 256, 256, 1, T, 8, 1, 0, 256, None) == -1
     assert b"2^30" in L.mm_last_error()
+
+
+def test_inputs_that_want_a_gradient_are_not_silently_cut_off():
+    """The 4-bit products refuse them; the layer on EXL3 experts, which took them before the router had gradients, warns."""
+    from types import SimpleNamespace
+
+    from mi355moe import moe, w4
+    W = SimpleNamespace(K=64, N=16, _device=torch.device("cpu"))
+    x = torch.zeros((2, 64), requires_grad=True)
+    with pytest.raises(RuntimeError, match="x requires a gradient"):
+        w4.linear(x, W)
+    store = object.__new__(w4.W4Store)
+    store.E, store.H, store.I, store.q13 = 4, 64, 32, torch.zeros(1)
+    ids, w = torch.zeros((2, 1), dtype=torch.int64), torch.ones((2, 1), requires_grad=True)
+    for args, name in (((x, ids, w.detach()), "x"), ((x.detach(), ids, w), "w")):
+        with pytest.raises(RuntimeError, match=f"{name} requires a gradient"):
+            moe.moe_forward(store, *args)
+        with torch.no_grad(), pytest.raises(ValueError, match="GPU"):
+            moe.moe_forward(store, *args)
+    with pytest.raises(ValueError, match="GPU"):
+        moe.moe_forward(store, x.detach(), ids, w.detach())
+
+    class Store:
+        E, H, I = 4, 64, 32
+
+        def mm_layer(self):
+            raise LookupError("reached the layer")
+
+    for T in (2, 40):
+        wt = torch.ones((T, 1), requires_grad=True)
+        a = (torch.zeros((T, 64)).half(), torch.zeros((T, 1), dtype=torch.int64))
+        with pytest.warns(UserWarning, match="no gradient"), pytest.raises(LookupError):
+            moe.moe_forward(Store(), *a, wt)
