@@ -117,7 +117,7 @@ def moe(store, x, ids, w, shared_expert=None, stream=None):
     if x.dim() != 2 or x.shape[1] != store.H:
         raise ValueError(f"w4.moe: x [T, {store.H}] expected (got {tuple(x.shape)})")
     T = x.shape[0]
-    if ids.shape != w.shape or ids.numel() == 0 and T or T and ids.numel() % T:
+    if ids.dim() != 2 or ids.shape != w.shape or ids.shape[0] != T or T and ids.shape[1] == 0:
         raise ValueError(f"w4.moe: ids and w must be [{T}, k] (got {tuple(ids.shape)} and {tuple(w.shape)})")
     shared = -1 if shared_expert is None else int(shared_expert)
     if shared_expert is not None and not 0 <= shared < store.E:
@@ -129,7 +129,7 @@ def moe(store, x, ids, w, shared_expert=None, stream=None):
         out = torch.empty((T, store.H), dtype=torch.float32, device=dev)
         if T == 0:
             return out
-        k = ids.numel() // T
+        k = ids.shape[1]
         x, ids, w = _lib.aligned(x), ids.long().contiguous(), w.float().contiguous()
         code = _DTYPES[x.dtype]
         wsb = _lib.load().mm_w4_moe_workspace(code, T, k, shared, store.E, store.H, store.I)

@@ -246,3 +246,18 @@ def test_inputs_that_want_a_gradient_are_not_silently_cut_off():
         a = (torch.zeros((T, 64)).half(), torch.zeros((T, 1), dtype=torch.int64))
         with pytest.warns(UserWarning, match="no gradient"), pytest.raises(LookupError):
             moe.moe_forward(Store(), *a, wt)
+
+
+def test_experts_take_picks_as_tokens_by_k_only():
+    """[k, T] has as many elements as [T, k], and would be read as other tokens' picks."""
+    from mi355moe import w4
+    store = object.__new__(w4.W4Store)
+    store.E, store.H, store.I, store.q13 = 4, 64, 32, torch.zeros(1)
+    x, ids = torch.zeros((6, 64)), torch.zeros((6, 2), dtype=torch.int64)
+    for bad in (ids.t(), ids.reshape(-1), ids.reshape(3, 4), ids.reshape(6, 2, 1), ids[:, 0]):
+        with pytest.raises(ValueError, match=r"ids and w must be \[6, k\]"):
+            w4.moe(store, x, bad, bad.float())
+    with pytest.raises(ValueError, match="GPU"):
+        w4.moe(store, x, ids, ids.float())
+    with pytest.raises(ValueError, match="GPU"):
+        w4.moe(store, x[:0], ids[:0], ids[:0].float())
