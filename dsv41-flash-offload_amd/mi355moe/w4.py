@@ -105,8 +105,8 @@ class W4Store:
                                  self.E, self.H, self.I, self.group, _DTYPES[scales13.dtype], self.limit)
 
     def mm_layer(self):
-        """The C ABI's mm_w4_layer_t for this store (kept alive by the store)."""
-        return self._c
+        """The EXL3 paths ask their store for its layer here: this one has none."""
+        raise TypeError("a W4Store holds no EXL3 layer: it runs on moe.moe_forward or w4.moe")
 
 
 def moe(store, x, ids, w, shared_expert=None, stream=None):

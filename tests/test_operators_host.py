@@ -261,3 +261,15 @@ def test_experts_take_picks_as_tokens_by_k_only():
         w4.moe(store, x, ids, ids.float())
     with pytest.raises(ValueError, match="GPU"):
         w4.moe(store, x[:0], ids[:0], ids[:0].float())
+
+
+def test_exl3_paths_refuse_a_store_of_4_bit_experts():
+    from mi355moe import moe, w4
+    store = object.__new__(w4.W4Store)
+    store.E, store.H, store.I = 4, 64, 32
+    x, ids, w = torch.zeros((2, 64)).half(), torch.zeros((2, 1), dtype=torch.int64), torch.ones((2, 1))
+    for call in (lambda: moe.decode_routes(store, x, ids, w, 2), lambda: moe.moe_prefill(store, x, ids, w),
+                 lambda: moe.fused_moe(store, x, ids, w, 32), lambda: moe.expert_gemv(store, x, ids, 2, 2, 1, 2),
+                 lambda: moe.grouped_gemm(store, x, ids)):
+        with pytest.raises(TypeError, match="W4Store.*moe.moe_forward"):
+            call()
