@@ -400,14 +400,14 @@ __device__ __forceinline__ void rb_tile(const GemmArgs& a, uint16_t* lds, int* s
             if constexpr (DX)
             {
                 // an infinite gradient times a zero part of the gate is NaN: such results are summed again from whole factors,
-                // so that they are what the formula gives (inf, or NaN)
+                // so that they are what the formula gives (inf, or NaN, which is where a sum ends: rows of padding cost little)
                 const int cs = scale[RB_H + c - c0];
 #pragma unroll
                 for (int m = 0; m < 4; ++m)
                     if (v[m] != v[m])
                     {
                         v[m] = 0.f;
-                        for (int e = 0; e < a.E; ++e)
+                        for (int e = 0; e < a.E && v[m] == v[m]; ++e)
                         {
                             const uint16_t* d = a.cols + (size_t)c * K + e;
                             v[m] = fmaf(ldexpf(h2f(d[0]) + h2f(d[(size_t)C * K]), -cs), a.gate[(size_t)e * H + h + m], v[m]);
