@@ -128,7 +128,7 @@ def moe_forward(store, x, ids, w, shared_expert=None, fat_threshold=FAT_THRESHOL
     warning here and are refused by w4.moe."""
     if isinstance(store, w4.W4Store):
         return w4.moe(store, x, ids, w, shared_expert=shared_expert, stream=stream)
-    name = _lib.wants_gradient(x=x, w=w)
+    name = _lib.wants_gradient(x=x, w=w) if x.requires_grad or w.requires_grad else None
     if name:
         warnings.warn(f"moe_forward: {name} requires a gradient, but the output carries no gradient (detach it, or call under "
                       "torch.no_grad())", stacklevel=2)

@@ -66,7 +66,8 @@ def linear(x, W, out_dtype=None, stream=None):
     shape, dev = x.shape, W._device
     if not shape or shape[-1] != W.K:
         raise ValueError(f"w4.linear: x [..., {W.K}] expected (got {tuple(shape)})")
-    _lib.no_gradient("w4.linear", x=x)
+    if x.requires_grad:
+        _lib.no_gradient("w4.linear", x=x)
     _lib.check_tensors("w4.linear", dev, x=x)
     M = x.numel() // W.K
     with _lib.on(dev, stream):
@@ -123,7 +124,8 @@ def moe(store, x, ids, w, shared_expert=None, stream=None):
     if shared_expert is not None and not 0 <= shared < store.E:
         raise ValueError(f"w4.moe: shared expert {shared} of {store.E}")
     dev = store.q13.device
-    _lib.no_gradient("w4.moe", x=x, w=w)
+    if x.requires_grad or w.requires_grad:
+        _lib.no_gradient("w4.moe", x=x, w=w)
     _lib.check_tensors("w4.moe", dev, x=x, ids=ids, w=w)
     with _lib.on(dev, stream):
         out = torch.empty((T, store.H), dtype=torch.float32, device=dev)
