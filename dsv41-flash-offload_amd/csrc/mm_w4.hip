@@ -1125,9 +1125,13 @@ int mm_w4_linear(const void* x, int x_dtype, int M, int K, int N, const mm_w4_t*
             else if (rows <= 32) launch(ic<2>{}, ic<1>{}, ic<8>{}, std::true_type{}, ic<1>{});
             else
             {
-                // workgroups of 128 columns and 16 MT tile rows: the least of the estimated times (us at 4,096 inputs)
+                // Workgroups of 128 columns and 16 MT tile rows: the least of the estimated times (us at 4,096 inputs): a round of 256
+                // workgroups is a chain of blocks, 20 us with four groups of waves, 41 with two; without groups the chain takes 42 however
+                // few the workgroups, and full grids 26 more for every 256. us measured (KG = 4, 2, 1): 64 rows by 1,024 columns 19, 36,
+                // 42; 300 by 4,096 37, 39, 42; 300 by 8,192 55, 40, 53; 600 by 4,096 56, 42, 56; 1,200 by 8,192 184, 153, 134. Over 40 to
+                // 2,400 rows by 128 to 16,384 columns the choice is within 5 % of the best (with 1,024 inputs within 17 %).
                 auto groups = [&](int mt) { return (size_t)((N + 127) / 128) * ((M + 16 * mt / P - 1) / (16 * mt / P)); };
-                const size_t t2 = 20 * ((groups(2) + 255) / 256), t5 = 41 * ((groups(5) + 255) / 256), t4 = 18 + 26 * groups(4) / 256;
+                const size_t t2 = 20 * ((groups(2) + 255) / 256), t5 = 41 * ((groups(5) + 255) / 256), t4 = std::max((size_t)42, 18 + 26 * groups(4) / 256);
                 if (t2 <= std::min(t4, t5)) launch(ic<2>{}, ic<2>{}, ic<4>{}, std::false_type{}, ic<4>{});
                 else if (t5 <= t4) launch(ic<5>{}, ic<2>{}, ic<4>{}, std::false_type{}, ic<2>{});
                 else launch(ic<4>{}, ic<2>{}, ic<4>{}, std::false_type{}, ic<1>{});
