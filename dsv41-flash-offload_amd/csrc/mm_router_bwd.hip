@@ -8,11 +8,11 @@
 // and what is left out of a product is 3 x 2^-22 of it (2^-33 of the row's largest where values lie far below that), so that rows of D
 // that sum to zero cancel what the gate's rows share as fp32 products do. (Two bf16 parts left up to 2^-13.7 of a product.)
 //
-// Four launches: the largest values that the powers of two come from; the parts of D, row-major for dx (its k is the expert) and transposed for dgate (its k is the token), and
-// of the transposed gate; both products; the sum of dgate's partial results in order, whose tokens are split over enough
-// workgroups to fill the GPU. 16,384 tokens x 4,096 x 384 experts: 389 us a call (357 with
-// two bf16 parts and no powers of two), the products bound by MFMA at 0.82 PFLOP/s of 16-bit work (a large library product reaches
-// 1.13); 700 tokens 39.7 us (35.9), bound by their few steps and the launches.
+// Four launches: the largest values that the powers of two come from; the parts of D, row-major for dx (its k is the expert) and
+// transposed for dgate (its k is the token), and of the transposed gate; both products; the sum of dgate's partial results in order,
+// whose tokens are split over enough workgroups to fill the GPU. 16,384 tokens x 4,096 x 384 experts: 376 to 389 us a call (345 to 357
+// with two bf16 parts and no powers of two), the products bound by MFMA at 0.84 PFLOP/s of 16-bit work (a large library product
+// reaches 1.13); 700 tokens 39.7 us (35.9), bound by their few steps and the launches.
 #include <algorithm>
 #include <type_traits>
 
@@ -29,7 +29,7 @@ typedef uint32_t rb_u4 __attribute__((ext_vector_type(4)));
 constexpr int RB_H = 128, RB_C = 128, RB_K = 64;
 // LDS row of a k-contiguous operand: eight 16-byte chunks, chunk q of row r at q ^ (r / 2): the 16 rows of an operand read lie in 16
 // distinct bank groups. Steps of 64 rather than 32 inputs, so that eight lanes read one row's 128 bytes: loads of 64 bytes a row
-// kept the address unit busy for twice as long (16,384 tokens: 384 us a call, 362 now).
+// kept the address unit busy for twice as long (16,384 tokens, before the powers of two: 384 us a call and 362).
 constexpr int RB_ROW = RB_K;
 constexpr int RB_XROW = RB_H + 16;       // LDS row of the token-major input tile (32 bytes of padding: transposed reads of four rows hit distinct banks)
 __device__ __forceinline__ int rb_at(int r, int q) { return r * RB_ROW + 8 * (q ^ ((r >> 1) & 7)); }

@@ -1,8 +1,8 @@
 // Products with 4-bit weights and group scales: y[m][n] = sum_k x[m][k] (q[n][k] - z[n][g]) s[n][g], g = k / G, for a few
 // rows of x (dense), and the routed experts of a MoE layer on such weights.
 //
-// Storage is the checkpoint's own: q int32 [N][K / 8] (k = 8 j + i in bits 4 i .. 4 i + 3 of word j), s fp16 or bf16 and
-// z uint8 (or none: 8) [N][K / G]. Nothing is laid out anew.
+// Storage: q int32 [N][K / 8] (k = 8 j + i in bits 4 i .. 4 i + 3 of word j), s fp16 or bf16 and z uint8 (or none: 8) [N][K / G],
+// read as they are given.
 //
 // A wave multiplies 16 MT rows of x with 16 NT rows of W on v_mfma_f32_16x16x32: x is the A operand (lane l: row l & 15,
 // k-group l >> 4), W the B operand (lane l: output column l & 15). A lane reads 16 bytes = 32 weights of one row, the four
@@ -11,7 +11,7 @@
 // which one more MFMA against ones gives in the lanes that hold the products,
 //   sum_k x (q - z) = sum_k x (16 + q) - (16 + z) X,
 // and the scale is one fp32 fma per output and group. Every product is exact in fp32; the fp32 accumulation is the only
-// rounding. fp32 inputs, and the SwiGLU output that the down product reads, are three bf16 parts whose sum is the value.
+// rounding, of sums that carry x (16 + q) and x (16 + z): an input may leave 2^-24 of 31 times itself where its weight is its zero point. fp32 inputs, and the SwiGLU output that the down product reads, are three bf16 parts whose sum is the value.
 #include <algorithm>
 #include <type_traits>
 
@@ -146,8 +146,8 @@ __device__ __forceinline__ void wave_fence()
 // Both operands go through LDS: the multiplier wants the 16 rows of a tile in neighbouring lanes, but a load of 16 bytes a lane
 // whose neighbours lie in different rows costs the address unit four times what one of neighbours in one row does. So four
 // lanes read the 64 bytes that a block has of a row of W, sixteen lanes the 256 bytes of a row of x, and the operands
-// are read back from LDS, where 16-byte chunk c of row r lies at c ^ r (x) or c ^ (r / 4) (W), so that neither side conflicts in the
-// banks. The next block's loads are in flight while a block is multiplied.
+// are read back from LDS, where 16-byte chunk c of row r lies at c ^ r (x) or c ^ (r / 4) (W), against conflicts in the
+// banks (those left are 30 % of the LDS cycles of the few-row kernels, whose LDS is busy a fifth of the time). The next block's loads are in flight while a block is multiplied.
 //
 // With OWN the wave keeps its rows of x to itself (waves split K); otherwise the NW waves of the workgroup share them (waves
 // split the columns), double-buffered, with a barrier a block.
@@ -534,9 +534,9 @@ __global__ __launch_bounds__(256) void k_w4_parts(const float* __restrict__ x, s
 // Dense. OWN: a workgroup takes 16 NT columns and its waves split K (up to 32 tile rows); else 16 NT columns a wave, and KG groups of
 // waves split K. A wave's block of 128 inputs is a chain of LDS reads, products and a barrier of some 1.2 us, of which more waves hide
 // more: 4 of them on a CU take 42 us for 64 rows of 8192 x 4096, 16 (KG = 4) take 20; 300 rows take 54 us in tiles of 64 rows,
-// 41 (490 TFLOP/s) in tiles of 80 with KG = 2, one workgroup a CU. Full grids have waves enough: 4,096 rows 424 us (648
-// TFLOP/s) with KG = 1, 514 with KG = 2. (Two to four blocks of loads in flight instead of one: 56-60 us at 300 rows, LDS operands a
-// block ahead: 59.) One row of 4096 x 4096 takes 3.9 us (2.2 TB/s; as many bytes copied take 3.5).
+// 41 (490 TFLOP/s) in tiles of 80 with KG = 2, one workgroup a CU. Full grids have waves enough: 2,400 rows 256 us with KG = 1, 306
+// with KG = 2; 4,096 rows 400 us (687 TFLOP/s). (Two to four blocks of loads in flight instead of one: 56-60 us at 300 rows, LDS operands a
+// block ahead: 59.) One row of 4096 x 4096 takes 4.6 us (1.9 TB/s).
 // ---------------------------------------------------------------------------------------------------------
 struct LinearArgs
 {
@@ -694,15 +694,17 @@ __device__ __forceinline__ void down_rows(const ExpertArgs& a, unsigned char* ld
 
 // Weight tiles of a workgroup in the gate/up and the down product of few rows.
 constexpr int W4_GU = 2, W4_DN = 2;
-// Waves per SIMD that they are compiled for: as many as need no scratch memory in the loops of the usual shapes (a few words at two
-// row tiles, which 24 tokens of 64 experts run on 3 % faster than with two waves).
+// Waves per SIMD that they are compiled for: as many as need no scratch memory with one row tile. With two row tiles it is 24 to 128 bytes a lane in
+// the down product and 24 to 144 in fp32 gate and up (G = 128 with zero points, 24 tokens of 64 experts: 76), and still 3 % faster there
+// than two waves without it.
 template <int G, bool ZP, int MT>
 constexpr int W4_OCC = MT == 1 && G == 128 && !ZP ? 4 : 3;
 
 // Few rows: one workgroup per record and 16 (32) columns, its four waves split K; one or two row tiles by the expert's routes, more
 // routes in more passes. Bound by no unit that a counter shows: 9 experts of 4096 / 2048 take 20.5 + 13.0 us, 32 experts of them (4
-// fp32 tokens) 58 + 32 us, 3.5 TB/s of weights, where a read alone in this pattern reaches 5.7 to 6.4; VALU 39 % busy, MFMA 18 %, address
-// unit 57 %, LDS 22 %. Waves that split the columns instead, as for many rows, would have each expert's few columns wait for the
+// fp32 tokens) 58 + 32 us, 3.5 TB/s of weights, where a read alone in this pattern reaches 5.6 to 5.9 (4.8 to 5.1 at nine experts' size); VALU 39 % busy, MFMA 18 %, address
+// unit 57 %, LDS 22 %. A wave has one block, 2 KB of weights, in flight, a CU 24 to 32 KB, which is 3.5 TB/s at 2 us a round
+// trip; more blocks in registers spill. Waves that split the columns instead, as for many rows, would have each expert's few columns wait for the
 // whole of K: 9 experts would be 9 x 32 workgroups of 32 blocks in a row.
 template <int XT, int P, int G, bool ZP, int MT>
 __global__ __launch_bounds__(256, (W4_OCC<G, ZP, MT>)) void k_w4_gate_up(ExpertArgs a)
@@ -741,7 +743,7 @@ __global__ __launch_bounds__(256, (W4_OCC<G, ZP, MT>)) void k_w4_down(ExpertArgs
 
 // Many rows: 64 columns (gate and up; down 64 NT) per workgroup, four waves that share the rows of x, KG groups of them that split K; up
 // to 16 MT tile rows a pass. 200 tokens of 32
-// experts of 1024 / 512 take 17 + 15 us (four blocks in a row), 4,000 of 4096 / 1024 1.2 ms in all (330 TFLOP/s, the down
+// experts of 1024 / 512 take 17 + 15 us (four blocks in a row), 4,000 of 64 experts of 4096 / 1024, four each, 1.2 to 1.3 ms in all (320 TFLOP/s, the down
 // product's three parts counted once).
 template <int XT, int P, int G, bool ZP, int MT, int KG>
 __global__ __launch_bounds__(256 * KG, 2) void k_w4_gate_up_many(ExpertArgs a)
@@ -940,8 +942,8 @@ static ExpertWs expert_ws(int x_dtype, int T, int k, int shared, int E, int H, i
     if (n > W4_SELF)
     {
         // Routes of a record, up to 16, 32 or 64 by the experts' average (us at 64 experts of 2048 / 1024, groups of 64): 6 routes an
-        // expert 92 in records of 16 and 97 of 32, 8 routes 102 and 97, 12 routes 131 and 102; 32 routes 157 in records of 32
-        // and 172 of 64, 40 routes 197 and 184, 128 routes 440 both, 256 routes 787 and 760.
+        // expert 86 in records of 16 and 90 of 32, 8 routes 100 and 92, 12 routes 129 and 96; 32 routes 145 in records of 32
+        // and 160 of 64, 40 routes 184 and 170, 128 routes 416 and 420, 256 routes 774 and 756.
         w.rows = n > (size_t)36 * E ? 64 : n > (size_t)7 * E ? 32 : 16;
         w.nrecs = (int)(std::min(n, (size_t)E) + n / w.rows);
         w.order = take(n * 4);
@@ -1027,8 +1029,8 @@ static int experts_launch(const mm_w4_layer_t* L, const void* x, int x_dtype, in
         a.nrec = nrec;
     }
     const bool many = s.rows > 16;
-    // At most one workgroup a CU: twice the waves in gate and up, half the columns in down (200 tokens of 32 experts of 1024 / 512 44.5 ->
-    // 40 us, 60 of 8 37 -> 32; with four workgroups a CU, 300 tokens of 64 experts of 2048 / 1024, 142 -> 160 and 163 us).
+    // At most one workgroup a CU: twice the waves in gate and up, half the columns in down (200 tokens of 32 experts of 1024 / 512 44 ->
+    // 40 us, 60 of 8 37 -> 29; with four workgroups a CU, 300 tokens of 64 experts of 2048 / 1024, 104 -> 132).
     auto few = [&](int columns) { return (size_t)columns * std::min(E, a.n) <= 256 && a.n <= 64 * E; };
     by_input(x_dtype, [&](auto xt, auto parts) {
         by_group(L->group, L->w13.zeros != nullptr, [&](auto g, auto zp) {

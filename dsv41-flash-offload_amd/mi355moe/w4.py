@@ -1,10 +1,11 @@
 """4-bit weights with group scales: dense products (W4Matrix, linear) and the routed experts of a layer (W4Store, moe).
 
-Tensors are taken as 4-bit checkpoints store them, and read in place:
+Tensors are read in place, in this layout (checkpoints that order the weights otherwise, or pack their zero points into
+words, are to be repacked first):
   q       int32 [N, K / 8]        weight k = 8 j + i of a row in bits 4 i .. 4 i + 3 of its word j
   scales  fp16 or bf16 [N, K / G] G = 32, 64 or 128 inputs per group
   zeros   uint8 [N, K / G], 0 to 16, or None (8): weight = (q - zero) * scale
-Products are exact, sums fp32. For serving: nothing here records itself in autograd, and inputs that
+Products are exact, sums fp32 (of x (16 + q) and x (16 + z), with the roundings of those). For serving: nothing here records itself in autograd, and inputs that
 require a gradient are refused. moe.moe_forward takes a W4Store as it takes
 an ExpertStore.
 """

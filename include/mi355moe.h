@@ -66,9 +66,10 @@ int mm_router_topk(const void* x_bf16, int T, int H, const float* gate, int E, i
  * dlogits fp32 [T][E] (NULL: none; of a loss on the logits such as mm_balance_loss) of its outputs,
  *   D = dlogits + scatter(w[t][j] (dw[t][j] - sum_i w[t][i] dw[t][i]) at ids[t][j]),
  *   dx bf16 [T][H] = D gate, dgate fp32 [E][H] = D^T x   (either NULL: not computed).
- * x, gate, ids and w as mm_router_topk took and gave them; infinite values give what IEEE products and sums of the formula give (ids outside [0, E) get no gradient, a pick named twice gets
- * both). fp32 factors are multiplied in parts with fp32 accumulation: exactly in dgate, in dx to 3 x 2^-22 of each product (and
- * 2^-33 of the largest of its row of D times the largest of its column of the gate). T <= 2^21, H a multiple of 16, E <= 1024, k <= 32; x, dx, dgate and the workspace 16-byte aligned. */
+ * x, gate, ids and w as mm_router_topk took and gave them; infinite values give what IEEE products and sums of the formula give
+ * (ids outside [0, E) get no gradient, a pick named twice gets both). fp32 factors are multiplied in parts with fp32 accumulation:
+ * exactly in dgate, in dx to 3 x 2^-22 of each product (and 2^-33 of the largest of its row of D times the largest of its column of
+ * the gate). T <= 2^21, H a multiple of 16, E <= 1024, k <= 32; x, dx, dgate and the workspace 16-byte aligned. */
 size_t mm_router_backward_workspace(int T, int H, int E);
 int mm_router_backward(const void* x_bf16, int T, int H, const float* gate, int E, int k, const int64_t* ids, const float* w,
                        const float* dw, const float* dlogits, void* dx_bf16, float* dgate, void* workspace,
@@ -268,7 +269,7 @@ int mm_fat_batched(const mm_layer_t* layer, const void* x, int x_dtype, int T, i
 
 /* ------------------------------------------------------------------------------------ 4-bit weights */
 
-/* A matrix [N][K] of 4-bit weights with group scales, in the storage of the checkpoints: w[n][k] = (q - z) s with q = bits
+/* A matrix [N][K] of 4-bit weights with group scales: w[n][k] = (q - z) s with q = bits
  * 4 (k % 8) .. + 3 of q[n][k / 8], s = scales[n][k / group] (fp16 or bf16) and z = zeros[n][k / group] (4-bit zero points, 0
  * .. 16; NULL: 8). group is 32, 64 or 128 and divides K. q is 16-byte aligned; rows are contiguous. */
 typedef struct mm_w4
@@ -278,7 +279,7 @@ typedef struct mm_w4
     const uint8_t* zeros;       /* [N][K / group] or NULL */
 } mm_w4_t;
 
-/* y [M][N] (y_dtype) = x [M][K] (x_dtype) W^T. Products are exact, sums fp32, the result is rounded once. x 16-byte aligned.
+/* y [M][N] (y_dtype) = x [M][K] (x_dtype) W^T. Products are exact, sums fp32 (of x (16 + q) and x (16 + z), with the roundings of those), the result is rounded once. x 16-byte aligned.
  * Built for few rows (decode steps); any M up to 2^20 works, at 32 to 80 rows (a third of fp32) per pass over the weights. K < 2^22, N <=
  * 2^26. Workspace: mm_w4_linear_workspace bytes (fp32 inputs only), 16-byte aligned. */
 size_t mm_w4_linear_workspace(int x_dtype, int M, int K);
@@ -297,7 +298,8 @@ typedef struct mm_w4_layer
 /* One MoE layer on 4-bit experts: out fp32 [T][H] = sum_j w[t,j] * expert_{ids[t,j]}(x_t) in ascending j (fp32 fma), ids
  * int64 [T*topk] (outside [0, E): contributes nothing), expert(x) = W2 (act(Wg x) * Wu x) with mm_moe_decode's activation and
  * clamp, nothing rounded below fp32 between x and out. shared >= 0 names an expert that every token is routed to besides, with weight 1,
- * added last (-1: none). The result of a token does not depend on the other tokens' order. An expert's weights are read once per 16 to 64 of its routes; a call of many tokens runs in
+ * added last (-1: none). The result of a token does not depend on the other tokens' order. An expert's gate and up weights are read once per 16 to 64 of its routes (fp32 inputs: 5, 10 or 32), its down weights once per 5, 10 or
+ * 32; a call of many tokens runs in
  * chunks of at most 8,192. No host synchronisation. E <= 1024, topk <= 1024, H and I multiples of the group, H I < 2^31; x and
  * out 16-byte aligned. Workspace: mm_w4_moe_workspace bytes (topk without the shared expert), 16-byte aligned. */
 size_t mm_w4_moe_workspace(int x_dtype, int T, int topk, int shared, int E, int H, int I);
