@@ -422,6 +422,7 @@ int mm_balance_loss(const void* logits, int dtype, const int64_t* ids, const uin
     const BalanceWs w = balance_ws(B, T, E);
     MM_CHECK_ARG(workspace_bytes >= w.total && (w.total == 0 || workspace), "mm_balance_loss: workspace too small (%zu < %zu)",
                  workspace_bytes, w.total);
+    MM_CHECK_ARG(w.total == 0 || ((uintptr_t)workspace & 15) == 0, "mm_balance_loss: workspace misaligned (16 bytes)");
     BalanceArgs a{};
     a.logits = logits;
     a.ids = ids;

@@ -83,7 +83,8 @@ int mm_router_backward(const void* x_bf16, int T, int H, const float* gate, int 
  *   loss fp32 [B] = E / (k tokens^2) sum_e counts[e] load[e]   (0 for a sequence without tokens).
  * One loss over a whole batch is B = 1. logits [B][T][E] of type MM_DTYPE_*; a logit of -inf is an expert that cannot be
  * picked, and a token whose logits are all -inf has no scores. Masked tokens' logits are never used. Sums are fp32 in a fixed order.
- * E <= 1024, k <= 32, B <= 65535, T <= 2^30 and T k < 2^31. Workspace: mm_balance_workspace(B, T, E) bytes (0: none). */
+ * E <= 1024, k <= 32, B <= 65535, T <= 2^30 and T k < 2^31. Workspace: mm_balance_workspace(B, T, E) bytes
+ * (0: none), 16-byte aligned. */
 #define MM_SCORE_SOFTMAX 0
 #define MM_SCORE_SIGMOID 1
 size_t mm_balance_workspace(int B, int T, int E);

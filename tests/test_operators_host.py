@@ -273,3 +273,13 @@ def test_exl3_paths_refuse_a_store_of_4_bit_experts():
                  lambda: moe.grouped_gemm(store, x, ids)):
         with pytest.raises(TypeError, match="W4Store.*moe.moe_forward"):
             call()
+
+
+def test_balance_refuses_a_misaligned_workspace():
+    """Its slices are counted with 32-bit atomics, which fault at odd addresses."""
+    from mi355moe import _lib
+    L = _lib.load()
+    need = L.mm_balance_workspace(1, 16384, 384)
+    for ws in (257, 258, 264):
+        assert L.mm_balance_loss(256, 2, 256, None, 1, 16384, 384, 8, 0, 256, 256, 256, 256, ws, need, None) == -1
+        assert b"misaligned" in L.mm_last_error()
