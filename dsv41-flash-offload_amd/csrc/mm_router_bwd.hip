@@ -189,7 +189,8 @@ __global__ __launch_bounds__(256) void k_rb_parts(const int64_t* __restrict__ id
     __shared__ int scale[64];
     if ((int)blockIdx.x >= tiles) return gate_parts(gate, E, H, Ek, gt, gmax, gs, tile, scale, blockIdx.x - tiles);
     const int ne = (E + 63) / 64, t0 = (int)blockIdx.x / ne * 64, e0 = (int)blockIdx.x % ne * 64, tid = threadIdx.x;
-    // all loads at once: the tile's logit gradients, and the rows' picks (their expert within the tile, or -1)
+    // all loads at once: the tile's logit gradients, and the rows' picks (their expert within the tile, -1 for another tile's, -2
+    // for none)
     float v[16];
 #pragma unroll
     for (int u = 0; u < 16; ++u)
@@ -205,7 +206,7 @@ __global__ __launch_bounds__(256) void k_rb_parts(const int64_t* __restrict__ id
         const int64_t e = ids[at];
         sw[i] = w[at];
         sd[i] = dw[at];
-        se[i] = e >= e0 && e < min(E, e0 + 64) ? (int)(e - e0) : -1;
+        se[i] = e < 0 || e >= E ? -2 : e >= e0 && e < e0 + 64 ? (int)(e - e0) : -1;
     }
 #pragma unroll
     for (int u = 0; u < 16; ++u) tile[(tid + 256 * u) >> 6][tid & 63] = v[u];
@@ -222,7 +223,7 @@ __global__ __launch_bounds__(256) void k_rb_parts(const int64_t* __restrict__ id
             for (int j = 0; j < k; ++j)
             {
                 const float p = sw[at + j] * (sd[at + j] - s);
-                m = max(m, finite_bits(p));
+                if (se[at + j] != -2) m = max(m, finite_bits(p));
                 if (se[at + j] >= 0) tile[tid][se[at + j]] += p;
             }
         }

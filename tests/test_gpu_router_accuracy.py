@@ -131,3 +131,18 @@ def test_balance_gradient_of_very_many_tokens(dev):
     assert d.shape == logits.shape
     assert bool((d[:, 0] == d[0, 0]).all()) and bool((d[:, 1] == -d[0, 0]).all())
     assert abs(float(d[0, 0]) - E * 0.5 * (3 - 2)) <= 2.0 ** -10
+
+
+@pytest.mark.parametrize("E", [20, 130])
+def test_dx_where_picks_of_no_expert_have_the_large_gradients(dev, E):
+    """They take part in the softmax's sum only; the row's scale is that of the picks of experts."""
+    from mi355moe import router
+    T, H = 70, 64
+    x, gate, _, _, _, _ = router_inputs(T, H, E, 1, E, dev)
+    ids = torch.tensor([3, -1, E]).repeat(T, 1).to(dev)
+    ids[::2, 0] = E - 1
+    w = torch.tensor([2.0 ** -30, 0.5, 0.5]).repeat(T, 1).to(dev)
+    dw = torch.tensor([1.0, 2.0 ** 20, -2.0 ** 20]).repeat(T, 1).to(dev)
+    dx, _ = router.topk_backward(x, gate, ids, w, dw, need_gate=False)
+    want = gate[ids[:, 0]].cpu().double() * (2.0 ** -30 * (1 - 2.0 ** -30))
+    close(dx, want, (2.0 ** -8 + 2.0 ** -19) * want.abs() + 2.0 ** -30 * 2.0 ** -33 * gate.abs().max().item())
