@@ -10,9 +10,9 @@
 //
 // Four launches: the largest values that the powers of two come from; the parts of D, row-major for dx (its k is the expert) and
 // transposed for dgate (its k is the token), and of the transposed gate; both products; the sum of dgate's partial results in order,
-// whose tokens are split over enough workgroups to fill the GPU. 16,384 tokens x 4,096 x 384 experts: 376 to 389 us a call (345 to 357
+// whose tokens are split over enough workgroups to fill the GPU. 16,384 tokens x 4,096 x 384 experts: 376 to 394 us a call (345 to 357
 // with two bf16 parts and no powers of two), the products bound by MFMA at 0.84 PFLOP/s of 16-bit work (a large library product
-// reaches 1.13); 700 tokens 39.7 us (35.9), bound by their few steps and the launches.
+// reaches 1.13); 700 tokens 40 us (35.9), bound by their few steps and the launches.
 #include <algorithm>
 #include <type_traits>
 
