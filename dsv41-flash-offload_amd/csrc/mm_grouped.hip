@@ -1,0 +1,598 @@
+// Products grouped by expert over ragged rows, for experts in 16-bit weights W [E][N][K]: rows offsets[e] .. offsets[e + 1] - 1 of
+// the plan's order belong to expert e, and with p such a row
+//   forward            y[p]  = W[e] x[p]                     contraction over K, both operands along their rows
+//   gradient of x      dx[p] = W[e]^T dy[p]                  contraction over N, W across its rows
+//   gradient of W      dW[e] = sum over p of dy[p] x[p]^T    contraction over the rows p, both operands across their rows
+// x (or dy) may have one row per token, which the plan's token list then picks, and rows may be summed per token.
+//
+// A workgroup of eight waves takes up to 256 rows by 256 columns on v_mfma_f32_16x16x32, block by block of 64 terms, with the
+// next blocks on their way into LDS by buffer loads that write it directly. An operand that lies along the contraction is kept as rows of 64
+// terms (128 bytes) and read in 16-byte chunks, chunk c of row r at c ^ (r & 7); one that lies across it is kept as 64 rows of the tile's
+// columns and read through the transposing LDS load, which gives a lane four terms of its column; its 32-byte pieces
+// lie at p ^ f(row), with f chosen so that the rows a wave reads together meet different banks. Products are exact in fp32 and summed in
+// fp32 by the matrix cores; a result is rounded once.
+#include <algorithm>
+#include <type_traits>
+
+#include "mm_common.h"
+#include "mm_decode.h"
+
+namespace mm {
+
+typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+typedef short s4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+
+template <int XT>
+__device__ __forceinline__ f4_t mfma(u4_t a, u4_t b, f4_t c)
+{
+    if constexpr (XT == MM_DTYPE_F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8_t, a), __builtin_bit_cast(bf8_t, b), c, 0, 0, 0);
+}
+template <int XT>
+__device__ __forceinline__ uint32_t pack2(float a, float b)
+{
+    return XT == MM_DTYPE_F16 ? (uint32_t)f2h(a) | (uint32_t)f2h(b) << 16 : (uint32_t)f2bf(a) | (uint32_t)f2bf(b) << 16;
+}
+__device__ __forceinline__ const void* scalar_ptr(const void* p)
+{
+    const uint64_t v = (uint64_t)(uintptr_t)p;
+    const uint32_t l = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+    const uint32_t h = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
+    return reinterpret_cast<const void*>((uintptr_t)((uint64_t)l | ((uint64_t)h << 32)));
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, uint32_t bytes)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(scalar_ptr(p)), (short)0, __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000);
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// Plan: the row tiles of a call
+// ---------------------------------------------------------------------------------------------------------
+constexpr int ROWS = 256, COLS = 256, TERMS = 64;      // the largest tile, and the terms of a block
+struct GroupTile
+{
+    int expert;            // -1: rows of no expert, which are zero
+    int row, rows;         // first row, rows (1 .. ROWS)
+    int first, count;      // the expert's tiles
+    int pad[3];
+};
+
+// Row tiles of n routes over E experts: whole ones, one for the rest of each expert that has rows, and those of no expert.
+constexpr long long tile_capacity(long long n, int E) { return n / ROWS + std::min<long long>(n, E) + 1; }
+
+// One thread per expert (and one for the routes of none): tiles in the experts' order.
+__global__ __launch_bounds__(1024) void k_group_tiles(const int32_t* __restrict__ offsets, int E, GroupTile* __restrict__ tiles, int32_t* __restrict__ ntiles)
+{
+    __shared__ int part[16];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    int run = 0;
+    for (int base = 0; base <= E; base += 1024)
+    {
+        const int e = base + t;
+        const int r0 = e <= E ? offsets[e] : 0, r1 = e <= E ? offsets[e + 1] : 0;
+        const int cnt = (r1 - r0 + ROWS - 1) / ROWS;
+        const int inc = wave_incl_scan(cnt);
+        __syncthreads();
+        if (lane == 63) part[wave] = inc;
+        __syncthreads();
+        int first = run + inc - cnt, total = 0;
+        for (int w = 0; w < 16; ++w)
+        {
+            if (w < wave) first += part[w];
+            total += part[w];
+        }
+        for (int i = 0; i < cnt; ++i)
+            tiles[first + i] = { e < E ? e : -1, r0 + i * ROWS, min(ROWS, r1 - r0 - i * ROWS), first, cnt, { 0, 0, 0 } };
+        run += total;
+    }
+    if (t == 0) *ntiles = run;
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// Operands: global memory to LDS
+// ---------------------------------------------------------------------------------------------------------
+// 16 bytes a lane, from `at` bytes into the buffer to lds + 16 lane.
+__device__ __forceinline__ void load16(__amdgpu_buffer_rsrc_t buf, unsigned char* lds, uint32_t at)
+{
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, lds, 16, at, 0, 0, 0);
+}
+constexpr uint32_t NOWHERE = 0xfffffff0u;              // past every buffer: reads zero
+
+// Rows of TERMS terms, R of them; LDS [R][64]. A wave's load is 8 rows of 128 bytes. Tiles of fewer rows than eight waves load
+// are loaded more than once, to the same place, so that every wave has as many loads in flight.
+template <int R>
+struct Along
+{
+    static constexpr int BYTES = R * 128, LOADS = std::max(1, R / 64);
+    __amdgpu_buffer_rsrc_t buf;
+    uint32_t at[LOADS];
+    int slot;             // the wave's first row
+    int chunk;            // the lane's chunk of a row's eight
+    // base: the tile's first row, or with `pick` the row that pick[] counts from; rows > 0; ld: bytes of a row; bytes: of the buffer
+    __device__ __forceinline__ void init(const void* base, uint32_t ld, int rows, uint32_t bytes, const int32_t* pick)
+    {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        buf = buffer(base, bytes);
+        slot = wave * LOADS * 8 % R;
+        chunk = (lane ^ (lane >> 3)) & 7;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+        {
+            const int r = slot + 8 * i + (lane >> 3);
+            // rows past the tile's are past the buffer, or the last row again: they are not stored
+            at[i] = (uint32_t)(pick ? pick[min(r, rows - 1)] : r) * ld + 16 * chunk;
+        }
+    }
+    __device__ __forceinline__ void load(unsigned char* lds, int block, int terms) const
+    {
+        // the last block of a contraction that is no multiple of 64: chunks past the row's end are zero
+        const bool in = TERMS * block + 8 * chunk < terms;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+            load16(buf, lds + (slot + 8 * i) * 128, in ? at[i] + 128 * block : NOWHERE);
+    }
+    // chunk kk * 4 + (lane >> 4) of row 16 b + (lane & 15)
+    __device__ static __forceinline__ uint32_t place(int first)
+    {
+        const int lane = threadIdx.x & 63;
+        return (uint32_t)(first + (lane & 15)) * 128 + 16 * ((lane >> 4) ^ (lane & 7));
+    }
+    __device__ static __forceinline__ u4_t read(const unsigned char* lds, uint32_t place, int b, int kk)
+    {
+        return *reinterpret_cast<const u4_t*>(lds + (place ^ (64 * kk)) + 2048 * b);
+    }
+};
+
+// 64 rows (terms) of R columns; LDS [64][R], 32-byte piece p of row k at p ^ swizzle(k).
+template <int R>
+struct Across
+{
+    static constexpr int BYTES = R * 128, LOADS = R / 64, RB = 2 * R, ROWS_LOAD = 1024 / RB;   // rows that one load covers
+    static_assert(R == 256 || R == 128, "columns");
+    struct Picks
+    {
+        int32_t row[LOADS];
+    };
+    const unsigned char* base;
+    uint32_t ld, at[LOADS];
+    int row[LOADS], slot;
+    // four rows of one 8-row group and the four groups that a wave reads at once
+    __device__ static __forceinline__ int swizzle(int k) { return ((k & 3) | ((k >> 3) & 3) << 2) & (R / 16 - 1); }
+    // base: column 0 of row 0; first: the tile's first column; width: columns of a row
+    __device__ __forceinline__ void init(const void* b, uint32_t ld_, int first, int width)
+    {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        base = static_cast<const unsigned char*>(b);
+        ld = ld_;
+        slot = wave * LOADS * ROWS_LOAD;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+        {
+            const int k = slot + ROWS_LOAD * i + lane / (RB / 16), s = lane % (RB / 16);
+            const int c = first + 8 * (((s >> 1) ^ swizzle(k)) * 2 + (s & 1));
+            row[i] = k;
+            at[i] = c < width ? k * ld + 2 * c : NOWHERE;
+        }
+    }
+    // rows 64 block .. of `terms`
+    __device__ __forceinline__ void load(unsigned char* lds, int block, int terms) const
+    {
+        const int left = terms - TERMS * block;
+        const __amdgpu_buffer_rsrc_t buf = buffer(base + (size_t)block * TERMS * ld, (uint32_t)max(0, min(left, TERMS)) * ld);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+            load16(buf, lds + (slot + ROWS_LOAD * i) * RB, at[i]);
+    }
+    // the same with the rows that `pick` names, taken a block ahead by next(); bytes: of the whole tensor
+    __device__ __forceinline__ void next(Picks& p, const int32_t* pick, int block, int terms) const
+    {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+        {
+            const int k = TERMS * block + row[i];
+            p.row[i] = k < terms ? pick[k] : -1;
+        }
+    }
+    __device__ __forceinline__ void load_picked(unsigned char* lds, const Picks& p, uint32_t bytes) const
+    {
+        const __amdgpu_buffer_rsrc_t buf = buffer(base, bytes);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+            load16(buf, lds + (slot + ROWS_LOAD * i) * RB, p.row[i] < 0 || at[i] == NOWHERE ? NOWHERE : (uint32_t)p.row[i] * ld + (at[i] - row[i] * ld));
+    }
+    // terms 32 kk + 8 (lane >> 4) .. + 7 of column 16 b + (lane & 15): the transposing load takes 4 rows of 16 columns from 16 lanes,
+    // lane 4 q + c giving row q, columns 4 c .. 4 c + 3, and leaves column i on lane i
+    __device__ static __forceinline__ uint32_t place(int first)
+    {
+        const int lane = threadIdx.x & 63, k = 8 * (lane >> 4) + ((lane & 15) >> 2);
+        return (uint32_t)k * RB + ((first / 16) ^ swizzle(k)) * 32 + (lane & 3) * 8;
+    }
+    __device__ static __forceinline__ u4_t read(const unsigned char* lds, uint32_t place, int b, int kk)
+    {
+        typedef __attribute__((address_space(3))) s4_t* at_t;
+        const unsigned char* p = lds + (place ^ (32 * b)) + 32 * kk * RB;
+        const u2_t lo = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_t)(p)));
+        const u2_t hi = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_t)(p + 4 * RB)));
+        return u4_t{ lo.x, lo.y, hi.x, hi.y };
+    }
+};
+
+// ---------------------------------------------------------------------------------------------------------
+// Tile: rows of M by columns of N; wave (wm, wn) has MB x NB blocks of 16 x 16.
+// ---------------------------------------------------------------------------------------------------------
+template <int R>
+struct Shape
+{
+    static constexpr int WN = R >= 128 ? 4 : 8, WM = 8 / WN, MB = std::max(1, R / 16 / WM), NB = COLS / 16 / WN;
+    static constexpr int STAGE = (R + COLS) * 128;
+    static constexpr int STAGES = R == 256 ? 2 : R >= 64 ? 3 : 4;
+    static_assert(STAGE * STAGES <= 160 * 1024, "LDS");
+};
+constexpr int LDS_ROWS = 144 * 1024;      // of the row tiles: 3 stages of 128 x 256
+
+template <int XT, typename M, typename N, typename S, bool MT, bool NT>
+__device__ __forceinline__ void multiply(const unsigned char* m, const unsigned char* n, uint32_t mp, uint32_t np, f4_t (&acc)[S::MB][S::NB])
+{
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+    {
+        u4_t b[S::NB], a[S::MB];
+#pragma unroll
+        for (int j = 0; j < S::NB; ++j) b[j] = N::read(n, np, j, kk);
+#pragma unroll
+        for (int i = 0; i < S::MB; ++i) a[i] = M::read(m, mp, i, kk);
+#pragma unroll
+        for (int i = 0; i < S::MB; ++i)
+#pragma unroll
+            for (int j = 0; j < S::NB; ++j) acc[i][j] = mfma<XT>(b[j], a[i], acc[i][j]);
+    }
+}
+
+// Lane (r, g) of a block holds columns 4 g .. 4 g + 3 of row r. For 16-bit outputs neighbouring blocks trade halves, so that a lane
+// stores eight columns.
+template <int XT, typename S>
+__device__ __forceinline__ void store(f4_t (&acc)[S::MB][S::NB], void* y, int type, size_t row0, int rows, int col0, int cols, size_t ld)
+{
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, g = lane >> 4, m0 = wave / S::WN * S::MB * 16, n0 = col0 + wave % S::WN * S::NB * 16;
+#pragma unroll
+    for (int i = 0; i < S::MB; ++i)
+    {
+        const int m = m0 + 16 * i + r;
+        const size_t at = (row0 + m) * ld;
+        if (type == MM_DTYPE_F32)
+        {
+#pragma unroll
+            for (int j = 0; j < S::NB; ++j)
+            {
+                const int n = n0 + 16 * j + 4 * g;
+                if (m < rows && n < cols) *reinterpret_cast<f4_t*>(static_cast<float*>(y) + at + n) = acc[i][j];
+            }
+            continue;
+        }
+#pragma unroll
+        for (int j = 0; j < S::NB; j += 2)
+        {
+            const auto lo = __builtin_amdgcn_permlane16_swap(pack2<XT>(acc[i][j][0], acc[i][j][1]), pack2<XT>(acc[i][j + 1][0], acc[i][j + 1][1]), false, false);
+            const auto hi = __builtin_amdgcn_permlane16_swap(pack2<XT>(acc[i][j][2], acc[i][j][3]), pack2<XT>(acc[i][j + 1][2], acc[i][j + 1][3]), false, false);
+            const int n = n0 + 16 * (j + (g & 1)) + 4 * (g & 2);
+            if (m < rows && n < cols) *reinterpret_cast<u4_t*>(static_cast<uint16_t*>(y) + at + n) = u4_t{ lo[0], hi[0], lo[1], hi[1] };
+        }
+    }
+}
+
+struct RowsArgs
+{
+    const uint16_t *x, *w;        // the rows (x or dy) and the weights
+    void* y;
+    const GroupTile* tiles;
+    const int32_t *ntiles, *token;     // token: row of x of each row, NULL: its own
+    size_t xbytes;
+    int terms, cols, type, zero, colt;      // zero: rows of no expert are stored (as zeros); colt: column tiles
+};
+
+// XCD x of eight runs workgroups x, x + 8, ..., and has its own L2: runs of 32 tiles (its CUs) stay on one XCD.
+__device__ __forceinline__ int tile_of_block(int b)
+{
+    const int x = b & 7, i = b >> 3;
+    return ((i >> 5) * 8 + x) * 32 + (i & 31);
+}
+
+template <int XT, bool ACROSS, int R>
+__device__ __forceinline__ void rows_tile(const RowsArgs& a, const GroupTile& t, int ct, unsigned char* lds)
+{
+    using S = Shape<R>;
+    using M = Along<R>;
+    using N = std::conditional_t<ACROSS, Across<COLS>, Along<COLS>>;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col0 = ct * COLS, blocks = (a.terms + TERMS - 1) / TERMS;
+    const uint16_t* w = a.w + (size_t)t.expert * a.terms * a.cols;
+    M m;
+    N n;
+    if (a.token) m.init(a.x, 2 * a.terms, t.rows, (uint32_t)a.xbytes, a.token + t.row);
+    else m.init(a.x + (size_t)t.row * a.terms, 2 * a.terms, t.rows, (uint32_t)t.rows * a.terms * 2, nullptr);
+    if constexpr (ACROSS) n.init(w, 2 * a.cols, col0, a.cols);
+    else n.init(w + (size_t)col0 * a.terms, 2 * a.terms, min(COLS, a.cols - col0), (uint32_t)min(COLS, a.cols - col0) * a.terms * 2, nullptr);
+    f4_t acc[S::MB][S::NB];
+#pragma unroll
+    for (int i = 0; i < S::MB; ++i)
+#pragma unroll
+        for (int j = 0; j < S::NB; ++j) acc[i][j] = f4_t{ 0.f, 0.f, 0.f, 0.f };
+    auto load = [&](int b) {
+        unsigned char* at = lds + b % S::STAGES * S::STAGE;
+        m.load(at, b, a.terms);
+        n.load(at + M::BYTES, b, a.terms);
+    };
+    constexpr int L = M::LOADS + N::LOADS, AHEAD = S::STAGES - 1;
+    const uint32_t mp = M::place(wave / S::WN * S::MB * 16), np = N::place(wave % S::WN * S::NB * 16);
+    for (int b = 0; b < AHEAD; ++b)
+        if (b < blocks) load(b);
+    for (int b = 0; b < blocks; ++b)
+    {
+        // block b has come once only the loads after it are out; the barrier shows it to every wave, and that all are past block b - 1
+        if (b + AHEAD <= blocks) wait_vmcnt<(AHEAD - 1) * L>();
+        else wait_vmcnt<0>();
+        lds_barrier();
+        if (b + AHEAD < blocks) load(b + AHEAD);
+        const unsigned char* at = lds + b % S::STAGES * S::STAGE;
+        multiply<XT, M, N, S, false, ACROSS>(at, at + M::BYTES, mp, np, acc);
+    }
+    store<XT, S>(acc, a.y, a.type, t.row, t.rows, col0, a.cols, a.cols);
+}
+
+template <int XT, bool ACROSS>
+__global__ __launch_bounds__(512, 2) void k_group_rows(RowsArgs a)
+{
+    __shared__ __align__(16) unsigned char lds[LDS_ROWS];
+    const int s = tile_of_block(blockIdx.x), nt = *a.ntiles;
+    if (s >= nt * a.colt) return;
+    // the tiles of an expert: row tiles next to each other, then the next column tile
+    const GroupTile f = a.tiles[s / a.colt];
+    const int l = s - f.first * a.colt;
+    const GroupTile t = a.tiles[f.first + l % f.count];
+    const int ct = l / f.count;
+    if (t.expert < 0)
+    {
+        if (!a.zero) return;
+        const int per = a.type == MM_DTYPE_F32 ? 4 : 8, n = min(COLS, a.cols - ct * COLS) / per;
+        for (int i = threadIdx.x; i < t.rows * n; i += 512)
+        {
+            const size_t at = (size_t)(t.row + i / n) * a.cols + ct * COLS + i % n * per;
+            *reinterpret_cast<u4_t*>(static_cast<unsigned char*>(a.y) + at * (16 / per)) = u4_t{ 0, 0, 0, 0 };
+        }
+        return;
+    }
+    if (t.rows > 128) rows_tile<XT, ACROSS, 256>(a, t, ct, lds);
+    else if (t.rows > 64) rows_tile<XT, ACROSS, 128>(a, t, ct, lds);
+    else if (t.rows > 32) rows_tile<XT, ACROSS, 64>(a, t, ct, lds);
+    else if (t.rows > 16) rows_tile<XT, ACROSS, 32>(a, t, ct, lds);
+    else rows_tile<XT, ACROSS, 16>(a, t, ct, lds);
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// Gradient of the weights: rows of dW[e] are columns of dy, its columns those of x; the terms are the expert's rows.
+// ---------------------------------------------------------------------------------------------------------
+struct WeightsArgs
+{
+    const uint16_t *dy, *x;
+    void* dw;
+    const int32_t *offsets, *token;
+    size_t pbytes;                // of the tensor that token picks from
+    int E, N, K, type, rowt, colt;
+};
+
+// Block b of both operands, and the tokens of the next one's rows. PICK: 0 neither tensor has rows per token, 1 dy has, 2 x has.
+using Terms = Across<256>;
+template <int PICK>
+__device__ __forceinline__ void load_terms(const Terms& m, const Terms& n, Terms::Picks& p, const int32_t* token, uint32_t bytes, unsigned char* at,
+                                           int b, int terms)
+{
+    if constexpr (PICK == 1) m.load_picked(at, p, bytes);
+    else m.load(at, b, terms);
+    if constexpr (PICK == 2) n.load_picked(at + Terms::BYTES, p, bytes);
+    else n.load(at + Terms::BYTES, b, terms);
+    if constexpr (PICK != 0) (PICK == 1 ? m : n).next(p, token, b + 1, terms);
+}
+
+template <int XT, int PICK>
+__global__ __launch_bounds__(512, 2) void k_group_weights(WeightsArgs a)
+{
+    using S = Shape<256>;
+    using O = Terms;
+    __shared__ __align__(16) unsigned char lds[S::STAGE * S::STAGES];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int s = tile_of_block(blockIdx.x);
+    if (s >= a.E * a.rowt * a.colt) return;
+    const int e = s / (a.rowt * a.colt), l = s - e * a.rowt * a.colt, row0 = l % a.rowt * ROWS, col0 = l / a.rowt * COLS;
+    const int p0 = a.offsets[e], terms = a.offsets[e + 1] - p0, blocks = (terms + TERMS - 1) / TERMS;
+    O m, n;
+    m.init(PICK == 1 ? a.dy : a.dy + (size_t)p0 * a.N, 2 * a.N, row0, a.N);
+    n.init(PICK == 2 ? a.x : a.x + (size_t)p0 * a.K, 2 * a.K, col0, a.K);
+    f4_t acc[S::MB][S::NB];
+#pragma unroll
+    for (int i = 0; i < S::MB; ++i)
+#pragma unroll
+        for (int j = 0; j < S::NB; ++j) acc[i][j] = f4_t{ 0.f, 0.f, 0.f, 0.f };
+    const int32_t* token = PICK != 0 ? a.token + p0 : nullptr;
+    O::Picks p;
+    const uint32_t mp = O::place(wave / S::WN * S::MB * 16), np = O::place(wave % S::WN * S::NB * 16);
+    if constexpr (PICK != 0) (PICK == 1 ? m : n).next(p, token, 0, terms);
+    if (blocks) load_terms<PICK>(m, n, p, token, (uint32_t)a.pbytes, lds, 0, terms);
+    for (int b = 0; b < blocks; ++b)
+    {
+        wait_vmcnt<0>();
+        lds_barrier();
+        if (b + 1 < blocks) load_terms<PICK>(m, n, p, token, (uint32_t)a.pbytes, lds + (b + 1) % 2 * S::STAGE, b + 1, terms);
+        const unsigned char* at = lds + b % 2 * S::STAGE;
+        multiply<XT, O, O, S, true, true>(at, at + O::BYTES, mp, np, acc);
+    }
+    store<XT, S>(acc, a.dw, a.type, (size_t)e * a.N + row0, min(ROWS, a.N - row0), col0, a.K, a.K);
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// Rows summed per token, in the order of its picks: out[t] = sum over j of rows[inv[t k + j]], picks of no expert left out.
+// ---------------------------------------------------------------------------------------------------------
+template <int OT>
+__global__ __launch_bounds__(256) void k_group_sum(const float* __restrict__ rows, const int32_t* __restrict__ inv, const int32_t* __restrict__ live,
+                                                   long long n4, int topk, int cols4, void* __restrict__ out)
+{
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n4) return;
+    const long long t = i / cols4;
+    const int c = (int)(i - t * cols4), end = *live;
+    f4_t s = f4_t{ 0.f, 0.f, 0.f, 0.f };
+    for (int j = 0; j < topk; ++j)
+    {
+        const int p = inv[t * topk + j];
+        if (p < end)
+        {
+            const f4_t v = reinterpret_cast<const f4_t*>(rows)[(size_t)p * cols4 + c];
+            s.x += v.x;
+            s.y += v.y;
+            s.z += v.z;
+            s.w += v.w;
+        }
+    }
+    if constexpr (OT == MM_DTYPE_F32) reinterpret_cast<f4_t*>(out)[i] = s;
+    else reinterpret_cast<u2_t*>(out)[i] = u2_t{ pack2<OT>(s.x, s.y), pack2<OT>(s.z, s.w) };
+}
+
+}  // namespace mm
+
+using namespace mm;
+
+namespace {
+
+constexpr long long MOST_BLOCKS = 0x7fffffffLL;
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// Checks that the products share; routes in *n.
+int check(const char* what, const mm_group_plan_t* p, int dtype, int K, int N, int out_type)
+{
+    MM_CHECK_ARG(p && p->offsets && p->order && p->token && p->inv && p->tiles && p->ntiles, "%s: incomplete plan", what);
+    MM_CHECK_ARG(p->T > 0 && p->topk > 0 && p->E > 0 && p->E <= 1024 && (long long)p->T * p->topk < (1LL << 31) - 256, "%s: bad plan", what);
+    MM_CHECK_ARG(dtype == MM_DTYPE_F16 || dtype == MM_DTYPE_BF16, "%s: rows and weights must be fp16 or bf16", what);
+    MM_CHECK_ARG(out_type == dtype || out_type == MM_DTYPE_F32, "%s: results must have the weights' type or fp32", what);
+    MM_CHECK_ARG(K > 0 && N > 0 && K % 8 == 0 && N % 8 == 0 && K <= 1 << 20 && N <= 1 << 20 && (long long)K * N < 1LL << 31,
+                 "%s: K and N must be multiples of 8, at most 2^20, and K N below 2^31 (K %d, N %d)", what, K, N);
+    return MM_OK;
+}
+
+template <bool ACROSS>
+int launch_rows(const char* what, const mm_group_plan_t* p, const void* x, const void* w, int dtype, int terms, int cols, int gather, int reduce,
+                void* y, int y_type, void* ws, size_t ws_bytes, mm_stream_t stream)
+{
+    const long long n = (long long)p->T * p->topk;
+    MM_CHECK_ARG(x && w && y, "%s: null pointer", what);
+    MM_CHECK_ARG(aligned16(x) && aligned16(w) && aligned16(y) && aligned16(ws), "%s: misaligned pointer", what);
+    const size_t need = reduce ? (size_t)n * cols * 4 : 0;
+    MM_CHECK_ARG(ws_bytes >= need && (!need || ws), "%s: workspace too small (%zu < %zu)", what, ws_bytes, need);
+    MM_CHECK_ARG(!gather || (long long)p->T * terms < 1LL << 31, "%s: rows per token must be below 4 GiB", what);
+    const hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
+    RowsArgs a = {};
+    a.x = static_cast<const uint16_t*>(x);
+    a.w = static_cast<const uint16_t*>(w);
+    a.y = reduce ? ws : y;
+    a.tiles = reinterpret_cast<const GroupTile*>(p->tiles);
+    a.ntiles = p->ntiles;
+    a.token = gather ? p->token : nullptr;
+    a.xbytes = (size_t)p->T * terms * 2;
+    a.terms = terms;
+    a.cols = cols;
+    a.type = reduce ? MM_DTYPE_F32 : y_type;
+    a.zero = !reduce;
+    a.colt = (cols + COLS - 1) / COLS;
+    const long long tiles = tile_capacity(n, p->E) * a.colt, blocks = (tiles + 255) / 256 * 256;
+    MM_CHECK_ARG(blocks <= MOST_BLOCKS, "%s: too many tiles", what);
+    auto kernel = dtype == MM_DTYPE_F16 ? k_group_rows<MM_DTYPE_F16, ACROSS> : k_group_rows<MM_DTYPE_BF16, ACROSS>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(512), 0, hs, a);
+    if (reduce)
+    {
+        const long long n4 = (long long)p->T * cols / 4;
+        MM_CHECK_ARG((n4 + 255) / 256 <= MOST_BLOCKS, "%s: too many tokens", what);
+        auto sum = y_type == MM_DTYPE_F32 ? k_group_sum<MM_DTYPE_F32> : y_type == MM_DTYPE_F16 ? k_group_sum<MM_DTYPE_F16> : k_group_sum<MM_DTYPE_BF16>;
+        hipLaunchKernelGGL(sum, dim3((unsigned)((n4 + 255) / 256)), dim3(256), 0, hs, static_cast<const float*>(ws), p->inv, p->offsets + p->E, n4,
+                           p->topk, cols / 4, y);
+    }
+    return check_launch(what);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t mm_group_tiles(int n, int E) { return n > 0 && E > 0 ? (size_t)tile_capacity(n, E) * sizeof(GroupTile) : 0; }
+
+int mm_group_plan(const int64_t* ids, const mm_group_plan_t* p, int32_t* counts, void* workspace, size_t workspace_bytes, mm_stream_t stream)
+{
+    MM_CHECK_ARG(p && p->offsets && p->order && p->token && p->inv && p->tiles && p->ntiles && counts && ids, "mm_group_plan: null pointer");
+    MM_CHECK_ARG(p->T > 0 && p->topk > 0 && p->E > 0 && p->E <= 1024 && (long long)p->T * p->topk < (1LL << 31) - 256,
+                 "mm_group_plan: need tokens, picks, 1 <= E <= 1024 and fewer than 2^31 - 256 routes");
+    MM_CHECK_ARG(aligned16(p->tiles), "mm_group_plan: misaligned tiles");
+    const int rc = permute_launch(ids, nullptr, p->T * p->topk, p->topk, p->E, counts, p->offsets, p->order, p->token, nullptr, p->inv, nullptr,
+                                  nullptr, workspace, workspace_bytes, stream);
+    if (rc != MM_OK) return rc;
+    hipLaunchKernelGGL(k_group_tiles, dim3(1), dim3(1024), 0, reinterpret_cast<hipStream_t>(stream), p->offsets, p->E,
+                       reinterpret_cast<GroupTile*>(p->tiles), p->ntiles);
+    return check_launch("mm_group_plan");
+}
+
+size_t mm_group_linear_workspace(int T, int topk, int cols, int reduce)
+{
+    return reduce && T > 0 && topk > 0 && cols > 0 ? (size_t)T * topk * cols * 4 : 0;
+}
+
+int mm_group_linear(const mm_group_plan_t* plan, const void* x, const void* w, int dtype, int K, int N, int gather, int reduce, void* y,
+                    int y_dtype, void* workspace, size_t workspace_bytes, mm_stream_t stream)
+{
+    if (const int rc = check("mm_group_linear", plan, dtype, K, N, y_dtype)) return rc;
+    return launch_rows<false>("mm_group_linear", plan, x, w, dtype, K, N, gather, reduce, y, y_dtype, workspace, workspace_bytes, stream);
+}
+
+int mm_group_linear_inputs(const mm_group_plan_t* plan, const void* dy, const void* w, int dtype, int K, int N, int gather, int reduce, void* dx,
+                           int dx_dtype, void* workspace, size_t workspace_bytes, mm_stream_t stream)
+{
+    if (const int rc = check("mm_group_linear_inputs", plan, dtype, K, N, dx_dtype)) return rc;
+    return launch_rows<true>("mm_group_linear_inputs", plan, dy, w, dtype, N, K, reduce, gather, dx, dx_dtype, workspace, workspace_bytes, stream);
+}
+
+int mm_group_linear_weights(const mm_group_plan_t* plan, const void* dy, const void* x, int dtype, int K, int N, int gather, int reduce, void* dw,
+                            int dw_dtype, mm_stream_t stream)
+{
+    if (const int rc = check("mm_group_linear_weights", plan, dtype, K, N, dw_dtype)) return rc;
+    MM_CHECK_ARG(dy && x && dw, "mm_group_linear_weights: null pointer");
+    MM_CHECK_ARG(aligned16(dy) && aligned16(x) && aligned16(dw), "mm_group_linear_weights: misaligned pointer");
+    MM_CHECK_ARG(!(gather && reduce), "mm_group_linear_weights: one of x and dy may have rows per token");
+    const int width = gather ? K : N;
+    MM_CHECK_ARG(!(gather || reduce) || (long long)plan->T * width < 1LL << 31, "mm_group_linear_weights: rows per token must be below 4 GiB");
+    WeightsArgs a = {};
+    a.dy = static_cast<const uint16_t*>(dy);
+    a.x = static_cast<const uint16_t*>(x);
+    a.dw = dw;
+    a.offsets = plan->offsets;
+    a.token = plan->token;
+    a.pbytes = (size_t)plan->T * width * 2;
+    a.E = plan->E;
+    a.N = N;
+    a.K = K;
+    a.type = dw_dtype;
+    a.rowt = (N + ROWS - 1) / ROWS;
+    a.colt = (K + COLS - 1) / COLS;
+    const long long tiles = (long long)plan->E * a.rowt * a.colt, blocks = (tiles + 255) / 256 * 256;
+    MM_CHECK_ARG(blocks <= MOST_BLOCKS, "mm_group_linear_weights: too many tiles");
+    const bool h = dtype == MM_DTYPE_F16;
+    auto kernel = gather ? (h ? k_group_weights<MM_DTYPE_F16, 2> : k_group_weights<MM_DTYPE_BF16, 2>)
+                : reduce ? (h ? k_group_weights<MM_DTYPE_F16, 1> : k_group_weights<MM_DTYPE_BF16, 1>)
+                         : (h ? k_group_weights<MM_DTYPE_F16, 0> : k_group_weights<MM_DTYPE_BF16, 0>);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(512), 0, reinterpret_cast<hipStream_t>(stream), a);
+    return check_launch("mm_group_linear_weights");
+}
+
+}  // extern "C"

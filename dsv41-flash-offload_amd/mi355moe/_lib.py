@@ -43,6 +43,13 @@ class MMW4Layer(ctypes.Structure):
                 ("limit", f32)]
 
 
+class MMGroupPlan(ctypes.Structure):
+    """Mirror of mm_group_plan_t."""
+
+    _fields_ = [("offsets", vp), ("order", vp), ("token", vp), ("inv", vp), ("tiles", vp), ("ntiles", vp), ("T", i32), ("topk", i32),
+                ("E", i32)]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     "mm_version": (i32, []),
@@ -76,6 +83,14 @@ _SIGS = {
     "mm_w4_linear": (i32, [vp, i32, i32, i32, i32, ctypes.POINTER(MMW4), i32, i32, vp, i32, vp, sz, vp]),
     "mm_w4_moe_workspace": (sz, [i32, i32, i32, i32, i32, i32, i32]),
     "mm_w4_moe": (i32, [ctypes.POINTER(MMW4Layer), vp, i32, i32, i32, vp, vp, i32, vp, vp, sz, vp]),
+    "mm_group_tiles": (sz, [i32, i32]),
+    "mm_group_plan": (i32, [vp, ctypes.POINTER(MMGroupPlan), vp, vp, sz, vp]),
+    "mm_group_linear_workspace": (sz, [i32, i32, i32, i32]),
+    "mm_group_linear": (i32, [ctypes.POINTER(MMGroupPlan), vp, vp, i32, i32, i32, i32, i32, vp, i32, vp, sz, vp]),
+    "mm_group_linear_inputs": (i32, [ctypes.POINTER(MMGroupPlan), vp, vp, i32, i32, i32, i32, i32, vp, i32, vp, sz, vp]),
+    "mm_group_linear_weights": (i32, [ctypes.POINTER(MMGroupPlan), vp, vp, i32, i32, i32, i32, i32, vp, i32, vp]),
+    "mm_gated": (i32, [ctypes.POINTER(MMGroupPlan), vp, i32, i32, i32, vp, f32, vp, vp, vp, vp]),
+    "mm_gated_backward": (i32, [ctypes.POINTER(MMGroupPlan), vp, vp, vp, vp, i32, i32, i32, vp, f32, vp, vp, vp, vp]),
     "mm_slot_point": (i32, [vp, vp, vp, vp, i32, vp, i32, vp]),
     "mm_stage_copy": (i32, [vp, vp, vp, i32, vp]),
     "mm_copy_stream": (i32, [i32, i32, vp, ctypes.POINTER(vp)]),

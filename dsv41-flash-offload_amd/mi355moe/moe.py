@@ -6,7 +6,7 @@ import warnings
 
 import torch
 
-from . import _lib, w4
+from . import _lib, dense, w4
 
 # Default fat-expert threshold of moe_forward (the reference image's VLLM_EXL3_FAT_THRESHOLD, docker/entrypoint.sh:69): calls
 # of at most this many tokens run on the decode path, larger ones go to mm_fused_moe.
@@ -122,12 +122,15 @@ def moe_forward(store, x, ids, w, shared_expert=None, fat_threshold=FAT_THRESHOL
     decode path. A larger call goes to mm_fused_moe, which takes the decode path or the grouped GEMM by its routes and
     experts. No call synchronises the host, so every call can be captured in a HIP graph.
 
-    A layer of 4-bit experts (w4.W4Store) runs on w4.moe, whatever the threshold.
+    A layer of 4-bit experts (w4.W4Store) runs on w4.moe, one of 16-bit experts (dense.DenseStore) on dense.moe, whatever the
+    threshold.
 
-    The output records no gradient, neither into x nor into w (router.topk's weights among them): inputs that require one get a
-    warning here and are refused by w4.moe."""
+    The output of a DenseStore has gradients into x, w and the weights. That of the others records none, neither into x nor into w
+    (router.topk's weights among them): inputs that require one get a warning here and are refused by w4.moe."""
     if isinstance(store, w4.W4Store):
         return w4.moe(store, x, ids, w, shared_expert=shared_expert, stream=stream)
+    if isinstance(store, dense.DenseStore):
+        return dense.moe(store, x, ids, w, shared_expert=shared_expert, stream=stream)
     name = _lib.wants_gradient(x=x, w=w) if x.requires_grad or w.requires_grad else None
     if name:
         warnings.warn(f"moe_forward: {name} requires a gradient, but the output carries no gradient (detach it, or call under "

@@ -307,6 +307,53 @@ size_t mm_w4_moe_workspace(int x_dtype, int T, int topk, int shared, int E, int 
 int mm_w4_moe(const mm_w4_layer_t* layer, const void* x, int x_dtype, int T, int topk, const int64_t* ids, const float* w,
               int shared, float* out, void* workspace, size_t workspace_bytes, mm_stream_t stream);
 
+/* ------------------------------------------------------------------------- experts in 16-bit weights, trainable */
+
+/* The order of a call's routes that the grouped products share: T tokens of topk picks each, sorted by expert (stable), picks
+ * outside [0, E) last. Device memory: offsets int32 [E + 2] (rows offsets[e] .. offsets[e + 1] - 1 belong to expert e, rows from
+ * offsets[E] on to none), order int32 [n] (flat route of each row, n = T topk < 2^31 - 256), token int32 [n] (order / topk), inv int32 [n]
+ * (row of each route), tiles (mm_group_tiles(n, E) bytes, 16-byte aligned) and ntiles int32 [1], the kernels' own. E <= 1024. */
+typedef struct mm_group_plan
+{
+    int32_t *offsets, *order, *token, *inv;
+    void* tiles;
+    int32_t* ntiles;
+    int T, topk, E;
+} mm_group_plan_t;
+
+/* Fills a plan's buffers from ids int64 [T][topk]. counts int32 [E + 1]: rows of each expert (and of none). Workspace:
+ * mm_permute_workspace(n, E) bytes. */
+size_t mm_group_tiles(int n, int E);
+int mm_group_plan(const int64_t* ids, const mm_group_plan_t* plan, int32_t* counts, void* workspace, size_t workspace_bytes,
+                  mm_stream_t stream);
+
+/* y[p] = W[e] x[p] over the rows p of each expert e: w [E][N][K] and x in dtype (fp16 or bf16), y in dtype or fp32, sums in fp32,
+ * rounded once. gather: x is [T][K] and row p reads row token[p], else [n][K]. reduce: y is [T][N], the sum of each token's rows in the order
+ * of its picks (from fp32 rows in the workspace: mm_group_linear_workspace(T, topk, N, reduce) bytes); else [n][N], rows of no expert
+ * zero. K and N multiples of 8, at most 2^20, K N < 2^31; tensors of rows per token below 4 GiB; all pointers 16-byte aligned. */
+size_t mm_group_linear_workspace(int T, int topk, int cols, int reduce);
+int mm_group_linear(const mm_group_plan_t* plan, const void* x, const void* w, int dtype, int K, int N, int gather, int reduce,
+                    void* y, int y_dtype, void* workspace, size_t workspace_bytes, mm_stream_t stream);
+/* Gradient of x: dx[p] = W[e]^T dy[p], of the same product: with gather dx is [T][K], summed per token (workspace:
+ * mm_group_linear_workspace(T, topk, K, gather)), with reduce dy is [T][N]. */
+int mm_group_linear_inputs(const mm_group_plan_t* plan, const void* dy, const void* w, int dtype, int K, int N, int gather, int reduce,
+                           void* dx, int dx_dtype, void* workspace, size_t workspace_bytes, mm_stream_t stream);
+/* Gradient of W: dw [E][N][K] (dtype or fp32) = sum over the rows of each expert of dy[p] x[p]^T; zero for experts without rows. */
+int mm_group_linear_weights(const mm_group_plan_t* plan, const void* dy, const void* x, int dtype, int K, int N, int gather, int reduce,
+                            void* dw, int dw_dtype, mm_stream_t stream);
+
+/* The activation between an expert's two products: rows gu [n][2 I] = [g | u] (fp16 or bf16) to h [n][I] =
+ * w min(silu(g), limit) clamp(u, -limit, limit) (limit 0: no clamp), w = weights[order[p]] of the plan's routes (fp32 [n]; NULL: 1);
+ * without a plan, row p's own. Rows of no expert give zeros. codes int8 [n][2 I] and exps int8 [n][2 I / 32] (both or neither; I a
+ * multiple of 32) take gu in 8 bits: codes times 2^exps per 32 neighbours, the least exponent (from -126 on) that keeps |code| <= 127, rounded to
+ * nearest even; 32 that hold an infinity or NaN have exponent 127 and come back as NaN. I a multiple of 8, at most 2^20. */
+int mm_gated(const mm_group_plan_t* plan, const void* gu, int dtype, int n, int I, const float* weights, float limit, void* h,
+             int8_t* codes, int8_t* exps, mm_stream_t stream);
+/* Its gradient, from gu or from its 8 bits (the other NULL): dgu [n][2 I] (zero where a clamp is passed), dweights fp32 [n] by route and
+ * h [n][I] once more (either may be NULL). */
+int mm_gated_backward(const mm_group_plan_t* plan, const void* dh, const void* gu, const int8_t* codes, const int8_t* exps, int dtype,
+                      int n, int I, const float* weights, float limit, void* dgu, float* dweights, void* h, mm_stream_t stream);
+
 /* ------------------------------------------------------------------------------------ expert placement */
 
 /* Slot-table repoint; replaces _ec_point's index_copy_ writes (ct/ct_vllm.py:268-279): items int64 [n][5] =
