@@ -109,7 +109,7 @@ constexpr uint32_t NOWHERE = 0xfffffff0u;              // past every buffer: rea
 template <int R>
 struct Along
 {
-    static constexpr int BYTES = R * 128, LOADS = std::max(1, R / 64);
+    static constexpr int BYTES = R * 128, LOADS = std::max(1, R / 64), READS = 1;
     __amdgpu_buffer_rsrc_t buf;
     uint32_t at[LOADS];
     int slot;             // the wave's first row
@@ -149,45 +149,57 @@ struct Along
     }
 };
 
-// 64 rows (terms) of R columns; LDS [64][R], 32-byte piece p of row k at p ^ swizzle(k).
-template <int R>
+// The transposing LDS load: 16 lanes read 4 rows of 16 columns, lane 4 q + c giving row q, columns 4 c .. 4 c + 3; lane i gets column i.
+// (__restrict__: without alias information the compiler waits for every load that writes LDS directly before each of these; the
+// waits and barriers in run() are the ones needed.)
+typedef __attribute__((address_space(3))) s4_t* lds_s4_t;
+__device__ __forceinline__ u2_t read_transposed(lds_s4_t __restrict__ p)
+{
+    return __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p));
+}
+
+// 64 rows (terms) of 256 columns; LDS [64][256], 32-byte piece p of row k at p ^ swizzle(k). A wave's load is two rows; loads 2 and 3 are
+// four rows below loads 0 and 1.
 struct Across
 {
-    static constexpr int BYTES = R * 128, LOADS = R / 64, RB = 2 * R, ROWS_LOAD = 1024 / RB;   // rows that one load covers
-    static_assert(R == 256 || R == 128, "columns");
+    static constexpr int BYTES = 256 * 128, LOADS = 4, READS = 2, RB = 512;
     struct Picks
     {
         int32_t row[LOADS];
     };
     const unsigned char* base;
-    uint32_t ld, at[LOADS];
-    int row[LOADS], slot;
-    // four rows of one 8-row group and the four groups that a wave reads at once
-    __device__ static __forceinline__ int swizzle(int k) { return ((k & 3) | ((k >> 3) & 3) << 2) & (R / 16 - 1); }
+    uint32_t ld, col[2];
+    int row, slot;                 // the lane's row of load 0, the wave's
+    // different for four rows of an 8-row group and for the four groups that a wave reads at once
+    __device__ static __forceinline__ int swizzle(int k) { return (k & 3) | ((k >> 3) & 3) << 2; }
     // base: column 0 of row 0; first: the tile's first column; width: columns of a row
     __device__ __forceinline__ void init(const void* b, uint32_t ld_, int first, int width)
     {
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int lane = threadIdx.x & 63, s = lane & 31;
         base = static_cast<const unsigned char*>(b);
         ld = ld_;
-        slot = wave * LOADS * ROWS_LOAD;
+        slot = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 8;
+        row = slot + (lane >> 5);
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i)
+        for (int i = 0; i < 2; ++i)
         {
-            const int k = slot + ROWS_LOAD * i + lane / (RB / 16), s = lane % (RB / 16);
-            const int c = first + 8 * (((s >> 1) ^ swizzle(k)) * 2 + (s & 1));
-            row[i] = k;
-            at[i] = c < width ? k * ld + 2 * c : NOWHERE;
+            const int c = first + 8 * (((s >> 1) ^ swizzle(row + 2 * i)) * 2 + (s & 1));
+            col[i] = c < width ? 2 * c : NOWHERE;
         }
     }
     // rows 64 block .. of `terms`
     __device__ __forceinline__ void load(unsigned char* lds, int block, int terms) const
     {
-        const int left = terms - TERMS * block;
-        const __amdgpu_buffer_rsrc_t buf = buffer(base + (size_t)block * TERMS * ld, (uint32_t)max(0, min(left, TERMS)) * ld);
+        const int left = min(terms - TERMS * block, TERMS);
+        const unsigned char* p = base + (size_t)block * TERMS * ld;
+        const __amdgpu_buffer_rsrc_t b0 = buffer(p, (uint32_t)max(0, left) * ld), b1 = buffer(p + 4 * (size_t)ld, (uint32_t)max(0, left - 4) * ld);
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-            load16(buf, lds + (slot + ROWS_LOAD * i) * RB, at[i]);
+        for (int i = 0; i < 2; ++i)
+        {
+            const uint32_t at = col[i] == NOWHERE ? NOWHERE : (row + 2 * i) * ld + col[i];
+            load16(b0, lds + (slot + 2 * i) * RB, at);
+            load16(b1, lds + (slot + 2 * i + 4) * RB, at);
+        }
     }
     // the same with the rows that `pick` names, taken a block ahead by next(); bytes: of the whole tensor
     __device__ __forceinline__ void next(Picks& p, const int32_t* pick, int block, int terms) const
@@ -195,8 +207,9 @@ struct Across
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
         {
-            const int k = TERMS * block + row[i];
-            p.row[i] = k < terms ? pick[k] : -1;
+            const int k = TERMS * block + row + 2 * i;
+            const int32_t r = pick[min(k, terms - 1)];
+            p.row[i] = k < terms ? r : -1;
         }
     }
     __device__ __forceinline__ void load_picked(unsigned char* lds, const Picks& p, uint32_t bytes) const
@@ -204,10 +217,9 @@ struct Across
         const __amdgpu_buffer_rsrc_t buf = buffer(base, bytes);
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
-            load16(buf, lds + (slot + ROWS_LOAD * i) * RB, p.row[i] < 0 || at[i] == NOWHERE ? NOWHERE : (uint32_t)p.row[i] * ld + (at[i] - row[i] * ld));
+            load16(buf, lds + (slot + 2 * i) * RB, p.row[i] < 0 || col[i & 1] == NOWHERE ? NOWHERE : (uint32_t)p.row[i] * ld + col[i & 1]);
     }
-    // terms 32 kk + 8 (lane >> 4) .. + 7 of column 16 b + (lane & 15): the transposing load takes 4 rows of 16 columns from 16 lanes,
-    // lane 4 q + c giving row q, columns 4 c .. 4 c + 3, and leaves column i on lane i
+    // terms 32 kk + 8 (lane >> 4) .. + 7 of column 16 b + (lane & 15)
     __device__ static __forceinline__ uint32_t place(int first)
     {
         const int lane = threadIdx.x & 63, k = 8 * (lane >> 4) + ((lane & 15) >> 2);
@@ -215,10 +227,8 @@ struct Across
     }
     __device__ static __forceinline__ u4_t read(const unsigned char* lds, uint32_t place, int b, int kk)
     {
-        typedef __attribute__((address_space(3))) s4_t* at_t;
         const unsigned char* p = lds + (place ^ (32 * b)) + 32 * kk * RB;
-        const u2_t lo = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_t)(p)));
-        const u2_t hi = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_t)(p + 4 * RB)));
+        const u2_t lo = read_transposed((lds_s4_t)p), hi = read_transposed((lds_s4_t)(p + 4 * RB));
         return u4_t{ lo.x, lo.y, hi.x, hi.y };
     }
 };
@@ -236,22 +246,80 @@ struct Shape
 };
 constexpr int LDS_ROWS = 144 * 1024;      // of the row tiles: 3 stages of 128 x 256
 
-template <int XT, typename M, typename N, typename S, bool MT, bool NT>
-__device__ __forceinline__ void multiply(const unsigned char* m, const unsigned char* n, uint32_t mp, uint32_t np, f4_t (&acc)[S::MB][S::NB])
+// Operands of half a block (32 terms).
+template <typename S>
+struct Half
+{
+    u4_t m[S::MB], n[S::NB];
+};
+template <typename M, typename N, typename S>
+__device__ __forceinline__ void read_half(Half<S>& h, const unsigned char* stage, uint32_t mp, uint32_t np, int kk)
 {
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
+    for (int j = 0; j < S::NB; ++j) h.n[j] = N::read(stage + M::BYTES, np, j, kk);
+#pragma unroll
+    for (int i = 0; i < S::MB; ++i) h.m[i] = M::read(stage, mp, i, kk);
+}
+template <int XT, typename S>
+__device__ __forceinline__ void multiply(const Half<S>& h, f4_t (&acc)[S::MB][S::NB])
+{
+#pragma unroll
+    for (int i = 0; i < S::MB; ++i)
+#pragma unroll
+        for (int j = 0; j < S::NB; ++j) acc[i][j] = mfma<XT>(h.n[j], h.m[i], acc[i][j]);
+}
+// The products of one half with READS LDS reads of the next between them.
+template <typename S, int READS>
+__device__ __forceinline__ void interleave()
+{
+    constexpr int PRODUCTS = S::MB * S::NB;
+#pragma unroll
+    for (int i = 0; i < READS; ++i)
     {
-        u4_t b[S::NB], a[S::MB];
-#pragma unroll
-        for (int j = 0; j < S::NB; ++j) b[j] = N::read(n, np, j, kk);
-#pragma unroll
-        for (int i = 0; i < S::MB; ++i) a[i] = M::read(m, mp, i, kk);
-#pragma unroll
-        for (int i = 0; i < S::MB; ++i)
-#pragma unroll
-            for (int j = 0; j < S::NB; ++j) acc[i][j] = mfma<XT>(b[j], a[i], acc[i][j]);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, std::max(1, PRODUCTS / READS), 0);
     }
+    __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS, 0);
+}
+
+// All blocks of a tile. Half a block's operands are read from LDS while the half before is multiplied, across the barrier too, which stands
+// in the middle of a block: a wave that waits there has half a block to multiply. Block b's place is free once every wave has
+// read its second half, so loads run STAGES blocks ahead. load(b) sends a wave's L loads of block b.
+template <int XT, typename M, typename N, typename S, int L, typename Load>
+__device__ __forceinline__ void run(unsigned char* lds, int blocks, uint32_t mp, uint32_t np, const Load& load, f4_t (&acc)[S::MB][S::NB])
+{
+    constexpr int READS = S::MB * M::READS + S::NB * N::READS;
+    Half<S> h0, h1;
+    for (int b = 0; b < S::STAGES; ++b)
+        if (b < blocks) load(b);
+    if (blocks >= S::STAGES) wait_vmcnt<(S::STAGES - 1) * L>();
+    else wait_vmcnt<0>();
+    lds_barrier();
+    read_half<M, N, S>(h0, lds, mp, np, 0);
+    int at = 0;
+#pragma clang loop unroll(disable)
+    for (int b = 0; b + 1 < blocks; ++b)
+    {
+        // (the places of the blocks are made from these two again each time, rather than kept in registers)
+        asm volatile("" : "+v"(mp), "+v"(np));
+        read_half<M, N, S>(h1, lds + at, mp, np, 1);
+        multiply<XT, S>(h0, acc);
+        interleave<S, READS>();
+        // block b + 1 has come once only the loads after it are out
+        if (b + S::STAGES <= blocks) wait_vmcnt<(S::STAGES - 2) * L>();
+        else wait_vmcnt<0>();
+        lds_barrier();
+        if (b + S::STAGES < blocks) load(b + S::STAGES);
+        at = at + S::STAGE == S::STAGES * S::STAGE ? 0 : at + S::STAGE;
+        asm volatile("" : "+v"(mp), "+v"(np));
+        read_half<M, N, S>(h0, lds + at, mp, np, 0);
+        multiply<XT, S>(h1, acc);
+        interleave<S, READS>();
+    }
+    read_half<M, N, S>(h1, lds + at, mp, np, 1);
+    multiply<XT, S>(h0, acc);
+    interleave<S, READS>();
+    multiply<XT, S>(h1, acc);
 }
 
 // Lane (r, g) of a block holds columns 4 g .. 4 g + 3 of row r. For 16-bit outputs neighbouring blocks trade halves, so that a lane
@@ -309,7 +377,7 @@ __device__ __forceinline__ void rows_tile(const RowsArgs& a, const GroupTile& t,
 {
     using S = Shape<R>;
     using M = Along<R>;
-    using N = std::conditional_t<ACROSS, Across<COLS>, Along<COLS>>;
+    using N = std::conditional_t<ACROSS, Across, Along<COLS>>;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col0 = ct * COLS, blocks = (a.terms + TERMS - 1) / TERMS;
     const uint16_t* w = a.w + (size_t)t.expert * a.terms * a.cols;
@@ -329,20 +397,8 @@ __device__ __forceinline__ void rows_tile(const RowsArgs& a, const GroupTile& t,
         m.load(at, b, a.terms);
         n.load(at + M::BYTES, b, a.terms);
     };
-    constexpr int L = M::LOADS + N::LOADS, AHEAD = S::STAGES - 1;
     const uint32_t mp = M::place(wave / S::WN * S::MB * 16), np = N::place(wave % S::WN * S::NB * 16);
-    for (int b = 0; b < AHEAD; ++b)
-        if (b < blocks) load(b);
-    for (int b = 0; b < blocks; ++b)
-    {
-        // block b has come once only the loads after it are out; the barrier shows it to every wave, and that all are past block b - 1
-        if (b + AHEAD <= blocks) wait_vmcnt<(AHEAD - 1) * L>();
-        else wait_vmcnt<0>();
-        lds_barrier();
-        if (b + AHEAD < blocks) load(b + AHEAD);
-        const unsigned char* at = lds + b % S::STAGES * S::STAGE;
-        multiply<XT, M, N, S, false, ACROSS>(at, at + M::BYTES, mp, np, acc);
-    }
+    run<XT, M, N, S, M::LOADS + N::LOADS>(lds, blocks, mp, np, load, acc);
     store<XT, S>(acc, a.y, a.type, t.row, t.rows, col0, a.cols, a.cols);
 }
 
@@ -388,15 +444,14 @@ struct WeightsArgs
 };
 
 // Block b of both operands, and the tokens of the next one's rows. PICK: 0 neither tensor has rows per token, 1 dy has, 2 x has.
-using Terms = Across<256>;
 template <int PICK>
-__device__ __forceinline__ void load_terms(const Terms& m, const Terms& n, Terms::Picks& p, const int32_t* token, uint32_t bytes, unsigned char* at,
+__device__ __forceinline__ void load_terms(const Across& m, const Across& n, Across::Picks& p, const int32_t* token, uint32_t bytes, unsigned char* at,
                                            int b, int terms)
 {
     if constexpr (PICK == 1) m.load_picked(at, p, bytes);
     else m.load(at, b, terms);
-    if constexpr (PICK == 2) n.load_picked(at + Terms::BYTES, p, bytes);
-    else n.load(at + Terms::BYTES, b, terms);
+    if constexpr (PICK == 2) n.load_picked(at + Across::BYTES, p, bytes);
+    else n.load(at + Across::BYTES, b, terms);
     if constexpr (PICK != 0) (PICK == 1 ? m : n).next(p, token, b + 1, terms);
 }
 
@@ -404,7 +459,7 @@ template <int XT, int PICK>
 __global__ __launch_bounds__(512, 2) void k_group_weights(WeightsArgs a)
 {
     using S = Shape<256>;
-    using O = Terms;
+    using O = Across;
     __shared__ __align__(16) unsigned char lds[S::STAGE * S::STAGES];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int s = tile_of_block(blockIdx.x);
@@ -423,15 +478,8 @@ __global__ __launch_bounds__(512, 2) void k_group_weights(WeightsArgs a)
     O::Picks p;
     const uint32_t mp = O::place(wave / S::WN * S::MB * 16), np = O::place(wave % S::WN * S::NB * 16);
     if constexpr (PICK != 0) (PICK == 1 ? m : n).next(p, token, 0, terms);
-    if (blocks) load_terms<PICK>(m, n, p, token, (uint32_t)a.pbytes, lds, 0, terms);
-    for (int b = 0; b < blocks; ++b)
-    {
-        wait_vmcnt<0>();
-        lds_barrier();
-        if (b + 1 < blocks) load_terms<PICK>(m, n, p, token, (uint32_t)a.pbytes, lds + (b + 1) % 2 * S::STAGE, b + 1, terms);
-        const unsigned char* at = lds + b % 2 * S::STAGE;
-        multiply<XT, O, O, S, true, true>(at, at + O::BYTES, mp, np, acc);
-    }
+    auto load = [&](int b) { load_terms<PICK>(m, n, p, token, (uint32_t)a.pbytes, lds + b % S::STAGES * S::STAGE, b, terms); };
+    if (blocks) run<XT, O, O, S, 2 * O::LOADS>(lds, blocks, mp, np, load, acc);
     store<XT, S>(acc, a.dw, a.type, (size_t)e * a.N + row0, min(ROWS, a.N - row0), col0, a.K, a.K);
 }
 
