@@ -34,10 +34,14 @@ __device__ __forceinline__ f4_t mfma(u4_t a, u4_t b, f4_t c)
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8_t, a), __builtin_bit_cast(bf8_t, b), c, 0, 0, 0);
 }
+typedef float f2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
+// two values rounded to nearest even, a in the low half
 template <int XT>
 __device__ __forceinline__ uint32_t pack2(float a, float b)
 {
-    return XT == MM_DTYPE_F16 ? (uint32_t)f2h(a) | (uint32_t)f2h(b) << 16 : (uint32_t)f2bf(a) | (uint32_t)f2bf(b) << 16;
+    if constexpr (XT == MM_DTYPE_F16) return (uint32_t)f2h(a) | (uint32_t)f2h(b) << 16;
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t{ a, b }), bf2_t));
 }
 __device__ __forceinline__ const void* scalar_ptr(const void* p)
 {
@@ -102,6 +106,13 @@ __device__ __forceinline__ void load16(__amdgpu_buffer_rsrc_t buf, unsigned char
 {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, lds, 16, at, 0, 0, 0);
 }
+// The lane, made again at each use: what follows from it is not kept in registers across a kernel's main loop.
+__device__ __forceinline__ int lane_here()
+{
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
 constexpr uint32_t NOWHERE = 0xfffffff0u;              // past every buffer: reads zero
 
 // Rows of TERMS terms, R of them; LDS [R][64]. A wave's load is 8 rows of 128 bytes. Tiles of fewer rows than eight waves load
@@ -158,27 +169,23 @@ __device__ __forceinline__ u2_t read_transposed(lds_s4_t __restrict__ p)
     return __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p));
 }
 
-// 64 rows (terms) of 256 columns; LDS [64][256], 32-byte piece p of row k at p ^ swizzle(k). A wave's load is two rows; loads 2 and 3 are
-// four rows below loads 0 and 1.
+// Blocks of B rows (terms) of 256 columns; LDS [B][256], 32-byte piece p of row k at p ^ swizzle(k). A wave's load is two rows.
+template <int B>
 struct Across
 {
-    static constexpr int BYTES = 256 * 128, LOADS = 4, READS = 2, RB = 512;
-    struct Picks
-    {
-        int32_t row[LOADS];
-    };
+    static constexpr int BYTES = B * 512, RB = 512, LOADS = B / 16, READS = 2;
     const unsigned char* base;
-    uint32_t ld, col[2];
+    uint32_t ld, col[2];           // loads 2 and 3 have the columns of 0 and 1
     int row, slot;                 // the lane's row of load 0, the wave's
     // different for four rows of an 8-row group and for the four groups that a wave reads at once
     __device__ static __forceinline__ int swizzle(int k) { return (k & 3) | ((k >> 3) & 3) << 2; }
     // base: column 0 of row 0; first: the tile's first column; width: columns of a row
     __device__ __forceinline__ void init(const void* b, uint32_t ld_, int first, int width)
     {
-        const int lane = threadIdx.x & 63, s = lane & 31;
+        const int lane = lane_here(), s = lane & 31;
         base = static_cast<const unsigned char*>(b);
         ld = ld_;
-        slot = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 8;
+        slot = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 2 * LOADS;
         row = slot + (lane >> 5);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -187,39 +194,53 @@ struct Across
             col[i] = c < width ? 2 * c : NOWHERE;
         }
     }
-    // rows 64 block .. of `terms`
+    // rows B block .. of `terms`
     __device__ __forceinline__ void load(unsigned char* lds, int block, int terms) const
     {
-        const int left = min(terms - TERMS * block, TERMS);
-        const unsigned char* p = base + (size_t)block * TERMS * ld;
-        const __amdgpu_buffer_rsrc_t b0 = buffer(p, (uint32_t)max(0, left) * ld), b1 = buffer(p + 4 * (size_t)ld, (uint32_t)max(0, left - 4) * ld);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-        {
-            const uint32_t at = col[i] == NOWHERE ? NOWHERE : (row + 2 * i) * ld + col[i];
-            load16(b0, lds + (slot + 2 * i) * RB, at);
-            load16(b1, lds + (slot + 2 * i + 4) * RB, at);
-        }
-    }
-    // the same with the rows that `pick` names, taken a block ahead by next(); bytes: of the whole tensor
-    __device__ __forceinline__ void next(Picks& p, const int32_t* pick, int block, int terms) const
-    {
+        const __amdgpu_buffer_rsrc_t buf = buffer(base + (size_t)block * B * ld, (uint32_t)max(0, min(terms - B * block, B)) * ld);
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
-        {
-            const int k = TERMS * block + row + 2 * i;
-            const int32_t r = pick[min(k, terms - 1)];
-            p.row[i] = k < terms ? r : -1;
-        }
+            load16(buf, lds + (slot + 2 * i) * RB, col[i & 1] == NOWHERE ? NOWHERE : (row + 2 * i) * ld + col[i & 1]);
     }
-    __device__ __forceinline__ void load_picked(unsigned char* lds, const Picks& p, uint32_t bytes) const
+    // The same with the rows that `pick` names. A lane holds the name of one of the wave's rows, for CHUNK blocks at once, and the next
+    // CHUNK blocks' are on their way: names read block by block would be waited for with all loads before them.
+    static constexpr int CHUNK = 64 / (2 * LOADS);
+    struct Picks
     {
+        int32_t cur, next;
+    };
+    __device__ __forceinline__ int32_t names(const int32_t* pick, int chunk, int terms) const
+    {
+        const int lane = lane_here(), k = B * (CHUNK * chunk + lane / (2 * LOADS)) + slot + lane % (2 * LOADS);
+        const int32_t r = pick[min(k, terms - 1)];
+        return k < terms ? r : -1;
+    }
+    __device__ __forceinline__ void first_names(Picks& p, const int32_t* pick, int terms) const
+    {
+        p.cur = names(pick, 0, terms);
+        p.next = names(pick, 1, terms);
+    }
+    // bytes: of the whole tensor
+    __device__ __forceinline__ void load_picked(unsigned char* lds, Picks& p, const int32_t* pick, uint32_t bytes, int block, int terms) const
+    {
+        const int at = block % CHUNK;
+        if (at == 0 && block)
+        {
+            p.cur = p.next;
+            p.next = names(pick, block / CHUNK + 1, terms);
+        }
         const __amdgpu_buffer_rsrc_t buf = buffer(base, bytes);
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
-            load16(buf, lds + (slot + 2 * i) * RB, p.row[i] < 0 || col[i & 1] == NOWHERE ? NOWHERE : (uint32_t)p.row[i] * ld + col[i & 1]);
+        {
+            const int32_t r0 = __builtin_amdgcn_readlane(p.cur, 2 * LOADS * at + 2 * i), r1 = __builtin_amdgcn_readlane(p.cur, 2 * LOADS * at + 2 * i + 1);
+            // (a row of none and a column past the width may not add up to a place again)
+            const uint32_t o0 = r0 < 0 ? NOWHERE : (uint32_t)r0 * ld, o1 = r1 < 0 ? NOWHERE : (uint32_t)r1 * ld;
+            const uint32_t o = threadIdx.x & 32 ? o1 : o0;
+            load16(buf, lds + (slot + 2 * i) * RB, o == NOWHERE || col[i & 1] == NOWHERE ? NOWHERE : o + col[i & 1]);
+        }
     }
-    // terms 32 kk + 8 (lane >> 4) .. + 7 of column 16 b + (lane & 15)
+    // terms 32 kk + 8 (lane >> 4) .. + 7 of column 16 b + (lane & 15); `first` a multiple of 16 times the blocks of a wave
     __device__ static __forceinline__ uint32_t place(int first)
     {
         const int lane = threadIdx.x & 63, k = 8 * (lane >> 4) + ((lane & 15) >> 2);
@@ -323,18 +344,20 @@ __device__ __forceinline__ void run(unsigned char* lds, int blocks, uint32_t mp,
 }
 
 // Lane (r, g) of a block holds columns 4 g .. 4 g + 3 of row r. For 16-bit outputs neighbouring blocks trade halves, so that a lane
-// stores eight columns.
-template <int XT, typename S>
+// stores eight columns. FULL: every row and column of the tile exists, type is 16 bits wide, and a wave sends exactly STORES<S> stores.
+template <typename S>
+constexpr int STORES = S::MB * S::NB / 2;
+template <int XT, typename S, bool FULL = false>
 __device__ __forceinline__ void store(f4_t (&acc)[S::MB][S::NB], void* y, int type, size_t row0, int rows, int col0, int cols, size_t ld)
 {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = lane_here(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4, m0 = wave / S::WN * S::MB * 16, n0 = col0 + wave % S::WN * S::NB * 16;
 #pragma unroll
     for (int i = 0; i < S::MB; ++i)
     {
         const int m = m0 + 16 * i + r;
         const size_t at = (row0 + m) * ld;
-        if (type == MM_DTYPE_F32)
+        if (!FULL && type == MM_DTYPE_F32)
         {
 #pragma unroll
             for (int j = 0; j < S::NB; ++j)
@@ -350,7 +373,7 @@ __device__ __forceinline__ void store(f4_t (&acc)[S::MB][S::NB], void* y, int ty
             const auto lo = __builtin_amdgcn_permlane16_swap(pack2<XT>(acc[i][j][0], acc[i][j][1]), pack2<XT>(acc[i][j + 1][0], acc[i][j + 1][1]), false, false);
             const auto hi = __builtin_amdgcn_permlane16_swap(pack2<XT>(acc[i][j][2], acc[i][j][3]), pack2<XT>(acc[i][j + 1][2], acc[i][j + 1][3]), false, false);
             const int n = n0 + 16 * (j + (g & 1)) + 4 * (g & 2);
-            if (m < rows && n < cols) *reinterpret_cast<u4_t*>(static_cast<uint16_t*>(y) + at + n) = u4_t{ lo[0], hi[0], lo[1], hi[1] };
+            if (FULL || (m < rows && n < cols)) *reinterpret_cast<u4_t*>(static_cast<uint16_t*>(y) + at + n) = u4_t{ lo[0], hi[0], lo[1], hi[1] };
         }
     }
 }
@@ -377,7 +400,7 @@ __device__ __forceinline__ void rows_tile(const RowsArgs& a, const GroupTile& t,
 {
     using S = Shape<R>;
     using M = Along<R>;
-    using N = std::conditional_t<ACROSS, Across, Along<COLS>>;
+    using N = std::conditional_t<ACROSS, Across<TERMS>, Along<COLS>>;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col0 = ct * COLS, blocks = (a.terms + TERMS - 1) / TERMS;
     const uint16_t* w = a.w + (size_t)t.expert * a.terms * a.cols;
@@ -443,44 +466,128 @@ struct WeightsArgs
     int E, N, K, type, rowt, colt;
 };
 
-// Block b of both operands, and the tokens of the next one's rows. PICK: 0 neither tensor has rows per token, 1 dy has, 2 x has.
+constexpr int W_TERMS = 32, W_STAGE = 2 * W_TERMS * 512, W_STAGES = 5;     // 160 KB of LDS
+using Terms = Across<W_TERMS>;
+using WShape = Shape<ROWS>;
+
+// A tile's operands. PICK: 0 neither tensor has rows per token, 1 dy has, 2 x has.
 template <int PICK>
-__device__ __forceinline__ void load_terms(const Across& m, const Across& n, Across::Picks& p, const int32_t* token, uint32_t bytes, unsigned char* at,
-                                           int b, int terms)
+struct WTile
 {
-    if constexpr (PICK == 1) m.load_picked(at, p, bytes);
-    else m.load(at, b, terms);
-    if constexpr (PICK == 2) n.load_picked(at + Across::BYTES, p, bytes);
-    else n.load(at + Across::BYTES, b, terms);
-    if constexpr (PICK != 0) (PICK == 1 ? m : n).next(p, token, b + 1, terms);
-}
+    Terms m, n;
+    Terms::Picks p;
+    const int32_t* token;
+    int e, row0, col0, terms, blocks;
+    __device__ __forceinline__ void init(const WeightsArgs& a, int s)
+    {
+        e = s / (a.rowt * a.colt);
+        const int l = s - e * a.rowt * a.colt;
+        row0 = l % a.rowt * ROWS;
+        col0 = l / a.rowt * COLS;
+        const int p0 = a.offsets[e];
+        terms = a.offsets[e + 1] - p0;
+        blocks = (terms + 2 * W_TERMS - 1) / (2 * W_TERMS) * 2;       // an even number: a last one past the terms is zero
+        m.init(PICK == 1 ? a.dy : a.dy + (size_t)p0 * a.N, 2 * a.N, row0, a.N);
+        n.init(PICK == 2 ? a.x : a.x + (size_t)p0 * a.K, 2 * a.K, col0, a.K);
+        token = PICK != 0 ? a.token + p0 : nullptr;
+    }
+    __device__ __forceinline__ void first_names()
+    {
+        if (!blocks) return;
+        if constexpr (PICK == 1) m.first_names(p, token, terms);
+        if constexpr (PICK == 2) n.first_names(p, token, terms);
+    }
+    __device__ __forceinline__ void load(const WeightsArgs& a, unsigned char* at, int b)
+    {
+        if constexpr (PICK == 1) m.load_picked(at, p, token, (uint32_t)a.pbytes, b, terms);
+        else m.load(at, b, terms);
+        if constexpr (PICK == 2) n.load_picked(at + Terms::BYTES, p, token, (uint32_t)a.pbytes, b, terms);
+        else n.load(at + Terms::BYTES, b, terms);
+    }
+    __device__ __forceinline__ void first_loads(const WeightsArgs& a, unsigned char* lds)
+    {
+#pragma unroll
+        for (int b = 0; b < W_STAGES; ++b)
+            if (b < blocks) load(a, lds + b * W_STAGE, b);
+    }
+};
 
 template <int XT, int PICK>
 __global__ __launch_bounds__(512, 2) void k_group_weights(WeightsArgs a)
 {
-    using S = Shape<256>;
-    using O = Across;
-    __shared__ __align__(16) unsigned char lds[S::STAGE * S::STAGES];
+    using S = WShape;
+    constexpr int L = 2 * Terms::LOADS, READS = (S::MB + S::NB) * Terms::READS;
+    __shared__ __align__(16) unsigned char lds[W_STAGE * W_STAGES];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int s = tile_of_block(blockIdx.x);
-    if (s >= a.E * a.rowt * a.colt) return;
-    const int e = s / (a.rowt * a.colt), l = s - e * a.rowt * a.colt, row0 = l % a.rowt * ROWS, col0 = l / a.rowt * COLS;
-    const int p0 = a.offsets[e], terms = a.offsets[e + 1] - p0, blocks = (terms + TERMS - 1) / TERMS;
-    O m, n;
-    m.init(PICK == 1 ? a.dy : a.dy + (size_t)p0 * a.N, 2 * a.N, row0, a.N);
-    n.init(PICK == 2 ? a.x : a.x + (size_t)p0 * a.K, 2 * a.K, col0, a.K);
-    f4_t acc[S::MB][S::NB];
+    const int total = a.E * a.rowt * a.colt;
+    uint32_t mp = Terms::place(wave / S::WN * S::MB * 16), np = Terms::place(wave % S::WN * S::NB * 16);
+    WTile<PICK> t;
+    int s = tile_of_block(blockIdx.x);
+    if (s >= total) return;
+    t.init(a, s);
+    t.first_names();
+    t.first_loads(a, lds);
+    bool behind = false;               // the last tile's stores were sent after this one's first loads
+    for (;;)
+    {
+        f4_t acc[S::MB][S::NB];
 #pragma unroll
-    for (int i = 0; i < S::MB; ++i)
+        for (int i = 0; i < S::MB; ++i)
 #pragma unroll
-        for (int j = 0; j < S::NB; ++j) acc[i][j] = f4_t{ 0.f, 0.f, 0.f, 0.f };
-    const int32_t* token = PICK != 0 ? a.token + p0 : nullptr;
-    O::Picks p;
-    const uint32_t mp = O::place(wave / S::WN * S::MB * 16), np = O::place(wave % S::WN * S::NB * 16);
-    if constexpr (PICK != 0) (PICK == 1 ? m : n).next(p, token, 0, terms);
-    auto load = [&](int b) { load_terms<PICK>(m, n, p, token, (uint32_t)a.pbytes, lds + b % S::STAGES * S::STAGE, b, terms); };
-    if (blocks) run<XT, O, O, S, 2 * O::LOADS>(lds, blocks, mp, np, load, acc);
-    store<XT, S>(acc, a.dw, a.type, (size_t)e * a.N + row0, min(ROWS, a.N - row0), col0, a.K, a.K);
+            for (int j = 0; j < S::NB; ++j) acc[i][j] = f4_t{ 0.f, 0.f, 0.f, 0.f };
+        const int blocks = t.blocks;
+        if (blocks)
+        {
+            // a block has come once only the loads after it are out, and the stores behind the first W_STAGES blocks
+            if (blocks < W_STAGES) wait_vmcnt<0>();
+            else if (behind) wait_vmcnt<(W_STAGES - 1) * L + STORES<S>>();
+            else wait_vmcnt<(W_STAGES - 1) * L>();
+            lds_barrier();
+            Half<S> h0, h1;
+            read_half<Terms, Terms, S>(h0, lds, mp, np, 0);
+            int at = 0;
+            // block b is multiplied while block b + 1 comes from LDS; loads run five blocks ahead
+            auto step = [&](const Half<S>& cur, Half<S>& next, int b) {
+                if (b + W_STAGES > blocks) wait_vmcnt<0>();
+                else if (behind && b + 1 < W_STAGES) wait_vmcnt<(W_STAGES - 2) * L + STORES<S>>();
+                else wait_vmcnt<(W_STAGES - 2) * L>();
+                lds_barrier();
+                if (b + W_STAGES < blocks) t.load(a, lds + at, b + W_STAGES);
+                at = at + W_STAGE == W_STAGES * W_STAGE ? 0 : at + W_STAGE;
+                asm volatile("" : "+v"(mp), "+v"(np));
+                read_half<Terms, Terms, S>(next, lds + at, mp, np, 0);
+                multiply<XT, S>(cur, acc);
+                interleave<S, READS>();
+            };
+            int b = 0;
+#pragma clang loop unroll(disable)
+            for (; b + 2 < blocks; b += 2)
+            {
+                step(h0, h1, b);
+                step(h1, h0, b + 1);
+            }
+            step(h0, h1, b);
+            multiply<XT, S>(h1, acc);
+        }
+        // the next tile's first blocks are on their way while this one's results are stored
+        const size_t row = (size_t)t.e * a.N + t.row0;
+        const int rows = min(ROWS, a.N - t.row0), col0 = t.col0;
+        s += gridDim.x;
+        const bool more = s < total;
+        if (more)
+        {
+            t.init(a, s);
+            t.first_names();
+            lds_barrier();             // every wave has read the last block
+            t.first_loads(a, lds);
+        }
+        asm volatile("" ::: "memory");                     // loads first: the waits count on it
+        behind = rows == ROWS && col0 + COLS <= a.K && a.type != MM_DTYPE_F32;
+        if (behind) store<XT, S, true>(acc, a.dw, a.type, row, rows, col0, a.K, a.K);
+        else store<XT, S>(acc, a.dw, a.type, row, rows, col0, a.K, a.K);
+        asm volatile("" ::: "memory");
+        if (!more) return;
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -633,13 +740,14 @@ int mm_group_linear_weights(const mm_group_plan_t* plan, const void* dy, const v
     a.type = dw_dtype;
     a.rowt = (N + ROWS - 1) / ROWS;
     a.colt = (K + COLS - 1) / COLS;
-    const long long tiles = (long long)plan->E * a.rowt * a.colt, blocks = (tiles + 255) / 256 * 256;
-    MM_CHECK_ARG(blocks <= MOST_BLOCKS, "mm_group_linear_weights: too many tiles");
+    const long long tiles = (long long)plan->E * a.rowt * a.colt;
+    MM_CHECK_ARG(tiles <= MOST_BLOCKS - 512, "mm_group_linear_weights: too many tiles");
+    const unsigned blocks = 256;             // one a CU
     const bool h = dtype == MM_DTYPE_F16;
     auto kernel = gather ? (h ? k_group_weights<MM_DTYPE_F16, 2> : k_group_weights<MM_DTYPE_BF16, 2>)
                 : reduce ? (h ? k_group_weights<MM_DTYPE_F16, 1> : k_group_weights<MM_DTYPE_BF16, 1>)
                          : (h ? k_group_weights<MM_DTYPE_F16, 0> : k_group_weights<MM_DTYPE_BF16, 0>);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(512), 0, reinterpret_cast<hipStream_t>(stream), a);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(512), 0, reinterpret_cast<hipStream_t>(stream), a);
     return check_launch("mm_group_linear_weights");
 }
 
