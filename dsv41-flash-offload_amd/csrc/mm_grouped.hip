@@ -64,10 +64,12 @@ struct GroupTile
     int expert;            // -1: rows of no expert, which are zero
     int row, rows;         // first row, rows (1 .. ROWS)
     int first, count;      // the expert's tiles
-    int pad[3];
+    int size;              // rows of the largest of them
+    int pad[2];
 };
 
-// Row tiles of n routes over E experts: whole ones, one for the rest of each expert that has rows, and those of no expert.
+// Row tiles of n routes over E experts: as few as an expert's rows need, of equal size (tiles of one expert that run side by side share its
+// weights in L2, as long as they take the same time: 341 rows as 256 + 85 read them twice), and those of no expert.
 constexpr long long tile_capacity(long long n, int E) { return n / ROWS + std::min<long long>(n, E) + 1; }
 
 // One thread per expert (and one for the routes of none): tiles in the experts' order.
@@ -91,8 +93,12 @@ __global__ __launch_bounds__(1024) void k_group_tiles(const int32_t* __restrict_
             if (w < wave) first += part[w];
             total += part[w];
         }
+        const int size = cnt ? (r1 - r0 + cnt - 1) / cnt : 0;
         for (int i = 0; i < cnt; ++i)
-            tiles[first + i] = { e < E ? e : -1, r0 + i * ROWS, min(ROWS, r1 - r0 - i * ROWS), first, cnt, { 0, 0, 0 } };
+        {
+            const int at = (int)((long long)(r1 - r0) * i / cnt), to = (int)((long long)(r1 - r0) * (i + 1) / cnt);
+            tiles[first + i] = { e < E ? e : -1, r0 + at, to - at, first, cnt, size, { 0, 0 } };
+        }
         run += total;
     }
     if (t == 0) *ntiles = run;
@@ -261,11 +267,12 @@ template <int R>
 struct Shape
 {
     static constexpr int WN = R >= 128 ? 4 : 8, WM = 8 / WN, MB = std::max(1, R / 16 / WM), NB = COLS / 16 / WN;
-    static constexpr int STAGE = (R + COLS) * 128;
-    static constexpr int STAGES = R == 256 ? 2 : R >= 64 ? 3 : 4;
-    static_assert(STAGE * STAGES <= 160 * 1024, "LDS");
+    // places in LDS for blocks of the rows and, more of them, of the columns: these are the weights, which come from farther away
+    static constexpr int SM = R >= 128 ? 2 : 3, SN = R == 256 ? 2 : R == 192 ? 3 : 4;
+    static constexpr int MSTAGE = R * 128, NSTAGE = COLS * 128;
+    static_assert(SM * MSTAGE + SN * NSTAGE <= 160 * 1024 && SN >= SM, "LDS");
 };
-constexpr int LDS_ROWS = 144 * 1024;      // of the row tiles: 3 stages of 128 x 256
+constexpr int LDS_ROWS = 160 * 1024;
 
 // Operands of half a block (32 terms).
 template <typename S>
@@ -274,12 +281,12 @@ struct Half
     u4_t m[S::MB], n[S::NB];
 };
 template <typename M, typename N, typename S>
-__device__ __forceinline__ void read_half(Half<S>& h, const unsigned char* stage, uint32_t mp, uint32_t np, int kk)
+__device__ __forceinline__ void read_half(Half<S>& h, const unsigned char* m, const unsigned char* n, uint32_t mp, uint32_t np, int kk)
 {
 #pragma unroll
-    for (int j = 0; j < S::NB; ++j) h.n[j] = N::read(stage + M::BYTES, np, j, kk);
+    for (int j = 0; j < S::NB; ++j) h.n[j] = N::read(n, np, j, kk);
 #pragma unroll
-    for (int i = 0; i < S::MB; ++i) h.m[i] = M::read(stage, mp, i, kk);
+    for (int i = 0; i < S::MB; ++i) h.m[i] = M::read(m, mp, i, kk);
 }
 template <int XT, typename S>
 __device__ __forceinline__ void multiply(const Half<S>& h, f4_t (&acc)[S::MB][S::NB])
@@ -304,40 +311,53 @@ __device__ __forceinline__ void interleave()
 }
 
 // All blocks of a tile. Half a block's operands are read from LDS while the half before is multiplied, across the barrier too, which stands
-// in the middle of a block: a wave that waits there has half a block to multiply. Block b's place is free once every wave has
-// read its second half, so loads run STAGES blocks ahead. load(b) sends a wave's L loads of block b.
-template <int XT, typename M, typename N, typename S, int L, typename Load>
-__device__ __forceinline__ void run(unsigned char* lds, int blocks, uint32_t mp, uint32_t np, const Load& load, f4_t (&acc)[S::MB][S::NB])
+// in the middle of a block: a wave that waits there has half a block to multiply. Block b's places are free once every wave has
+// read its second half, so loads run SM and SN blocks ahead.
+template <int XT, typename M, typename N, typename S>
+__device__ __forceinline__ void run(unsigned char* lds, const M& m, const N& n, int terms, uint32_t mp, uint32_t np, f4_t (&acc)[S::MB][S::NB])
 {
-    constexpr int READS = S::MB * M::READS + S::NB * N::READS;
+    constexpr int READS = S::MB * M::READS + S::NB * N::READS, SM = S::SM, SN = S::SN;
+    constexpr int AFTER = SN > SM ? N::LOADS : 0, EACH = M::LOADS + N::LOADS;      // loads after a block's last one, and in each block after
+    unsigned char *ml = lds, *nl = lds + SM * S::MSTAGE;
+    const int blocks = (terms + TERMS - 1) / TERMS;
     Half<S> h0, h1;
-    for (int b = 0; b < S::STAGES; ++b)
-        if (b < blocks) load(b);
-    if (blocks >= S::STAGES) wait_vmcnt<(S::STAGES - 1) * L>();
+    // in the order of the loop: m of block b after n of block b + SN - SM - 1, before n of block b + SN - SM
+#pragma unroll
+    for (int b = 0; b < SN; ++b)
+    {
+        const int bm = b - (SN - SM);
+        if (bm >= 0 && bm < blocks) m.load(ml + bm * S::MSTAGE, bm, terms);
+        if (b < blocks) n.load(nl + b * S::NSTAGE, b, terms);
+    }
+    // block 0 has come once only what was sent after it is out
+    if (blocks >= SN) wait_vmcnt<AFTER + (SM - 1) * EACH>();
     else wait_vmcnt<0>();
     lds_barrier();
-    read_half<M, N, S>(h0, lds, mp, np, 0);
-    int at = 0;
+    read_half<M, N, S>(h0, ml, nl, mp, np, 0);
+    int am = 0, an = 0;
 #pragma clang loop unroll(disable)
     for (int b = 0; b + 1 < blocks; ++b)
     {
         // (the places of the blocks are made from these two again each time, rather than kept in registers)
         asm volatile("" : "+v"(mp), "+v"(np));
-        read_half<M, N, S>(h1, lds + at, mp, np, 1);
+        read_half<M, N, S>(h1, ml + am, nl + an, mp, np, 1);
         multiply<XT, S>(h0, acc);
         interleave<S, READS>();
-        // block b + 1 has come once only the loads after it are out
-        if (b + S::STAGES <= blocks) wait_vmcnt<(S::STAGES - 2) * L>();
+        // the same for block b + 1
+        if (b + SN <= blocks) wait_vmcnt<AFTER + (SM - 2) * EACH>();
         else wait_vmcnt<0>();
         lds_barrier();
-        if (b + S::STAGES < blocks) load(b + S::STAGES);
-        at = at + S::STAGE == S::STAGES * S::STAGE ? 0 : at + S::STAGE;
+        if (b + SM < blocks) m.load(ml + am, b + SM, terms);
+        asm volatile("" ::: "memory");
+        if (b + SN < blocks) n.load(nl + an, b + SN, terms);
+        am = am + S::MSTAGE == SM * S::MSTAGE ? 0 : am + S::MSTAGE;
+        an = an + S::NSTAGE == SN * S::NSTAGE ? 0 : an + S::NSTAGE;
         asm volatile("" : "+v"(mp), "+v"(np));
-        read_half<M, N, S>(h0, lds + at, mp, np, 0);
+        read_half<M, N, S>(h0, ml + am, nl + an, mp, np, 0);
         multiply<XT, S>(h1, acc);
         interleave<S, READS>();
     }
-    read_half<M, N, S>(h1, lds + at, mp, np, 1);
+    read_half<M, N, S>(h1, ml + am, nl + an, mp, np, 1);
     multiply<XT, S>(h0, acc);
     interleave<S, READS>();
     multiply<XT, S>(h1, acc);
@@ -378,6 +398,14 @@ __device__ __forceinline__ void store(f4_t (&acc)[S::MB][S::NB], void* y, int ty
     }
 }
 
+// Tile l of `rows` x `cols` tiles: bands of eight row tiles, column by column, so that the 32 tiles an XCD works on share few operands.
+__device__ __forceinline__ void tile_in_bands(int l, int rows, int cols, int& r, int& c)
+{
+    const int band = l / (8 * cols), in = l - band * 8 * cols, h = min(8, rows - 8 * band);
+    c = in / h;
+    r = 8 * band + in - c * h;
+}
+
 struct RowsArgs
 {
     const uint16_t *x, *w;        // the rows (x or dy) and the weights
@@ -402,7 +430,7 @@ __device__ __forceinline__ void rows_tile(const RowsArgs& a, const GroupTile& t,
     using M = Along<R>;
     using N = std::conditional_t<ACROSS, Across<TERMS>, Along<COLS>>;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col0 = ct * COLS, blocks = (a.terms + TERMS - 1) / TERMS;
+    const int col0 = ct * COLS;
     const uint16_t* w = a.w + (size_t)t.expert * a.terms * a.cols;
     M m;
     N n;
@@ -415,13 +443,8 @@ __device__ __forceinline__ void rows_tile(const RowsArgs& a, const GroupTile& t,
     for (int i = 0; i < S::MB; ++i)
 #pragma unroll
         for (int j = 0; j < S::NB; ++j) acc[i][j] = f4_t{ 0.f, 0.f, 0.f, 0.f };
-    auto load = [&](int b) {
-        unsigned char* at = lds + b % S::STAGES * S::STAGE;
-        m.load(at, b, a.terms);
-        n.load(at + M::BYTES, b, a.terms);
-    };
     const uint32_t mp = M::place(wave / S::WN * S::MB * 16), np = N::place(wave % S::WN * S::NB * 16);
-    run<XT, M, N, S, M::LOADS + N::LOADS>(lds, blocks, mp, np, load, acc);
+    run<XT, M, N, S>(lds, m, n, a.terms, mp, np, acc);
     store<XT, S>(acc, a.y, a.type, t.row, t.rows, col0, a.cols, a.cols);
 }
 
@@ -431,11 +454,10 @@ __global__ __launch_bounds__(512, 2) void k_group_rows(RowsArgs a)
     __shared__ __align__(16) unsigned char lds[LDS_ROWS];
     const int s = tile_of_block(blockIdx.x), nt = *a.ntiles;
     if (s >= nt * a.colt) return;
-    // the tiles of an expert: row tiles next to each other, then the next column tile
-    const GroupTile f = a.tiles[s / a.colt];
-    const int l = s - f.first * a.colt;
-    const GroupTile t = a.tiles[f.first + l % f.count];
-    const int ct = l / f.count;
+    const GroupTile f = a.tiles[s / a.colt];             // one of the same expert
+    int rt, ct;
+    tile_in_bands(s - f.first * a.colt, f.count, a.colt, rt, ct);
+    const GroupTile t = a.tiles[f.first + rt];
     if (t.expert < 0)
     {
         if (!a.zero) return;
@@ -447,10 +469,11 @@ __global__ __launch_bounds__(512, 2) void k_group_rows(RowsArgs a)
         }
         return;
     }
-    if (t.rows > 128) rows_tile<XT, ACROSS, 256>(a, t, ct, lds);
-    else if (t.rows > 64) rows_tile<XT, ACROSS, 128>(a, t, ct, lds);
-    else if (t.rows > 32) rows_tile<XT, ACROSS, 64>(a, t, ct, lds);
-    else if (t.rows > 16) rows_tile<XT, ACROSS, 32>(a, t, ct, lds);
+    if (t.size > 192) rows_tile<XT, ACROSS, 256>(a, t, ct, lds);
+    else if (t.size > 128) rows_tile<XT, ACROSS, 192>(a, t, ct, lds);
+    else if (t.size > 64) rows_tile<XT, ACROSS, 128>(a, t, ct, lds);
+    else if (t.size > 32) rows_tile<XT, ACROSS, 64>(a, t, ct, lds);
+    else if (t.size > 16) rows_tile<XT, ACROSS, 32>(a, t, ct, lds);
     else rows_tile<XT, ACROSS, 16>(a, t, ct, lds);
 }
 
@@ -481,9 +504,10 @@ struct WTile
     __device__ __forceinline__ void init(const WeightsArgs& a, int s)
     {
         e = s / (a.rowt * a.colt);
-        const int l = s - e * a.rowt * a.colt;
-        row0 = l % a.rowt * ROWS;
-        col0 = l / a.rowt * COLS;
+        int rt, ct;
+        tile_in_bands(s - e * a.rowt * a.colt, a.rowt, a.colt, rt, ct);
+        row0 = rt * ROWS;
+        col0 = ct * COLS;
         const int p0 = a.offsets[e];
         terms = a.offsets[e + 1] - p0;
         blocks = (terms + 2 * W_TERMS - 1) / (2 * W_TERMS) * 2;       // an even number: a last one past the terms is zero
@@ -544,7 +568,7 @@ __global__ __launch_bounds__(512, 2) void k_group_weights(WeightsArgs a)
             else wait_vmcnt<(W_STAGES - 1) * L>();
             lds_barrier();
             Half<S> h0, h1;
-            read_half<Terms, Terms, S>(h0, lds, mp, np, 0);
+            read_half<Terms, Terms, S>(h0, lds, lds + Terms::BYTES, mp, np, 0);
             int at = 0;
             // block b is multiplied while block b + 1 comes from LDS; loads run five blocks ahead
             auto step = [&](const Half<S>& cur, Half<S>& next, int b) {
@@ -555,7 +579,7 @@ __global__ __launch_bounds__(512, 2) void k_group_weights(WeightsArgs a)
                 if (b + W_STAGES < blocks) t.load(a, lds + at, b + W_STAGES);
                 at = at + W_STAGE == W_STAGES * W_STAGE ? 0 : at + W_STAGE;
                 asm volatile("" : "+v"(mp), "+v"(np));
-                read_half<Terms, Terms, S>(next, lds + at, mp, np, 0);
+                read_half<Terms, Terms, S>(next, lds + at, lds + at + Terms::BYTES, mp, np, 0);
                 multiply<XT, S>(cur, acc);
                 interleave<S, READS>();
             };
