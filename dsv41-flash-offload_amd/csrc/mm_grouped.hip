@@ -364,36 +364,59 @@ __device__ __forceinline__ void run(unsigned char* lds, const M& m, const N& n, 
 }
 
 // Lane (r, g) of a block holds columns 4 g .. 4 g + 3 of row r. For 16-bit outputs neighbouring blocks trade halves, so that a lane
-// stores eight columns. FULL: every row and column of the tile exists, type is 16 bits wide, and a wave sends exactly STORES<S> stores.
+// has eight columns; then lanes r and r ^ 8 trade, so that a store writes 128 bytes of eight rows rather than 64 of sixteen: whole
+// cache lines, which leave for memory once. FULL: every row and column of the tile exists, type is 16 bits wide, and a wave sends exactly
+// STORES<S> stores.
 template <typename S>
 constexpr int STORES = S::MB * S::NB / 2;
+__device__ __forceinline__ void trade_rows(u4_t& a, u4_t& b, bool low)
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+        const uint32_t got = (uint32_t)xor_lane_i<8>((int)(low ? b[i] : a[i]));
+        a[i] = low ? a[i] : got;
+        b[i] = low ? got : b[i];
+    }
+}
 template <int XT, typename S, bool FULL = false>
 __device__ __forceinline__ void store(f4_t (&acc)[S::MB][S::NB], void* y, int type, size_t row0, int rows, int col0, int cols, size_t ld)
 {
     const int lane = lane_here(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4, m0 = wave / S::WN * S::MB * 16, n0 = col0 + wave % S::WN * S::NB * 16;
+    const bool low = r < 8;
+    // two 16-byte pieces of row r, `step` columns apart, as pieces of rows r & 7 and (r & 7) + 8
+    auto pair = [&](u4_t a, u4_t b, int i, int n, int step, int size) {
+        trade_rows(a, b, low);
+        const int m = m0 + 16 * i + (r & 7), c = low ? n : n + step;
+        unsigned char* at = static_cast<unsigned char*>(y) + ((row0 + m) * ld + c) * size;
+        if (FULL || (m < rows && c < cols)) *reinterpret_cast<u4_t*>(at) = a;
+        if (FULL || (m + 8 < rows && c < cols)) *reinterpret_cast<u4_t*>(at + 8 * ld * size) = b;
+    };
 #pragma unroll
     for (int i = 0; i < S::MB; ++i)
     {
-        const int m = m0 + 16 * i + r;
-        const size_t at = (row0 + m) * ld;
         if (!FULL && type == MM_DTYPE_F32)
         {
 #pragma unroll
-            for (int j = 0; j < S::NB; ++j)
-            {
-                const int n = n0 + 16 * j + 4 * g;
-                if (m < rows && n < cols) *reinterpret_cast<f4_t*>(static_cast<float*>(y) + at + n) = acc[i][j];
-            }
+            for (int j = 0; j < S::NB; j += 2)
+                pair(__builtin_bit_cast(u4_t, acc[i][j]), __builtin_bit_cast(u4_t, acc[i][j + 1]), i, n0 + 16 * j + 4 * g, 16, 4);
             continue;
         }
+        u4_t v[S::NB / 2];
 #pragma unroll
         for (int j = 0; j < S::NB; j += 2)
         {
             const auto lo = __builtin_amdgcn_permlane16_swap(pack2<XT>(acc[i][j][0], acc[i][j][1]), pack2<XT>(acc[i][j + 1][0], acc[i][j + 1][1]), false, false);
             const auto hi = __builtin_amdgcn_permlane16_swap(pack2<XT>(acc[i][j][2], acc[i][j][3]), pack2<XT>(acc[i][j + 1][2], acc[i][j + 1][3]), false, false);
-            const int n = n0 + 16 * (j + (g & 1)) + 4 * (g & 2);
-            if (FULL || (m < rows && n < cols)) *reinterpret_cast<u4_t*>(static_cast<uint16_t*>(y) + at + n) = u4_t{ lo[0], hi[0], lo[1], hi[1] };
+            v[j / 2] = u4_t{ lo[0], hi[0], lo[1], hi[1] };
+        }
+        const int n = n0 + 16 * (g & 1) + 4 * (g & 2);
+        if constexpr (S::NB == 4) pair(v[0], v[1], i, n, 32, 2);
+        else
+        {
+            const int m = m0 + 16 * i + r;
+            if (m < rows && n < cols) *reinterpret_cast<u4_t*>(static_cast<uint16_t*>(y) + (row0 + m) * ld + n) = v[0];
         }
     }
 }
