@@ -58,7 +58,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, uint32_t
 // ---------------------------------------------------------------------------------------------------------
 // Plan: the row tiles of a call
 // ---------------------------------------------------------------------------------------------------------
-constexpr int ROWS = 256, COLS = 256, TERMS = 64;      // the largest tile, and the terms of a block
+constexpr int ROWS = 256, FEW_ROWS = 64, TERMS = 64;      // rows of the largest tile, and of the largest small one; terms of a block
 struct GroupTile
 {
     int expert;            // -1: rows of no expert, which are zero
@@ -68,40 +68,54 @@ struct GroupTile
     int pad[2];
 };
 
-// Row tiles of n routes over E experts: as few as an expert's rows need, of equal size (tiles of one expert that run side by side share its
-// weights in L2, as long as they take the same time: 341 rows as 256 + 85 read them twice), and those of no expert.
-constexpr long long tile_capacity(long long n, int E) { return n / ROWS + std::min<long long>(n, E) + 1; }
+// Row tiles of n routes over E experts: as few of at most `rows` as an expert's rows need, of equal size (tiles of one expert that run side
+// by side share its weights in L2, as long as they take the same time: 341 rows as 256 + 85 read them twice), and those of no expert. A
+// plan has two lists, of large tiles and of small ones, and their numbers.
+constexpr long long tile_capacity(long long n, int E, int rows) { return n / rows + std::min<long long>(n, E) + 1; }
 
-// One thread per expert (and one for the routes of none): tiles in the experts' order.
-__global__ __launch_bounds__(1024) void k_group_tiles(const int32_t* __restrict__ offsets, int E, GroupTile* __restrict__ tiles, int32_t* __restrict__ ntiles)
+__global__ __launch_bounds__(1024) void k_group_tiles(const int32_t* __restrict__ offsets, int E, GroupTile* __restrict__ tiles, GroupTile* __restrict__ few,
+                                                      int32_t* __restrict__ ntiles)
 {
-    __shared__ int part[16];
+    __shared__ int part[16], start[1026], first[1026];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    int run = 0;
-    for (int base = 0; base <= E; base += 1024)
+    for (int i = t; i < E + 2; i += 1024) start[i] = offsets[i];
+    for (int list = 0; list < 2; ++list)
     {
-        const int e = base + t;
-        const int r0 = e <= E ? offsets[e] : 0, r1 = e <= E ? offsets[e + 1] : 0;
-        const int cnt = (r1 - r0 + ROWS - 1) / ROWS;
-        const int inc = wave_incl_scan(cnt);
-        __syncthreads();
-        if (lane == 63) part[wave] = inc;
-        __syncthreads();
-        int first = run + inc - cnt, total = 0;
-        for (int w = 0; w < 16; ++w)
+        const int most = list ? FEW_ROWS : ROWS;
+        GroupTile* out = list ? few : tiles;
+        int run = 0;
+        for (int base = 0; base <= E; base += 1024)
         {
-            if (w < wave) first += part[w];
-            total += part[w];
+            __syncthreads();
+            const int e = base + t, cnt = e <= E ? (start[e + 1] - start[e] + most - 1) / most : 0, inc = wave_incl_scan(cnt);
+            if (lane == 63) part[wave] = inc;
+            __syncthreads();
+            int at = run + inc - cnt, total = 0;
+            for (int w = 0; w < 16; ++w)
+            {
+                if (w < wave) at += part[w];
+                total += part[w];
+            }
+            if (e <= E) first[e] = at;
+            run += total;
         }
-        const int size = cnt ? (r1 - r0 + cnt - 1) / cnt : 0;
-        for (int i = 0; i < cnt; ++i)
+        if (t == 0)
         {
-            const int at = (int)((long long)(r1 - r0) * i / cnt), to = (int)((long long)(r1 - r0) * (i + 1) / cnt);
-            tiles[first + i] = { e < E ? e : -1, r0 + at, to - at, first, cnt, size, { 0, 0 } };
+            first[E + 1] = run;
+            ntiles[list] = run;
         }
-        run += total;
+        __syncthreads();
+        for (int i = t; i < run; i += 1024)
+        {
+            // the expert (E: none) whose tiles i is among
+            int e = 0;
+            for (int step = 1024; step; step >>= 1)
+                if (e + step <= E && first[e + step] <= i) e += step;
+            const int cnt = first[e + 1] - first[e], r0 = start[e], n = start[e + 1] - r0, k = i - first[e];
+            const int at = (int)((long long)n * k / cnt), to = (int)((long long)n * (k + 1) / cnt);
+            out[i] = { e < E ? e : -1, r0 + at, to - at, first[e], cnt, (n + cnt - 1) / cnt, { 0, 0 } };
+        }
     }
-    if (t == 0) *ntiles = run;
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -121,12 +135,12 @@ __device__ __forceinline__ int lane_here()
 }
 constexpr uint32_t NOWHERE = 0xfffffff0u;              // past every buffer: reads zero
 
-// Rows of TERMS terms, R of them; LDS [R][64]. A wave's load is 8 rows of 128 bytes. Tiles of fewer rows than eight waves load
-// are loaded more than once, to the same place, so that every wave has as many loads in flight.
-template <int R>
+// Rows of TERMS terms, R of them, loaded by W waves; LDS [R][64]. A wave's load is 8 rows of 128 bytes. Tiles of fewer rows than the waves
+// load are loaded more than once, to the same place, so that every wave has as many loads in flight.
+template <int R, int W>
 struct Along
 {
-    static constexpr int BYTES = R * 128, LOADS = std::max(1, R / 64), READS = 1;
+    static constexpr int BYTES = R * 128, LOADS = std::max(1, R / (8 * W)), READS = 1;
     __amdgpu_buffer_rsrc_t buf;
     uint32_t at[LOADS];
     int slot;             // the wave's first row
@@ -175,28 +189,33 @@ __device__ __forceinline__ u2_t read_transposed(lds_s4_t __restrict__ p)
     return __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p));
 }
 
-// Blocks of B rows (terms) of 256 columns; LDS [B][256], 32-byte piece p of row k at p ^ swizzle(k). A wave's load is two rows.
-template <int B>
+// Blocks of B rows (terms) of C columns, loaded by W waves; LDS [B][C], 32-byte piece p of row k at p ^ swizzle(k).
+template <int B, int C, int W>
 struct Across
 {
-    static constexpr int BYTES = B * 512, RB = 512, LOADS = B / 16, READS = 2;
+    // EACH: rows of a wave's load; OWN: rows of a wave
+    static constexpr int BYTES = 2 * B * C, RB = 2 * C, EACH = 512 / C, OWN = B / W, LOADS = OWN / EACH, READS = 2;
+    // loads whose rows have the same swizzle share their columns: of C = 256 those four rows apart, of C = 128 those within eight rows
+    static constexpr int KINDS = 2;
+    static constexpr int kind(int i) { return C == 256 ? i % 2 : i / 2; }
+    static_assert((C == 256 && OWN <= 8) || (C == 128 && OWN == 16), "rows of a wave");
     const unsigned char* base;
-    uint32_t ld, col[2];           // loads 2 and 3 have the columns of 0 and 1
+    uint32_t ld, col[KINDS];
     int row, slot;                 // the lane's row of load 0, the wave's
-    // different for four rows of an 8-row group and for the four groups that a wave reads at once
-    __device__ static __forceinline__ int swizzle(int k) { return (k & 3) | ((k >> 3) & 3) << 2; }
+    // different for four rows of an 8-row group and for the groups that a wave reads at once, as far as the pieces go
+    __device__ static __forceinline__ int swizzle(int k) { return ((k & 3) | ((k >> 3) & 3) << 2) & (C / 16 - 1); }
     // base: column 0 of row 0; first: the tile's first column; width: columns of a row
     __device__ __forceinline__ void init(const void* b, uint32_t ld_, int first, int width)
     {
-        const int lane = lane_here(), s = lane & 31;
+        const int lane = lane_here(), s = lane % (RB / 16);
         base = static_cast<const unsigned char*>(b);
         ld = ld_;
-        slot = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 2 * LOADS;
-        row = slot + (lane >> 5);
+        slot = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * OWN;
+        row = slot + lane / (RB / 16);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < KINDS; ++i)
         {
-            const int c = first + 8 * (((s >> 1) ^ swizzle(row + 2 * i)) * 2 + (s & 1));
+            const int c = first + 8 * (((s >> 1) ^ swizzle(row + (C == 256 ? 2 : 8) * i)) * 2 + (s & 1));
             col[i] = c < width ? 2 * c : NOWHERE;
         }
     }
@@ -206,18 +225,18 @@ struct Across
         const __amdgpu_buffer_rsrc_t buf = buffer(base + (size_t)block * B * ld, (uint32_t)max(0, min(terms - B * block, B)) * ld);
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
-            load16(buf, lds + (slot + 2 * i) * RB, col[i & 1] == NOWHERE ? NOWHERE : (row + 2 * i) * ld + col[i & 1]);
+            load16(buf, lds + (slot + EACH * i) * RB, col[kind(i)] == NOWHERE ? NOWHERE : (row + EACH * i) * ld + col[kind(i)]);
     }
     // The same with the rows that `pick` names. A lane holds the name of one of the wave's rows, for CHUNK blocks at once, and the next
     // CHUNK blocks' are on their way: names read block by block would be waited for with all loads before them.
-    static constexpr int CHUNK = 64 / (2 * LOADS);
+    static constexpr int CHUNK = 64 / OWN;
     struct Picks
     {
         int32_t cur, next;
     };
     __device__ __forceinline__ int32_t names(const int32_t* pick, int chunk, int terms) const
     {
-        const int lane = lane_here(), k = B * (CHUNK * chunk + lane / (2 * LOADS)) + slot + lane % (2 * LOADS);
+        const int lane = lane_here(), k = B * (CHUNK * chunk + lane / OWN) + slot + lane % OWN;
         const int32_t r = pick[min(k, terms - 1)];
         return k < terms ? r : -1;
     }
@@ -236,14 +255,20 @@ struct Across
             p.next = names(pick, block / CHUNK + 1, terms);
         }
         const __amdgpu_buffer_rsrc_t buf = buffer(base, bytes);
+        const int mine = (threadIdx.x & 63) / (RB / 16);
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
         {
-            const int32_t r0 = __builtin_amdgcn_readlane(p.cur, 2 * LOADS * at + 2 * i), r1 = __builtin_amdgcn_readlane(p.cur, 2 * LOADS * at + 2 * i + 1);
             // (a row of none and a column past the width may not add up to a place again)
-            const uint32_t o0 = r0 < 0 ? NOWHERE : (uint32_t)r0 * ld, o1 = r1 < 0 ? NOWHERE : (uint32_t)r1 * ld;
-            const uint32_t o = threadIdx.x & 32 ? o1 : o0;
-            load16(buf, lds + (slot + 2 * i) * RB, o == NOWHERE || col[i & 1] == NOWHERE ? NOWHERE : o + col[i & 1]);
+            uint32_t o = NOWHERE;
+#pragma unroll
+            for (int q = 0; q < EACH; ++q)
+            {
+                const int32_t r = __builtin_amdgcn_readlane(p.cur, OWN * at + EACH * i + q);
+                const uint32_t v = r < 0 ? NOWHERE : (uint32_t)r * ld;
+                o = mine == q ? v : o;
+            }
+            load16(buf, lds + (slot + EACH * i) * RB, o == NOWHERE || col[kind(i)] == NOWHERE ? NOWHERE : o + col[kind(i)]);
         }
     }
     // terms 32 kk + 8 (lane >> 4) .. + 7 of column 16 b + (lane & 15); `first` a multiple of 16 times the blocks of a wave
@@ -263,16 +288,18 @@ struct Across
 // ---------------------------------------------------------------------------------------------------------
 // Tile: rows of M by columns of N; wave (wm, wn) has MB x NB blocks of 16 x 16.
 // ---------------------------------------------------------------------------------------------------------
-template <int R>
+// One workgroup of eight waves a CU, or two of four.
+template <int C>
+constexpr int LDS_BYTES = C == 256 ? 160 * 1024 : 76 * 1024;
+template <int R, int C>
 struct Shape
 {
-    static constexpr int WN = R >= 128 ? 4 : 8, WM = 8 / WN, MB = std::max(1, R / 16 / WM), NB = COLS / 16 / WN;
-    // places in LDS for blocks of the rows and, more of them, of the columns: these are the weights, which come from farther away
-    static constexpr int SM = R >= 128 ? 2 : 3, SN = R == 256 ? 2 : R == 192 ? 3 : 4;
-    static constexpr int MSTAGE = R * 128, NSTAGE = COLS * 128;
-    static_assert(SM * MSTAGE + SN * NSTAGE <= 160 * 1024 && SN >= SM, "LDS");
+    static constexpr int WAVES = C / 32, WN = R >= 128 ? 4 : WAVES, WM = WAVES / WN, MB = std::max(1, R / 16 / WM), NB = C / 16 / WN;
+    // places in LDS for blocks of the rows and of the columns: these are the weights, which come from farther away when tiles have few rows
+    static constexpr int SM = R >= 128 ? 2 : 3, SN = R == 256 ? 2 : R == 192 || (C == 128 && R == 64) ? 3 : 4;
+    static constexpr int MSTAGE = R * 128, NSTAGE = C * 128, LDS = SM * MSTAGE + SN * NSTAGE;
+    static_assert(LDS <= LDS_BYTES<C> && SN >= SM, "LDS");
 };
-constexpr int LDS_ROWS = 160 * 1024;
 
 // Operands of half a block (32 terms).
 template <typename S>
@@ -446,21 +473,21 @@ __device__ __forceinline__ int tile_of_block(int b)
     return ((i >> 5) * 8 + x) * 32 + (i & 31);
 }
 
-template <int XT, bool ACROSS, int R>
+template <int XT, bool ACROSS, int R, int C>
 __device__ __forceinline__ void rows_tile(const RowsArgs& a, const GroupTile& t, int ct, unsigned char* lds)
 {
-    using S = Shape<R>;
-    using M = Along<R>;
-    using N = std::conditional_t<ACROSS, Across<TERMS>, Along<COLS>>;
+    using S = Shape<R, C>;
+    using M = Along<R, S::WAVES>;
+    using N = std::conditional_t<ACROSS, Across<TERMS, C, S::WAVES>, Along<C, S::WAVES>>;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col0 = ct * COLS;
+    const int col0 = ct * C;
     const uint16_t* w = a.w + (size_t)t.expert * a.terms * a.cols;
     M m;
     N n;
     if (a.token) m.init(a.x, 2 * a.terms, t.rows, (uint32_t)a.xbytes, a.token + t.row);
     else m.init(a.x + (size_t)t.row * a.terms, 2 * a.terms, t.rows, (uint32_t)t.rows * a.terms * 2, nullptr);
     if constexpr (ACROSS) n.init(w, 2 * a.cols, col0, a.cols);
-    else n.init(w + (size_t)col0 * a.terms, 2 * a.terms, min(COLS, a.cols - col0), (uint32_t)min(COLS, a.cols - col0) * a.terms * 2, nullptr);
+    else n.init(w + (size_t)col0 * a.terms, 2 * a.terms, min(C, a.cols - col0), (uint32_t)min(C, a.cols - col0) * a.terms * 2, nullptr);
     f4_t acc[S::MB][S::NB];
 #pragma unroll
     for (int i = 0; i < S::MB; ++i)
@@ -471,33 +498,113 @@ __device__ __forceinline__ void rows_tile(const RowsArgs& a, const GroupTile& t,
     store<XT, S>(acc, a.y, a.type, t.row, t.rows, col0, a.cols, a.cols);
 }
 
-template <int XT, bool ACROSS>
-__global__ __launch_bounds__(512, 2) void k_group_rows(RowsArgs a)
+// Columns ct C .. of rows of no expert.
+template <int C>
+__device__ __forceinline__ void zero_tile(const RowsArgs& a, const GroupTile& t, int ct)
 {
-    __shared__ __align__(16) unsigned char lds[LDS_ROWS];
+    if (!a.zero) return;
+    const int per = a.type == MM_DTYPE_F32 ? 4 : 8, n = min(C, a.cols - ct * C) / per;
+    for (int i = threadIdx.x; i < t.rows * n; i += blockDim.x)
+    {
+        const size_t at = (size_t)(t.row + i / n) * a.cols + ct * C + i % n * per;
+        *reinterpret_cast<u4_t*>(static_cast<unsigned char*>(a.y) + at * (16 / per)) = u4_t{ 0, 0, 0, 0 };
+    }
+}
+
+// C = 256: large tiles. C = 128: small ones of at most FEW_ROWS rows, for calls that have too few large tiles for the GPU.
+template <int XT, bool ACROSS, int C>
+__global__ __launch_bounds__(2 * C, 2) void k_group_rows(RowsArgs a)
+{
+    __shared__ __align__(16) unsigned char lds[LDS_BYTES<C>];
     const int s = tile_of_block(blockIdx.x), nt = *a.ntiles;
     if (s >= nt * a.colt) return;
     const GroupTile f = a.tiles[s / a.colt];             // one of the same expert
     int rt, ct;
     tile_in_bands(s - f.first * a.colt, f.count, a.colt, rt, ct);
     const GroupTile t = a.tiles[f.first + rt];
-    if (t.expert < 0)
+    if (t.expert < 0) return zero_tile<C>(a, t, ct);
+    if constexpr (C == 256)
     {
-        if (!a.zero) return;
-        const int per = a.type == MM_DTYPE_F32 ? 4 : 8, n = min(COLS, a.cols - ct * COLS) / per;
-        for (int i = threadIdx.x; i < t.rows * n; i += 512)
-        {
-            const size_t at = (size_t)(t.row + i / n) * a.cols + ct * COLS + i % n * per;
-            *reinterpret_cast<u4_t*>(static_cast<unsigned char*>(a.y) + at * (16 / per)) = u4_t{ 0, 0, 0, 0 };
-        }
-        return;
+        if (t.size > 192) return rows_tile<XT, ACROSS, 256, C>(a, t, ct, lds);
+        if (t.size > 128) return rows_tile<XT, ACROSS, 192, C>(a, t, ct, lds);
+        if (t.size > 64) return rows_tile<XT, ACROSS, 128, C>(a, t, ct, lds);
     }
-    if (t.size > 192) rows_tile<XT, ACROSS, 256>(a, t, ct, lds);
-    else if (t.size > 128) rows_tile<XT, ACROSS, 192>(a, t, ct, lds);
-    else if (t.size > 64) rows_tile<XT, ACROSS, 128>(a, t, ct, lds);
-    else if (t.size > 32) rows_tile<XT, ACROSS, 64>(a, t, ct, lds);
-    else if (t.size > 16) rows_tile<XT, ACROSS, 32>(a, t, ct, lds);
-    else rows_tile<XT, ACROSS, 16>(a, t, ct, lds);
+    if (t.size > 32) rows_tile<XT, ACROSS, 64, C>(a, t, ct, lds);
+    else if (t.size > 16) rows_tile<XT, ACROSS, 32, C>(a, t, ct, lds);
+    else rows_tile<XT, ACROSS, 16, C>(a, t, ct, lds);
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// A few rows per expert (a decode step): bound by reading the weights, once. A workgroup takes a small tile's rows by 16 columns; its
+// four waves split the terms, 32 each of 128, straight from memory into the operands' registers, and their sums are added through LDS.
+// ---------------------------------------------------------------------------------------------------------
+template <int XT, int MB>
+__device__ __forceinline__ void few_tile(const RowsArgs& a, const GroupTile& t, int col0, f4_t* lds)
+{
+    constexpr int AHEAD = MB == 1 ? 8 : MB == 2 ? 6 : 4;           // loads in flight of each operand row
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const uint32_t ld = 2 * a.terms;
+    const __amdgpu_buffer_rsrc_t wb = buffer(a.w + ((size_t)t.expert * a.cols + col0) * a.terms, (uint32_t)min(16, a.cols - col0) * ld);
+    const __amdgpu_buffer_rsrc_t xb = a.token ? buffer(a.x, (uint32_t)a.xbytes) : buffer(a.x + (size_t)t.row * a.terms, (uint32_t)t.rows * ld);
+    // columns past the last one are past the buffer; rows past the tile's are its last row again, and not stored
+    uint32_t xo[MB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+    {
+        const int m = min(16 * i + r, t.rows - 1);
+        xo[i] = (uint32_t)(a.token ? a.token[t.row + m] : m) * ld;
+    }
+    f4_t acc[MB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i) acc[i] = f4_t{ 0.f, 0.f, 0.f, 0.f };
+    u4_t w[AHEAD], x[AHEAD][MB];
+    auto load = [&](int b, u4_t& wv, u4_t (&xv)[MB]) {
+        const uint32_t k = 16 * g + 64 * wave + 256 * b;             // bytes into a row
+        wv = __builtin_amdgcn_raw_buffer_load_b128(wb, k < ld ? r * ld + k : NOWHERE, 0, 0);
+#pragma unroll
+        for (int i = 0; i < MB; ++i) xv[i] = __builtin_amdgcn_raw_buffer_load_b128(xb, k < ld ? xo[i] + k : NOWHERE, 0, 0);
+    };
+    const int blocks = (a.terms + 127) / 128;
+#pragma unroll
+    for (int q = 0; q < AHEAD; ++q) load(q, w[q], x[q]);             // (past the terms: zero)
+    for (int b = 0; b < blocks; b += AHEAD)
+    {
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q)
+        {
+#pragma unroll
+            for (int i = 0; i < MB; ++i) acc[i] = mfma<XT>(w[q], x[q][i], acc[i]);
+            load(b + AHEAD + q, w[q], x[q]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MB; ++i) lds[(wave * MB + i) * 64 + lane] = acc[i];
+    __syncthreads();
+    for (int i = wave; i < MB; i += 4)
+    {
+        f4_t v = lds[i * 64 + lane];
+#pragma unroll
+        for (int u = 1; u < 4; ++u) v += lds[(u * MB + i) * 64 + lane];
+        const int m = 16 * i + r, n = col0 + 4 * g;
+        if (m >= t.rows || n >= a.cols) continue;
+        const size_t at = (size_t)(t.row + m) * a.cols + n;
+        if (a.type == MM_DTYPE_F32) *reinterpret_cast<f4_t*>(static_cast<float*>(a.y) + at) = v;
+        else *reinterpret_cast<u2_t*>(static_cast<uint16_t*>(a.y) + at) = u2_t{ pack2<XT>(v[0], v[1]), pack2<XT>(v[2], v[3]) };
+    }
+}
+
+template <int XT>
+__global__ __launch_bounds__(256) void k_group_few(RowsArgs a)
+{
+    __shared__ f4_t lds[4 * 4 * 64];
+    const int s = tile_of_block(blockIdx.x), nt = *a.ntiles;
+    if (s >= nt * a.colt) return;
+    const GroupTile t = a.tiles[s / a.colt];
+    const int ct = s % a.colt;
+    if (t.expert < 0) return zero_tile<16>(a, t, ct);
+    if (t.rows > 32) few_tile<XT, 4>(a, t, 16 * ct, lds);
+    else if (t.rows > 16) few_tile<XT, 2>(a, t, 16 * ct, lds);
+    else few_tile<XT, 1>(a, t, 16 * ct, lds);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -513,8 +620,9 @@ struct WeightsArgs
 };
 
 constexpr int W_TERMS = 32, W_STAGE = 2 * W_TERMS * 512, W_STAGES = 5;     // 160 KB of LDS
-using Terms = Across<W_TERMS>;
-using WShape = Shape<ROWS>;
+constexpr int COLS = 256;
+using Terms = Across<W_TERMS, COLS, 8>;
+using WShape = Shape<ROWS, COLS>;
 
 // A tile's operands. PICK: 0 neither tensor has rows per token, 1 dy has, 2 x has.
 template <int PICK>
@@ -702,19 +810,30 @@ int launch_rows(const char* what, const mm_group_plan_t* p, const void* x, const
     a.x = static_cast<const uint16_t*>(x);
     a.w = static_cast<const uint16_t*>(w);
     a.y = reduce ? ws : y;
-    a.tiles = reinterpret_cast<const GroupTile*>(p->tiles);
-    a.ntiles = p->ntiles;
     a.token = gather ? p->token : nullptr;
     a.xbytes = (size_t)p->T * terms * 2;
     a.terms = terms;
     a.cols = cols;
     a.type = reduce ? MM_DTYPE_F32 : y_type;
     a.zero = !reduce;
-    a.colt = (cols + COLS - 1) / COLS;
-    const long long tiles = tile_capacity(n, p->E) * a.colt, blocks = (tiles + 255) / 256 * 256;
+    // The form by the tiles there will be (the routes' experts are not known here): large ones as soon as they nearly fill the GPU (512 rows of
+    // each of 8 experts of 4096 x 4096, 320 tiles by this estimate: 115 us, small ones 195), else small ones (1,000 rows of one expert, 48
+    // tiles: 98 and 38 us). Forward, few rows of many experts are a little faster in small tiles too (64 of 64: 448 and 418 us; 128: 477
+    // and 525), the gradient of the inputs is not (359 and 393). A few routes that leave most CUs without a small tile are split over the terms
+    // instead (one of 4096 x 4096: 28 and 9 us; eight: 43 and 45).
+    const long long met = std::min<long long>(n, p->E), large = std::max(met, n / ROWS + met / 2) * ((cols + 255) / 256);
+    const bool few = !ACROSS && n <= 16 && n * ((cols + 127) / 128) < 256;
+    const bool small = !few && (large < 192 || (!ACROSS && n <= 64 * met));
+    const int most = few || small ? FEW_ROWS : ROWS, width = few ? 16 : small ? 128 : 256;
+    a.tiles = reinterpret_cast<const GroupTile*>(p->tiles) + (most == FEW_ROWS ? tile_capacity(n, p->E, ROWS) : 0);
+    a.ntiles = p->ntiles + (most == FEW_ROWS);
+    a.colt = (cols + width - 1) / width;
+    const long long tiles = tile_capacity(n, p->E, most) * a.colt, blocks = (tiles + 255) / 256 * 256;
     MM_CHECK_ARG(blocks <= MOST_BLOCKS, "%s: too many tiles", what);
-    auto kernel = dtype == MM_DTYPE_F16 ? k_group_rows<MM_DTYPE_F16, ACROSS> : k_group_rows<MM_DTYPE_BF16, ACROSS>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(512), 0, hs, a);
+    const bool h = dtype == MM_DTYPE_F16;
+    if (few) hipLaunchKernelGGL((h ? k_group_few<MM_DTYPE_F16> : k_group_few<MM_DTYPE_BF16>), dim3((unsigned)blocks), dim3(256), 0, hs, a);
+    else if (small) hipLaunchKernelGGL((h ? k_group_rows<MM_DTYPE_F16, ACROSS, 128> : k_group_rows<MM_DTYPE_BF16, ACROSS, 128>), dim3((unsigned)blocks), dim3(256), 0, hs, a);
+    else hipLaunchKernelGGL((h ? k_group_rows<MM_DTYPE_F16, ACROSS, 256> : k_group_rows<MM_DTYPE_BF16, ACROSS, 256>), dim3((unsigned)blocks), dim3(512), 0, hs, a);
     if (reduce)
     {
         const long long n4 = (long long)p->T * cols / 4;
@@ -730,7 +849,10 @@ int launch_rows(const char* what, const mm_group_plan_t* p, const void* x, const
 
 extern "C" {
 
-size_t mm_group_tiles(int n, int E) { return n > 0 && E > 0 ? (size_t)tile_capacity(n, E) * sizeof(GroupTile) : 0; }
+size_t mm_group_tiles(int n, int E)
+{
+    return n > 0 && E > 0 ? (size_t)(tile_capacity(n, E, ROWS) + tile_capacity(n, E, FEW_ROWS)) * sizeof(GroupTile) : 0;
+}
 
 int mm_group_plan(const int64_t* ids, const mm_group_plan_t* p, int32_t* counts, void* workspace, size_t workspace_bytes, mm_stream_t stream)
 {
@@ -742,7 +864,8 @@ int mm_group_plan(const int64_t* ids, const mm_group_plan_t* p, int32_t* counts,
                                   nullptr, workspace, workspace_bytes, stream);
     if (rc != MM_OK) return rc;
     hipLaunchKernelGGL(k_group_tiles, dim3(1), dim3(1024), 0, reinterpret_cast<hipStream_t>(stream), p->offsets, p->E,
-                       reinterpret_cast<GroupTile*>(p->tiles), p->ntiles);
+                       reinterpret_cast<GroupTile*>(p->tiles), reinterpret_cast<GroupTile*>(p->tiles) + tile_capacity((long long)p->T * p->topk, p->E, ROWS),
+                       p->ntiles);
     return check_launch("mm_group_plan");
 }
 

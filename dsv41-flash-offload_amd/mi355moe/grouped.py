@@ -40,7 +40,7 @@ class Plan:
             tiles = lib.mm_group_tiles(n, E)
             # one buffer: tiles, offsets [E + 2], counts [E + 1], ntiles, order, token, inv [n]
             at = [tiles // 4]
-            for size in (E + 2, E + 1, 1, n, n, n):
+            for size in (E + 2, E + 1, 2, n, n, n):
                 at.append(at[-1] + size)
             make = torch.empty if n else torch.zeros
             self._buf = buf = make(at[-1], dtype=torch.int32, device=dev)

@@ -312,7 +312,7 @@ int mm_w4_moe(const mm_w4_layer_t* layer, const void* x, int x_dtype, int T, int
 /* The order of a call's routes that the grouped products share: T tokens of topk picks each, sorted by expert (stable), picks
  * outside [0, E) last. Device memory: offsets int32 [E + 2] (rows offsets[e] .. offsets[e + 1] - 1 belong to expert e, rows from
  * offsets[E] on to none), order int32 [n] (flat route of each row, n = T topk < 2^31 - 256), token int32 [n] (order / topk), inv int32 [n]
- * (row of each route), tiles (mm_group_tiles(n, E) bytes, 16-byte aligned) and ntiles int32 [1], the kernels' own. E <= 1024. */
+ * (row of each route), tiles (mm_group_tiles(n, E) bytes, 16-byte aligned) and ntiles int32 [2], the kernels' own. E <= 1024. */
 typedef struct mm_group_plan
 {
     int32_t *offsets, *order, *token, *inv;
