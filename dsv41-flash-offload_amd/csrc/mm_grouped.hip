@@ -73,12 +73,32 @@ struct GroupTile
 // plan has two lists, of large tiles and of small ones, and their numbers.
 constexpr long long tile_capacity(long long n, int E, int rows) { return n / rows + std::min<long long>(n, E) + 1; }
 
-__global__ __launch_bounds__(1024) void k_group_tiles(const int32_t* __restrict__ offsets, int E, GroupTile* __restrict__ tiles, GroupTile* __restrict__ few,
-                                                      int32_t* __restrict__ ntiles)
+struct PlanLds
 {
-    __shared__ int part[16], start[1026], first[1026];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    for (int i = t; i < E + 2; i += 1024) start[i] = offsets[i];
+    int part[16], start[1026], first[1026];
+};
+
+// Exclusive sums over the workgroup's 1024 threads; the total in `total`.
+__device__ __forceinline__ int scan_1024(int v, int* part, int& total)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, inc = wave_incl_scan(v);
+    __syncthreads();
+    if (lane == 63) part[wave] = inc;
+    __syncthreads();
+    int at = inc - v;
+    total = 0;
+    for (int w = 0; w < 16; ++w)
+    {
+        if (w < wave) at += part[w];
+        total += part[w];
+    }
+    return at;
+}
+
+// Both lists from start[0 .. E + 1], the first row of each expert and of none.
+__device__ __forceinline__ void write_tiles(PlanLds& l, int E, GroupTile* tiles, GroupTile* few, int32_t* ntiles)
+{
+    const int t = threadIdx.x;
     for (int list = 0; list < 2; ++list)
     {
         const int most = list ? FEW_ROWS : ROWS;
@@ -86,22 +106,15 @@ __global__ __launch_bounds__(1024) void k_group_tiles(const int32_t* __restrict_
         int run = 0;
         for (int base = 0; base <= E; base += 1024)
         {
-            __syncthreads();
-            const int e = base + t, cnt = e <= E ? (start[e + 1] - start[e] + most - 1) / most : 0, inc = wave_incl_scan(cnt);
-            if (lane == 63) part[wave] = inc;
-            __syncthreads();
-            int at = run + inc - cnt, total = 0;
-            for (int w = 0; w < 16; ++w)
-            {
-                if (w < wave) at += part[w];
-                total += part[w];
-            }
-            if (e <= E) first[e] = at;
+            const int e = base + t;
+            int total;
+            const int at = scan_1024(e <= E ? (l.start[e + 1] - l.start[e] + most - 1) / most : 0, l.part, total);
+            if (e <= E) l.first[e] = run + at;
             run += total;
         }
         if (t == 0)
         {
-            first[E + 1] = run;
+            l.first[E + 1] = run;
             ntiles[list] = run;
         }
         __syncthreads();
@@ -110,12 +123,104 @@ __global__ __launch_bounds__(1024) void k_group_tiles(const int32_t* __restrict_
             // the expert (E: none) whose tiles i is among
             int e = 0;
             for (int step = 1024; step; step >>= 1)
-                if (e + step <= E && first[e + step] <= i) e += step;
-            const int cnt = first[e + 1] - first[e], r0 = start[e], n = start[e + 1] - r0, k = i - first[e];
+                if (e + step <= E && l.first[e + step] <= i) e += step;
+            const int cnt = l.first[e + 1] - l.first[e], r0 = l.start[e], n = l.start[e + 1] - r0, k = i - l.first[e];
             const int at = (int)((long long)n * k / cnt), to = (int)((long long)n * (k + 1) / cnt);
-            out[i] = { e < E ? e : -1, r0 + at, to - at, first[e], cnt, (n + cnt - 1) / cnt, { 0, 0 } };
+            out[i] = { e < E ? e : -1, r0 + at, to - at, l.first[e], cnt, (n + cnt - 1) / cnt, { 0, 0 } };
         }
+        __syncthreads();
     }
+}
+
+__global__ __launch_bounds__(1024) void k_group_tiles(const int32_t* __restrict__ offsets, int E, GroupTile* __restrict__ tiles, GroupTile* __restrict__ few,
+                                                      int32_t* __restrict__ ntiles)
+{
+    __shared__ PlanLds l;
+    for (int i = threadIdx.x; i < E + 2; i += 1024) l.start[i] = offsets[i];
+    __syncthreads();
+    write_tiles(l, E, tiles, few, ntiles);
+}
+
+// The whole plan of up to PLAN_ROUTES routes in one workgroup (701 tokens of 4 picks: 17 + 4 us as a permutation and its tiles). A wave takes
+// a run of routes, 64 at a time: lanes that hold the same expert find each other by one ballot per bit, so that a route's place among its
+// expert's is the wave's count so far and the lanes before it; counts of the waves before come on top.
+constexpr int PLAN_ROUTES = 8192, PLAN_ROUNDS = PLAN_ROUTES / 1024;
+__global__ __launch_bounds__(1024) void k_group_plan(const int64_t* __restrict__ ids, int n, int topk, int E, int bits, int32_t* __restrict__ counts,
+                                                     int32_t* __restrict__ offsets, int32_t* __restrict__ order, int32_t* __restrict__ token,
+                                                     int32_t* __restrict__ inv, GroupTile* __restrict__ tiles, GroupTile* __restrict__ few,
+                                                     int32_t* __restrict__ ntiles)
+{
+    __shared__ PlanLds l;
+    __shared__ uint16_t hist[16][1026];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, rounds = (n + 1023) / 1024, s0 = wave * rounds * 64 + lane;
+    int e[PLAN_ROUNDS], p[PLAN_ROUNDS];
+#pragma unroll
+    for (int r = 0; r < PLAN_ROUNDS; ++r)
+    {
+        const int s = s0 + 64 * r;
+        const int64_t id = r < rounds && s < n ? ids[s] : 0;
+        e[r] = id >= 0 && id < E ? (int)id : E;
+    }
+    for (int i = t; i < 16 * 1026 / 2; i += 1024) reinterpret_cast<uint32_t*>(hist)[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < PLAN_ROUNDS; ++r)
+    {
+        if (r >= rounds) break;
+        const bool in = s0 + 64 * r < n;
+        uint64_t same = __ballot(in);
+        for (int b = 0; b < bits; ++b)
+        {
+            const uint64_t one = __ballot((e[r] >> b) & 1);
+            same &= (e[r] >> b) & 1 ? one : ~one;
+        }
+        const int before = __popcll(same & ((1ull << lane) - 1)), had = hist[wave][e[r]];
+        __builtin_amdgcn_wave_barrier();
+        p[r] = had + before;
+        if (in && before == 0) hist[wave][e[r]] = (uint16_t)(had + __popcll(same));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    int run = 0;
+    for (int base = 0; base <= E; base += 1024)
+    {
+        const int x = base + t;
+        int c = 0;
+        if (x <= E)
+            for (int w = 0; w < 16; ++w)
+            {
+                const int h = hist[w][x];
+                hist[w][x] = (uint16_t)c;
+                c += h;
+            }
+        int total;
+        const int at = run + scan_1024(c, l.part, total);
+        if (x <= E)
+        {
+            l.start[x] = at;
+            offsets[x] = at;
+            counts[x] = c;
+        }
+        run += total;
+    }
+    if (t == 0)
+    {
+        l.start[E + 1] = n;
+        offsets[E + 1] = n;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < PLAN_ROUNDS; ++r)
+    {
+        const int s = s0 + 64 * r;
+        if (r >= rounds || s >= n) break;
+        const int at = l.start[e[r]] + hist[wave][e[r]] + p[r];
+        order[at] = s;
+        token[at] = s / topk;
+        inv[s] = at;
+    }
+    write_tiles(l, E, tiles, few, ntiles);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -860,12 +965,22 @@ int mm_group_plan(const int64_t* ids, const mm_group_plan_t* p, int32_t* counts,
     MM_CHECK_ARG(p->T > 0 && p->topk > 0 && p->E > 0 && p->E <= 1024 && (long long)p->T * p->topk < (1LL << 31) - 256,
                  "mm_group_plan: need tokens, picks, 1 <= E <= 1024 and fewer than 2^31 - 256 routes");
     MM_CHECK_ARG(aligned16(p->tiles), "mm_group_plan: misaligned tiles");
-    const int rc = permute_launch(ids, nullptr, p->T * p->topk, p->topk, p->E, counts, p->offsets, p->order, p->token, nullptr, p->inv, nullptr,
-                                  nullptr, workspace, workspace_bytes, stream);
-    if (rc != MM_OK) return rc;
-    hipLaunchKernelGGL(k_group_tiles, dim3(1), dim3(1024), 0, reinterpret_cast<hipStream_t>(stream), p->offsets, p->E,
-                       reinterpret_cast<GroupTile*>(p->tiles), reinterpret_cast<GroupTile*>(p->tiles) + tile_capacity((long long)p->T * p->topk, p->E, ROWS),
-                       p->ntiles);
+    const int n = p->T * p->topk;
+    const hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
+    GroupTile* tiles = reinterpret_cast<GroupTile*>(p->tiles);
+    GroupTile* few = tiles + tile_capacity(n, p->E, ROWS);
+    if (n <= PLAN_ROUTES)
+    {
+        int bits = 1;
+        while (p->E >> bits) ++bits;
+        hipLaunchKernelGGL(k_group_plan, dim3(1), dim3(1024), 0, hs, ids, n, p->topk, p->E, bits, counts, p->offsets, p->order, p->token, p->inv, tiles,
+                           few, p->ntiles);
+        return check_launch("mm_group_plan");
+    }
+    if (const int rc = permute_launch(ids, nullptr, n, p->topk, p->E, counts, p->offsets, p->order, p->token, nullptr, p->inv, nullptr, nullptr,
+                                      workspace, workspace_bytes, stream))
+        return rc;
+    hipLaunchKernelGGL(k_group_tiles, dim3(1), dim3(1024), 0, hs, p->offsets, p->E, tiles, few, p->ntiles);
     return check_launch("mm_group_plan");
 }
 
