@@ -62,7 +62,7 @@ class _Moe(torch.autograd.Function):
         need_x, need_w, need_13, need_2 = ctx.needs_input_grad[:4]
         plan, up = ctx.plan, w13.flatten(1, 2)
         kept = grouped.Saved8(*kept, x.dtype) if ctx.save8 else kept[0]
-        dout = dout.to(x.dtype)                      # the products take 16-bit operands
+        dout = _lib.aligned(dout.to(x.dtype))        # the products take 16-bit operands
         dx = dw = d13 = d2 = None
         dh, _ = grouped.linear_backward(dout, None, w2, plan, reduce=True, need_w=False)
         dgu, dw, h = grouped.swiglu_backward(dh, kept, plan, w, ctx.limit, need_weights=need_w, need_h=need_2)
@@ -95,4 +95,5 @@ def moe(store, x, ids, w, shared_expert=None, stream=None):
         if shared >= 0:
             ids = torch.cat([ids, torch.full((T, 1), shared, dtype=torch.long, device=dev)], 1)
             w = torch.cat([w, torch.ones((T, 1), dtype=torch.float32, device=dev)], 1)
-        return _captured_apply("dense.moe", _Moe, (x, w, store.w13, store.w2), x, w, store.w13, store.w2, ids, store.limit, store.save8)
+        return _captured_apply("dense.moe", _Moe, (x, w, store.w13, store.w2), x, w, store.w13, store.w2, ids, store.limit, store.save8,
+                               instead="the *_forward and *_backward functions of grouped")

@@ -218,6 +218,10 @@ def swiglu_backward(dh, kept, plan=None, weights=None, limit=10.0, need_weights=
         raise ValueError(f"swiglu_backward: gu [n, 2 I] expected (got {tuple(kept.shape)})")
     n, I = (kept.codes if saved else kept).shape[0], (kept.codes if saved else kept).shape[1] // 2
     _check_swiglu("swiglu_backward", n, kept.dtype, I, plan, weights, limit)
+    if saved:
+        for name, t, shape in (("codes", kept.codes, (n, 2 * I)), ("exps", kept.exps, (n, 2 * I // SAVE_GROUP))):
+            if t.dtype != torch.int8 or tuple(t.shape) != shape or not t.is_contiguous() or I % SAVE_GROUP:
+                raise ValueError(f"swiglu_backward: {name} must be contiguous int8 {list(shape)}, I a multiple of {SAVE_GROUP} (got {t.dtype} {tuple(t.shape)})")
     if dh.dtype != kept.dtype or tuple(dh.shape) != (n, I):
         raise ValueError(f"swiglu_backward: dh must be {kept.dtype} {[n, I]} (got {dh.dtype} {tuple(dh.shape)})")
     dev = dh.device

@@ -20,8 +20,8 @@ def _capture_stream(device):
     return _lib.raw_stream(device) if device.type == "cuda" else None
 
 
-def _captured_apply(what, fn, leaves, *args):
-    """fn.apply(*args). Under stream capture, a leaf among its inputs may not have its gradient node in an autograd graph from before
+def _captured_apply(what, fn, leaves, *args, instead=None):
+    """fn.apply(*args), for `what`, whose kernels without autograd are `instead`. Under stream capture, a leaf among its inputs may not have its gradient node in an autograd graph from before
     the capture: the captured backward would go to that node's stream, which invalidates the capture and ends the process. (A node that
     a captured call made belongs to that capture's stream, and passes in captures of that stream only.)"""
     leaves = [t for t in leaves if t.requires_grad and t.is_leaf]
@@ -37,7 +37,7 @@ def _captured_apply(what, fn, leaves, *args):
         notes(t)["mi355moe seen"] = True                      # gone with the node if no graph holds it
         if notes(t).pop("mi355moe seen", None):
             raise RuntimeError(f"{what}: an input has an autograd graph from before the stream capture; drop it first, or capture "
-                               f"{what}_forward and {what}_backward")
+                               f"{instead or f'{what}_forward and {what}_backward'}")
     out = fn.apply(*args)
     for t in leaves:
         notes(t)["mi355moe captured"] = (t.device, _capture_stream(t.device))
