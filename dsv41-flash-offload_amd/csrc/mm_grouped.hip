@@ -245,22 +245,22 @@ constexpr uint32_t NOWHERE = 0xfffffff0u;              // past every buffer: rea
 template <int R, int W>
 struct Along
 {
-    static constexpr int BYTES = R * 128, LOADS = std::max(1, R / (8 * W)), READS = 1;
+    static constexpr int BYTES = R * 128, LOADS = (R + 8 * W - 1) / (8 * W), READS = 1;
     __amdgpu_buffer_rsrc_t buf;
     uint32_t at[LOADS];
-    int slot;             // the wave's first row
+    int slot[LOADS];      // first rows of the wave's loads
     int chunk;            // the lane's chunk of a row's eight
     // base: the tile's first row, or with `pick` the row that pick[] counts from; rows > 0; ld: bytes of a row; bytes: of the buffer
     __device__ __forceinline__ void init(const void* base, uint32_t ld, int rows, uint32_t bytes, const int32_t* pick)
     {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         buf = buffer(base, bytes);
-        slot = wave * LOADS * 8 % R;
         chunk = (lane ^ (lane >> 3)) & 7;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
         {
-            const int r = slot + 8 * i + (lane >> 3);
+            slot[i] = (wave * LOADS + i) * 8 % R;
+            const int r = slot[i] + (lane >> 3);
             // rows past the tile's are past the buffer, or the last row again: they are not stored
             at[i] = (uint32_t)(pick ? pick[min(r, rows - 1)] : r) * ld + 16 * chunk;
         }
@@ -271,7 +271,7 @@ struct Along
         const bool in = TERMS * block + 8 * chunk < terms;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
-            load16(buf, lds + (slot + 8 * i) * 128, in ? at[i] + 128 * block : NOWHERE);
+            load16(buf, lds + slot[i] * 128, in ? at[i] + 128 * block : NOWHERE);
     }
     // chunk kk * 4 + (lane >> 4) of row 16 b + (lane & 15)
     __device__ static __forceinline__ uint32_t place(int first)
@@ -399,9 +399,9 @@ constexpr int LDS_BYTES = C == 256 ? 160 * 1024 : 76 * 1024;
 template <int R, int C>
 struct Shape
 {
-    static constexpr int WAVES = C / 32, WN = R >= 128 ? 4 : WAVES, WM = WAVES / WN, MB = std::max(1, R / 16 / WM), NB = C / 16 / WN;
+    static constexpr int WAVES = C / 32, WN = R > 64 ? 4 : WAVES, WM = WAVES / WN, MB = std::max(1, R / 16 / WM), NB = C / 16 / WN;
     // places in LDS for blocks of the rows and of the columns: these are the weights, which come from farther away when tiles have few rows
-    static constexpr int SM = R >= 128 ? 2 : 3, SN = R == 256 ? 2 : R == 192 || (C == 128 && R == 64) ? 3 : 4;
+    static constexpr int SM = R > 64 ? 2 : 3, SN = R > 192 ? 2 : R > 128 || (C == 128 && R == 64) ? 3 : 4;
     static constexpr int MSTAGE = R * 128, NSTAGE = C * 128, LDS = SM * MSTAGE + SN * NSTAGE;
     static_assert(LDS <= LDS_BYTES<C> && SN >= SM, "LDS");
 };
@@ -630,9 +630,12 @@ __global__ __launch_bounds__(2 * C, 2) void k_group_rows(RowsArgs a)
     if (t.expert < 0) return zero_tile<C>(a, t, ct);
     if constexpr (C == 256)
     {
-        if (t.size > 192) return rows_tile<XT, ACROSS, 256, C>(a, t, ct, lds);
-        if (t.size > 128) return rows_tile<XT, ACROSS, 192, C>(a, t, ct, lds);
-        if (t.size > 64) return rows_tile<XT, ACROSS, 128, C>(a, t, ct, lds);
+        if (t.size > 224) return rows_tile<XT, ACROSS, 256, C>(a, t, ct, lds);
+        if (t.size > 192) return rows_tile<XT, ACROSS, 224, C>(a, t, ct, lds);
+        if (t.size > 160) return rows_tile<XT, ACROSS, 192, C>(a, t, ct, lds);
+        if (t.size > 128) return rows_tile<XT, ACROSS, 160, C>(a, t, ct, lds);
+        if (t.size > 96) return rows_tile<XT, ACROSS, 128, C>(a, t, ct, lds);
+        if (t.size > 64) return rows_tile<XT, ACROSS, 96, C>(a, t, ct, lds);
     }
     if (t.size > 32) rows_tile<XT, ACROSS, 64, C>(a, t, ct, lds);
     else if (t.size > 16) rows_tile<XT, ACROSS, 32, C>(a, t, ct, lds);
