@@ -643,76 +643,63 @@ __global__ __launch_bounds__(2 * C, 2) void k_group_rows(RowsArgs a)
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// A few rows per expert (a decode step): bound by reading the weights, once. A workgroup takes a small tile's rows by 16 columns; its
-// four waves split the terms, 32 each of 128, straight from memory into the operands' registers, and their sums are added through LDS.
+// A few routes, of a decode step: bound by reading the weights, once, and by the time a chain of blocks takes where few workgroups share
+// them. A workgroup takes a tile's rows (at most 16) by 16 columns; its four waves split the terms, 32 each of 128, straight from memory into
+// the operands' registers, and their sums are added through LDS.
 // ---------------------------------------------------------------------------------------------------------
-template <int XT, int MB>
+constexpr int FEW_ROUTES = 16;
+template <int XT>
 __device__ __forceinline__ void few_tile(const RowsArgs& a, const GroupTile& t, int col0, f4_t* lds)
 {
-    constexpr int AHEAD = MB == 1 ? 8 : MB == 2 ? 6 : 4;           // loads in flight of each operand row
+    constexpr int AHEAD = 8;                                         // blocks of 128 terms on their way
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     const uint32_t ld = 2 * a.terms;
     const __amdgpu_buffer_rsrc_t wb = buffer(a.w + ((size_t)t.expert * a.cols + col0) * a.terms, (uint32_t)min(16, a.cols - col0) * ld);
     const __amdgpu_buffer_rsrc_t xb = a.token ? buffer(a.x, (uint32_t)a.xbytes) : buffer(a.x + (size_t)t.row * a.terms, (uint32_t)t.rows * ld);
     // columns past the last one are past the buffer; rows past the tile's are its last row again, and not stored
-    uint32_t xo[MB];
-#pragma unroll
-    for (int i = 0; i < MB; ++i)
-    {
-        const int m = min(16 * i + r, t.rows - 1);
-        xo[i] = (uint32_t)(a.token ? a.token[t.row + m] : m) * ld;
-    }
-    f4_t acc[MB];
-#pragma unroll
-    for (int i = 0; i < MB; ++i) acc[i] = f4_t{ 0.f, 0.f, 0.f, 0.f };
-    u4_t w[AHEAD], x[AHEAD][MB];
-    auto load = [&](int b, u4_t& wv, u4_t (&xv)[MB]) {
-        const uint32_t k = 16 * g + 64 * wave + 256 * b;             // bytes into a row
+    const int m = min(r, t.rows - 1);
+    const uint32_t xo = (uint32_t)(a.token ? a.token[t.row + m] : m) * ld;
+    f4_t acc = f4_t{ 0.f, 0.f, 0.f, 0.f };
+    u4_t w[AHEAD], x[AHEAD];
+    auto load = [&](int b, u4_t& wv, u4_t& xv) {
+        const uint32_t k = 16 * g + 64 * wave + 256 * b;             // bytes into a row; past the terms: zero
         wv = __builtin_amdgcn_raw_buffer_load_b128(wb, k < ld ? r * ld + k : NOWHERE, 0, 0);
-#pragma unroll
-        for (int i = 0; i < MB; ++i) xv[i] = __builtin_amdgcn_raw_buffer_load_b128(xb, k < ld ? xo[i] + k : NOWHERE, 0, 0);
+        xv = __builtin_amdgcn_raw_buffer_load_b128(xb, k < ld ? xo + k : NOWHERE, 0, 0);
     };
     const int blocks = (a.terms + 127) / 128;
 #pragma unroll
-    for (int q = 0; q < AHEAD; ++q) load(q, w[q], x[q]);             // (past the terms: zero)
+    for (int q = 0; q < AHEAD; ++q) load(q, w[q], x[q]);
     for (int b = 0; b < blocks; b += AHEAD)
     {
 #pragma unroll
         for (int q = 0; q < AHEAD; ++q)
         {
-#pragma unroll
-            for (int i = 0; i < MB; ++i) acc[i] = mfma<XT>(w[q], x[q][i], acc[i]);
+            acc = mfma<XT>(w[q], x[q], acc);
             load(b + AHEAD + q, w[q], x[q]);
         }
     }
-#pragma unroll
-    for (int i = 0; i < MB; ++i) lds[(wave * MB + i) * 64 + lane] = acc[i];
+    lds[threadIdx.x] = acc;
     __syncthreads();
-    for (int i = wave; i < MB; i += 4)
-    {
-        f4_t v = lds[i * 64 + lane];
+    if (wave) return;
 #pragma unroll
-        for (int u = 1; u < 4; ++u) v += lds[(u * MB + i) * 64 + lane];
-        const int m = 16 * i + r, n = col0 + 4 * g;
-        if (m >= t.rows || n >= a.cols) continue;
-        const size_t at = (size_t)(t.row + m) * a.cols + n;
-        if (a.type == MM_DTYPE_F32) *reinterpret_cast<f4_t*>(static_cast<float*>(a.y) + at) = v;
-        else *reinterpret_cast<u2_t*>(static_cast<uint16_t*>(a.y) + at) = u2_t{ pack2<XT>(v[0], v[1]), pack2<XT>(v[2], v[3]) };
-    }
+    for (int u = 1; u < 4; ++u) acc += lds[u * 64 + lane];
+    const int n = col0 + 4 * g;
+    if (r >= t.rows || n >= a.cols) return;
+    const size_t at = (size_t)(t.row + r) * a.cols + n;
+    if (a.type == MM_DTYPE_F32) *reinterpret_cast<f4_t*>(static_cast<float*>(a.y) + at) = acc;
+    else *reinterpret_cast<u2_t*>(static_cast<uint16_t*>(a.y) + at) = u2_t{ pack2<XT>(acc[0], acc[1]), pack2<XT>(acc[2], acc[3]) };
 }
 
 template <int XT>
 __global__ __launch_bounds__(256) void k_group_few(RowsArgs a)
 {
-    __shared__ f4_t lds[4 * 4 * 64];
+    __shared__ f4_t lds[256];
     const int s = tile_of_block(blockIdx.x), nt = *a.ntiles;
     if (s >= nt * a.colt) return;
     const GroupTile t = a.tiles[s / a.colt];
     const int ct = s % a.colt;
-    if (t.expert < 0) return zero_tile<16>(a, t, ct);
-    if (t.rows > 32) few_tile<XT, 4>(a, t, 16 * ct, lds);
-    else if (t.rows > 16) few_tile<XT, 2>(a, t, 16 * ct, lds);
-    else few_tile<XT, 1>(a, t, 16 * ct, lds);
+    if (t.expert < 0) zero_tile<16>(a, t, ct);
+    else few_tile<XT>(a, t, 16 * ct, lds);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -930,7 +917,7 @@ int launch_rows(const char* what, const mm_group_plan_t* p, const void* x, const
     // and 525), the gradient of the inputs is not (359 and 393). A few routes that leave most CUs without a small tile are split over the terms
     // instead (one of 4096 x 4096: 28 and 9 us; eight: 43 and 45).
     const long long met = std::min<long long>(n, p->E), large = std::max(met, n / ROWS + met / 2) * ((cols + 255) / 256);
-    const bool few = !ACROSS && n <= 16 && n * ((cols + 127) / 128) < 256;
+    const bool few = !ACROSS && n <= FEW_ROUTES && n * ((cols + 127) / 128) < 256;
     const bool small = !few && (large < 192 || (!ACROSS && n <= 64 * met));
     const int most = few || small ? FEW_ROWS : ROWS, width = few ? 16 : small ? 128 : 256;
     a.tiles = reinterpret_cast<const GroupTile*>(p->tiles) + (most == FEW_ROWS ? tile_capacity(n, p->E, ROWS) : 0);

@@ -90,7 +90,7 @@ def run_all(dev, x, dy, w, ids, gather, reduce, out_dtype=None, stream=None):
 
 
 COUNTS = {"edges": [0, 1, 15, 16, 17, 0, 31, 32, 33, 63, 64, 65, 2], "tiles": [127, 128, 129, 0, 255, 256, 257], "long": [5, 800, 0, 301],
-          "few": [1, 0, 0, 2, 1], "one": [0, 0, 1], "none": [0, 0]}
+          "sizes": [90, 97, 128, 129, 150, 161, 180, 193, 210, 225, 256, 257, 5, 300, 20, 700, 40], "few": [1, 0, 0, 2, 1], "one": [0, 0, 1], "none": [0, 0]}
 
 
 @pytest.mark.parametrize("rows,k,none,K,N,dtype,gather,reduce", [
@@ -102,6 +102,11 @@ COUNTS = {"edges": [0, 1, 15, 16, 17, 0, 31, 32, 33, 63, 64, 65, 2], "tiles": [1
     ("tiles", 8, 3, 8, 512, HF, False, True),
     ("long", 2, 300, 264, 136, BF, True, False),
     ("long", 5, 1, 1032, 8, HF, False, True),
+    # enough large tiles for every form of them: of columns forward, of inputs backward
+    ("sizes", 1, 5, 72, 4096, BF, False, False),
+    ("sizes", 2, 300, 4096, 72, HF, True, False),
+    ("sizes", 3, 4, 200, 3848, HF, False, True),
+    ("sizes", 4, 1, 3848, 136, BF, False, True),
     ("few", 1, 0, 1024, 512, BF, True, False),
     ("few", 2, 1, 512, 1024, HF, False, True),
     ("one", 1, 0, 8, 8, BF, False, False),
@@ -248,14 +253,13 @@ def act_error(gu):
     return (g + 8) * 2.0 ** -23
 
 
-@pytest.mark.parametrize("T,k,E,I,dtype,limit,weighted,none", [
-    (1, 1, 1, 8, BF, LIMIT, False, 0), (1, 8, 384, 2048, BF, LIMIT, True, 0), (40, 3, 5, 520, HF, LIMIT, True, 17), (70, 2, 9, 64, BF, 0.0, True, 3),
-    (9, 4, 4, 2304, HF, 1.5, False, 5), (300, 1, 2, 32, BF, 0.25, True, 300), (5, 2, 3, 4128, BF, 7.0, True, 0)])
-@pytest.mark.parametrize("save8", [False, True])
+GATED = [(1, 1, 1, 8, BF, LIMIT, False, 0), (1, 8, 384, 2048, BF, LIMIT, True, 0), (40, 3, 5, 520, HF, LIMIT, True, 17), (70, 2, 9, 64, BF, 0.0, True, 3),
+         (9, 4, 4, 2304, HF, 1.5, False, 5), (300, 1, 2, 32, BF, 0.25, True, 300), (5, 2, 3, 4128, BF, 7.0, True, 0)]
+
+
+@pytest.mark.parametrize("T,k,E,I,dtype,limit,weighted,none,save8", [c + (s,) for s in (False, True) for c in GATED if not s or c[3] % 32 == 0])
 def test_gated(dev, T, k, E, I, dtype, limit, weighted, none, save8):
     from mi355moe import grouped
-    if save8 and I % 32:
-        pytest.skip("8 bits take whole groups of 32")
     g = torch.Generator().manual_seed(T + I)
     n = T * k
     ids = torch.randint(0, E, (n,), generator=g)
