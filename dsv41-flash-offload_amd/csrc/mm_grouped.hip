@@ -75,60 +75,78 @@ constexpr long long tile_capacity(long long n, int E, int rows) { return n / row
 
 struct PlanLds
 {
-    int part[16], start[1026], first[1026];
+    int part[3][16], start[1026], first[2][1026];
+};
+struct Sums
+{
+    int v[3];
 };
 
-// Exclusive sums over the workgroup's 1024 threads; the total in `total`.
-__device__ __forceinline__ int scan_1024(int v, int* part, int& total)
+// Exclusive sums of three values over the workgroup's 1024 threads; the totals are added to `run`.
+__device__ __forceinline__ Sums scan_1024(const Sums& x, PlanLds& l, Sums& run)
 {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, inc = wave_incl_scan(v);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    Sums at;
+    int inc[3];
     __syncthreads();
-    if (lane == 63) part[wave] = inc;
-    __syncthreads();
-    int at = inc - v;
-    total = 0;
-    for (int w = 0; w < 16; ++w)
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
     {
-        if (w < wave) at += part[w];
-        total += part[w];
+        inc[i] = wave_incl_scan(x.v[i]);
+        if (lane == 63) l.part[i][wave] = inc[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+    {
+        at.v[i] = run.v[i] + inc[i] - x.v[i];
+#pragma unroll
+        for (int w = 0; w < 16; ++w)
+        {
+            const int p = l.part[i][w];
+            at.v[i] += w < wave ? p : 0;
+            run.v[i] += p;
+        }
     }
     return at;
 }
 
-// Both lists from start[0 .. E + 1], the first row of each expert and of none.
-__device__ __forceinline__ void write_tiles(PlanLds& l, int E, GroupTile* tiles, GroupTile* few, int32_t* ntiles)
+// First row and first tiles of expert x (E: none), which has c rows, and behind the last one; every thread of the workgroup takes part.
+// Returns the first row.
+__device__ __forceinline__ int place_expert(PlanLds& l, int x, int c, int E, Sums& run)
 {
-    const int t = threadIdx.x;
-    for (int list = 0; list < 2; ++list)
+    const Sums at = scan_1024(Sums{ { c, (c + ROWS - 1) / ROWS, (c + FEW_ROWS - 1) / FEW_ROWS } }, l, run);
+    if (x <= E)
     {
-        const int most = list ? FEW_ROWS : ROWS;
-        GroupTile* out = list ? few : tiles;
-        int run = 0;
-        for (int base = 0; base <= E; base += 1024)
-        {
-            const int e = base + t;
-            int total;
-            const int at = scan_1024(e <= E ? (l.start[e + 1] - l.start[e] + most - 1) / most : 0, l.part, total);
-            if (e <= E) l.first[e] = run + at;
-            run += total;
-        }
-        if (t == 0)
-        {
-            l.first[E + 1] = run;
-            ntiles[list] = run;
-        }
-        __syncthreads();
-        for (int i = t; i < run; i += 1024)
-        {
-            // the expert (E: none) whose tiles i is among
-            int e = 0;
-            for (int step = 1024; step; step >>= 1)
-                if (e + step <= E && l.first[e + step] <= i) e += step;
-            const int cnt = l.first[e + 1] - l.first[e], r0 = l.start[e], n = l.start[e + 1] - r0, k = i - l.first[e];
-            const int at = (int)((long long)n * k / cnt), to = (int)((long long)n * (k + 1) / cnt);
-            out[i] = { e < E ? e : -1, r0 + at, to - at, l.first[e], cnt, (n + cnt - 1) / cnt, { 0, 0 } };
-        }
-        __syncthreads();
+        l.start[x] = at.v[0];
+        l.first[0][x] = at.v[1];
+        l.first[1][x] = at.v[2];
+    }
+    if (x == E)
+    {
+        l.start[E + 1] = at.v[0] + c;
+        l.first[0][E + 1] = at.v[1] + (c + ROWS - 1) / ROWS;
+        l.first[1][E + 1] = at.v[2] + (c + FEW_ROWS - 1) / FEW_ROWS;
+    }
+    return at.v[0];
+}
+
+// Both lists, of places that are there for every thread to read.
+__device__ __forceinline__ void write_tiles(const PlanLds& l, int E, GroupTile* tiles, GroupTile* few, int32_t* ntiles)
+{
+    const int n0 = l.first[0][E + 1], n1 = l.first[1][E + 1];
+    if (threadIdx.x < 2) ntiles[threadIdx.x] = threadIdx.x ? n1 : n0;
+    for (int j = threadIdx.x; j < n0 + n1; j += 1024)
+    {
+        const int list = j >= n0, i = list ? j - n0 : j;
+        const int* first = l.first[list];
+        // the expert (E: none) whose tiles i is among
+        int e = 0;
+        for (int step = 1024; step; step >>= 1)
+            if (e + step <= E && first[e + step] <= i) e += step;
+        const int cnt = first[e + 1] - first[e], r0 = l.start[e], n = l.start[e + 1] - r0, k = i - first[e];
+        const int at = (int)((long long)n * k / cnt), to = (int)((long long)n * (k + 1) / cnt);
+        (list ? few : tiles)[i] = { e < E ? e : -1, r0 + at, to - at, first[e], cnt, (n + cnt - 1) / cnt, { 0, 0 } };
     }
 }
 
@@ -136,7 +154,12 @@ __global__ __launch_bounds__(1024) void k_group_tiles(const int32_t* __restrict_
                                                       int32_t* __restrict__ ntiles)
 {
     __shared__ PlanLds l;
-    for (int i = threadIdx.x; i < E + 2; i += 1024) l.start[i] = offsets[i];
+    Sums run = {};
+    for (int base = 0; base <= E; base += 1024)
+    {
+        const int x = base + threadIdx.x;
+        place_expert(l, x, x <= E ? offsets[x + 1] - offsets[x] : 0, E, run);
+    }
     __syncthreads();
     write_tiles(l, E, tiles, few, ntiles);
 }
@@ -182,33 +205,30 @@ __global__ __launch_bounds__(1024) void k_group_plan(const int64_t* __restrict__
         __builtin_amdgcn_wave_barrier();
     }
     __syncthreads();
-    int run = 0;
+    Sums run = {};
     for (int base = 0; base <= E; base += 1024)
     {
         const int x = base + t;
-        int c = 0;
-        if (x <= E)
-            for (int w = 0; w < 16; ++w)
-            {
-                const int h = hist[w][x];
-                hist[w][x] = (uint16_t)c;
-                c += h;
-            }
-        int total;
-        const int at = run + scan_1024(c, l.part, total);
+        int h[16], c = 0;
         if (x <= E)
         {
-            l.start[x] = at;
+#pragma unroll
+            for (int w = 0; w < 16; ++w) h[w] = hist[w][x];
+#pragma unroll
+            for (int w = 0; w < 16; ++w)
+            {
+                hist[w][x] = (uint16_t)c;
+                c += h[w];
+            }
+        }
+        const int at = place_expert(l, x, c, E, run);
+        if (x <= E)
+        {
             offsets[x] = at;
             counts[x] = c;
         }
-        run += total;
     }
-    if (t == 0)
-    {
-        l.start[E + 1] = n;
-        offsets[E + 1] = n;
-    }
+    if (t == 0) offsets[E + 1] = n;
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < PLAN_ROUNDS; ++r)
@@ -396,12 +416,14 @@ struct Across
 // One workgroup of eight waves a CU, or two of four.
 template <int C>
 constexpr int LDS_BYTES = C == 256 ? 160 * 1024 : 76 * 1024;
-template <int R, int C>
+template <int R, int C, bool FAR = false>
 struct Shape
 {
     static constexpr int WAVES = C / 32, WN = R > 64 ? 4 : WAVES, WM = WAVES / WN, MB = std::max(1, R / 16 / WM), NB = C / 16 / WN;
-    // places in LDS for blocks of the rows and of the columns: these are the weights, which come from farther away when tiles have few rows
-    static constexpr int SM = R > 64 ? 2 : 3, SN = R > 192 ? 2 : R > 128 || (C == 128 && R == 64) ? 3 : 4;
+    // Places in LDS for blocks of the rows and of the columns: these are the weights, which come from farther away where tiles have few rows, and
+    // FAR, where no other tile reads them (98,304 rows of 384 experts, 256 each: 3,300 us with two places, 3,180 with three; 131,072 of 8
+    // experts: 3,389 and 3,461).
+    static constexpr int SM = R > 64 ? 2 : 3, SN = R > 192 ? (FAR ? 3 : 2) : R > 128 || (C == 128 && R == 64) ? 3 : 4;
     static constexpr int MSTAGE = R * 128, NSTAGE = C * 128, LDS = SM * MSTAGE + SN * NSTAGE;
     static_assert(LDS <= LDS_BYTES<C> && SN >= SM, "LDS");
 };
@@ -578,10 +600,10 @@ __device__ __forceinline__ int tile_of_block(int b)
     return ((i >> 5) * 8 + x) * 32 + (i & 31);
 }
 
-template <int XT, bool ACROSS, int R, int C>
+template <int XT, bool ACROSS, int R, int C, bool FAR = false>
 __device__ __forceinline__ void rows_tile(const RowsArgs& a, const GroupTile& t, int ct, unsigned char* lds)
 {
-    using S = Shape<R, C>;
+    using S = Shape<R, C, FAR>;
     using M = Along<R, S::WAVES>;
     using N = std::conditional_t<ACROSS, Across<TERMS, C, S::WAVES>, Along<C, S::WAVES>>;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -630,6 +652,11 @@ __global__ __launch_bounds__(2 * C, 2) void k_group_rows(RowsArgs a)
     if (t.expert < 0) return zero_tile<C>(a, t, ct);
     if constexpr (C == 256)
     {
+        if (t.count == 1 && t.size > 192)
+        {
+            if (t.size > 224) return rows_tile<XT, ACROSS, 256, C, true>(a, t, ct, lds);
+            return rows_tile<XT, ACROSS, 224, C, true>(a, t, ct, lds);
+        }
         if (t.size > 224) return rows_tile<XT, ACROSS, 256, C>(a, t, ct, lds);
         if (t.size > 192) return rows_tile<XT, ACROSS, 224, C>(a, t, ct, lds);
         if (t.size > 160) return rows_tile<XT, ACROSS, 192, C>(a, t, ct, lds);
