@@ -544,8 +544,16 @@ __device__ __forceinline__ void store(f4_t (&acc)[S::MB][S::NB], void* y, int ty
         trade_rows(a, b, low);
         const int m = m0 + 16 * i + (r & 7), c = low ? n : n + step;
         unsigned char* at = static_cast<unsigned char*>(y) + ((row0 + m) * ld + c) * size;
-        if (FULL || (m < rows && c < cols)) *reinterpret_cast<u4_t*>(at) = a;
-        if (FULL || (m + 8 < rows && c < cols)) *reinterpret_cast<u4_t*>(at + 8 * ld * size) = b;
+        if constexpr (FULL)
+        {
+            __builtin_nontemporal_store(a, reinterpret_cast<u4_t*>(at));
+            __builtin_nontemporal_store(b, reinterpret_cast<u4_t*>(at + 8 * ld * size));
+        }
+        else
+        {
+            if (m < rows && c < cols) *reinterpret_cast<u4_t*>(at) = a;
+            if (m + 8 < rows && c < cols) *reinterpret_cast<u4_t*>(at + 8 * ld * size) = b;
+        }
     };
 #pragma unroll
     for (int i = 0; i < S::MB; ++i)
@@ -789,6 +797,25 @@ struct WTile
     }
 };
 
+// Waits until at most `blocks` blocks of L loads are out (up to 4), and with `stores` STORES stores behind them.
+template <int L, int STORES>
+__device__ __forceinline__ void wait_blocks(int blocks, bool stores)
+{
+    if (stores)
+    {
+        if (blocks >= 4) wait_vmcnt<4 * L + STORES>();
+        else if (blocks == 3) wait_vmcnt<3 * L + STORES>();
+        else if (blocks == 2) wait_vmcnt<2 * L + STORES>();
+        else if (blocks == 1) wait_vmcnt<L + STORES>();
+        else wait_vmcnt<STORES>();
+    }
+    else if (blocks == 3) wait_vmcnt<3 * L>();
+    else if (blocks >= 4) wait_vmcnt<4 * L>();
+    else if (blocks == 2) wait_vmcnt<2 * L>();
+    else if (blocks == 1) wait_vmcnt<L>();
+    else wait_vmcnt<0>();
+}
+
 template <int XT, int PICK>
 __global__ __launch_bounds__(512, 2) void k_group_weights(WeightsArgs a)
 {
@@ -816,18 +843,14 @@ __global__ __launch_bounds__(512, 2) void k_group_weights(WeightsArgs a)
         if (blocks)
         {
             // a block has come once only the loads after it are out, and the stores behind the first W_STAGES blocks
-            if (blocks < W_STAGES) wait_vmcnt<0>();
-            else if (behind) wait_vmcnt<(W_STAGES - 1) * L + STORES<S>>();
-            else wait_vmcnt<(W_STAGES - 1) * L>();
+            wait_blocks<L, STORES<S>>(min(blocks, W_STAGES) - 1, behind);
             lds_barrier();
             Half<S> h0, h1;
             read_half<Terms, Terms, S>(h0, lds, lds + Terms::BYTES, mp, np, 0);
             int at = 0;
             // block b is multiplied while block b + 1 comes from LDS; loads run five blocks ahead
             auto step = [&](const Half<S>& cur, Half<S>& next, int b) {
-                if (b + W_STAGES > blocks) wait_vmcnt<0>();
-                else if (behind && b + 1 < W_STAGES) wait_vmcnt<(W_STAGES - 2) * L + STORES<S>>();
-                else wait_vmcnt<(W_STAGES - 2) * L>();
+                wait_blocks<L, STORES<S>>(min(blocks - b - 2, W_STAGES - 2), behind && b + 1 < W_STAGES);
                 lds_barrier();
                 if (b + W_STAGES < blocks) t.load(a, lds + at, b + W_STAGES);
                 at = at + W_STAGE == W_STAGES * W_STAGE ? 0 : at + W_STAGE;
