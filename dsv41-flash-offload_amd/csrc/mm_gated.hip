@@ -25,7 +25,7 @@ struct GatedArgs
     int8_t *codes, *exps;
     uint16_t *h, *dgu;
     float* dweights;
-    int I;
+    int n, I;
     float limit;                       // infinite: no clamp
 };
 
@@ -85,7 +85,8 @@ __device__ __forceinline__ float within(float v, float l) { return v > l ? l : v
 template <int XT, bool SAVE>
 __global__ __launch_bounds__(256) void k_gated(GatedArgs a)
 {
-    const size_t row = blockIdx.x;
+    const size_t row = (size_t)blockIdx.y * gridDim.x + blockIdx.x;
+    if (row >= (size_t)a.n) return;
     const bool live = !a.live || (int)row < *a.live;
     const float w = !live ? 0.f : a.weights ? a.weights[a.order ? a.order[row] : row] : 1.f;
     for (int base = 0; base < a.I; base += 8 * blockDim.x)
@@ -130,7 +131,8 @@ template <int XT, bool SAVED>
 __global__ __launch_bounds__(256) void k_gated_backward(GatedArgs a)
 {
     __shared__ float part[4];
-    const size_t row = blockIdx.x;
+    const size_t row = (size_t)blockIdx.y * gridDim.x + blockIdx.x;
+    if (row >= (size_t)a.n) return;
     const bool live = !a.live || (int)row < *a.live;
     const int route = a.order ? a.order[row] : (int)row;
     const float w = !live ? 0.f : a.weights ? a.weights[route] : 1.f;
@@ -195,7 +197,7 @@ int check(const char* what, const mm_group_plan_t* p, int dtype, int n, int I, f
     MM_CHECK_ARG(!p || (p->offsets && p->order), "%s: incomplete plan", what);
     MM_CHECK_ARG(!p || (p->T > 0 && p->topk > 0 && p->E > 0 && p->E <= 1024 && (long long)p->T * p->topk == n), "%s: the plan has other rows", what);
     MM_CHECK_ARG(dtype == MM_DTYPE_F16 || dtype == MM_DTYPE_BF16, "%s: rows must be fp16 or bf16", what);
-    MM_CHECK_ARG(n > 0 && I > 0 && I % 8 == 0 && I <= 1 << 20, "%s: need rows, I a multiple of 8 and at most 2^20 (n %d, I %d)", what, n, I);
+    MM_CHECK_ARG(n > 0 && n <= 1 << 30 && I > 0 && I % 8 == 0 && I <= 1 << 20, "%s: need 1 to 2^30 rows, I a multiple of 8 and at most 2^20 (n %d, I %d)", what, n, I);
     MM_CHECK_ARG(limit >= 0.f, "%s: negative limit", what);
     MM_CHECK_ARG(!codes == !exps, "%s: codes and exponents go together", what);
     MM_CHECK_ARG(!codes || I % SAVE_GROUP == 0, "%s: 8 bits need I a multiple of 32 (I %d)", what, I);
@@ -203,17 +205,24 @@ int check(const char* what, const mm_group_plan_t* p, int dtype, int n, int I, f
     return MM_OK;
 }
 
-GatedArgs args(const mm_group_plan_t* p, int I, const float* weights, float limit)
+GatedArgs args(const mm_group_plan_t* p, int n, int I, const float* weights, float limit)
 {
     GatedArgs a = {};
     a.weights = weights;
     a.order = p ? p->order : nullptr;
     a.live = p ? p->offsets + p->E : nullptr;
+    a.n = n;
     a.I = I;
     a.limit = limit == 0.f ? INFINITY : limit;
     return a;
 }
 
+// a row each; a launch has less than 2^32 threads in a dimension
+dim3 grid(int n)
+{
+    const int x = n < 1 << 20 ? n : 1 << 20;
+    return dim3((unsigned)x, (unsigned)(((long long)n + x - 1) / x));
+}
 dim3 threads(int I) { return dim3(I >= 2048 ? 256 : (I + 511) / 512 * 64); }
 
 }  // namespace
@@ -226,14 +235,14 @@ int mm_gated(const mm_group_plan_t* plan, const void* gu, int dtype, int n, int 
     if (const int rc = check("mm_gated", plan, dtype, n, I, limit, codes, exps)) return rc;
     MM_CHECK_ARG(gu && h, "mm_gated: null pointer");
     MM_CHECK_ARG(at(gu, 16) && at(h, 16), "mm_gated: misaligned pointer");
-    GatedArgs a = args(plan, I, weights, limit);
+    GatedArgs a = args(plan, n, I, weights, limit);
     a.gu = static_cast<const uint16_t*>(gu);
     a.h = static_cast<uint16_t*>(h);
     a.codes = codes;
     a.exps = exps;
     const bool f = dtype == MM_DTYPE_F16;
     auto kernel = codes ? (f ? k_gated<MM_DTYPE_F16, true> : k_gated<MM_DTYPE_BF16, true>) : (f ? k_gated<MM_DTYPE_F16, false> : k_gated<MM_DTYPE_BF16, false>);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)n), threads(I), 0, reinterpret_cast<hipStream_t>(stream), a);
+    hipLaunchKernelGGL(kernel, grid(n), threads(I), 0, reinterpret_cast<hipStream_t>(stream), a);
     return check_launch("mm_gated");
 }
 
@@ -243,7 +252,7 @@ int mm_gated_backward(const mm_group_plan_t* plan, const void* dh, const void* g
     if (const int rc = check("mm_gated_backward", plan, dtype, n, I, limit, codes, exps)) return rc;
     MM_CHECK_ARG(dh && dgu && !gu != !codes, "mm_gated_backward: null pointer, or both forms of the rows");
     MM_CHECK_ARG(at(dh, 16) && at(gu, 16) && at(dgu, 16) && at(h, 16), "mm_gated_backward: misaligned pointer");
-    GatedArgs a = args(plan, I, weights, limit);
+    GatedArgs a = args(plan, n, I, weights, limit);
     a.dh = static_cast<const uint16_t*>(dh);
     a.gu = static_cast<const uint16_t*>(gu);
     a.codes_in = codes;
@@ -254,7 +263,7 @@ int mm_gated_backward(const mm_group_plan_t* plan, const void* dh, const void* g
     const bool f = dtype == MM_DTYPE_F16;
     auto kernel = codes ? (f ? k_gated_backward<MM_DTYPE_F16, true> : k_gated_backward<MM_DTYPE_BF16, true>)
                         : (f ? k_gated_backward<MM_DTYPE_F16, false> : k_gated_backward<MM_DTYPE_BF16, false>);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)n), threads(I), 0, reinterpret_cast<hipStream_t>(stream), a);
+    hipLaunchKernelGGL(kernel, grid(n), threads(I), 0, reinterpret_cast<hipStream_t>(stream), a);
     return check_launch("mm_gated_backward");
 }
 

@@ -258,6 +258,8 @@ __device__ __forceinline__ int lane_here()
     asm volatile("" : "+v"(lane));
     return lane;
 }
+// Loads and stores before it are sent before those after it: waits for memory count what was sent since.
+__device__ __forceinline__ void keep_order() { asm volatile("" ::: "memory"); }
 constexpr uint32_t NOWHERE = 0xfffffff0u;              // past every buffer: reads zero
 
 // Rows of TERMS terms, R of them, loaded by W waves; LDS [R][64]. A wave's load is 8 rows of 128 bytes. Tiles of fewer rows than the waves
@@ -481,7 +483,9 @@ __device__ __forceinline__ void run(unsigned char* lds, const M& m, const N& n, 
     {
         const int bm = b - (SN - SM);
         if (bm >= 0 && bm < blocks) m.load(ml + bm * S::MSTAGE, bm, terms);
+        keep_order();
         if (b < blocks) n.load(nl + b * S::NSTAGE, b, terms);
+        keep_order();
     }
     // block 0 has come once only what was sent after it is out
     if (blocks >= SN) wait_vmcnt<AFTER + (SM - 1) * EACH>();
@@ -502,7 +506,7 @@ __device__ __forceinline__ void run(unsigned char* lds, const M& m, const N& n, 
         else wait_vmcnt<0>();
         lds_barrier();
         if (b + SM < blocks) m.load(ml + am, b + SM, terms);
-        asm volatile("" ::: "memory");
+        keep_order();
         if (b + SN < blocks) n.load(nl + an, b + SN, terms);
         am = am + S::MSTAGE == SM * S::MSTAGE ? 0 : am + S::MSTAGE;
         an = an + S::NSTAGE == SN * S::NSTAGE ? 0 : an + S::NSTAGE;
@@ -793,7 +797,10 @@ struct WTile
     {
 #pragma unroll
         for (int b = 0; b < W_STAGES; ++b)
+        {
             if (b < blocks) load(a, lds + b * W_STAGE, b);
+            keep_order();
+        }
     }
 };
 
@@ -881,11 +888,11 @@ __global__ __launch_bounds__(512, 2) void k_group_weights(WeightsArgs a)
             lds_barrier();             // every wave has read the last block
             t.first_loads(a, lds);
         }
-        asm volatile("" ::: "memory");                     // loads first: the waits count on it
+        keep_order();                  // the stores behind the loads
         behind = rows == ROWS && col0 + COLS <= a.K && a.type != MM_DTYPE_F32;
         if (behind) store<XT, S, true>(acc, a.dw, a.type, row, rows, col0, a.K, a.K);
         else store<XT, S>(acc, a.dw, a.type, row, rows, col0, a.K, a.K);
-        asm volatile("" ::: "memory");
+        keep_order();
         if (!more) return;
     }
 }
@@ -897,25 +904,27 @@ template <int OT>
 __global__ __launch_bounds__(256) void k_group_sum(const float* __restrict__ rows, const int32_t* __restrict__ inv, const int32_t* __restrict__ live,
                                                    long long n4, int topk, int cols4, void* __restrict__ out)
 {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n4) return;
-    const long long t = i / cols4;
-    const int c = (int)(i - t * cols4), end = *live;
-    f4_t s = f4_t{ 0.f, 0.f, 0.f, 0.f };
-    for (int j = 0; j < topk; ++j)
+    const int end = *live;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n4; i += (long long)gridDim.x * 256)
     {
-        const int p = inv[t * topk + j];
-        if (p < end)
+        const long long t = i / cols4;
+        const int c = (int)(i - t * cols4);
+        f4_t s = f4_t{ 0.f, 0.f, 0.f, 0.f };
+        for (int j = 0; j < topk; ++j)
         {
-            const f4_t v = reinterpret_cast<const f4_t*>(rows)[(size_t)p * cols4 + c];
-            s.x += v.x;
-            s.y += v.y;
-            s.z += v.z;
-            s.w += v.w;
+            const int p = inv[t * topk + j];
+            if (p < end)
+            {
+                const f4_t v = reinterpret_cast<const f4_t*>(rows)[(size_t)p * cols4 + c];
+                s.x += v.x;
+                s.y += v.y;
+                s.z += v.z;
+                s.w += v.w;
+            }
         }
+        if constexpr (OT == MM_DTYPE_F32) reinterpret_cast<f4_t*>(out)[i] = s;
+        else reinterpret_cast<u2_t*>(out)[i] = u2_t{ pack2<OT>(s.x, s.y), pack2<OT>(s.z, s.w) };
     }
-    if constexpr (OT == MM_DTYPE_F32) reinterpret_cast<f4_t*>(out)[i] = s;
-    else reinterpret_cast<u2_t*>(out)[i] = u2_t{ pack2<OT>(s.x, s.y), pack2<OT>(s.z, s.w) };
 }
 
 }  // namespace mm
@@ -924,15 +933,15 @@ using namespace mm;
 
 namespace {
 
-constexpr long long MOST_BLOCKS = 0x7fffffffLL;
+constexpr long long MOST_ROUTES = 1LL << 30, MOST_THREADS = (1LL << 32) - 1;      // of a launch
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-// Checks that the products share; routes in *n.
+// Checks that the products share.
 int check(const char* what, const mm_group_plan_t* p, int dtype, int K, int N, int out_type)
 {
     MM_CHECK_ARG(p && p->offsets && p->order && p->token && p->inv && p->tiles && p->ntiles, "%s: incomplete plan", what);
-    MM_CHECK_ARG(p->T > 0 && p->topk > 0 && p->E > 0 && p->E <= 1024 && (long long)p->T * p->topk < (1LL << 31) - 256, "%s: bad plan", what);
+    MM_CHECK_ARG(p->T > 0 && p->topk > 0 && p->E > 0 && p->E <= 1024 && (long long)p->T * p->topk <= MOST_ROUTES, "%s: bad plan", what);
     MM_CHECK_ARG(dtype == MM_DTYPE_F16 || dtype == MM_DTYPE_BF16, "%s: rows and weights must be fp16 or bf16", what);
     MM_CHECK_ARG(out_type == dtype || out_type == MM_DTYPE_F32, "%s: results must have the weights' type or fp32", what);
     MM_CHECK_ARG(K > 0 && N > 0 && K % 8 == 0 && N % 8 == 0 && K <= 1 << 20 && N <= 1 << 20 && (long long)K * N < 1LL << 31,
@@ -974,7 +983,7 @@ int launch_rows(const char* what, const mm_group_plan_t* p, const void* x, const
     a.ntiles = p->ntiles + (most == FEW_ROWS);
     a.colt = (cols + width - 1) / width;
     const long long tiles = tile_capacity(n, p->E, most) * a.colt, blocks = (tiles + 255) / 256 * 256;
-    MM_CHECK_ARG(blocks <= MOST_BLOCKS, "%s: too many tiles", what);
+    MM_CHECK_ARG(blocks * (few || small ? 256 : 512) <= MOST_THREADS, "%s: too many tiles", what);
     const bool h = dtype == MM_DTYPE_F16;
     if (few) hipLaunchKernelGGL((h ? k_group_few<MM_DTYPE_F16> : k_group_few<MM_DTYPE_BF16>), dim3((unsigned)blocks), dim3(256), 0, hs, a);
     else if (small) hipLaunchKernelGGL((h ? k_group_rows<MM_DTYPE_F16, ACROSS, 128> : k_group_rows<MM_DTYPE_BF16, ACROSS, 128>), dim3((unsigned)blocks), dim3(256), 0, hs, a);
@@ -982,9 +991,8 @@ int launch_rows(const char* what, const mm_group_plan_t* p, const void* x, const
     if (reduce)
     {
         const long long n4 = (long long)p->T * cols / 4;
-        MM_CHECK_ARG((n4 + 255) / 256 <= MOST_BLOCKS, "%s: too many tokens", what);
         auto sum = y_type == MM_DTYPE_F32 ? k_group_sum<MM_DTYPE_F32> : y_type == MM_DTYPE_F16 ? k_group_sum<MM_DTYPE_F16> : k_group_sum<MM_DTYPE_BF16>;
-        hipLaunchKernelGGL(sum, dim3((unsigned)((n4 + 255) / 256)), dim3(256), 0, hs, static_cast<const float*>(ws), p->inv, p->offsets + p->E, n4,
+        hipLaunchKernelGGL(sum, dim3((unsigned)std::min<long long>((n4 + 255) / 256, 1 << 22)), dim3(256), 0, hs, static_cast<const float*>(ws), p->inv, p->offsets + p->E, n4,
                            p->topk, cols / 4, y);
     }
     return check_launch(what);
@@ -1002,8 +1010,8 @@ size_t mm_group_tiles(int n, int E)
 int mm_group_plan(const int64_t* ids, const mm_group_plan_t* p, int32_t* counts, void* workspace, size_t workspace_bytes, mm_stream_t stream)
 {
     MM_CHECK_ARG(p && p->offsets && p->order && p->token && p->inv && p->tiles && p->ntiles && counts && ids, "mm_group_plan: null pointer");
-    MM_CHECK_ARG(p->T > 0 && p->topk > 0 && p->E > 0 && p->E <= 1024 && (long long)p->T * p->topk < (1LL << 31) - 256,
-                 "mm_group_plan: need tokens, picks, 1 <= E <= 1024 and fewer than 2^31 - 256 routes");
+    MM_CHECK_ARG(p->T > 0 && p->topk > 0 && p->E > 0 && p->E <= 1024 && (long long)p->T * p->topk <= MOST_ROUTES,
+                 "mm_group_plan: need tokens, picks, 1 <= E <= 1024 and at most 2^30 routes");
     MM_CHECK_ARG(aligned16(p->tiles), "mm_group_plan: misaligned tiles");
     const int n = p->T * p->topk;
     const hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
@@ -1066,7 +1074,7 @@ int mm_group_linear_weights(const mm_group_plan_t* plan, const void* dy, const v
     a.rowt = (N + ROWS - 1) / ROWS;
     a.colt = (K + COLS - 1) / COLS;
     const long long tiles = (long long)plan->E * a.rowt * a.colt;
-    MM_CHECK_ARG(tiles <= MOST_BLOCKS - 512, "mm_group_linear_weights: too many tiles");
+    MM_CHECK_ARG(tiles <= 1LL << 30, "mm_group_linear_weights: too many tiles");
     const unsigned blocks = 256;             // one a CU
     const bool h = dtype == MM_DTYPE_F16;
     auto kernel = gather ? (h ? k_group_weights<MM_DTYPE_F16, 2> : k_group_weights<MM_DTYPE_BF16, 2>)

@@ -43,8 +43,7 @@ class DenseStore:
 
 class _Moe(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, w13, w2, ids, limit, save8):
-        keep = any(ctx.needs_input_grad)
+    def forward(ctx, x, w, w13, w2, ids, limit, save8, keep):
         plan = grouped.Plan(ids, w13.shape[0])
         gu = grouped.linear_forward(x, w13.flatten(1, 2), plan, gather=True)
         h, kept = grouped.swiglu_forward(gu, plan, w, limit, save8 and keep)
@@ -70,7 +69,7 @@ class _Moe(torch.autograd.Function):
             _, d2 = grouped.linear_backward(dout, h, w2, plan, reduce=True, need_x=False)
         if need_x or need_13:
             dx, d13 = grouped.linear_backward(dgu, x, up, plan, gather=True, need_x=need_x, need_w=need_13)
-        return dx, dw, None if d13 is None else d13.view_as(w13), d2, None, None, None
+        return dx, dw, None if d13 is None else d13.view_as(w13), d2, None, None, None, None
 
 
 def moe(store, x, ids, w, shared_expert=None, stream=None):
@@ -95,5 +94,7 @@ def moe(store, x, ids, w, shared_expert=None, stream=None):
         if shared >= 0:
             ids = torch.cat([ids, torch.full((T, 1), shared, dtype=torch.long, device=dev)], 1)
             w = torch.cat([w, torch.ones((T, 1), dtype=torch.float32, device=dev)], 1)
-        return _captured_apply("dense.moe", _Moe, (x, w, store.w13, store.w2), x, w, store.w13, store.w2, ids, store.limit, store.save8,
+        leaves = (x, w, store.w13, store.w2)
+        keep = torch.is_grad_enabled() and any(t.requires_grad for t in leaves)
+        return _captured_apply("dense.moe", _Moe, leaves, *leaves, ids, store.limit, store.save8, keep,
                                instead="the *_forward and *_backward functions of grouped")

@@ -32,8 +32,8 @@ class Plan:
             raise ValueError(f"Plan: need 1 <= E <= 1024 (got {E})")
         (self.T, self.k), self.E, dev = ids.shape, int(E), ids.device
         n = self.n = self.T * self.k
-        if n >= 2 ** 31 - 256:
-            raise ValueError(f"Plan: {n} routes, fewer than 2^31 - 256 expected")
+        if n > 2 ** 30:
+            raise ValueError(f"Plan: {n} routes, at most 2^30 expected")
         _lib.check_tensors("Plan", dev)
         with _lib.on(dev, stream):
             lib = _lib.load()

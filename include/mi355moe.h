@@ -311,7 +311,7 @@ int mm_w4_moe(const mm_w4_layer_t* layer, const void* x, int x_dtype, int T, int
 
 /* The order of a call's routes that the grouped products share: T tokens of topk picks each, sorted by expert (stable), picks
  * outside [0, E) last. Device memory: offsets int32 [E + 2] (rows offsets[e] .. offsets[e + 1] - 1 belong to expert e, rows from
- * offsets[E] on to none), order int32 [n] (flat route of each row, n = T topk < 2^31 - 256), token int32 [n] (order / topk), inv int32 [n]
+ * offsets[E] on to none), order int32 [n] (flat route of each row, n = T topk <= 2^30), token int32 [n] (order / topk), inv int32 [n]
  * (row of each route), tiles (mm_group_tiles(n, E) bytes, 16-byte aligned) and ntiles int32 [2], the kernels' own. E <= 1024. */
 typedef struct mm_group_plan
 {
@@ -330,7 +330,8 @@ int mm_group_plan(const int64_t* ids, const mm_group_plan_t* plan, int32_t* coun
 /* y[p] = W[e] x[p] over the rows p of each expert e: w [E][N][K] and x in dtype (fp16 or bf16), y in dtype or fp32, sums in fp32,
  * rounded once. gather: x is [T][K] and row p reads row token[p], else [n][K]. reduce: y is [T][N], the sum of each token's rows in the order
  * of its picks (from fp32 rows in the workspace: mm_group_linear_workspace(T, topk, N, reduce) bytes); else [n][N], rows of no expert
- * zero. K and N multiples of 8, at most 2^20, K N < 2^31; tensors of rows per token below 4 GiB; all pointers 16-byte aligned. */
+ * zero. K and N multiples of 8, at most 2^20, K N < 2^31; tensors of rows per token below 4 GiB; tiles of a call within one launch (2^32
+ * threads: 2^30 rows of 1,024 columns, say); all pointers 16-byte aligned. Sums are in an order of the call's sizes: a call repeats bit for bit. */
 size_t mm_group_linear_workspace(int T, int topk, int cols, int reduce);
 int mm_group_linear(const mm_group_plan_t* plan, const void* x, const void* w, int dtype, int K, int N, int gather, int reduce,
                     void* y, int y_dtype, void* workspace, size_t workspace_bytes, mm_stream_t stream);

@@ -335,8 +335,8 @@ def test_8_bits_hold_what_they_say(dev, dtype):
     top = x.double().unflatten(1, (-1, 32)).abs().amax(-1, keepdim=True).expand(-1, -1, 32).flatten(1)
     assert ((values - x.double()).abs()[fine] <= (top / 127).clamp(min=2.0 ** -127)[fine]).all()
     dgu, _, _ = grouped.swiglu_backward(torch.ones((len(tops) + 2, 32), dtype=dtype, device=dev), kept)
-    assert dgu[-1, 32:].isnan().logical_not().all() or dgu[-1].isnan().any()      # no fault; NaN values give NaN gradients
-    assert dgu[:-2].isfinite().logical_or(torch.tensor(tops[:len(tops)]).to(dev)[:, None] > 1e4).all()
+    # a gate of NaN passes into du, an up of NaN into dg; their own derivatives are cut
+    assert dgu[:-2].isfinite().all() and dgu[-2, 32:].isnan().all() and dgu[-1, :32].isnan().all()
 
 
 def test_clamps_keep_nan_and_cut_gradients(dev):

@@ -115,7 +115,7 @@ def test_c_argument_errors():
     err(L.mm_group_plan(None, p(), 256, None, 0, None), b"null")
     err(L.mm_group_plan(256, p(T=0), 256, None, 0, None), b"need tokens")
     err(L.mm_group_plan(256, p(E=1025), 256, None, 0, None), b"E <= 1024")
-    err(L.mm_group_plan(256, p(T=1 << 28, k=8), 256, None, 0, None), b"2^31")
+    err(L.mm_group_plan(256, p(T=1 << 28, k=8), 256, None, 0, None), b"2^30")
     err(L.mm_group_plan(256, p(tiles=264), 256, None, 0, None), b"misaligned")
     err(L.mm_group_plan(256, p(T=1 << 16), 256, None, 0, None), b"workspace")
     row = [256, 256, 1, 16, 24, 0, 0, 256, 1, None, 0, None]
@@ -155,7 +155,7 @@ def test_c_argument_errors():
         a[at] = value
         err(L.mm_gated(p(), *a), text)
     err(L.mm_gated(p(), 256, 1, 8, 40, None, 10.0, 256, 256, 256, None), b"multiple of 32")
-    err(L.mm_gated(None, 256, 1, 0, 32, None, 10.0, 256, None, None, None), b"need rows")
+    err(L.mm_gated(None, 256, 1, 0, 32, None, 10.0, 256, None, None, None), b"2^30 rows")
     b = [256, 256, None, None, 1, 8, 32, None, 10.0, 256, None, None, None]
     for at, value, text in [(0, None, b"null"), (1, None, b"null"), (9, None, b"null"), (4, 3, b"fp16 or bf16"), (11, 264, b"misaligned"), (2, 256, b"go together")]:
         a = list(b)
