@@ -150,97 +150,173 @@ __device__ __forceinline__ void write_tiles(const PlanLds& l, int E, GroupTile* 
     }
 }
 
-__global__ __launch_bounds__(1024) void k_group_tiles(const int32_t* __restrict__ offsets, int E, GroupTile* __restrict__ tiles, GroupTile* __restrict__ few,
-                                                      int32_t* __restrict__ ntiles)
+// A workgroup's run of routes: a wave takes a part of it, 64 routes at a time. Lanes that hold the same expert find each other by one ballot per
+// bit, so that a route's place among its expert's is the wave's count so far and the lanes before it; counts of the waves before come on top.
+constexpr int PLAN_ROUNDS = 8, PLAN_ROUTES = 1024 * PLAN_ROUNDS;      // of a workgroup
+struct RouteLds
+{
+    uint16_t hist[16][1026];
+};
+struct Routes
+{
+    int e[PLAN_ROUNDS], p[PLAN_ROUNDS], s0, rounds, end;
+    __device__ __forceinline__ int route(int r) const { return s0 + 64 * r; }
+    // routes s .. end - 1, at most PLAN_ROUTES; every thread of the workgroup takes part
+    __device__ __forceinline__ void init(RouteLds& l, const int64_t* __restrict__ ids, int s, int to, int E, int bits)
+    {
+        const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+        rounds = (to - s + 1023) / 1024;
+        s0 = s + wave * rounds * 64 + lane;
+        end = to;
+#pragma unroll
+        for (int r = 0; r < PLAN_ROUNDS; ++r)
+        {
+            const int64_t id = r < rounds && route(r) < end ? ids[route(r)] : 0;
+            e[r] = id >= 0 && id < E ? (int)id : E;
+        }
+        for (int i = t; i < 16 * 1026 / 2; i += 1024) reinterpret_cast<uint32_t*>(l.hist)[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < PLAN_ROUNDS; ++r)
+        {
+            if (r >= rounds) break;
+            const bool in = route(r) < end;
+            uint64_t same = __ballot(in);
+            for (int b = 0; b < bits; ++b)
+            {
+                const uint64_t one = __ballot((e[r] >> b) & 1);
+                same &= (e[r] >> b) & 1 ? one : ~one;
+            }
+            const int before = __popcll(same & ((1ull << lane) - 1)), had = l.hist[wave][e[r]];
+            __builtin_amdgcn_wave_barrier();
+            p[r] = had + before;
+            if (in && before == 0) l.hist[wave][e[r]] = (uint16_t)(had + __popcll(same));
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+        __syncthreads();
+    }
+    // the waves' counts of expert x as the count of the waves before each; returns their sum
+    __device__ __forceinline__ static int count(RouteLds& l, int x)
+    {
+        int h[16], c = 0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) h[w] = l.hist[w][x];
+#pragma unroll
+        for (int w = 0; w < 16; ++w)
+        {
+            l.hist[w][x] = (uint16_t)c;
+            c += h[w];
+        }
+        return c;
+    }
+    // start(e): the row of the workgroup's first route of expert e
+    template <typename Start>
+    __device__ __forceinline__ void write(const RouteLds& l, int topk, const Start& start, int32_t* order, int32_t* token, int32_t* inv) const
+    {
+        const int wave = threadIdx.x >> 6;
+#pragma unroll
+        for (int r = 0; r < PLAN_ROUNDS; ++r)
+        {
+            const int s = route(r);
+            if (r >= rounds || s >= end) break;
+            const int at = start(e[r]) + l.hist[wave][e[r]] + p[r];
+            order[at] = s;
+            token[at] = s / topk;
+            inv[s] = at;
+        }
+    }
+};
+
+struct PlanArgs
+{
+    const int64_t* ids;
+    int32_t *counts, *offsets, *order, *token, *inv, *ntiles;
+    GroupTile *tiles, *few;
+    int32_t* hist;              // [workgroups][E + 1]
+    int n, topk, E, bits, run, groups;       // run: routes of a workgroup
+};
+
+// The whole plan in one workgroup and launch (701 tokens of 4 picks: 6.6 us; as a permutation and its tiles 21).
+__global__ __launch_bounds__(1024) void k_group_plan(PlanArgs a)
 {
     __shared__ PlanLds l;
+    __shared__ RouteLds h;
+    Routes q;
+    q.init(h, a.ids, 0, a.n, a.E, a.bits);
     Sums run = {};
-    for (int base = 0; base <= E; base += 1024)
+    for (int base = 0; base <= a.E; base += 1024)
     {
-        const int x = base + threadIdx.x;
-        place_expert(l, x, x <= E ? offsets[x + 1] - offsets[x] : 0, E, run);
+        const int x = base + threadIdx.x, c = x <= a.E ? Routes::count(h, x) : 0, at = place_expert(l, x, c, a.E, run);
+        if (x > a.E) continue;
+        a.offsets[x] = at;
+        a.counts[x] = c;
+        if (x == a.E) a.offsets[x + 1] = a.n;
     }
     __syncthreads();
-    write_tiles(l, E, tiles, few, ntiles);
+    q.write(h, a.topk, [&](int e) { return l.start[e]; }, a.order, a.token, a.inv);
+    write_tiles(l, a.E, a.tiles, a.few, a.ntiles);
 }
 
-// The whole plan of up to PLAN_ROUTES routes in one workgroup (701 tokens of 4 picks: 17 + 4 us as a permutation and its tiles). A wave takes
-// a run of routes, 64 at a time: lanes that hold the same expert find each other by one ballot per bit, so that a route's place among its
-// expert's is the wave's count so far and the lanes before it; counts of the waves before come on top.
-constexpr int PLAN_ROUTES = 8192, PLAN_ROUNDS = PLAN_ROUTES / 1024;
-__global__ __launch_bounds__(1024) void k_group_plan(const int64_t* __restrict__ ids, int n, int topk, int E, int bits, int32_t* __restrict__ counts,
-                                                     int32_t* __restrict__ offsets, int32_t* __restrict__ order, int32_t* __restrict__ token,
-                                                     int32_t* __restrict__ inv, GroupTile* __restrict__ tiles, GroupTile* __restrict__ few,
-                                                     int32_t* __restrict__ ntiles)
+// Larger plans: each workgroup's counts, their sums, the rows.
+__global__ __launch_bounds__(1024) void k_group_count(PlanArgs a)
+{
+    __shared__ int c[1026];
+    for (int x = threadIdx.x; x <= a.E; x += 1024) c[x] = 0;
+    __syncthreads();
+    const int s = blockIdx.x * a.run, to = min(a.n, s + a.run);
+    for (int i = s + threadIdx.x; i < to; i += 1024)
+    {
+        const int64_t id = a.ids[i];
+        atomicAdd(&c[id >= 0 && id < a.E ? (int)id : a.E], 1);
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x <= a.E; x += 1024) a.hist[(size_t)blockIdx.x * (a.E + 1) + x] = c[x];
+}
+__global__ __launch_bounds__(1024) void k_group_sums(PlanArgs a)
 {
     __shared__ PlanLds l;
-    __shared__ uint16_t hist[16][1026];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, rounds = (n + 1023) / 1024, s0 = wave * rounds * 64 + lane;
-    int e[PLAN_ROUNDS], p[PLAN_ROUNDS];
-#pragma unroll
-    for (int r = 0; r < PLAN_ROUNDS; ++r)
-    {
-        const int s = s0 + 64 * r;
-        const int64_t id = r < rounds && s < n ? ids[s] : 0;
-        e[r] = id >= 0 && id < E ? (int)id : E;
-    }
-    for (int i = t; i < 16 * 1026 / 2; i += 1024) reinterpret_cast<uint32_t*>(hist)[i] = 0;
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < PLAN_ROUNDS; ++r)
-    {
-        if (r >= rounds) break;
-        const bool in = s0 + 64 * r < n;
-        uint64_t same = __ballot(in);
-        for (int b = 0; b < bits; ++b)
-        {
-            const uint64_t one = __ballot((e[r] >> b) & 1);
-            same &= (e[r] >> b) & 1 ? one : ~one;
-        }
-        const int before = __popcll(same & ((1ull << lane) - 1)), had = hist[wave][e[r]];
-        __builtin_amdgcn_wave_barrier();
-        p[r] = had + before;
-        if (in && before == 0) hist[wave][e[r]] = (uint16_t)(had + __popcll(same));
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-    }
-    __syncthreads();
     Sums run = {};
-    for (int base = 0; base <= E; base += 1024)
+    for (int base = 0; base <= a.E; base += 1024)
     {
-        const int x = base + t;
-        int h[16], c = 0;
-        if (x <= E)
-        {
-#pragma unroll
-            for (int w = 0; w < 16; ++w) h[w] = hist[w][x];
-#pragma unroll
-            for (int w = 0; w < 16; ++w)
+        const int x = base + threadIdx.x;
+        int c = 0;
+        if (x <= a.E)
+            for (int g = 0; g < a.groups; g += 16)
             {
-                hist[w][x] = (uint16_t)c;
-                c += h[w];
-            }
-        }
-        const int at = place_expert(l, x, c, E, run);
-        if (x <= E)
-        {
-            offsets[x] = at;
-            counts[x] = c;
-        }
-    }
-    if (t == 0) offsets[E + 1] = n;
-    __syncthreads();
+                int v[16];
 #pragma unroll
-    for (int r = 0; r < PLAN_ROUNDS; ++r)
-    {
-        const int s = s0 + 64 * r;
-        if (r >= rounds || s >= n) break;
-        const int at = l.start[e[r]] + hist[wave][e[r]] + p[r];
-        order[at] = s;
-        token[at] = s / topk;
-        inv[s] = at;
+                for (int i = 0; i < 16; ++i) v[i] = g + i < a.groups ? a.hist[(size_t)(g + i) * (a.E + 1) + x] : 0;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                {
+                    if (g + i < a.groups) a.hist[(size_t)(g + i) * (a.E + 1) + x] = c;
+                    c += v[i];
+                }
+            }
+        const int at = place_expert(l, x, c, a.E, run);
+        if (x > a.E) continue;
+        a.offsets[x] = at;
+        a.counts[x] = c;
+        if (x == a.E) a.offsets[x + 1] = a.n;
     }
-    write_tiles(l, E, tiles, few, ntiles);
+    __syncthreads();
+    write_tiles(l, a.E, a.tiles, a.few, a.ntiles);
+}
+__global__ __launch_bounds__(1024) void k_group_order(PlanArgs a)
+{
+    __shared__ int start[1026];
+    __shared__ RouteLds h;
+    Routes q;
+    const int s = blockIdx.x * a.run;
+    q.init(h, a.ids, s, min(a.n, s + a.run), a.E, a.bits);
+    for (int x = threadIdx.x; x <= a.E; x += 1024)
+    {
+        start[x] = a.offsets[x] + a.hist[(size_t)blockIdx.x * (a.E + 1) + x];
+        Routes::count(h, x);
+    }
+    __syncthreads();
+    q.write(h, a.topk, [&](int e) { return start[e]; }, a.order, a.token, a.inv);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -935,6 +1011,15 @@ namespace {
 
 constexpr long long MOST_ROUTES = 1LL << 30, MOST_THREADS = (1LL << 32) - 1;      // of a launch
 
+// Plans of up to PLAN_ONE routes take one launch (4,096 routes 9.0 us, 8,192 17.5), larger ones three (8,200 routes 11.8 us, 131,072 22.4).
+constexpr int PLAN_ONE = 4096;
+// Routes of a workgroup: few enough that the workgroups fill the GPU, many enough that their counts are soon added.
+static_assert(PLAN_ONE <= PLAN_ROUTES, "a workgroup's routes");
+int plan_run(int n)
+{
+    return 1024 * (int)std::min<long long>(PLAN_ROUNDS, ((long long)n + (128 << 10) - 1) / (128 << 10));
+}
+
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // Checks that the products share.
@@ -1007,6 +1092,12 @@ size_t mm_group_tiles(int n, int E)
     return n > 0 && E > 0 ? (size_t)(tile_capacity(n, E, ROWS) + tile_capacity(n, E, FEW_ROWS)) * sizeof(GroupTile) : 0;
 }
 
+size_t mm_group_plan_workspace(int n, int E)
+{
+    if (n <= PLAN_ONE || E <= 0) return 0;
+    return (size_t)(((long long)n + plan_run(n) - 1) / plan_run(n)) * (E + 1) * sizeof(int32_t);
+}
+
 int mm_group_plan(const int64_t* ids, const mm_group_plan_t* p, int32_t* counts, void* workspace, size_t workspace_bytes, mm_stream_t stream)
 {
     MM_CHECK_ARG(p && p->offsets && p->order && p->token && p->inv && p->tiles && p->ntiles && counts && ids, "mm_group_plan: null pointer");
@@ -1014,21 +1105,34 @@ int mm_group_plan(const int64_t* ids, const mm_group_plan_t* p, int32_t* counts,
                  "mm_group_plan: need tokens, picks, 1 <= E <= 1024 and at most 2^30 routes");
     MM_CHECK_ARG(aligned16(p->tiles), "mm_group_plan: misaligned tiles");
     const int n = p->T * p->topk;
+    const size_t need = mm_group_plan_workspace(n, p->E);
+    MM_CHECK_ARG(workspace_bytes >= need && (!need || workspace), "mm_group_plan: workspace too small (%zu < %zu)", workspace_bytes, need);
+    MM_CHECK_ARG(((uintptr_t)workspace & 3) == 0, "mm_group_plan: misaligned workspace");
     const hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
-    GroupTile* tiles = reinterpret_cast<GroupTile*>(p->tiles);
-    GroupTile* few = tiles + tile_capacity(n, p->E, ROWS);
-    if (n <= PLAN_ROUTES)
+    PlanArgs a = {};
+    a.ids = ids;
+    a.counts = counts;
+    a.offsets = p->offsets;
+    a.order = p->order;
+    a.token = p->token;
+    a.inv = p->inv;
+    a.ntiles = p->ntiles;
+    a.tiles = reinterpret_cast<GroupTile*>(p->tiles);
+    a.few = a.tiles + tile_capacity(n, p->E, ROWS);
+    a.hist = static_cast<int32_t*>(workspace);
+    a.n = n;
+    a.topk = p->topk;
+    a.E = p->E;
+    a.run = plan_run(n);
+    a.groups = (int)(((long long)n + a.run - 1) / a.run);
+    for (a.bits = 1; p->E >> a.bits;) ++a.bits;
+    if (!need) hipLaunchKernelGGL(k_group_plan, dim3(1), dim3(1024), 0, hs, a);
+    else
     {
-        int bits = 1;
-        while (p->E >> bits) ++bits;
-        hipLaunchKernelGGL(k_group_plan, dim3(1), dim3(1024), 0, hs, ids, n, p->topk, p->E, bits, counts, p->offsets, p->order, p->token, p->inv, tiles,
-                           few, p->ntiles);
-        return check_launch("mm_group_plan");
+        hipLaunchKernelGGL(k_group_count, dim3(a.groups), dim3(1024), 0, hs, a);
+        hipLaunchKernelGGL(k_group_sums, dim3(1), dim3(1024), 0, hs, a);
+        hipLaunchKernelGGL(k_group_order, dim3(a.groups), dim3(1024), 0, hs, a);
     }
-    if (const int rc = permute_launch(ids, nullptr, n, p->topk, p->E, counts, p->offsets, p->order, p->token, nullptr, p->inv, nullptr, nullptr,
-                                      workspace, workspace_bytes, stream))
-        return rc;
-    hipLaunchKernelGGL(k_group_tiles, dim3(1), dim3(1024), 0, hs, p->offsets, p->E, tiles, few, p->ntiles);
     return check_launch("mm_group_plan");
 }
 

@@ -84,6 +84,7 @@ _SIGS = {
     "mm_w4_moe_workspace": (sz, [i32, i32, i32, i32, i32, i32, i32]),
     "mm_w4_moe": (i32, [ctypes.POINTER(MMW4Layer), vp, i32, i32, i32, vp, vp, i32, vp, vp, sz, vp]),
     "mm_group_tiles": (sz, [i32, i32]),
+    "mm_group_plan_workspace": (sz, [i32, i32]),
     "mm_group_plan": (i32, [vp, ctypes.POINTER(MMGroupPlan), vp, vp, sz, vp]),
     "mm_group_linear_workspace": (sz, [i32, i32, i32, i32]),
     "mm_group_linear": (i32, [ctypes.POINTER(MMGroupPlan), vp, vp, i32, i32, i32, i32, i32, vp, i32, vp, sz, vp]),

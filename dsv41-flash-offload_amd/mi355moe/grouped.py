@@ -51,7 +51,7 @@ class Plan:
             self._ref, self.device = ctypes.byref(self._c), dev
             if n:
                 ids = ids.contiguous()
-                wsb = lib.mm_permute_workspace(n, E)
+                wsb = lib.mm_group_plan_workspace(n, E)
                 ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
                 _lib.call("mm_group_plan", ids.data_ptr(), self._ref, a + 4 * at[1], _p(ws), wsb, _lib.raw_stream(dev))
 

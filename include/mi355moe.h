@@ -322,8 +322,9 @@ typedef struct mm_group_plan
 } mm_group_plan_t;
 
 /* Fills a plan's buffers from ids int64 [T][topk]. counts int32 [E + 1]: rows of each expert (and of none). Workspace:
- * mm_permute_workspace(n, E) bytes. */
+ * mm_group_plan_workspace(n, E) bytes, 4-byte aligned. */
 size_t mm_group_tiles(int n, int E);
+size_t mm_group_plan_workspace(int n, int E);
 int mm_group_plan(const int64_t* ids, const mm_group_plan_t* plan, int32_t* counts, void* workspace, size_t workspace_bytes,
                   mm_stream_t stream);
 

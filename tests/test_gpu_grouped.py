@@ -125,7 +125,8 @@ def test_products(dev, rows, k, none, K, N, dtype, gather, reduce):
 
 
 @pytest.mark.parametrize("T,k,E,K,N", [(1, 1, 1, 64, 64), (1, 8, 384, 512, 256), (3, 2, 1024, 64, 72), (700, 6, 64, 128, 320), (5000, 2, 9, 64, 64),
-                                         (1024, 8, 384, 64, 64), (1025, 8, 1024, 8, 16), (8192, 1, 1, 8, 8), (127, 9, 1023, 16, 8), (65, 1, 512, 8, 8)])
+                                         (1024, 4, 384, 64, 64), (1025, 4, 1024, 8, 16), (4096, 1, 1, 8, 8), (4097, 1, 1, 8, 8), (127, 9, 1023, 16, 8), (65, 1, 512, 8, 8),
+                                         (40000, 8, 1024, 8, 8), (131073, 1, 3, 8, 8), (16384, 8, 384, 8, 16)])
 def test_plan(dev, T, k, E, K, N):
     """The order by its definition, for one kernel's calls and for many; picks of none last."""
     from mi355moe import grouped
