@@ -76,7 +76,7 @@ def _check_linear(what, w, plan, gather, reduce):
 def _check_rows(what, name, t, rows, width, dtype):
     if t.dtype != dtype:
         raise TypeError(f"{what}: {name} must have w's type {dtype} (got {t.dtype})")
-    if t.dim() != 2 or tuple(t.shape) != (rows, width):
+    if t.shape != (rows, width):
         raise ValueError(f"{what}: {name} must be {[rows, width]} (got {tuple(t.shape)})")
 
 
@@ -181,7 +181,7 @@ def _check_swiglu(what, rows, dtype, width, plan, weights, limit):
         raise ValueError(f"{what}: limit must not be negative (got {limit})")
     if weights is not None:
         shape = (rows,) if plan is None else (plan.T, plan.k)
-        if weights.dtype != torch.float32 or tuple(weights.shape) != shape:
+        if weights.dtype != torch.float32 or weights.shape != shape:
             raise ValueError(f"{what}: weights must be fp32 {list(shape)} (got {weights.dtype} {tuple(weights.shape)})")
 
 
@@ -189,23 +189,25 @@ def swiglu_forward(gu, plan=None, weights=None, limit=10.0, save8=False, stream=
     """(h, kept) of rows gu [n, 2 I] = [g | u]: h [n, I] = w min(silu(g), limit) clamp(u, -limit, limit) (limit 0: no clamp), with the
     routing weights fp32 [T, k] of the plan's routes (without a plan [n]; None: 1); rows of no expert are zero (mm_gated). kept is what
     swiglu_backward takes: gu, or with `save8` a Saved8 of it, in the same pass (I a multiple of 32)."""
-    if gu.dim() != 2 or gu.shape[1] % 2:
-        raise ValueError(f"swiglu: gu [n, 2 I] expected (got {tuple(gu.shape)})")
-    n, I, dev = gu.shape[0], gu.shape[1] // 2, gu.device
-    _check_swiglu("swiglu", n, gu.dtype, I, plan, weights, limit)
+    # (a decode step's call takes as long as its launch: little is done twice here)
+    shape, dev, dtype = gu.shape, gu.device, gu.dtype
+    if len(shape) != 2 or shape[1] % 2:
+        raise ValueError(f"swiglu: gu [n, 2 I] expected (got {tuple(shape)})")
+    n, I = shape[0], shape[1] // 2
+    _check_swiglu("swiglu", n, dtype, I, plan, weights, limit)
     if save8 and I % SAVE_GROUP:
         raise ValueError(f"swiglu: save8 needs I a multiple of {SAVE_GROUP} (got {I})")
     _lib.check_tensors("swiglu", dev if plan is None else plan.device, gu=gu, weights=weights)
     with _lib.on(dev, stream):
-        h = torch.empty((n, I), dtype=gu.dtype, device=dev)
+        h = torch.empty((n, I), dtype=dtype, device=dev)
         kept = gu
         if save8:
             kept = Saved8(torch.empty((n, 2 * I), dtype=torch.int8, device=dev),
-                          torch.empty((n, 2 * I // SAVE_GROUP), dtype=torch.int8, device=dev), gu.dtype)
+                          torch.empty((n, 2 * I // SAVE_GROUP), dtype=torch.int8, device=dev), dtype)
         if n:
             gu = _lib.aligned(gu)
             weights = None if weights is None else weights.contiguous()
-            _lib.call("mm_gated", None if plan is None else plan._ref, gu.data_ptr(), _DTYPES[gu.dtype], n, I, _p(weights), float(limit), h.data_ptr(),
+            _lib.call("mm_gated", None if plan is None else plan._ref, gu.data_ptr(), _DTYPES[dtype], n, I, _p(weights), float(limit), h.data_ptr(),
                       kept.codes.data_ptr() if save8 else None, kept.exps.data_ptr() if save8 else None, _lib.raw_stream(dev))
     return h, kept
 
