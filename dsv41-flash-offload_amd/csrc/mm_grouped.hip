@@ -613,8 +613,30 @@ __device__ __forceinline__ void trade_rows(u4_t& a, u4_t& b, bool low)
         b[i] = low ? got : b[i];
     }
 }
+// Rows that are summed per token into a bf16 result are kept in between as fp16 times a power of two per 32 columns of a row, from their
+// largest finite value: each is within 2^-11 of itself (2^-39 of that largest where it is far below), an eighth of the result's own half step, at
+// half the bytes of fp32. 131,072 rows of 64 experts, 4,096 columns, summed by eights: 2,048 terms 2,630 us with fp32 rows, 2,310 so; 4,096 terms
+// 4,330 and 3,990; 3,600 rows of 5,120: 339 and 327.
+constexpr int ROWS_SCALED = 3, SCALE_COLS = 32;
+// the exponent for a lane's eight values and those of the other lanes of its row
+__device__ __forceinline__ int row_exponent(const f4_t& a, const f4_t& b)
+{
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+        const float u = fabsf(a[i]), v = fabsf(b[i]);
+        top = fmaxf(top, fmaxf(u < INFINITY ? u : 0.f, v < INFINITY ? v : 0.f));
+    }
+    top = fmaxf(top, xor_lane<16>(top));
+    top = fmaxf(top, xor_lane<32>(top));
+    return max(-126, (int)(__float_as_uint(top) >> 23) - 127 - 14);      // the largest below 2^15
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
 template <int XT, typename S, bool FULL = false>
-__device__ __forceinline__ void store(f4_t (&acc)[S::MB][S::NB], void* y, int type, size_t row0, int rows, int col0, int cols, size_t ld)
+__device__ __forceinline__ void store(f4_t (&acc)[S::MB][S::NB], void* y, int type, size_t row0, int rows, int col0, int cols, size_t ld,
+                                      int8_t* exps = nullptr)
 {
     const int lane = lane_here(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4, m0 = wave / S::WN * S::MB * 16, n0 = col0 + wave % S::WN * S::NB * 16;
@@ -645,12 +667,25 @@ __device__ __forceinline__ void store(f4_t (&acc)[S::MB][S::NB], void* y, int ty
                 pair(__builtin_bit_cast(u4_t, acc[i][j]), __builtin_bit_cast(u4_t, acc[i][j + 1]), i, n0 + 16 * j + 4 * g, 16, 4);
             continue;
         }
+        if (!FULL && type == ROWS_SCALED)
+        {
+#pragma unroll
+            for (int j = 0; j < S::NB; j += 2)
+            {
+                const int e = row_exponent(acc[i][j], acc[i][j + 1]), m = m0 + 16 * i + r, n = n0 + 16 * j;
+                acc[i][j] *= power_of_two(-e);
+                acc[i][j + 1] *= power_of_two(-e);
+                if (g == j / 2 && m < rows && n < cols) exps[(row0 + m) * ((ld + SCALE_COLS - 1) / SCALE_COLS) + n / SCALE_COLS] = (int8_t)e;
+            }
+        }
         u4_t v[S::NB / 2];
 #pragma unroll
         for (int j = 0; j < S::NB; j += 2)
         {
-            const auto lo = __builtin_amdgcn_permlane16_swap(pack2<XT>(acc[i][j][0], acc[i][j][1]), pack2<XT>(acc[i][j + 1][0], acc[i][j + 1][1]), false, false);
-            const auto hi = __builtin_amdgcn_permlane16_swap(pack2<XT>(acc[i][j][2], acc[i][j][3]), pack2<XT>(acc[i][j + 1][2], acc[i][j + 1][3]), false, false);
+            const bool half = !FULL && type == ROWS_SCALED;
+            auto pack = [&](float a, float b) { return half ? pack2<MM_DTYPE_F16>(a, b) : pack2<XT>(a, b); };
+            const auto lo = __builtin_amdgcn_permlane16_swap(pack(acc[i][j][0], acc[i][j][1]), pack(acc[i][j + 1][0], acc[i][j + 1][1]), false, false);
+            const auto hi = __builtin_amdgcn_permlane16_swap(pack(acc[i][j][2], acc[i][j][3]), pack(acc[i][j + 1][2], acc[i][j + 1][3]), false, false);
             v[j / 2] = u4_t{ lo[0], hi[0], lo[1], hi[1] };
         }
         const int n = n0 + 16 * (g & 1) + 4 * (g & 2);
@@ -677,6 +712,7 @@ struct RowsArgs
     void* y;
     const GroupTile* tiles;
     const int32_t *ntiles, *token;     // token: row of x of each row, NULL: its own
+    int8_t* exps;                      // of ROWS_SCALED rows
     size_t xbytes;
     int terms, cols, type, zero, colt;      // zero: rows of no expert are stored (as zeros); colt: column tiles
 };
@@ -710,7 +746,7 @@ __device__ __forceinline__ void rows_tile(const RowsArgs& a, const GroupTile& t,
         for (int j = 0; j < S::NB; ++j) acc[i][j] = f4_t{ 0.f, 0.f, 0.f, 0.f };
     const uint32_t mp = M::place(wave / S::WN * S::MB * 16), np = N::place(wave % S::WN * S::NB * 16);
     run<XT, M, N, S>(lds, m, n, a.terms, mp, np, acc);
-    store<XT, S>(acc, a.y, a.type, t.row, t.rows, col0, a.cols, a.cols);
+    store<XT, S>(acc, a.y, a.type, t.row, t.rows, col0, a.cols, a.cols, a.exps);
 }
 
 // Columns ct C .. of rows of no expert.
@@ -1003,6 +1039,36 @@ __global__ __launch_bounds__(256) void k_group_sum(const float* __restrict__ row
     }
 }
 
+// The same of rows as ROWS_SCALED keeps them, into bf16.
+__global__ __launch_bounds__(256) void k_group_sum_scaled(const uint16_t* __restrict__ rows, const int8_t* __restrict__ exps, const int32_t* __restrict__ inv,
+                                                          const int32_t* __restrict__ live, long long n8, int topk, int cols8, void* __restrict__ out)
+{
+    const int end = *live, groups = (cols8 + 3) / 4;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n8; i += (long long)gridDim.x * 256)
+    {
+        const long long t = i / cols8;
+        const int c = (int)(i - t * cols8);
+        float s[8] = {};
+        for (int j = 0; j < topk; ++j)
+        {
+            const int p = inv[t * topk + j];
+            if (p >= end) continue;
+            const u4_t v = reinterpret_cast<const u4_t*>(rows)[(size_t)p * cols8 + c];
+            const float f = power_of_two(exps[(size_t)p * groups + c / 4]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+            {
+                s[2 * k] = fmaf(h2f((uint16_t)v[k]), f, s[2 * k]);
+                s[2 * k + 1] = fmaf(h2f((uint16_t)(v[k] >> 16)), f, s[2 * k + 1]);
+            }
+        }
+        u4_t o;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = pack2<MM_DTYPE_BF16>(s[2 * k], s[2 * k + 1]);
+        reinterpret_cast<u4_t*>(out)[i] = o;
+    }
+}
+
 }  // namespace mm
 
 using namespace mm;
@@ -1034,6 +1100,13 @@ int check(const char* what, const mm_group_plan_t* p, int dtype, int K, int N, i
     return MM_OK;
 }
 
+// Whether rows to be summed are kept scaled (those of the few-route form are not: they are few).
+bool scaled_rows(long long n, int y_type) { return y_type == MM_DTYPE_BF16 && n > FEW_ROUTES; }
+size_t sum_workspace(long long n, int cols, int y_type)
+{
+    return scaled_rows(n, y_type) ? (size_t)n * cols * 2 + (size_t)n * ((cols + SCALE_COLS - 1) / SCALE_COLS) : (size_t)n * cols * 4;
+}
+
 template <bool ACROSS>
 int launch_rows(const char* what, const mm_group_plan_t* p, const void* x, const void* w, int dtype, int terms, int cols, int gather, int reduce,
                 void* y, int y_type, void* ws, size_t ws_bytes, mm_stream_t stream)
@@ -1041,7 +1114,7 @@ int launch_rows(const char* what, const mm_group_plan_t* p, const void* x, const
     const long long n = (long long)p->T * p->topk;
     MM_CHECK_ARG(x && w && y, "%s: null pointer", what);
     MM_CHECK_ARG(aligned16(x) && aligned16(w) && aligned16(y) && aligned16(ws), "%s: misaligned pointer", what);
-    const size_t need = reduce ? (size_t)n * cols * 4 : 0;
+    const size_t need = reduce ? sum_workspace(n, cols, y_type) : 0;
     MM_CHECK_ARG(ws_bytes >= need && (!need || ws), "%s: workspace too small (%zu < %zu)", what, ws_bytes, need);
     MM_CHECK_ARG(!gather || (long long)p->T * terms < 1LL << 31, "%s: rows per token must be below 4 GiB", what);
     const hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
@@ -1053,7 +1126,9 @@ int launch_rows(const char* what, const mm_group_plan_t* p, const void* x, const
     a.xbytes = (size_t)p->T * terms * 2;
     a.terms = terms;
     a.cols = cols;
-    a.type = reduce ? MM_DTYPE_F32 : y_type;
+    const bool scaled = reduce && scaled_rows(n, y_type);
+    a.type = scaled ? ROWS_SCALED : reduce ? MM_DTYPE_F32 : y_type;
+    a.exps = scaled ? static_cast<int8_t*>(ws) + (size_t)n * cols * 2 : nullptr;
     a.zero = !reduce;
     // The form by the tiles there will be (the routes' experts are not known here): large ones as soon as they nearly fill the GPU (512 rows of
     // each of 8 experts of 4096 x 4096, 320 tiles by this estimate: 115 us, small ones 195), else small ones (1,000 rows of one expert, 48
@@ -1073,7 +1148,13 @@ int launch_rows(const char* what, const mm_group_plan_t* p, const void* x, const
     if (few) hipLaunchKernelGGL((h ? k_group_few<MM_DTYPE_F16> : k_group_few<MM_DTYPE_BF16>), dim3((unsigned)blocks), dim3(256), 0, hs, a);
     else if (small) hipLaunchKernelGGL((h ? k_group_rows<MM_DTYPE_F16, ACROSS, 128> : k_group_rows<MM_DTYPE_BF16, ACROSS, 128>), dim3((unsigned)blocks), dim3(256), 0, hs, a);
     else hipLaunchKernelGGL((h ? k_group_rows<MM_DTYPE_F16, ACROSS, 256> : k_group_rows<MM_DTYPE_BF16, ACROSS, 256>), dim3((unsigned)blocks), dim3(512), 0, hs, a);
-    if (reduce)
+    if (scaled)
+    {
+        const long long n8 = (long long)p->T * cols / 8;
+        hipLaunchKernelGGL(k_group_sum_scaled, dim3((unsigned)std::min<long long>((n8 + 255) / 256, 1 << 22)), dim3(256), 0, hs,
+                           static_cast<const uint16_t*>(ws), a.exps, p->inv, p->offsets + p->E, n8, p->topk, cols / 8, y);
+    }
+    else if (reduce)
     {
         const long long n4 = (long long)p->T * cols / 4;
         auto sum = y_type == MM_DTYPE_F32 ? k_group_sum<MM_DTYPE_F32> : y_type == MM_DTYPE_F16 ? k_group_sum<MM_DTYPE_F16> : k_group_sum<MM_DTYPE_BF16>;
@@ -1136,9 +1217,9 @@ int mm_group_plan(const int64_t* ids, const mm_group_plan_t* p, int32_t* counts,
     return check_launch("mm_group_plan");
 }
 
-size_t mm_group_linear_workspace(int T, int topk, int cols, int reduce)
+size_t mm_group_linear_workspace(int T, int topk, int cols, int reduce, int y_dtype)
 {
-    return reduce && T > 0 && topk > 0 && cols > 0 ? (size_t)T * topk * cols * 4 : 0;
+    return reduce && T > 0 && topk > 0 && cols > 0 ? sum_workspace((long long)T * topk, cols, y_dtype) : 0;
 }
 
 int mm_group_linear(const mm_group_plan_t* plan, const void* x, const void* w, int dtype, int K, int N, int gather, int reduce, void* y,

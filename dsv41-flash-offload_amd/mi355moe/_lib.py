@@ -86,7 +86,7 @@ _SIGS = {
     "mm_group_tiles": (sz, [i32, i32]),
     "mm_group_plan_workspace": (sz, [i32, i32]),
     "mm_group_plan": (i32, [vp, ctypes.POINTER(MMGroupPlan), vp, vp, sz, vp]),
-    "mm_group_linear_workspace": (sz, [i32, i32, i32, i32]),
+    "mm_group_linear_workspace": (sz, [i32, i32, i32, i32, i32]),
     "mm_group_linear": (i32, [ctypes.POINTER(MMGroupPlan), vp, vp, i32, i32, i32, i32, i32, vp, i32, vp, sz, vp]),
     "mm_group_linear_inputs": (i32, [ctypes.POINTER(MMGroupPlan), vp, vp, i32, i32, i32, i32, i32, vp, i32, vp, sz, vp]),
     "mm_group_linear_weights": (i32, [ctypes.POINTER(MMGroupPlan), vp, vp, i32, i32, i32, i32, i32, vp, i32, vp]),

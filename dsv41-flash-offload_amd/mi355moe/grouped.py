@@ -99,7 +99,7 @@ def linear_forward(x, w, plan, gather=False, reduce=False, out_dtype=None, strea
         y = torch.empty((plan.T if reduce else plan.n, N), dtype=out_dtype, device=dev)
         if plan.n:
             x = _lib.aligned(x)
-            wsb = plan.n * N * 4 if reduce else 0
+            wsb = _lib.load().mm_group_linear_workspace(plan.T, plan.k, N, 1, out_code) if reduce else 0
             ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
             _lib.call("mm_group_linear", plan._ref, x.data_ptr(), w.data_ptr(), code, K, N, int(gather), int(reduce), y.data_ptr(), out_code,
                       _p(ws), wsb, _lib.raw_stream(dev))
@@ -124,7 +124,7 @@ def linear_backward(dy, x, w, plan, gather=False, reduce=False, need_x=True, nee
         if need_x:
             dx = torch.empty((plan.T if gather else plan.n, K), dtype=w.dtype, device=dev)
             if plan.n:
-                wsb = plan.n * K * 4 if gather else 0
+                wsb = _lib.load().mm_group_linear_workspace(plan.T, plan.k, K, 1, code) if gather else 0
                 ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
                 _lib.call("mm_group_linear_inputs", plan._ref, dy.data_ptr(), w.data_ptr(), code, K, N, int(gather), int(reduce), dx.data_ptr(),
                           code, _p(ws), wsb, _lib.raw_stream(dev))

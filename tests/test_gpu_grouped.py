@@ -3,7 +3,9 @@
 Tolerances: products of 16-bit values are exact in fp32. A sum of K terms passes through at most K fp32 roundings, each at most 2^-23 of the
 sum of the terms' magnitudes, whatever the order (matrix cores may truncate: a whole unit instead of a half); as a random walk the same
 roundings come to sqrt(K) 2^-23 of the root of the sum of squares, which the 2-norm of the error over all outputs is held to (twice).
-Results are rounded once to their type (half a step, and half the smallest subnormal)."""
+Results are rounded once to their type (half a step, and half the smallest subnormal). Rows that are summed per token into bf16 are kept in between
+in 11 bits under a power of two per 32 columns: off by at most 2^-11 of themselves (half a step of fp16), and by half of fp16's smallest subnormal where
+the largest of the 32 is at least 2^14 times it: 2^-25 / 2^14 of that largest."""
 import pytest
 import torch
 
@@ -60,16 +62,25 @@ def products(x, dy, w, ids, gather, reduce):
     sq = [v.sqrt() for v in all_(xr ** 2, dr ** 2, w ** 2)]
     most = int(torch.bincount(expert[expert < E], minlength=E).max()) if E else 0
     terms = (K + k, N + k, max(most, 1))
-    return dict(zip(("forward", "inputs", "weights"), zip(res, mag, sq, terms)))
+    # what the rows that are summed per token may be off by as they are kept
+    rows = [None, None, None]
+    if (reduce or gather) and w.dtype == torch.float64 and T * k > 16:
+        each = torch.zeros((T * k, N if reduce else K)).double()
+        for e in range(E):
+            r = (expert == e).nonzero()[:, 0]
+            each[r] = xr[r] @ w[e].t() if reduce else dr[r] @ w[e]
+        rows[0 if reduce else 1] = torch.zeros((T, each.shape[1])).double().index_add_(0, token, 2.0 ** -11 * each.abs() + 2.0 ** -39 * each.abs().amax(1, keepdim=True))
+    return dict(zip(("forward", "inputs", "weights"), zip(res, mag, sq, terms, rows)))
 
 
 def check(got, want):
-    ref, mag, sq, terms = want
+    ref, mag, sq, terms, rows = want
     half, tiny = HALF[got.dtype], TINY[got.dtype]
+    kept = rows if rows is not None and got.dtype == BF else torch.zeros(1).double()
     assert got.shape == ref.shape
-    within(got, ref, terms * 2.0 ** -23 * mag + half * ref.abs() + tiny)
+    within(got, ref, terms * 2.0 ** -23 * mag + half * (ref.abs() + kept) + kept + tiny)
     err = (got.cpu().double() - ref).norm()
-    assert err <= 2 * terms ** 0.5 * 2.0 ** -23 * sq.norm() + half * ref.norm() + tiny * ref.numel() ** 0.5
+    assert err <= 2 * terms ** 0.5 * 2.0 ** -23 * sq.norm() + half * (ref.norm() + kept.norm()) + kept.norm() + tiny * ref.numel() ** 0.5
 
 
 def inputs(g, ids, E, K, N, dtype, gather, reduce):
@@ -175,6 +186,29 @@ def test_infinite_and_nan_rows_stay_their_own(dev):
     assert torch.equal(got[rows.to(dev)], clean[rows.to(dev)])
     ref = torch.sign(w[0][:, 3].float()) * float("inf")
     assert torch.equal(got[5].cpu().float(), ref) and got[50].isnan().all() and got[119].isinf().all()
+
+
+def test_summed_rows_of_all_sizes(dev):
+    """Rows kept between product and sum: columns 2^60 apart, rows of zeros, values at bf16's ends, an infinity beside large finite values."""
+    from mi355moe import grouped
+    g = torch.Generator().manual_seed(5)
+    ids = picks(g, [30, 50], 2)
+    T = ids.shape[0]
+    x, w = torch.randn((2 * T, 64), generator=g).to(BF), torch.randn((2, 200, 64), generator=g)
+    w *= 2.0 ** torch.randint(-30, 31, (2, 200, 1), generator=g)
+    w[:, 40:80] = 0
+    x[:8] *= 2.0 ** -90
+    x[8:12] *= 2.0 ** 90
+    w = w.to(BF)
+    plan = grouped.Plan(ids.to(dev), 2)
+    y = grouped.linear_forward(x.to(dev), w.to(dev), plan, reduce=True)
+    dy = torch.zeros((T, 200)).to(BF)
+    check(y, products(x, dy, w, ids, False, True)["forward"])
+    w[0, 3, 5] = float("inf")
+    y = grouped.linear_forward(x.to(dev), w.to(dev), plan, reduce=True).cpu()
+    rows = grouped.linear_forward(x.to(dev), w.to(dev), plan, out_dtype=torch.float32).cpu()
+    want = torch.zeros((T, 200)).index_add_(0, order_of(ids, 2)[0] // 2, rows)
+    assert torch.equal(y.isfinite(), want.to(BF).isfinite()) and torch.equal(y.isnan(), want.isnan())
 
 
 def test_products_repeat_and_take_views(dev):

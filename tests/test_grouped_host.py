@@ -109,8 +109,9 @@ def test_c_argument_errors():
         f = dict(offsets=256, order=256, token=256, inv=256, tiles=256, ntiles=256, T=T, topk=k, E=E) | kw
         return ctypes.byref(_lib.MMGroupPlan(*f.values()))
 
-    assert L.mm_group_tiles(8, 3) > 0 and L.mm_group_tiles(0, 3) == 0 and L.mm_group_linear_workspace(4, 2, 24, 1) == 4 * 2 * 24 * 4
-    assert L.mm_group_linear_workspace(4, 2, 24, 0) == 0
+    assert L.mm_group_tiles(8, 3) > 0 and L.mm_group_tiles(0, 3) == 0 and L.mm_group_linear_workspace(4, 2, 24, 1, 1) == 4 * 2 * 24 * 4
+    assert L.mm_group_linear_workspace(4, 2, 24, 0, 1) == 0 and L.mm_group_linear_workspace(9, 2, 72, 1, 2) == 18 * 72 * 4
+    assert L.mm_group_linear_workspace(9, 2, 72, 1, 0) == 18 * 72 * 4 and L.mm_group_linear_workspace(9, 2, 72, 1, 1) == 18 * (72 * 2 + 3)
     err(L.mm_group_plan(256, p(order=None), 256, None, 0, None), b"null")
     err(L.mm_group_plan(None, p(), 256, None, 0, None), b"null")
     err(L.mm_group_plan(256, p(T=0), 256, None, 0, None), b"need tokens")
