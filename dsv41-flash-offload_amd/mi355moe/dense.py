@@ -43,7 +43,13 @@ class DenseStore:
 
 class _Moe(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, w13, w2, ids, limit, save8, keep):
+    def forward(ctx, x, w, w13, w2, ids, shared, limit, save8, keep):
+        ctx.w = w.dtype, w.shape[1]
+        ids, w = ids.long(), w.float()
+        if shared >= 0:
+            one = (x.shape[0], 1)
+            ids = torch.cat([ids, torch.full(one, shared, dtype=torch.long, device=x.device)], 1)
+            w = torch.cat([w, torch.ones(one, dtype=torch.float32, device=x.device)], 1)
         plan = grouped.Plan(ids, w13.shape[0])
         gu = grouped.linear_forward(x, w13.flatten(1, 2), plan, gather=True)
         h, kept = grouped.swiglu_forward(gu, plan, w, limit, save8 and keep)
@@ -69,7 +75,10 @@ class _Moe(torch.autograd.Function):
             _, d2 = grouped.linear_backward(dout, h, w2, plan, reduce=True, need_x=False)
         if need_x or need_13:
             dx, d13 = grouped.linear_backward(dgu, x, up, plan, gather=True, need_x=need_x, need_w=need_13)
-        return dx, dw, None if d13 is None else d13.view_as(w13), d2, None, None, None, None
+        if dw is not None:
+            dtype, k = ctx.w
+            dw = dw[:, :k].to(dtype)
+        return dx, dw, None if d13 is None else d13.view_as(w13), d2, None, None, None, None, None
 
 
 def moe(store, x, ids, w, shared_expert=None, stream=None):
@@ -90,11 +99,7 @@ def moe(store, x, ids, w, shared_expert=None, stream=None):
     dev = store.w13.device
     _lib.check_tensors("dense.moe", dev, x=x, ids=ids, w=w)
     with _lib.on(dev, stream):
-        ids, w = ids.long(), w.float()
-        if shared >= 0:
-            ids = torch.cat([ids, torch.full((T, 1), shared, dtype=torch.long, device=dev)], 1)
-            w = torch.cat([w, torch.ones((T, 1), dtype=torch.float32, device=dev)], 1)
         leaves = (x, w, store.w13, store.w2)
         keep = torch.is_grad_enabled() and any(t.requires_grad for t in leaves)
-        return _captured_apply("dense.moe", _Moe, leaves, *leaves, ids, store.limit, store.save8, keep,
+        return _captured_apply("dense.moe", _Moe, leaves, *leaves, ids, shared, store.limit, store.save8, keep,
                                instead="the *_forward and *_backward functions of grouped")

@@ -21,9 +21,10 @@ def _capture_stream(device):
 
 
 def _captured_apply(what, fn, leaves, *args, instead=None):
-    """fn.apply(*args), for `what`, whose kernels without autograd are `instead`. Under stream capture, a leaf among its inputs may not have its gradient node in an autograd graph from before
-    the capture: the captured backward would go to that node's stream, which invalidates the capture and ends the process. (A node that
-    a captured call made belongs to that capture's stream, and passes in captures of that stream only.)"""
+    """fn.apply(*args), for `what`, whose kernels without autograd are `instead`. Under stream capture, a leaf among its inputs may not
+    have its gradient node in an autograd graph from before the capture: the captured backward would go to that node's stream, which
+    invalidates the capture and ends the process. (A node that a captured call made belongs to that capture's stream, and passes in
+    captures of that stream only.)"""
     leaves = [t for t in leaves if t.requires_grad and t.is_leaf]
     if not (leaves and torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing()):
         return fn.apply(*args)

@@ -232,6 +232,35 @@ def test_captured_training_step(dev):
             assert torch.equal(a, b)
 
 
+def test_captured_step_with_a_shared_expert(dev):
+    """The routing weights as a leaf in 64 bits, beside a shared expert, inside a capture: their gradient has their type and shape."""
+    from mi355moe import dense
+    g = torch.Generator().manual_seed(17)
+    x, w13, w2, ids, w = (t.to(dev) for t in tensors(g, 30, 2, 4, 64, 32, HF))
+    store = dense.DenseStore(w13.requires_grad_(), w2)
+    w = w.double().requires_grad_()
+
+    def step():
+        return torch.autograd.grad(dense.moe(store, x, ids, w, shared_expert=3).sum(), (w, w13))
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    assert outs[0].dtype == torch.float64 and outs[0].shape == w.shape
+    for i in range(3):
+        x.copy_(torch.randn(x.shape, generator=g))
+        print(f"replay {i}", flush=True)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, step()):
+            assert torch.equal(a, b)
+
+
 def test_two_streams_at_once(dev):
     """Calls of one plan on two streams do not touch each other's workspaces."""
     from mi355moe import grouped

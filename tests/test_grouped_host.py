@@ -183,3 +183,19 @@ def test_a_captured_layer_names_what_to_capture_instead(monkeypatch):
     with pytest.raises(RuntimeError, match="dense.moe: .* or capture the others"):
         router._captured_apply("dense.moe", Double, (t,), t, instead="the others")
     del eager
+
+
+@pytest.mark.parametrize("dtype,shared", [(torch.float32, None), (torch.float32, 1), (torch.bfloat16, None), (torch.float64, 0)])
+def test_a_layer_names_the_callers_own_tensors_as_leaves(monkeypatch, dtype, shared):
+    """Under capture the leaves are looked at for older graphs: the routing weights as the caller has them, not a copy with another type or
+    the shared expert's column."""
+    import contextlib
+    from mi355moe import _lib, dense
+    monkeypatch.setattr(_lib, "check_tensors", lambda *a, **k: None)
+    monkeypatch.setattr(_lib, "on", lambda *a: contextlib.nullcontext())
+    seen = []
+    monkeypatch.setattr(dense, "_captured_apply", lambda what, fn, leaves, *args, **k: seen.append(leaves))
+    store = dense.DenseStore(torch.zeros(2, 2, 8, 8, dtype=torch.bfloat16), torch.zeros(2, 8, 8, dtype=torch.bfloat16))
+    x, w = torch.zeros(3, 8, dtype=torch.bfloat16), torch.zeros(3, 1, dtype=dtype, requires_grad=True)
+    dense.moe(store, x, torch.zeros(3, 1, dtype=torch.int64), w, shared_expert=shared)
+    assert [id(t) for t in seen[0]] == [id(t) for t in (x, w, store.w13, store.w2)]
