@@ -363,13 +363,17 @@ struct Along
             at[i] = (uint32_t)(pick ? pick[min(r, rows - 1)] : r) * ld + 16 * chunk;
         }
     }
-    __device__ __forceinline__ void load(unsigned char* lds, int block, int terms) const
+    // Loads of a block, one by one. (The last block of a contraction that is no multiple of 64: chunks past the row's end are zero; so are
+    // blocks past the last one.)
+    struct Block
     {
-        // the last block of a contraction that is no multiple of 64: chunks past the row's end are zero
-        const bool in = TERMS * block + 8 * chunk < terms;
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-            load16(buf, lds + slot[i] * 128, in ? at[i] + 128 * block : NOWHERE);
+        uint32_t at;
+        bool in;
+    };
+    __device__ __forceinline__ Block block(int b, int terms) const { return { 128u * b, TERMS * b + 8 * chunk < terms }; }
+    __device__ __forceinline__ void load(const Block& b, unsigned char* lds, int i) const
+    {
+        load16(buf, lds + slot[i] * 128, b.in ? at[i] + b.at : NOWHERE);
     }
     // chunk kk * 4 + (lane >> 4) of row 16 b + (lane & 15)
     __device__ static __forceinline__ uint32_t place(int first)
@@ -422,13 +426,24 @@ struct Across
             col[i] = c < width ? 2 * c : NOWHERE;
         }
     }
-    // rows B block .. of `terms`
-    __device__ __forceinline__ void load(unsigned char* lds, int block, int terms) const
+    // rows B b .. of `terms`, one load of them at a time
+    struct Block
     {
-        const __amdgpu_buffer_rsrc_t buf = buffer(base + (size_t)block * B * ld, (uint32_t)max(0, min(terms - B * block, B)) * ld);
+        __amdgpu_buffer_rsrc_t buf;
+    };
+    __device__ __forceinline__ Block block(int b, int terms) const
+    {
+        return { buffer(base + (size_t)b * B * ld, (uint32_t)max(0, min(terms - B * b, B)) * ld) };
+    }
+    __device__ __forceinline__ void load(const Block& b, unsigned char* lds, int i) const
+    {
+        load16(b.buf, lds + (slot + EACH * i) * RB, col[kind(i)] == NOWHERE ? NOWHERE : (row + EACH * i) * ld + col[kind(i)]);
+    }
+    __device__ __forceinline__ void load(unsigned char* lds, int b, int terms) const
+    {
+        const Block at = block(b, terms);
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-            load16(buf, lds + (slot + EACH * i) * RB, col[kind(i)] == NOWHERE ? NOWHERE : (row + EACH * i) * ld + col[kind(i)]);
+        for (int i = 0; i < LOADS; ++i) load(at, lds, i);
     }
     // The same with the rows that `pick` names. A lane holds the name of one of the wave's rows, for CHUNK blocks at once, and the next
     // CHUNK blocks' are on their way: names read block by block would be waited for with all loads before them.
@@ -528,28 +543,37 @@ __device__ __forceinline__ void multiply(const Half<S>& h, f4_t (&acc)[S::MB][S:
 #pragma unroll
         for (int j = 0; j < S::NB; ++j) acc[i][j] = mfma<XT>(h.n[j], h.m[i], acc[i][j]);
 }
-// The products of one half with READS LDS reads of the next between them.
-template <typename S, int READS>
+// The products of one half with the LDS reads of the next between them (of N's NB operands, then of M's), and LOADS loads.
+template <typename M, typename N, typename S, int LOADS = 0>
 __device__ __forceinline__ void interleave()
 {
-    constexpr int PRODUCTS = S::MB * S::NB;
+    constexpr int PRODUCTS = S::MB * S::NB, OPS = S::MB + S::NB, STEPS = std::max(OPS, LOADS), EACH = std::min(std::max(1, PRODUCTS / STEPS), PRODUCTS);
 #pragma unroll
-    for (int i = 0; i < READS; ++i)
+    for (int i = 0; i < STEPS; ++i)
     {
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, std::max(1, PRODUCTS / READS), 0);
+        if (i < S::NB) __builtin_amdgcn_sched_group_barrier(0x100, N::READS, 0);
+        else if (i < OPS) __builtin_amdgcn_sched_group_barrier(0x100, M::READS, 0);
+        if (i < LOADS) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+        if (EACH * (i + 1) <= PRODUCTS) __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS, 0);
+    if (PRODUCTS > EACH * STEPS) __builtin_amdgcn_sched_group_barrier(0x008, std::max(1, PRODUCTS - EACH * STEPS), 0);
 }
 
 // All blocks of a tile. Half a block's operands are read from LDS while the half before is multiplied, across the barrier too, which stands
 // in the middle of a block: a wave that waits there has half a block to multiply. Block b's places are free once every wave has
-// read its second half, so loads run SM and SN blocks ahead.
+// read its second half, so loads run SM and SN blocks ahead, past the last block too: those read zeros, and what is waited for is the same in
+// every block (gradient of the inputs of 131,072 rows of 384 experts 4,750 us with branches around them, 4,655 so).
 template <int XT, typename M, typename N, typename S>
 __device__ __forceinline__ void run(unsigned char* lds, const M& m, const N& n, int terms, uint32_t mp, uint32_t np, f4_t (&acc)[S::MB][S::NB])
 {
-    constexpr int READS = S::MB * M::READS + S::NB * N::READS, SM = S::SM, SN = S::SN;
+    constexpr int SM = S::SM, SN = S::SN;
     constexpr int AFTER = SN > SM ? N::LOADS : 0, EACH = M::LOADS + N::LOADS;      // loads after a block's last one, and in each block after
+    constexpr int OPS = S::MB + S::NB;
+    // Whether a block's loads are sent between the products, or together after the barrier: the first where two LDS reads make an operand of the
+    // weights (gradient of the inputs, 131,072 rows of 64 experts, 4,096 x 2,048: 1,816 us, together 1,870; of 384 experts, 4,096 x 4,096:
+    // 4,570 and 4,670), the second elsewhere (forward of 16,384 rows, 4,096 x 4,096: 646 and 639 us) and in small tiles (4,200 rows of
+    // 64 experts, 5,120 x 4,608: 618 and 608).
+    constexpr bool SPREAD = N::READS == 2 && S::MB * S::WM * 16 > 128;
     unsigned char *ml = lds, *nl = lds + SM * S::MSTAGE;
     const int blocks = (terms + TERMS - 1) / TERMS;
     Half<S> h0, h1;
@@ -558,14 +582,20 @@ __device__ __forceinline__ void run(unsigned char* lds, const M& m, const N& n, 
     for (int b = 0; b < SN; ++b)
     {
         const int bm = b - (SN - SM);
-        if (bm >= 0 && bm < blocks) m.load(ml + bm * S::MSTAGE, bm, terms);
+        if (bm >= 0)
+        {
+            const typename M::Block k = m.block(bm, terms);
+#pragma unroll
+            for (int i = 0; i < M::LOADS; ++i) m.load(k, ml + bm * S::MSTAGE, i);
+        }
         keep_order();
-        if (b < blocks) n.load(nl + b * S::NSTAGE, b, terms);
+        const typename N::Block k = n.block(b, terms);
+#pragma unroll
+        for (int i = 0; i < N::LOADS; ++i) n.load(k, nl + b * S::NSTAGE, i);
         keep_order();
     }
     // block 0 has come once only what was sent after it is out
-    if (blocks >= SN) wait_vmcnt<AFTER + (SM - 1) * EACH>();
-    else wait_vmcnt<0>();
+    wait_vmcnt<AFTER + (SM - 1) * EACH>();
     lds_barrier();
     read_half<M, N, S>(h0, ml, nl, mp, np, 0);
     int am = 0, an = 0;
@@ -576,25 +606,45 @@ __device__ __forceinline__ void run(unsigned char* lds, const M& m, const N& n, 
         asm volatile("" : "+v"(mp), "+v"(np));
         read_half<M, N, S>(h1, ml + am, nl + an, mp, np, 1);
         multiply<XT, S>(h0, acc);
-        interleave<S, READS>();
+        interleave<M, N, S>();
         // the same for block b + 1
-        if (b + SN <= blocks) wait_vmcnt<AFTER + (SM - 2) * EACH>();
-        else wait_vmcnt<0>();
+        wait_vmcnt<AFTER + (SM - 2) * EACH>();
         lds_barrier();
-        if (b + SM < blocks) m.load(ml + am, b + SM, terms);
-        keep_order();
-        if (b + SN < blocks) n.load(nl + an, b + SN, terms);
+        unsigned char *mt = ml + am, *nt = nl + an;
         am = am + S::MSTAGE == SM * S::MSTAGE ? 0 : am + S::MSTAGE;
         an = an + S::NSTAGE == SN * S::NSTAGE ? 0 : an + S::NSTAGE;
         asm volatile("" : "+v"(mp), "+v"(np));
-        read_half<M, N, S>(h0, ml + am, nl + an, mp, np, 0);
+        const typename M::Block km = m.block(b + SM, terms);
+        const typename N::Block kn = n.block(b + SN, terms);
+        if constexpr (!SPREAD)
+        {
+#pragma unroll
+            for (int i = 0; i < M::LOADS; ++i) m.load(km, mt, i);
+            keep_order();
+#pragma unroll
+            for (int i = 0; i < N::LOADS; ++i) n.load(kn, nt, i);
+            read_half<M, N, S>(h0, ml + am, nl + an, mp, np, 0);
+        }
+        else
+        {
+#pragma unroll
+            for (int i = 0; i < std::max(OPS, EACH); ++i)
+            {
+                if (i < S::NB) h0.n[i] = N::read(nl + an, np, i, 0);
+                else if (i < OPS) h0.m[i - S::NB] = M::read(ml + am, mp, i - S::NB, 0);
+                if (i == M::LOADS) keep_order();
+                if (i < M::LOADS) m.load(km, mt, i);
+                else if (i < EACH) n.load(kn, nt, i - M::LOADS);
+            }
+        }
         multiply<XT, S>(h1, acc);
-        interleave<S, READS>();
+        interleave<M, N, S, SPREAD ? EACH : 0>();
     }
     read_half<M, N, S>(h1, ml + am, nl + an, mp, np, 1);
     multiply<XT, S>(h0, acc);
-    interleave<S, READS>();
+    interleave<M, N, S>();
     multiply<XT, S>(h1, acc);
+    wait_vmcnt<0>();       // loads past the last block, which write zeros to LDS
 }
 
 // Lane (r, g) of a block holds columns 4 g .. 4 g + 3 of row r. For 16-bit outputs neighbouring blocks trade halves, so that a lane
@@ -939,7 +989,7 @@ template <int XT, int PICK>
 __global__ __launch_bounds__(512, 2) void k_group_weights(WeightsArgs a)
 {
     using S = WShape;
-    constexpr int L = 2 * Terms::LOADS, READS = (S::MB + S::NB) * Terms::READS;
+    constexpr int L = 2 * Terms::LOADS;
     __shared__ __align__(16) unsigned char lds[W_STAGE * W_STAGES];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int total = a.E * a.rowt * a.colt;
@@ -976,7 +1026,7 @@ __global__ __launch_bounds__(512, 2) void k_group_weights(WeightsArgs a)
                 asm volatile("" : "+v"(mp), "+v"(np));
                 read_half<Terms, Terms, S>(next, lds + at, lds + at + Terms::BYTES, mp, np, 0);
                 multiply<XT, S>(cur, acc);
-                interleave<S, READS>();
+                interleave<Terms, Terms, S>();
             };
             int b = 0;
 #pragma clang loop unroll(disable)
