@@ -653,14 +653,15 @@ __device__ __forceinline__ void run(unsigned char* lds, const M& m, const N& n, 
 // STORES<S> stores.
 template <typename S>
 constexpr int STORES = S::MB * S::NB / 2;
-__device__ __forceinline__ void trade_rows(u4_t& a, u4_t& b, bool low)
+__device__ __forceinline__ void trade_rows(u4_t& a, u4_t& b)
 {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
     {
-        const uint32_t got = (uint32_t)xor_lane_i<8>((int)(low ? b[i] : a[i]));
-        a[i] = low ? a[i] : got;
-        b[i] = low ? got : b[i];
+        // lanes 8 .. 15 of 16 take b of the lane 8 below, lanes 0 .. 7 take a of the lane 8 above
+        const int x = (int)a[i], y = (int)b[i];
+        a[i] = (uint32_t)__builtin_amdgcn_update_dpp(x, y, 0x128, 0xF, 0xC, false);
+        b[i] = (uint32_t)__builtin_amdgcn_update_dpp(y, x, 0x128, 0xF, 0x3, false);
     }
 }
 // Rows that are summed per token into a bf16 result are kept in between as fp16 times a power of two per 32 columns of a row, from their
@@ -693,7 +694,7 @@ __device__ __forceinline__ void store(f4_t (&acc)[S::MB][S::NB], void* y, int ty
     const bool low = r < 8;
     // two 16-byte pieces of row r, `step` columns apart, as pieces of rows r & 7 and (r & 7) + 8
     auto pair = [&](u4_t a, u4_t b, int i, int n, int step, int size) {
-        trade_rows(a, b, low);
+        trade_rows(a, b);
         const int m = m0 + 16 * i + (r & 7), c = low ? n : n + step;
         unsigned char* at = static_cast<unsigned char*>(y) + ((row0 + m) * ld + c) * size;
         if constexpr (FULL)
