@@ -650,7 +650,7 @@ __device__ __forceinline__ void run(unsigned char* lds, const M& m, const N& n, 
 // Lane (r, g) of a block holds columns 4 g .. 4 g + 3 of row r. For 16-bit outputs neighbouring blocks trade halves, so that a lane
 // has eight columns; then lanes r and r ^ 8 trade, so that a store writes 128 bytes of eight rows rather than 64 of sixteen: whole
 // cache lines, which leave for memory once. FULL: every row and column of the tile exists, type is 16 bits wide, and a wave sends exactly
-// STORES<S> stores.
+// STORES<S> stores. SUMMED: type may be ROWS_SCALED.
 template <typename S>
 constexpr int STORES = S::MB * S::NB / 2;
 __device__ __forceinline__ void trade_rows(u4_t& a, u4_t& b)
@@ -685,7 +685,7 @@ __device__ __forceinline__ int row_exponent(const f4_t& a, const f4_t& b)
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
-template <int XT, typename S, bool FULL = false>
+template <int XT, typename S, bool FULL = false, bool SUMMED = false>
 __device__ __forceinline__ void store(f4_t (&acc)[S::MB][S::NB], void* y, int type, size_t row0, int rows, int col0, int cols, size_t ld,
                                       int8_t* exps = nullptr)
 {
@@ -718,7 +718,7 @@ __device__ __forceinline__ void store(f4_t (&acc)[S::MB][S::NB], void* y, int ty
                 pair(__builtin_bit_cast(u4_t, acc[i][j]), __builtin_bit_cast(u4_t, acc[i][j + 1]), i, n0 + 16 * j + 4 * g, 16, 4);
             continue;
         }
-        if (!FULL && type == ROWS_SCALED)
+        if (SUMMED && type == ROWS_SCALED)
         {
 #pragma unroll
             for (int j = 0; j < S::NB; j += 2)
@@ -733,7 +733,7 @@ __device__ __forceinline__ void store(f4_t (&acc)[S::MB][S::NB], void* y, int ty
 #pragma unroll
         for (int j = 0; j < S::NB; j += 2)
         {
-            const bool half = !FULL && type == ROWS_SCALED;
+            const bool half = SUMMED && type == ROWS_SCALED;
             auto pack = [&](float a, float b) { return half ? pack2<MM_DTYPE_F16>(a, b) : pack2<XT>(a, b); };
             const auto lo = __builtin_amdgcn_permlane16_swap(pack(acc[i][j][0], acc[i][j][1]), pack(acc[i][j + 1][0], acc[i][j + 1][1]), false, false);
             const auto hi = __builtin_amdgcn_permlane16_swap(pack(acc[i][j][2], acc[i][j][3]), pack(acc[i][j + 1][2], acc[i][j + 1][3]), false, false);
@@ -797,7 +797,7 @@ __device__ __forceinline__ void rows_tile(const RowsArgs& a, const GroupTile& t,
         for (int j = 0; j < S::NB; ++j) acc[i][j] = f4_t{ 0.f, 0.f, 0.f, 0.f };
     const uint32_t mp = M::place(wave / S::WN * S::MB * 16), np = N::place(wave % S::WN * S::NB * 16);
     run<XT, M, N, S>(lds, m, n, a.terms, mp, np, acc);
-    store<XT, S>(acc, a.y, a.type, t.row, t.rows, col0, a.cols, a.cols, a.exps);
+    store<XT, S, false, XT == MM_DTYPE_BF16>(acc, a.y, a.type, t.row, t.rows, col0, a.cols, a.cols, a.exps);
 }
 
 // Columns ct C .. of rows of no expert.

@@ -89,7 +89,8 @@ def _check_out(what, dtype, w):
 def linear_forward(x, w, plan, gather=False, reduce=False, out_dtype=None, stream=None):
     """Row p of expert e times w[e] transposed (mm_group_linear): x [n, K] in the plan's order, or with `gather` [T, K], one row per
     token; w [E, N, K] (fp16 or bf16, as x). Returns [n, N], zero in rows of no expert, or with `reduce` [T, N], each token's rows summed
-    in the order of its picks; in w's type or fp32 (`out_dtype`), rounded once."""
+    in the order of its picks; in w's type or fp32 (`out_dtype`), rounded once (rows to be summed into bf16, of more than 16 routes, are
+    kept in between in 11 bits under a power of two per 32 columns)."""
     N, K, code = _check_linear("linear", w, plan, gather, reduce)
     _check_rows("linear", "x", x, plan.T if gather else plan.n, K, w.dtype)
     out_dtype = w.dtype if out_dtype is None else out_dtype
@@ -108,7 +109,8 @@ def linear_forward(x, w, plan, gather=False, reduce=False, out_dtype=None, strea
 
 def linear_backward(dy, x, w, plan, gather=False, reduce=False, need_x=True, need_w=True, dw_dtype=None, stream=None):
     """(dx, dw) of linear_forward from dy [n, N] (with `reduce` [T, N]), in w's type; dw also in fp32 (`dw_dtype`). None for one that is
-    not needed; x may be None without dw. Experts without rows have a dw of zeros (mm_group_linear_inputs, mm_group_linear_weights)."""
+    not needed; x may be None without dw. With `gather` dx is [T, K], rows summed per token as by linear_forward. Experts without rows have a
+    dw of zeros (mm_group_linear_inputs, mm_group_linear_weights)."""
     N, K, code = _check_linear("linear_backward", w, plan, gather, reduce)
     _check_rows("linear_backward", "dy", dy, plan.T if reduce else plan.n, N, w.dtype)
     dw_dtype = w.dtype if dw_dtype is None else dw_dtype
