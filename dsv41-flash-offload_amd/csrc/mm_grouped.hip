@@ -814,8 +814,8 @@ __device__ __forceinline__ void zero_tile(const RowsArgs& a, const GroupTile& t,
     }
 }
 
-// Bound by products where experts have many rows (131,072 rows of one expert, 4,096 x 4,096: 3,360 us, 1.3 PFLOP/s; of 64 3,510; of 384 4,300),
-// by reading the weights where they have few (64 experts of 66 rows, 5,120 x 4,608: 598 us, 5 TB/s). A tile's start and end take some 10 us.
+// Bound by products where experts have many rows (131,072 rows of one expert, 4,096 x 4,096: 3,360 us, 1.3 PFLOP/s; of 64 3,510; of 384 4,290),
+// by reading the weights where they have few (64 experts of 66 rows, 5,120 x 4,608: 593 us, 5 TB/s). A tile's start and end take some 10 us.
 // C = 256: large tiles. C = 128: small ones of at most FEW_ROWS rows, for calls that have too few large tiles for the GPU.
 template <int XT, bool ACROSS, int C>
 __global__ __launch_bounds__(2 * C, 2) void k_group_rows(RowsArgs a)
