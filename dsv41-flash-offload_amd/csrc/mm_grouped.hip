@@ -649,9 +649,9 @@ __device__ __forceinline__ void run(unsigned char* lds, const M& m, const N& n, 
 
 // Lane (r, g) of a block holds columns 4 g .. 4 g + 3 of row r. For 16-bit outputs neighbouring blocks trade halves, so that a lane
 // has eight columns; then lanes r and r ^ 8 trade, so that a store writes 128 bytes of eight rows rather than 64 of sixteen: whole
-// cache lines, which leave for memory once, past the caches that hold the operands (down of 131,072 rows of 64 experts, summed: 2,275 us through
-// them, 2,215 so; 65,536 rows of 1,024 columns 165 and 156; the gradient of the inputs 1,824 and 1,790). FULL: every row and column of the tile exists, type is 16 bits wide, and a wave sends exactly
-// STORES<S> stores. SUMMED: type may be ROWS_SCALED.
+// cache lines, which leave for memory once, past the caches that hold the operands (down of 131,072 rows of 64 experts, fp32 rows summed: 2,646 us through
+// them, 2,611 so; 4,200 rows of 5,120 columns 314 and 297; the gradient of the inputs, not summed, 1,824 and 1,790). FULL: every row and column of the tile exists, type is 16 bits wide, and a wave sends exactly
+// STORES<S> stores.
 template <typename S>
 constexpr int STORES = S::MB * S::NB / 2;
 __device__ __forceinline__ void trade_rows(u4_t& a, u4_t& b)
@@ -665,30 +665,8 @@ __device__ __forceinline__ void trade_rows(u4_t& a, u4_t& b)
         b[i] = (uint32_t)__builtin_amdgcn_update_dpp(y, x, 0x128, 0xF, 0x3, false);
     }
 }
-// Rows that are summed per token into a bf16 result are kept in between as fp16 times a power of two per 32 columns of a row, from their
-// largest finite value: each is within 2^-11 of itself (2^-39 of that largest where it is far below), an eighth of the result's own half step, at
-// half the bytes of fp32. 131,072 rows of 64 experts, 4,096 columns, summed by eights: 2,048 terms 2,630 us with fp32 rows, 2,310 so; 4,096 terms
-// 4,330 and 3,990; 3,600 rows of 5,120: 339 and 327.
-constexpr int ROWS_SCALED = 3, SCALE_COLS = 32;
-// the exponent for a lane's eight values and those of the other lanes of its row
-__device__ __forceinline__ int row_exponent(const f4_t& a, const f4_t& b)
-{
-    float top = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-    {
-        const float u = fabsf(a[i]), v = fabsf(b[i]);
-        top = fmaxf(top, fmaxf(u < INFINITY ? u : 0.f, v < INFINITY ? v : 0.f));
-    }
-    top = fmaxf(top, xor_lane<16>(top));
-    top = fmaxf(top, xor_lane<32>(top));
-    return max(-126, (int)(__float_as_uint(top) >> 23) - 127 - 14);      // the largest below 2^15
-}
-__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
-
-template <int XT, typename S, bool FULL = false, bool SUMMED = false>
-__device__ __forceinline__ void store(f4_t (&acc)[S::MB][S::NB], void* y, int type, size_t row0, int rows, int col0, int cols, size_t ld,
-                                      int8_t* exps = nullptr)
+template <int XT, typename S, bool FULL = false>
+__device__ __forceinline__ void store(f4_t (&acc)[S::MB][S::NB], void* y, int type, size_t row0, int rows, int col0, int cols, size_t ld)
 {
     const int lane = lane_here(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4, m0 = wave / S::WN * S::MB * 16, n0 = col0 + wave % S::WN * S::NB * 16;
@@ -719,25 +697,12 @@ __device__ __forceinline__ void store(f4_t (&acc)[S::MB][S::NB], void* y, int ty
                 pair(__builtin_bit_cast(u4_t, acc[i][j]), __builtin_bit_cast(u4_t, acc[i][j + 1]), i, n0 + 16 * j + 4 * g, 16, 4);
             continue;
         }
-        if (SUMMED && type == ROWS_SCALED)
-        {
-#pragma unroll
-            for (int j = 0; j < S::NB; j += 2)
-            {
-                const int e = row_exponent(acc[i][j], acc[i][j + 1]), m = m0 + 16 * i + r, n = n0 + 16 * j;
-                acc[i][j] *= power_of_two(-e);
-                acc[i][j + 1] *= power_of_two(-e);
-                if (g == j / 2 && m < rows && n < cols) exps[(row0 + m) * ((ld + SCALE_COLS - 1) / SCALE_COLS) + n / SCALE_COLS] = (int8_t)e;
-            }
-        }
         u4_t v[S::NB / 2];
 #pragma unroll
         for (int j = 0; j < S::NB; j += 2)
         {
-            const bool half = SUMMED && type == ROWS_SCALED;
-            auto pack = [&](float a, float b) { return half ? pack2<MM_DTYPE_F16>(a, b) : pack2<XT>(a, b); };
-            const auto lo = __builtin_amdgcn_permlane16_swap(pack(acc[i][j][0], acc[i][j][1]), pack(acc[i][j + 1][0], acc[i][j + 1][1]), false, false);
-            const auto hi = __builtin_amdgcn_permlane16_swap(pack(acc[i][j][2], acc[i][j][3]), pack(acc[i][j + 1][2], acc[i][j + 1][3]), false, false);
+            const auto lo = __builtin_amdgcn_permlane16_swap(pack2<XT>(acc[i][j][0], acc[i][j][1]), pack2<XT>(acc[i][j + 1][0], acc[i][j + 1][1]), false, false);
+            const auto hi = __builtin_amdgcn_permlane16_swap(pack2<XT>(acc[i][j][2], acc[i][j][3]), pack2<XT>(acc[i][j + 1][2], acc[i][j + 1][3]), false, false);
             v[j / 2] = u4_t{ lo[0], hi[0], lo[1], hi[1] };
         }
         const int n = n0 + 16 * (g & 1) + 4 * (g & 2);
@@ -764,9 +729,8 @@ struct RowsArgs
     void* y;
     const GroupTile* tiles;
     const int32_t *ntiles, *token;     // token: row of x of each row, NULL: its own
-    int8_t* exps;                      // of ROWS_SCALED rows
     size_t xbytes;
-    int terms, cols, type, zero, colt;      // zero: rows of no expert are stored (as zeros); colt: column tiles
+    int terms, cols, wcols, type, zero, colt;      // cols of the wcols that W has, from w on; zero: rows of no expert are stored (as zeros); colt: column tiles
 };
 
 // XCD x of eight runs workgroups x, x + 8, ..., and has its own L2: runs of 32 tiles (its CUs) stay on one XCD.
@@ -784,12 +748,12 @@ __device__ __forceinline__ void rows_tile(const RowsArgs& a, const GroupTile& t,
     using N = std::conditional_t<ACROSS, Across<TERMS, C, S::WAVES>, Along<C, S::WAVES>>;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col0 = ct * C;
-    const uint16_t* w = a.w + (size_t)t.expert * a.terms * a.cols;
+    const uint16_t* w = a.w + (size_t)t.expert * a.terms * a.wcols;
     M m;
     N n;
     if (a.token) m.init(a.x, 2 * a.terms, t.rows, (uint32_t)a.xbytes, a.token + t.row);
     else m.init(a.x + (size_t)t.row * a.terms, 2 * a.terms, t.rows, (uint32_t)t.rows * a.terms * 2, nullptr);
-    if constexpr (ACROSS) n.init(w, 2 * a.cols, col0, a.cols);
+    if constexpr (ACROSS) n.init(w, 2 * a.wcols, col0, a.cols);
     else n.init(w + (size_t)col0 * a.terms, 2 * a.terms, min(C, a.cols - col0), (uint32_t)min(C, a.cols - col0) * a.terms * 2, nullptr);
     f4_t acc[S::MB][S::NB];
 #pragma unroll
@@ -798,7 +762,7 @@ __device__ __forceinline__ void rows_tile(const RowsArgs& a, const GroupTile& t,
         for (int j = 0; j < S::NB; ++j) acc[i][j] = f4_t{ 0.f, 0.f, 0.f, 0.f };
     const uint32_t mp = M::place(wave / S::WN * S::MB * 16), np = N::place(wave % S::WN * S::NB * 16);
     run<XT, M, N, S>(lds, m, n, a.terms, mp, np, acc);
-    store<XT, S, false, XT == MM_DTYPE_BF16>(acc, a.y, a.type, t.row, t.rows, col0, a.cols, a.cols, a.exps);
+    store<XT, S>(acc, a.y, a.type, t.row, t.rows, col0, a.cols, a.cols);
 }
 
 // Columns ct C .. of rows of no expert.
@@ -859,7 +823,7 @@ __device__ __forceinline__ void few_tile(const RowsArgs& a, const GroupTile& t, 
     constexpr int AHEAD = 8;                                         // blocks of 128 terms on their way
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     const uint32_t ld = 2 * a.terms;
-    const __amdgpu_buffer_rsrc_t wb = buffer(a.w + ((size_t)t.expert * a.cols + col0) * a.terms, (uint32_t)min(16, a.cols - col0) * ld);
+    const __amdgpu_buffer_rsrc_t wb = buffer(a.w + ((size_t)t.expert * a.wcols + col0) * a.terms, (uint32_t)min(16, a.cols - col0) * ld);
     const __amdgpu_buffer_rsrc_t xb = a.token ? buffer(a.x, (uint32_t)a.xbytes) : buffer(a.x + (size_t)t.row * a.terms, (uint32_t)t.rows * ld);
     // columns past the last one are past the buffer; rows past the tile's are its last row again, and not stored
     const int m = min(r, t.rows - 1);
@@ -1068,12 +1032,12 @@ __global__ __launch_bounds__(512, 2) void k_group_weights(WeightsArgs a)
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// Rows summed per token, in the order of its picks: out[t] = sum over j of rows[inv[t k + j]], picks of no expert left out. Bound by
-// memory (4,200 scaled rows of 5,120 columns: 13 us, 3.9 TB/s).
+// Rows summed per token, in the order of its picks: out[t] = sum over j of rows[inv[t k + j]], picks of no expert left out; cols4 and ocols4: fours of
+// columns of the rows and of out. Bound by memory (4,200 rows of 5,120 columns into bf16: 19.7 us, 4.7 TB/s).
 // ---------------------------------------------------------------------------------------------------------
 template <int OT>
 __global__ __launch_bounds__(256) void k_group_sum(const float* __restrict__ rows, const int32_t* __restrict__ inv, const int32_t* __restrict__ live,
-                                                   long long n4, int topk, int cols4, void* __restrict__ out)
+                                                   long long n4, int topk, int cols4, int ocols4, void* __restrict__ out)
 {
     const int end = *live;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n4; i += (long long)gridDim.x * 256)
@@ -1093,38 +1057,9 @@ __global__ __launch_bounds__(256) void k_group_sum(const float* __restrict__ row
                 s.w += v.w;
             }
         }
-        if constexpr (OT == MM_DTYPE_F32) reinterpret_cast<f4_t*>(out)[i] = s;
-        else reinterpret_cast<u2_t*>(out)[i] = u2_t{ pack2<OT>(s.x, s.y), pack2<OT>(s.z, s.w) };
-    }
-}
-
-// The same of rows as ROWS_SCALED keeps them, into bf16.
-__global__ __launch_bounds__(256) void k_group_sum_scaled(const uint16_t* __restrict__ rows, const int8_t* __restrict__ exps, const int32_t* __restrict__ inv,
-                                                          const int32_t* __restrict__ live, long long n8, int topk, int cols8, void* __restrict__ out)
-{
-    const int end = *live, groups = (cols8 + 3) / 4;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n8; i += (long long)gridDim.x * 256)
-    {
-        const long long t = i / cols8;
-        const int c = (int)(i - t * cols8);
-        float s[8] = {};
-        for (int j = 0; j < topk; ++j)
-        {
-            const int p = inv[t * topk + j];
-            if (p >= end) continue;
-            const u4_t v = reinterpret_cast<const u4_t*>(rows)[(size_t)p * cols8 + c];
-            const float f = power_of_two(exps[(size_t)p * groups + c / 4]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-            {
-                s[2 * k] = fmaf(h2f((uint16_t)v[k]), f, s[2 * k]);
-                s[2 * k + 1] = fmaf(h2f((uint16_t)(v[k] >> 16)), f, s[2 * k + 1]);
-            }
-        }
-        u4_t o;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) o[k] = pack2<MM_DTYPE_BF16>(s[2 * k], s[2 * k + 1]);
-        reinterpret_cast<u4_t*>(out)[i] = o;
+        const size_t o = (size_t)t * ocols4 + c;
+        if constexpr (OT == MM_DTYPE_F32) reinterpret_cast<f4_t*>(out)[o] = s;
+        else reinterpret_cast<u2_t*>(out)[o] = u2_t{ pack2<OT>(s.x, s.y), pack2<OT>(s.z, s.w) };
     }
 }
 
@@ -1159,11 +1094,20 @@ int check(const char* what, const mm_group_plan_t* p, int dtype, int K, int N, i
     return MM_OK;
 }
 
-// Whether rows to be summed are kept scaled (those of the few-route form are not: they are few).
-bool scaled_rows(long long n, int y_type) { return y_type == MM_DTYPE_BF16 && n > FEW_ROUTES; }
+// Rows that are summed per token are fp32 until their sum is rounded: where rows cancel, fewer bits would be the result's whole error. All columns' rows
+// at once take 4 cols bytes a row. The least workspace is that too, but for a bf16 result of many routes about half: the product and the sum then go by bands
+// of columns, which costs a short call its second launches, a long one little (down of 131,072 rows of 64 experts 2,611 us at once, 2,499 in two bands; 384
+// experts 2,884 and 2,953; gradient of 4,200 rows of 5,120 columns 564 and 651).
 size_t sum_workspace(long long n, int cols, int y_type)
 {
-    return scaled_rows(n, y_type) ? (size_t)n * cols * 2 + (size_t)n * ((cols + SCALE_COLS - 1) / SCALE_COLS) : (size_t)n * cols * 4;
+    const int half = 2 * cols + (cols + 31) / 32;
+    return (size_t)n * (y_type == MM_DTYPE_BF16 && n > FEW_ROUTES ? std::max(half, 32) : 4 * cols);
+}
+// Columns of a band: all of them if their rows fit, else whole column tiles, or a multiple of eight.
+int band_columns(size_t ws_bytes, long long n, int cols)
+{
+    const int fit = (int)std::min<size_t>(ws_bytes / n / 4, cols);
+    return fit == cols ? cols : fit >= 256 ? fit & ~255 : fit & ~7;
 }
 
 template <bool ACROSS>
@@ -1179,46 +1123,41 @@ int launch_rows(const char* what, const mm_group_plan_t* p, const void* x, const
     const hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
     RowsArgs a = {};
     a.x = static_cast<const uint16_t*>(x);
-    a.w = static_cast<const uint16_t*>(w);
-    a.y = reduce ? ws : y;
     a.token = gather ? p->token : nullptr;
     a.xbytes = (size_t)p->T * terms * 2;
     a.terms = terms;
-    a.cols = cols;
-    const bool scaled = reduce && scaled_rows(n, y_type);
-    a.type = scaled ? ROWS_SCALED : reduce ? MM_DTYPE_F32 : y_type;
-    a.exps = scaled ? static_cast<int8_t*>(ws) + (size_t)n * cols * 2 : nullptr;
+    a.wcols = cols;
+    a.type = reduce ? MM_DTYPE_F32 : y_type;
     a.zero = !reduce;
-    // The form by the tiles there will be (the routes' experts are not known here): large ones as soon as they nearly fill the GPU (512 rows of
-    // each of 8 experts of 4096 x 4096, 320 tiles by this estimate: 115 us, small ones 195), else small ones (1,000 rows of one expert, 48
-    // tiles: 98 and 38 us). Forward, few rows of many experts are a little faster in small tiles too (64 of 64: 448 and 418 us; 128: 477
-    // and 525), the gradient of the inputs is not (359 and 393). A few routes that leave most CUs without a small tile are split over the terms
-    // instead (one of 4096 x 4096: 28 and 9 us; eight: 43 and 45).
-    const long long met = std::min<long long>(n, p->E), large = std::max(met, n / ROWS + met / 2) * ((cols + 255) / 256);
-    const bool few = !ACROSS && n <= FEW_ROUTES && n * ((cols + 127) / 128) < 256;
-    const bool small = !few && (large < 192 || (!ACROSS && n <= 64 * met));
-    const int most = few || small ? FEW_ROWS : ROWS, width = few ? 16 : small ? 128 : 256;
-    a.tiles = reinterpret_cast<const GroupTile*>(p->tiles) + (most == FEW_ROWS ? tile_capacity(n, p->E, ROWS) : 0);
-    a.ntiles = p->ntiles + (most == FEW_ROWS);
-    a.colt = (cols + width - 1) / width;
-    const long long tiles = tile_capacity(n, p->E, most) * a.colt, blocks = (tiles + 255) / 256 * 256;
-    MM_CHECK_ARG(blocks * (few || small ? 256 : 512) <= MOST_THREADS, "%s: too many tiles", what);
     const bool h = dtype == MM_DTYPE_F16;
-    if (few) hipLaunchKernelGGL((h ? k_group_few<MM_DTYPE_F16> : k_group_few<MM_DTYPE_BF16>), dim3((unsigned)blocks), dim3(256), 0, hs, a);
-    else if (small) hipLaunchKernelGGL((h ? k_group_rows<MM_DTYPE_F16, ACROSS, 128> : k_group_rows<MM_DTYPE_BF16, ACROSS, 128>), dim3((unsigned)blocks), dim3(256), 0, hs, a);
-    else hipLaunchKernelGGL((h ? k_group_rows<MM_DTYPE_F16, ACROSS, 256> : k_group_rows<MM_DTYPE_BF16, ACROSS, 256>), dim3((unsigned)blocks), dim3(512), 0, hs, a);
-    if (scaled)
+    const int band = reduce ? band_columns(ws_bytes, n, cols) : cols;
+    for (int c0 = 0; c0 < cols; c0 += band)
     {
-        const long long n8 = (long long)p->T * cols / 8;
-        hipLaunchKernelGGL(k_group_sum_scaled, dim3((unsigned)std::min<long long>((n8 + 255) / 256, 1 << 22)), dim3(256), 0, hs,
-                           static_cast<const uint16_t*>(ws), a.exps, p->inv, p->offsets + p->E, n8, p->topk, cols / 8, y);
-    }
-    else if (reduce)
-    {
-        const long long n4 = (long long)p->T * cols / 4;
+        a.cols = std::min(band, cols - c0);
+        a.w = static_cast<const uint16_t*>(w) + (size_t)c0 * (ACROSS ? 1 : terms);
+        a.y = reduce ? ws : y;
+        // The form by the tiles there will be (the routes' experts are not known here): large ones as soon as they nearly fill the GPU (512 rows of
+        // each of 8 experts of 4096 x 4096, 320 tiles by this estimate: 115 us, small ones 195), else small ones (1,000 rows of one expert, 48
+        // tiles: 98 and 38 us). Forward, few rows of many experts are a little faster in small tiles too (64 of 64: 448 and 418 us; 128: 477
+        // and 525), the gradient of the inputs is not (359 and 393). A few routes that leave most CUs without a small tile are split over the terms
+        // instead (one of 4096 x 4096: 28 and 9 us; eight: 43 and 45).
+        const long long met = std::min<long long>(n, p->E), large = std::max(met, n / ROWS + met / 2) * ((a.cols + 255) / 256);
+        const bool few = !ACROSS && n <= FEW_ROUTES && n * ((a.cols + 127) / 128) < 256;
+        const bool small = !few && (large < 192 || (!ACROSS && n <= 64 * met));
+        const int most = few || small ? FEW_ROWS : ROWS, width = few ? 16 : small ? 128 : 256;
+        a.tiles = reinterpret_cast<const GroupTile*>(p->tiles) + (most == FEW_ROWS ? tile_capacity(n, p->E, ROWS) : 0);
+        a.ntiles = p->ntiles + (most == FEW_ROWS);
+        a.colt = (a.cols + width - 1) / width;
+        const long long tiles = tile_capacity(n, p->E, most) * a.colt, blocks = (tiles + 255) / 256 * 256;
+        MM_CHECK_ARG(blocks * (few || small ? 256 : 512) <= MOST_THREADS, "%s: too many tiles", what);
+        if (few) hipLaunchKernelGGL((h ? k_group_few<MM_DTYPE_F16> : k_group_few<MM_DTYPE_BF16>), dim3((unsigned)blocks), dim3(256), 0, hs, a);
+        else if (small) hipLaunchKernelGGL((h ? k_group_rows<MM_DTYPE_F16, ACROSS, 128> : k_group_rows<MM_DTYPE_BF16, ACROSS, 128>), dim3((unsigned)blocks), dim3(256), 0, hs, a);
+        else hipLaunchKernelGGL((h ? k_group_rows<MM_DTYPE_F16, ACROSS, 256> : k_group_rows<MM_DTYPE_BF16, ACROSS, 256>), dim3((unsigned)blocks), dim3(512), 0, hs, a);
+        if (!reduce) break;
+        const long long n4 = (long long)p->T * a.cols / 4;
         auto sum = y_type == MM_DTYPE_F32 ? k_group_sum<MM_DTYPE_F32> : y_type == MM_DTYPE_F16 ? k_group_sum<MM_DTYPE_F16> : k_group_sum<MM_DTYPE_BF16>;
         hipLaunchKernelGGL(sum, dim3((unsigned)std::min<long long>((n4 + 255) / 256, 1 << 22)), dim3(256), 0, hs, static_cast<const float*>(ws), p->inv, p->offsets + p->E, n4,
-                           p->topk, cols / 4, y);
+                           p->topk, a.cols / 4, cols / 4, static_cast<unsigned char*>(y) + (size_t)c0 * (y_type == MM_DTYPE_F32 ? 4 : 2));
     }
     return check_launch(what);
 }

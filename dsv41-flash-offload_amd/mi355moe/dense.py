@@ -85,8 +85,7 @@ def moe(store, x, ids, w, shared_expert=None, stream=None):
     """out fp32 [T, H] = sum_j w[t, j] * expert_{ids[t, j]}(x_t) (+ expert `shared_expert` with weight 1), expert(x) = W2 (min(silu(Wg x),
     limit) clamp(Wu x)), with gradients into x, w and the store's weights. x [T, H] in the weights' type, ids int64 and w [T, k]; ids
     outside [0, E) contribute nothing and get no gradient. Gate and up rows, the weighted activation and, backward, the gradients between the
-    products are rounded to the weights' type (the products' operands), and the rows of a bf16 dx are kept as grouped.linear_forward says;
-    sums are fp32. Under stream capture as router.topk."""
+    products are rounded to the weights' type (the products' operands); sums are fp32. Under stream capture as router.topk."""
     if x.dtype != store.w13.dtype:
         raise TypeError(f"dense.moe: x must have the weights' type {store.w13.dtype} (got {x.dtype})")
     if x.dim() != 2 or x.shape[1] != store.H:

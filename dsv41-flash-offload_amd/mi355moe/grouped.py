@@ -86,11 +86,15 @@ def _check_out(what, dtype, w):
     return _OUT[dtype]
 
 
+def _rows_workspace(plan, cols):
+    """Bytes of all rows to be summed, in fp32: what results of fp32 need, and more than the least for bf16, which would take more launches."""
+    return _lib.load().mm_group_linear_workspace(plan.T, plan.k, cols, 1, _lib.DTYPE_F32)
+
+
 def linear_forward(x, w, plan, gather=False, reduce=False, out_dtype=None, stream=None):
     """Row p of expert e times w[e] transposed (mm_group_linear): x [n, K] in the plan's order, or with `gather` [T, K], one row per
     token; w [E, N, K] (fp16 or bf16, as x). Returns [n, N], zero in rows of no expert, or with `reduce` [T, N], each token's rows summed
-    in the order of its picks; in w's type or fp32 (`out_dtype`), rounded once (rows to be summed into bf16, of more than 16 routes, are
-    kept in between in 11 bits under a power of two per 32 columns)."""
+    in the order of its picks; in w's type or fp32 (`out_dtype`). Rows and sums are fp32, results are rounded once."""
     N, K, code = _check_linear("linear", w, plan, gather, reduce)
     _check_rows("linear", "x", x, plan.T if gather else plan.n, K, w.dtype)
     out_dtype = w.dtype if out_dtype is None else out_dtype
@@ -100,7 +104,7 @@ def linear_forward(x, w, plan, gather=False, reduce=False, out_dtype=None, strea
         y = torch.empty((plan.T if reduce else plan.n, N), dtype=out_dtype, device=dev)
         if plan.n:
             x = _lib.aligned(x)
-            wsb = _lib.load().mm_group_linear_workspace(plan.T, plan.k, N, 1, out_code) if reduce else 0
+            wsb = _rows_workspace(plan, N) if reduce else 0
             ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
             _lib.call("mm_group_linear", plan._ref, x.data_ptr(), w.data_ptr(), code, K, N, int(gather), int(reduce), y.data_ptr(), out_code,
                       _p(ws), wsb, _lib.raw_stream(dev))
@@ -126,7 +130,7 @@ def linear_backward(dy, x, w, plan, gather=False, reduce=False, need_x=True, nee
         if need_x:
             dx = torch.empty((plan.T if gather else plan.n, K), dtype=w.dtype, device=dev)
             if plan.n:
-                wsb = _lib.load().mm_group_linear_workspace(plan.T, plan.k, K, 1, code) if gather else 0
+                wsb = _rows_workspace(plan, K) if gather else 0
                 ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
                 _lib.call("mm_group_linear_inputs", plan._ref, dy.data_ptr(), w.data_ptr(), code, K, N, int(gather), int(reduce), dx.data_ptr(),
                           code, _p(ws), wsb, _lib.raw_stream(dev))

@@ -330,15 +330,15 @@ int mm_group_plan(const int64_t* ids, const mm_group_plan_t* plan, int32_t* coun
 
 /* y[p] = W[e] x[p] over the rows p of each expert e: w [E][N][K] and x in dtype (fp16 or bf16), y in dtype or fp32, sums in fp32,
  * rounded once. gather: x is [T][K] and row p reads row token[p], else [n][K]. reduce: y is [T][N], the sum of each token's rows in the order
- * of its picks (from rows in the workspace, mm_group_linear_workspace(T, topk, N, reduce, y_dtype) bytes: fp32, or for a bf16 y of more than 16
- * routes fp16 times a power of two per 32 columns of a row, within 2^-11 of each value); else [n][N], rows of no expert
- * zero. K and N multiples of 8, at most 2^20, K N < 2^31; tensors of rows per token below 4 GiB; tiles of a call within one launch (2^32
+ * of its picks, from fp32 rows in the workspace; else [n][N], rows of no expert zero. Workspace: n N 4 bytes hold all the rows, and
+ * mm_group_linear_workspace(T, topk, N, reduce, y_dtype) bytes are enough (the same, for a bf16 y of more than 16 routes about half: the columns then go
+ * in bands, with the same results). K and N multiples of 8, at most 2^20, K N < 2^31; tensors of rows per token below 4 GiB; tiles of a call within one launch (2^32
  * threads: 2^30 rows of 1,024 columns, say); all pointers 16-byte aligned. Sums are in an order of the call's sizes: a call repeats bit for bit. */
 size_t mm_group_linear_workspace(int T, int topk, int cols, int reduce, int y_dtype);
 int mm_group_linear(const mm_group_plan_t* plan, const void* x, const void* w, int dtype, int K, int N, int gather, int reduce,
                     void* y, int y_dtype, void* workspace, size_t workspace_bytes, mm_stream_t stream);
 /* Gradient of x: dx[p] = W[e]^T dy[p], of the same product: with gather dx is [T][K], summed per token (workspace:
- * mm_group_linear_workspace(T, topk, K, gather, dx_dtype)), with reduce dy is [T][N]. */
+ * mm_group_linear_workspace(T, topk, K, gather, dx_dtype) bytes, n K 4 for all the rows at once), with reduce dy is [T][N]. */
 int mm_group_linear_inputs(const mm_group_plan_t* plan, const void* dy, const void* w, int dtype, int K, int N, int gather, int reduce,
                            void* dx, int dx_dtype, void* workspace, size_t workspace_bytes, mm_stream_t stream);
 /* Gradient of W: dw [E][N][K] (dtype or fp32) = sum over the rows of each expert of dy[p] x[p]^T; zero for experts without rows. */
