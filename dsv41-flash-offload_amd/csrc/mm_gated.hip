@@ -2,6 +2,7 @@
 // step keeps the activation's input: with [g | u] a row, w its routing weight and L the clamp,
 //   h = w a c,  a = min(g s, L),  c = clamp(u, -L, L),  s = 1 / (1 + exp(-g))
 //   dg = w dh c s (1 + g (1 - s)) [g s <= L],  du = w dh a [|u| <= L],  dw = sum over the columns of dh a c
+// (a clamp that is there cuts the gradient of NaN too; without one, NaN and infinities go the formula's way),
 // and per 32 neighbours of a row, with e the least exponent that has all |x| <= 127 2^e,
 //   code = x 2^-e rounded to a whole number (ties to even),  x again = code 2^e, within 2^(e - 1) <= max |x| / 127:
 // the scaling is exact, so the codes' rounding is the only one. 32 that hold an infinity or a NaN come back as NaN.
@@ -138,6 +139,7 @@ __global__ __launch_bounds__(256) void k_gated_backward(GatedArgs a)
     const bool live = !a.live || (int)row < *a.live;
     const int route = a.order ? a.order[row] : (int)row;
     const float w = !live ? 0.f : a.weights ? a.weights[route] : 1.f;
+    const bool free = a.limit == INFINITY;
     float sum = 0.f;
     for (int at = 8 * threadIdx.x; at < a.I; at += 8 * blockDim.x)
     {
@@ -165,8 +167,8 @@ __global__ __launch_bounds__(256) void k_gated_backward(GatedArgs a)
             for (int i = 0; i < 8; ++i)
             {
                 const float s = logistic(g[i]), v = g[i] * s, act = below(v, a.limit), c = within(u[i], a.limit), wd = w * d[i];
-                dg[i] = v <= a.limit ? wd * c * s * (1.f + g[i] * (1.f - s)) : 0.f;
-                du[i] = fabsf(u[i]) <= a.limit ? wd * act : 0.f;
+                dg[i] = free || v <= a.limit ? wd * c * s * (1.f + g[i] * (1.f - s)) : 0.f;
+                du[i] = free || fabsf(u[i]) <= a.limit ? wd * act : 0.f;
                 h[i] = w * act * c;
                 sum = fmaf(d[i], act * c, sum);
             }

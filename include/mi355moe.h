@@ -352,8 +352,8 @@ int mm_group_linear_weights(const mm_group_plan_t* plan, const void* dy, const v
  * nearest even; 32 that hold an infinity or NaN have exponent 127 and come back as NaN. I a multiple of 8, at most 2^20. */
 int mm_gated(const mm_group_plan_t* plan, const void* gu, int dtype, int n, int I, const float* weights, float limit, void* h,
              int8_t* codes, int8_t* exps, mm_stream_t stream);
-/* Its gradient, from gu or from its 8 bits (the other NULL): dgu [n][2 I] (zero where a clamp is passed), dweights fp32 [n] by route and
- * h [n][I] once more (either may be NULL). */
+/* Its gradient, from gu or from its 8 bits (the other NULL): dgu [n][2 I] (zero where a clamp is passed or met by
+ * NaN; a limit of 0 or infinity is no clamp), dweights fp32 [n] by route and h [n][I] once more (either may be NULL). */
 int mm_gated_backward(const mm_group_plan_t* plan, const void* dh, const void* gu, const int8_t* codes, const int8_t* exps, int dtype,
                       int n, int I, const float* weights, float limit, void* dgu, float* dweights, void* h, mm_stream_t stream);
 
