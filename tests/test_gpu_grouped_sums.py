@@ -121,3 +121,25 @@ def test_columns_of_all_sizes(dev):
     rounded_once(grouped.linear_forward(r.to(dev), w.to(dev), plan, reduce=True), ref, mag, terms + 2)
     w = w.transpose(1, 2).contiguous()
     rounded_once(grouped.linear_backward(r.to(dev), None, w.to(dev), plan, gather=True, need_w=False)[0], ref, mag, terms + 2)
+
+
+@pytest.mark.parametrize("turn", [False, True])
+def test_long_sums_take_no_more_than_half_the_rows(dev, turn):
+    """320,000 rows of 4,096 columns are 5.2 GB in fp32: a bf16 result asks for less than 3, and has the same bits."""
+    from mi355moe import grouped
+    g = torch.Generator(device=dev).manual_seed(9)
+    T, k, E, terms, cols = 40000, 8, 8, 64, 4096
+    ids = torch.randint(-1, E, (T, k), generator=g, device=dev)
+    r = torch.randn((T * k, terms), generator=g, device=dev).to(BF)
+    w = torch.randn((E, terms, cols) if turn else (E, cols, terms), generator=g, device=dev).to(BF)
+    plan = grouped.Plan(ids, E)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = grouped.linear_backward(r, None, w, plan, gather=True, need_w=False)[0] if turn else grouped.linear_forward(r, w, plan, reduce=True)
+    torch.cuda.synchronize()
+    out = 2 * T * cols
+    assert torch.cuda.max_memory_allocated() - before - out < 3e9
+    exact = call_c("mm_group_linear_inputs" if turn else "mm_group_linear", plan, r, w, torch.float32, 4 * T * k * cols)
+    assert torch.equal(got, exact.to(BF))
