@@ -4,7 +4,7 @@
 //   dg = w dh c s (1 + g (1 - s)) [g s <= L],  du = w dh a [|u| <= L],  dw = sum over the columns of dh a c
 // (a clamp that is there cuts the gradient of NaN too; without one, NaN and infinities go the formula's way),
 // and per 32 neighbours of a row, with e the least exponent that has all |x| <= 127 2^e,
-//   code = x 2^-e rounded to a whole number (ties to even),  x again = code 2^e, within 2^(e - 1) <= max |x| / 127:
+//   code = x 2^-e rounded to a whole number (ties to even),  x again = code 2^e, within 2^(e - 1) <= max |x| / 127 (2^-127 at e = -126, the least):
 // the scaling is exact, so the codes' rounding is the only one. 32 that hold an infinity or a NaN come back as NaN.
 #include "mm_common.h"
 #include "mm_decode.h"
@@ -83,7 +83,7 @@ __device__ __forceinline__ float below(float v, float l) { return v > l ? l : v;
 __device__ __forceinline__ float within(float v, float l) { return v > l ? l : v < -l ? -l : v; }
 
 // A workgroup takes a row, a thread eight columns of g and of u; a loop over rows instead took 4 % longer. Bound by memory (131,072 rows of
-// 2,048: with codes 367 us, 5.9 TB/s; 4,200 rows of 2,304 without them 13 us, 4.5 TB/s).
+// 2,048: with codes 365 us, 5.9 TB/s; 4,200 rows of 2,304 without them 14 us, 4.2 TB/s).
 template <int XT, bool SAVE>
 __global__ __launch_bounds__(256) void k_gated(GatedArgs a)
 {
@@ -129,7 +129,7 @@ __global__ __launch_bounds__(256) void k_gated(GatedArgs a)
     }
 }
 
-// The same shape. Bound by memory (131,072 rows of 2,048 from codes 489 us, with h again 5.6 TB/s; 4,200 rows of 2,304 from 16 bits 19 us).
+// The same shape. Bound by memory (131,072 rows of 2,048 from codes 476 us, with h again 5.7 TB/s; 4,200 rows of 2,304 from 16 bits 19 us).
 template <int XT, bool SAVED>
 __global__ __launch_bounds__(256) void k_gated_backward(GatedArgs a)
 {

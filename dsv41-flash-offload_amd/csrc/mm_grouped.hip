@@ -1136,7 +1136,7 @@ int launch_rows(const char* what, const mm_group_plan_t* p, const void* x, const
         a.cols = std::min(band, cols - c0);
         a.w = static_cast<const uint16_t*>(w) + (size_t)c0 * (ACROSS ? 1 : terms);
         a.y = reduce ? ws : y;
-        // The form by the tiles there will be (the routes' experts are not known here): large ones as soon as they nearly fill the GPU (512 rows of
+        // The form by the tiles there will be (the routes' experts are not known here; measured with equal experts): large ones as soon as they nearly fill the GPU (512 rows of
         // each of 8 experts of 4096 x 4096, 320 tiles by this estimate: 115 us, small ones 195), else small ones (1,000 rows of one expert, 48
         // tiles: 98 and 38 us). Forward, few rows of many experts are a little faster in small tiles too (64 of 64: 448 and 418 us; 128: 477
         // and 525), the gradient of the inputs is not (359 and 393). A few routes that leave most CUs without a small tile are split over the terms

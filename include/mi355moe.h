@@ -333,7 +333,7 @@ int mm_group_plan(const int64_t* ids, const mm_group_plan_t* plan, int32_t* coun
  * of its picks, from fp32 rows in the workspace; else [n][N], rows of no expert zero. Workspace: n N 4 bytes hold all the rows, and
  * mm_group_linear_workspace(T, topk, N, reduce, y_dtype) bytes are enough (the same, for a bf16 y of more than 16 routes about half: the columns then go
  * in bands, with the same results). K and N multiples of 8, at most 2^20, K N < 2^31; tensors of rows per token below 4 GiB; tiles of a call within one launch (2^32
- * threads: 2^30 rows of 256 columns, say); all pointers 16-byte aligned. Sums are in an order of the call's sizes: a call repeats bit for bit. */
+ * threads, 512 of them for 256 rows by 256 columns); all pointers 16-byte aligned. Sums are in an order of the call's sizes: a call repeats bit for bit. */
 size_t mm_group_linear_workspace(int T, int topk, int cols, int reduce, int y_dtype);
 int mm_group_linear(const mm_group_plan_t* plan, const void* x, const void* w, int dtype, int K, int N, int gather, int reduce,
                     void* y, int y_dtype, void* workspace, size_t workspace_bytes, mm_stream_t stream);

@@ -3,7 +3,7 @@ import ctypes
 
 
 def test_tiles_of_a_call_fit_one_launch():
-    """2^30 rows of 512 columns are two tiles of 512 threads per 256 rows, 2^32 threads and more; the header's 256 columns are half of that."""
+    """2^30 rows of 512 columns are two tiles of 512 threads per 256 rows, 2^32 threads and more."""
     from mi355moe import _lib
     L = _lib.load()
     plan = ctypes.byref(_lib.MMGroupPlan(*[256] * 6, 1 << 30, 1, 3))
